@@ -285,6 +285,89 @@ typedef struct sqa_append_args {
 
 SQA_API int sqa_cache_append(const sqa_append_args* args, void* stream);
 
+/* ---- Block-scaled 8-bit cache ----
+ * An e4m3 cache (SQA_KV_FP8_E4M3) with one fp32 scale per page (16 tokens) and KV
+ * head, K and V apart: a cached element stands for scale * e4m3.  Scales are device
+ * arrays [num_pages, num_kv_heads], `page_stride` floats from page to page
+ * (0 = num_kv_heads; larger for a view of a bigger array).  No upstream counterpart. */
+typedef struct sqa_scales {
+  float* key;
+  float* value;
+  int64_t page_stride;
+} sqa_scales;
+
+/* Quantising append: sqa_cache_append's tokens and slots (and its handling of bad
+ * lengths and pages), for new K/V of type new_dtype (SQA_DTYPE_F16 or
+ * SQA_DTYPE_BF16; args->kv_dtype is SQA_KV_FP8_E4M3).  Any q_len >= 1.  Per touched
+ * page and head, K and V apart: need = the smallest power of two (2^-100 at least)
+ * that brings the finite new values within 448 * need; scale = need for a page whose
+ * first slot is new, else the larger of need and the old scale, where the page's older
+ * tokens are stored again at the grown scale.  Values are rounded to nearest even
+ * and saturate at 448 * scale; NaN stays NaN.  Slots behind the last new token keep
+ * their bytes.  One page twice in a call races. */
+SQA_API int sqa_cache_append_scaled(const sqa_append_args* args, const sqa_scales* scales, int32_t new_dtype,
+                                    void* stream);
+
+/* sqa_forward over a block-scaled cache: K = key_scale * e4m3, V = value_scale * e4m3.
+ * args as for sqa_forward with kv_dtype = SQA_KV_FP8_E4M3, except: with `out`, out_lse
+ * may be given too (fp32 [batch, q_len, num_q_heads], as in partial mode); kernel must
+ * be 0 and cluster 0 or 1.  Scales are finite; key scales have any sign, value scales are
+ * not negative.  Needs sqa_scaled_workspace_bytes() bytes of workspace, zeroed
+ * once with sqa_workspace_init; the status word is read with sqa_read_device_status. */
+SQA_API size_t sqa_scaled_workspace_bytes(const sqa_args* args, int device, int* status);
+SQA_API int sqa_forward_scaled(const sqa_args* args, const sqa_scales* scales, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* ---- Accumulated attention weight, and eviction by it ----
+ * scores: fp32 [num_pages, num_kv_heads, 16], one value per cached token and KV head.
+ * With w(b, h, t) = the sum over the rows (q_len draft tokens x 4 query heads) that see
+ * token t of exp(sm_scale * q.k_t - lse[row]): the last q_len tokens of a sequence (new
+ * in this step) get scores = w, the earlier ones scores += w; slots behind the sequence
+ * are left.  args: query, key_cache (16-bit of args->dtype, or e4m3 with `scales`, of
+ * which only `key` is read), block_tables, seq_lens, mask_lens and sm_scale as for
+ * sqa_forward; value_cache and the outputs are not used.  lse: fp32 [batch, q_len,
+ * num_q_heads], the natural-log log-sum-exp that the step's attention returned (a
+ * row of -inf counts nothing).  The SQA_DEV_* bits are ORed into *status (may be NULL).
+ * Pages must not be shared between sequences.  Asynchronous on `stream`. */
+SQA_API int sqa_accumulate_weights(const sqa_args* args, const float* lse, const sqa_scales* scales, float* scores,
+                                   uint32_t* status, void* stream);
+
+/* Per sequence and KV head with n = seq_lens[b] > budget, keep the first `sinks` tokens,
+ * the last `recent`, and of the others the budget - sinks - recent of the highest score
+ * (NaN counts as the lowest, equal scores: the earlier token first).  Kept tokens move,
+ * in order, to positions 0 .. budget - 1 of the sequence's own pages: K, V and scores.
+ * A block-scaled cache (`scales`, with kv_dtype = SQA_KV_FP8_E4M3) gets, for every page
+ * written, the smallest power-of-two scale for the values it now holds.
+ * new_lens[b] = min(n, budget) and kept[b, h, i] = the position that target i came from
+ * (-1 behind the last).  A sequence of at most `budget` tokens is left, and so is one
+ * with a negative length, more pages than max_pages, or a page id outside the
+ * cache (SQA_DEV_SEQ_TOO_SHORT / SEQ_TOO_LONG / BAD_PAGE, new_lens = n, kept = -1).
+ * Pages must not be shared between sequences or listed twice. */
+typedef struct sqa_evict_args {
+  void* key_cache;             /* as in sqa_args */
+  void* value_cache;
+  float* scores;               /* [num_pages, num_kv_heads, 16] */
+  const int32_t* block_tables; /* [batch, max_pages] */
+  const int32_t* seq_lens;     /* [batch] */
+  int32_t* new_lens;           /* [batch]; not seq_lens itself */
+  int32_t* kept;               /* [batch, num_kv_heads, budget] */
+  uint32_t* status;            /* device status word or NULL */
+  int32_t batch;
+  int32_t num_kv_heads;
+  int32_t head_dim;            /* must be 128 */
+  int32_t page_size;           /* must be 16  */
+  int32_t num_pages;
+  int32_t max_pages;
+  int32_t kv_layout;           /* SQA_KV_NHD or SQA_KV_HND */
+  int32_t kv_dtype;            /* SQA_KV_SAME (2-byte elements) or SQA_KV_FP8_E4M3 with scales */
+  int32_t budget;              /* tokens to keep, >= 1 and >= sinks + recent */
+  int32_t recent;
+  int32_t sinks;
+  int64_t page_stride;         /* elements from page to page, 0 = contiguous (as in sqa_args) */
+} sqa_evict_args;
+
+SQA_API int sqa_cache_evict(const sqa_evict_args* args, const sqa_scales* scales, void* stream);
+
 /* ---- Long-context split across the GPUs of one node ----
  * One sequence's pages are cut into contiguous ranges, one per rank (one
  * process per GPU); every rank computes the shard form of the operator over

@@ -10,3 +10,11 @@ from .paged_mtp_attention import (  # noqa: F401
     paged_mtp_attention_partial,
     paged_mtp_attention_reference,
 )
+from .scaled_cache import (  # noqa: F401
+    append_scaled_reference,
+    attention_scaled_reference,
+    evict_reference,
+    page_scale,
+    round_e4m3,
+    weights_reference,
+)

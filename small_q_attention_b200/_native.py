@@ -55,6 +55,11 @@ EXPORTED_SYMBOLS = (
     "sqa_abi_version",
     "sqa_selected_kernel",
     "sqa_cache_append",
+    "sqa_cache_append_scaled",
+    "sqa_scaled_workspace_bytes",
+    "sqa_forward_scaled",
+    "sqa_accumulate_weights",
+    "sqa_cache_evict",
     "sqa_lc_handle_bytes",
     "sqa_lc_create",
     "sqa_lc_connect",
@@ -125,6 +130,43 @@ class SqaArgs(ctypes.Structure):
     ]
 
 
+class SqaScales(ctypes.Structure):
+    """Mirror of ``struct sqa_scales``."""
+
+    _fields_ = [
+        ("key", ctypes.c_void_p),
+        ("value", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+    ]
+
+
+class SqaEvictArgs(ctypes.Structure):
+    """Mirror of ``struct sqa_evict_args``."""
+
+    _fields_ = [
+        ("key_cache", ctypes.c_void_p),
+        ("value_cache", ctypes.c_void_p),
+        ("scores", ctypes.c_void_p),
+        ("block_tables", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("new_lens", ctypes.c_void_p),
+        ("kept", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("batch", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("kv_layout", ctypes.c_int32),
+        ("kv_dtype", ctypes.c_int32),
+        ("budget", ctypes.c_int32),
+        ("recent", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+        ("page_stride", ctypes.c_int64),
+    ]
+
+
 _lib = None
 # Reentrant: torch_ext() holds it while it loads the C library through library().
 _lock = threading.RLock()
@@ -169,6 +211,16 @@ def library(path: Path | None = None):
         lib.sqa_selected_kernel.restype = ctypes.c_int
         lib.sqa_cache_append.argtypes = [ctypes.POINTER(SqaAppendArgs), vp]
         lib.sqa_cache_append.restype = ctypes.c_int
+        lib.sqa_cache_append_scaled.argtypes = [ctypes.POINTER(SqaAppendArgs), ctypes.POINTER(SqaScales), i32, vp]
+        lib.sqa_cache_append_scaled.restype = ctypes.c_int
+        lib.sqa_scaled_workspace_bytes.argtypes = [ctypes.POINTER(SqaArgs), ctypes.c_int, ctypes.POINTER(ctypes.c_int)]
+        lib.sqa_scaled_workspace_bytes.restype = sz
+        lib.sqa_forward_scaled.argtypes = [ctypes.POINTER(SqaArgs), ctypes.POINTER(SqaScales), vp, sz, vp]
+        lib.sqa_forward_scaled.restype = ctypes.c_int
+        lib.sqa_accumulate_weights.argtypes = [ctypes.POINTER(SqaArgs), vp, ctypes.POINTER(SqaScales), vp, vp, vp]
+        lib.sqa_accumulate_weights.restype = ctypes.c_int
+        lib.sqa_cache_evict.argtypes = [ctypes.POINTER(SqaEvictArgs), ctypes.POINTER(SqaScales), vp]
+        lib.sqa_cache_evict.restype = ctypes.c_int
         lib.sqa_lc_handle_bytes.argtypes = []
         lib.sqa_lc_handle_bytes.restype = sz
         lib.sqa_lc_create.argtypes = [i32, i32, i64, ctypes.POINTER(vp), vp]

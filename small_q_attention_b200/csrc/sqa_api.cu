@@ -535,6 +535,102 @@ int sqa_forward_timed(const sqa_args* a, void* workspace, size_t workspace_bytes
   return forward_impl(a, workspace, workspace_bytes, stream, event_before, event_after);
 }
 
+namespace {
+// The checks of a block-scaled call beyond validate() and its pointers.
+int validate_scales(const sqa_args* a, const sqa_scales* s) {
+  if (!s || a->kv_dtype != SQA_KV_FP8_E4M3) return SQA_ERR_INVALID_ARGUMENT;
+  if (s->page_stride < 0 || (s->page_stride > 0 && s->page_stride < a->num_kv_heads)) return SQA_ERR_INVALID_ARGUMENT;
+  return SQA_OK;
+}
+
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+ScaledParams scaled_params(const sqa_args* a, const sqa_scales* s) {
+  ScaledParams p = {};
+  p.q = a->query;
+  p.k_cache = a->key_cache;
+  p.v_cache = a->value_cache;
+  p.k_scales = s ? s->key : nullptr;
+  p.v_scales = s ? s->value : nullptr;
+  p.block_tables = a->block_tables;
+  p.seq_lens = a->seq_lens;
+  p.mask_lens = a->mask_lens;
+  p.page_stride = a->page_stride > 0 ? a->page_stride : (int64_t)kPageSize * a->num_kv_heads * kHeadDim;
+  p.scale_stride = s && s->page_stride > 0 ? s->page_stride : a->num_kv_heads;
+  p.batch = a->batch;
+  p.q_len = a->q_len;
+  p.hq = a->num_q_heads;
+  p.hkv = a->num_kv_heads;
+  p.max_pages = a->max_pages;
+  p.num_pages = a->num_pages;
+  p.hnd = a->kv_layout == SQA_KV_HND;
+  p.bf16 = a->dtype == SQA_DTYPE_BF16;
+  p.scale_log2 = 1.4426950408889634f * (a->sm_scale > 0.f ? a->sm_scale : 1.f / sqrtf((float)kHeadDim));
+  p.out_scale = a->out_scale != 0.f ? a->out_scale : 1.f;
+  return p;
+}
+}  // namespace
+
+size_t sqa_scaled_workspace_bytes(const sqa_args* a, int device, int* status) {
+  (void)device;
+  int st = validate(a);
+  if (st == SQA_OK && a->kv_dtype != SQA_KV_FP8_E4M3) st = SQA_ERR_INVALID_ARGUMENT;
+  if (st == SQA_OK && (a->kernel != 0 || a->cluster > 1)) st = SQA_ERR_UNSUPPORTED;
+  if (status) *status = st;
+  return st == SQA_OK ? kAlign : 0;
+}
+
+int sqa_forward_scaled(const sqa_args* a, const sqa_scales* scales, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  int st = SQA_OK;
+  const size_t need = sqa_scaled_workspace_bytes(a, -1, &st);
+  if (st != SQA_OK) return st;
+  st = validate_scales(a, scales);
+  if (st != SQA_OK) return st;
+  if (a->batch == 0) return SQA_OK;
+  if (!a->query || !a->key_cache || !a->value_cache || !a->block_tables || !a->seq_lens || !scales->key || !scales->value)
+    return SQA_ERR_INVALID_ARGUMENT;
+  // 16-bit rows with or without the log-sum-exp, or fp32 rows with it
+  if ((a->out != nullptr) == (a->out_partial != nullptr) || (a->out_partial && !a->out_lse))
+    return SQA_ERR_INVALID_ARGUMENT;
+  if (!aligned16(a->query) || !aligned16(a->key_cache) || !aligned16(a->value_cache) || !aligned16(a->out) ||
+      !aligned16(a->out_partial))
+    return SQA_ERR_INVALID_ARGUMENT;
+  if (!aligned4(a->block_tables) || !aligned4(a->seq_lens) || !aligned4(a->mask_lens) || !aligned4(a->out_lse) ||
+      !aligned4(scales->key) || !aligned4(scales->value))
+    return SQA_ERR_INVALID_ARGUMENT;
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & (kAlign - 1))) return SQA_ERR_INVALID_ARGUMENT;
+  if (workspace_bytes < need) return SQA_ERR_WORKSPACE_TOO_SMALL;
+  ScaledParams p = scaled_params(a, scales);
+  p.out = a->out;
+  p.out_o = a->out_partial;
+  p.out_lse = a->out_lse;
+  p.status = static_cast<unsigned int*>(workspace);
+  return launch_scaled_attention(p, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? SQA_OK : SQA_ERR_CUDA;
+}
+
+int sqa_accumulate_weights(const sqa_args* a, const float* lse, const sqa_scales* scales, float* scores,
+                           uint32_t* status, void* stream) {
+  int st = validate(a);
+  if (st != SQA_OK) return st;
+  if (a->kernel != 0 || a->cluster > 1) return SQA_ERR_UNSUPPORTED;
+  if (a->kv_dtype == SQA_KV_FP8_E4M3) st = validate_scales(a, scales);  // e4m3 caches carry their scales
+  else if (scales) st = SQA_ERR_INVALID_ARGUMENT;
+  if (st != SQA_OK) return st;
+  if (a->batch == 0) return SQA_OK;
+  if (!a->query || !a->key_cache || !a->block_tables || !a->seq_lens || !lse || !scores || (scales && !scales->key))
+    return SQA_ERR_INVALID_ARGUMENT;
+  if (!aligned16(a->query) || !aligned16(a->key_cache)) return SQA_ERR_INVALID_ARGUMENT;
+  if (!aligned4(a->block_tables) || !aligned4(a->seq_lens) || !aligned4(a->mask_lens) || !aligned4(lse) ||
+      !aligned4(scores) || !aligned4(status) || (scales && !aligned4(scales->key)))
+    return SQA_ERR_INVALID_ARGUMENT;
+  ScaledParams p = scaled_params(a, scales);
+  p.lse = lse;
+  p.scores = scores;
+  p.status = status;
+  return launch_weights(p, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? SQA_OK : SQA_ERR_CUDA;
+}
+
 int sqa_merge_partials(const float* parts_o, const float* parts_lse, int32_t num_parts, int64_t rows,
                        void* out, float* out_o, float* out_lse, void* stream) {
   if (!parts_o || !parts_lse || num_parts <= 0 || rows < 0) return SQA_ERR_INVALID_ARGUMENT;

@@ -1,0 +1,452 @@
+// sqa_evict.cu -- eviction from the paged cache by accumulated attention weight.
+//
+// Per (sequence b, KV head h) with n = seq_lens[b] > budget, the kept tokens are the
+// first `sinks`, the last `recent` and, of the others, the budget - sinks - recent
+// with the highest score (NaN counts as the lowest; equal scores: the earlier token).
+// They move, in order of position, to positions 0 .. budget - 1 of the same pages:
+// K, V and score.  Every page of a block-scaled cache that is written gets the scale
+// of the values that it now holds.  Sequences of at most `budget` tokens are left.
+//
+// A thread-block cluster of C CTAs works on one (b, h):
+//
+// 1. Selection.  Each CTA holds a slice of the scores as order-preserving 32-bit keys.
+//    A radix search over the range [lo, hi] that still holds the wanted rank: 256 equal
+//    bins, histograms summed over the cluster through distributed shared memory, one
+//    cluster barrier a pass, until the range is one key or a bin edge cuts off exactly
+//    the wanted count (three or four passes).  The range is taken from the scores
+//    themselves, so that the bins are used evenly (scores share their leading bits; a
+//    fixed digit would send them all to one bin and serialise its counter).
+// 2. Ranks.  A kept token's target is a sum of counts of earlier slices (shared through
+//    the cluster) and of a block scan; kept[] lists the kept positions.
+// 3. Moves, in place and in waves of C x 8 target pages: a warp loads the 16 source rows
+//    of its target page (K, V, scores, source scales) into registers, the cluster meets
+//    at a barrier, then every warp writes its page.  A source is never before its
+//    target, and the sources of later waves lie in pages behind this wave's targets, so
+//    nothing is overwritten before it is read.  A warp has a page's K and V (8 KB for
+//    16-bit elements) in flight at once.
+#include "small_q_attention.h"
+#include "sqa_internal.h"
+#include "sqa_ptx.cuh"
+#include "sqa_scaled.cuh"
+
+namespace sqa {
+namespace {
+
+constexpr int kEvictThreads = 256;
+constexpr int kEvictWarps = kEvictThreads / 32;
+constexpr int kEvictMaxCluster = 8;
+constexpr int kKeyCap = 12288;  // keys of a slice held in shared memory (48 KB); further ones are read again
+
+struct EvictParams {
+  uint8_t* k_cache;
+  uint8_t* v_cache;
+  float* k_scales;
+  float* v_scales;
+  float* scores;  // [num_pages, hkv, 16]
+  const int32_t* block_tables;
+  const int32_t* seq_lens;
+  int32_t* new_lens;
+  int32_t* kept;  // [batch, hkv, budget]
+  unsigned int* status;
+  long long page_stride;   // bytes
+  long long scale_stride;  // floats
+  int hkv, num_pages, max_pages, hnd;
+  int budget, recent, sinks;
+  int cluster, key_cap;
+};
+
+struct EvictShared {
+  unsigned int hist[2][256];
+  unsigned int exchange[2];  // read by the other CTAs of the cluster
+  unsigned int counts[2];    // this slice's (above, equal), read by the others
+  unsigned int warp_a[kEvictWarps], warp_b[kEvictWarps];
+  unsigned int pick[2];
+};
+
+__device__ __forceinline__ unsigned int ld_cluster_u32(const void* p, int rank) {
+  unsigned int v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_map(smem_u32(p), (uint32_t)rank)) : "memory");
+  return v;
+}
+
+// Order-preserving key of a score; NaN lowest, the two zeros equal.
+__device__ __forceinline__ unsigned int score_key(float f) {
+  if (f != f) return 0u;
+  const unsigned int u = __float_as_uint(f == 0.f ? 0.f : f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+template <int E>  // bytes per cached element: 2 (16-bit) or 1 (block-scaled e4m3)
+__global__ void __launch_bounds__(kEvictThreads, 2) sqa_cache_evict_kernel(const EvictParams p) {
+  extern __shared__ unsigned int keys[];  // key_cap
+  __shared__ EvictShared sh;
+  grid_dependency_wait();
+  allow_dependent_launch();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int C = p.cluster;
+  const int rank = (int)blockIdx.x % C;
+  const int seg = (int)blockIdx.x / C;
+  const int b = seg / p.hkv, h = seg - b * p.hkv;
+  const int len = __ldg(p.seq_lens + b);
+  const int32_t* table = p.block_tables + (size_t)b * p.max_pages;
+  int32_t* const kept = p.kept + (size_t)seg * p.budget;
+
+  // Sequences that stay as they are: short ones, and those whose length or pages are bad.
+  unsigned int err = 0;
+  const int pages = (max(len, 0) + kPageSize - 1) / kPageSize;
+  if (len < 0) err = 4u;                 // SQA_DEV_SEQ_TOO_SHORT
+  else if (pages > p.max_pages) err = 2u;  // SQA_DEV_SEQ_TOO_LONG
+  else if (len > p.budget) {
+    int bad = 0;
+    for (int i = tid; i < pages; i += kEvictThreads) {
+      const int id = __ldg(table + i);
+      bad |= id < 0 || id >= p.num_pages;
+    }
+    if (__syncthreads_or(bad)) err = 8u;  // SQA_DEV_BAD_PAGE
+  }
+  if (err || len <= p.budget) {  // the same for every CTA of the cluster
+    for (int i = rank * kEvictThreads + tid; i < p.budget; i += C * kEvictThreads)
+      kept[i] = (!err && i < len) ? i : -1;
+    if (h == 0 && rank == 0 && tid == 0) {
+      p.new_lens[b] = len;
+      if (err && p.status) atomicOr(p.status, err);
+    }
+    return;
+  }
+  if (h == 0 && rank == 0 && tid == 0) p.new_lens[b] = p.budget;
+
+  // ---- 1. the key of the last score that is kept
+  const int middle = len - p.sinks - p.recent;  // candidates
+  const int want = p.budget - p.sinks - p.recent;
+  const int per = (middle + C - 1) / C;
+  const int a0 = p.sinks + min(middle, rank * per);
+  const int count = p.sinks + min(middle, (rank + 1) * per) - a0;
+  auto read_key = [&](int i) {
+    const int t = a0 + i;
+    return score_key(__ldcg(p.scores + ((size_t)__ldg(table + t / kPageSize) * p.hkv + h) * kPageSize + t % kPageSize));
+  };
+  auto key_at = [&](int i) { return i < p.key_cap ? keys[i] : read_key(i); };
+  unsigned int lo = 0xffffffffu, hi = 0u;
+  for (int i = tid; i < count; i += kEvictThreads) {
+    const unsigned int k = read_key(i);
+    if (i < p.key_cap) keys[i] = k;
+    lo = min(lo, k);
+    hi = max(hi, k);
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if (lane == 0) {
+    sh.warp_a[warp] = lo;
+    sh.warp_b[warp] = hi;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < kEvictWarps; ++w) {
+      lo = min(lo, sh.warp_a[w]);
+      hi = max(hi, sh.warp_b[w]);
+    }
+    sh.exchange[0] = lo;
+    sh.exchange[1] = hi;
+  }
+  cluster_sync_all();
+  lo = 0xffffffffu;
+  hi = 0u;
+  for (int r = 0; r < C; ++r) {
+    lo = min(lo, ld_cluster_u32(&sh.exchange[0], r));
+    hi = max(hi, ld_cluster_u32(&sh.exchange[1], r));
+  }
+  // Kept: every key > above, and of the keys == lo the first `need` (none once `exact`).
+  // Invariant: the keys above hi number want - need, those in [lo, hi] at least need.
+  int need = want;
+  bool exact = want == 0;      // nothing from [lo, hi] is needed
+  unsigned int above = hi;     // keys > above are kept whatever else
+  for (int pass = 0; !exact && lo < hi; ++pass) {
+    unsigned int* const hist = sh.hist[pass & 1];
+    const int shift = max(0, 24 - __clz(hi - lo));  // (hi - lo) >> shift < 256
+    hist[tid] = 0u;
+    __syncthreads();
+    for (int i = tid; i < count; i += kEvictThreads) {
+      const unsigned int k = key_at(i);
+      if (k >= lo && k <= hi) atomicAdd(&hist[(k - lo) >> shift], 1u);
+    }
+    cluster_sync_all();  // also: every CTA is done with the other histogram
+    // thread t: bin 255 - t, so that an inclusive scan counts from the top
+    const int bin = 255 - tid;
+    unsigned int n = 0;
+    for (int r = 0; r < C; ++r) n += ld_cluster_u32(&hist[bin], r);
+    unsigned int incl = n;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const unsigned int y = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += y;
+    }
+    if (lane == 31) sh.warp_a[warp] = incl;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) incl += sh.warp_a[w];
+    if (incl >= (unsigned int)need && incl - n < (unsigned int)need) {  // exactly one thread
+      sh.pick[0] = (unsigned int)bin;
+      sh.pick[1] = incl;
+    }
+    __syncthreads();
+    const unsigned int j = sh.pick[0], upto = sh.pick[1];  // keys of bins >= j in the range
+    const unsigned int in_bin = ld_cluster_u32(&hist[j], 0);
+    unsigned int total = in_bin;
+    for (int r = 1; r < C; ++r) total += ld_cluster_u32(&hist[j], r);
+    const unsigned int edge = lo + (j << shift);
+    hi = edge + min(hi - edge, (1u << shift) - 1u);
+    lo = edge;
+    above = hi;
+    if (upto == (unsigned int)need && lo > 0u) {  // the whole bin is kept: its lower edge is the limit
+      above = lo - 1u;
+      exact = true;
+    } else {
+      need -= (int)(upto - total);
+    }
+  }
+  if (exact) need = 0;
+  const unsigned int last = exact ? above : lo;  // kept: key > last, and the first `need` with key == last
+
+  // ---- 2. ranks: (above, equal) counts of this slice and of the ones before it
+  unsigned int gt = 0, eq = 0;
+  for (int i = tid; i < count; i += kEvictThreads) {
+    const unsigned int k = key_at(i);
+    gt += k > last;
+    eq += k == last;
+  }
+  gt = __reduce_add_sync(0xffffffffu, gt);
+  eq = __reduce_add_sync(0xffffffffu, eq);
+  __syncthreads();  // warp_a is free
+  if (lane == 0) {
+    sh.warp_a[warp] = gt;
+    sh.warp_b[warp] = eq;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < kEvictWarps; ++w) {
+      gt += sh.warp_a[w];
+      eq += sh.warp_b[w];
+    }
+    sh.counts[0] = gt;
+    sh.counts[1] = eq;
+  }
+  cluster_sync_all();
+  unsigned int gt_before = 0, eq_before = 0;
+  for (int r = 0; r < rank; ++r) {
+    gt_before += ld_cluster_u32(&sh.counts[0], r);
+    eq_before += ld_cluster_u32(&sh.counts[1], r);
+  }
+  for (int base = 0; base < count; base += kEvictThreads) {
+    const int i = base + tid;
+    const unsigned int k = i < count ? key_at(i) : 0u;
+    const bool is_gt = i < count && k > last, is_eq = i < count && k == last;
+    const unsigned int m_gt = __ballot_sync(0xffffffffu, is_gt), m_eq = __ballot_sync(0xffffffffu, is_eq);
+    __syncthreads();  // the last tile's counts have been read
+    if (lane == 0) {
+      sh.warp_a[warp] = __popc(m_gt);
+      sh.warp_b[warp] = __popc(m_eq);
+    }
+    __syncthreads();
+    unsigned int g = gt_before, e = eq_before;
+    for (int w = 0; w < kEvictWarps; ++w) {
+      const unsigned int wg = sh.warp_a[w], we = sh.warp_b[w];
+      if (w < warp) {
+        g += wg;
+        e += we;
+      }
+      gt_before += wg;
+      eq_before += we;
+    }
+    const unsigned int under = (1u << lane) - 1u;
+    g += __popc(m_gt & under);
+    e += __popc(m_eq & under);
+    if (is_gt || (is_eq && e < (unsigned int)need)) kept[p.sinks + g + min(e, (unsigned int)need)] = a0 + i;
+  }
+  for (int i = rank * kEvictThreads + tid; i < p.sinks; i += C * kEvictThreads) kept[i] = i;
+  for (int i = rank * kEvictThreads + tid; i < p.recent; i += C * kEvictThreads)
+    kept[p.budget - p.recent + i] = len - p.recent + i;
+  cluster_sync_all();  // kept[] is complete, for every CTA of the cluster
+
+  // ---- 3. moves, C x 8 target pages a wave
+  constexpr int kLanesPerRow = kHeadDim * E / 16;     // 16 (16-bit) or 8 (e4m3) lanes hold a row
+  constexpr int kRowsPerLoad = 32 / kLanesPerRow;     // rows a warp loads at once
+  constexpr int kLoads = kPageSize / kRowsPerLoad;
+  const int sub = lane / kLanesPerRow;
+  const size_t head = p.hnd ? (size_t)h * kPageSize * kHeadDim * E : (size_t)h * kHeadDim * E;
+  const size_t row = p.hnd ? (size_t)kHeadDim * E : (size_t)p.hkv * kHeadDim * E;  // bytes from slot to slot
+  const size_t in_row = head + (lane % kLanesPerRow) * 16;
+  const int targets = (p.budget + kPageSize - 1) / kPageSize;
+  for (int base = 0; base < targets; base += C * kEvictWarps) {
+    const int target = base + rank * kEvictWarps + warp;
+    const int rows = target < targets ? min(kPageSize, p.budget - target * kPageSize) : 0;
+    uint4 k[kLoads], v[kLoads];
+    float score = 0.f, ks = 0.f, vs = 0.f;
+    int to = 0;
+    if (rows > 0) {
+      to = __ldg(table + target);
+      int from = 0, slot = 0;
+      if (lane < rows) {
+        const int t = __ldcg(kept + target * kPageSize + lane);
+        from = __ldg(table + t / kPageSize);
+        slot = t % kPageSize;
+        score = __ldcg(p.scores + ((size_t)from * p.hkv + h) * kPageSize + slot);
+        if constexpr (E == 1) {
+          ks = __ldcg(p.k_scales + (size_t)from * p.scale_stride + h);
+          vs = __ldcg(p.v_scales + (size_t)from * p.scale_stride + h);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int r = i * kRowsPerLoad + sub;
+        const int rf = __shfl_sync(0xffffffffu, from, r), rs = __shfl_sync(0xffffffffu, slot, r);
+        const size_t at = (size_t)rf * p.page_stride + rs * row + in_row;
+        k[i] = v[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < rows) {
+          k[i] = __ldcg(reinterpret_cast<const uint4*>(p.k_cache + at));
+          v[i] = __ldcg(reinterpret_cast<const uint4*>(p.v_cache + at));
+        }
+      }
+    }
+    cluster_sync_all();  // every source of this wave has been read
+    if (rows > 0) {
+      if constexpr (E == 1) {
+        // values at their source page's scale, then the target page's scale from what it now holds
+        auto rescale = [&](uint4(&x)[kLoads], float source) {
+          float amax = 0.f, s[kLoads];
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i) {
+            s[i] = __shfl_sync(0xffffffffu, source, i * kRowsPerLoad + sub);
+            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float2 a = unpack_e4m3x2(w[c]), d = unpack_e4m3x2(w[c] >> 16);
+              amax = fmaxf(amax, fmaxf(fmaxf(finite_abs(a.x * s[i]), finite_abs(a.y * s[i])),
+                                       fmaxf(finite_abs(d.x * s[i]), finite_abs(d.y * s[i]))));
+            }
+          }
+          const float scale = page_scale(warp_max(amax));
+          const float inv = 1.f / scale;  // a power of two: multiplying by it is dividing by scale
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i) {
+            uint32_t* const w = reinterpret_cast<uint32_t*>(&x[i]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float2 a = unpack_e4m3x2(w[c]), d = unpack_e4m3x2(w[c] >> 16);
+              w[c] = pack_e4m3x4(a.x * s[i] * inv, a.y * s[i] * inv, d.x * s[i] * inv, d.y * s[i] * inv);
+            }
+          }
+          return scale;
+        };
+        const float new_ks = rescale(k, ks), new_vs = rescale(v, vs);
+        if (lane == 0) {
+          p.k_scales[(size_t)to * p.scale_stride + h] = new_ks;
+          p.v_scales[(size_t)to * p.scale_stride + h] = new_vs;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int r = i * kRowsPerLoad + sub;
+        if (r < rows) {
+          const size_t at = (size_t)to * p.page_stride + r * row + in_row;
+          *reinterpret_cast<uint4*>(p.k_cache + at) = k[i];
+          *reinterpret_cast<uint4*>(p.v_cache + at) = v[i];
+        }
+      }
+      if (lane < rows) p.scores[((size_t)to * p.hkv + h) * kPageSize + lane] = score;
+    }
+  }
+}
+
+template <int E>
+cudaError_t launch_evict(const EvictParams& p, int segments, cudaStream_t stream) {
+  auto kernel = sqa_cache_evict_kernel<E>;
+  const int smem = p.key_cap * (int)sizeof(unsigned int);
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         kKeyCap * (int)sizeof(unsigned int));
+  if (err != cudaSuccess) return err;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(segments * p.cluster));
+  cfg.blockDim = dim3(kEvictThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  err = cudaLaunchKernelEx(&cfg, kernel, p);
+  return err != cudaSuccess ? err : cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace sqa
+
+using namespace sqa;
+
+extern "C" SQA_API int sqa_cache_evict(const sqa_evict_args* a, const sqa_scales* scales, void* stream) {
+  if (a == nullptr) return SQA_ERR_INVALID_ARGUMENT;
+  if (a->head_dim != kHeadDim || a->page_size != kPageSize) return SQA_ERR_UNSUPPORTED;
+  if (a->batch < 0 || a->num_kv_heads <= 0 || a->num_pages <= 0 || a->max_pages <= 0) return SQA_ERR_INVALID_ARGUMENT;
+  if (a->kv_layout != SQA_KV_NHD && a->kv_layout != SQA_KV_HND) return SQA_ERR_UNSUPPORTED;
+  if (a->kv_dtype != SQA_KV_SAME && a->kv_dtype != SQA_KV_FP8_E4M3) return SQA_ERR_UNSUPPORTED;
+  const bool fp8 = a->kv_dtype == SQA_KV_FP8_E4M3;
+  if (fp8 != (scales != nullptr)) return SQA_ERR_INVALID_ARGUMENT;  // e4m3 caches carry their scales
+  if (a->budget < 1 || a->recent < 0 || a->sinks < 0 || (int64_t)a->recent + a->sinks > a->budget)
+    return SQA_ERR_INVALID_ARGUMENT;
+  if (a->page_stride < 0 || (a->page_stride > 0 && (a->page_stride < (int64_t)kPageSize * a->num_kv_heads * kHeadDim ||
+                                                    a->page_stride % (fp8 ? 16 : 8) != 0)))
+    return SQA_ERR_INVALID_ARGUMENT;
+  if (scales && (scales->page_stride < 0 || (scales->page_stride > 0 && scales->page_stride < a->num_kv_heads)))
+    return SQA_ERR_INVALID_ARGUMENT;
+  // positions and grid sizes are 32-bit
+  if (a->max_pages > (1 << 26) || a->budget > (1 << 30) || (int64_t)a->batch * a->num_kv_heads > (1 << 27))
+    return SQA_ERR_UNSUPPORTED;
+  if (a->batch == 0) return SQA_OK;
+  if (!a->key_cache || !a->value_cache || !a->scores || !a->block_tables || !a->seq_lens || !a->new_lens || !a->kept ||
+      a->new_lens == a->seq_lens || (scales && (!scales->key || !scales->value)))
+    return SQA_ERR_INVALID_ARGUMENT;
+  const uintptr_t wide = reinterpret_cast<uintptr_t>(a->key_cache) | reinterpret_cast<uintptr_t>(a->value_cache);
+  uintptr_t narrow = reinterpret_cast<uintptr_t>(a->scores) | reinterpret_cast<uintptr_t>(a->block_tables) |
+                     reinterpret_cast<uintptr_t>(a->seq_lens) | reinterpret_cast<uintptr_t>(a->new_lens) |
+                     reinterpret_cast<uintptr_t>(a->kept) | reinterpret_cast<uintptr_t>(a->status);
+  if (scales) narrow |= reinterpret_cast<uintptr_t>(scales->key) | reinterpret_cast<uintptr_t>(scales->value);
+  if ((wide & 15u) || (narrow & 3u)) return SQA_ERR_INVALID_ARGUMENT;
+
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return SQA_ERR_CUDA;
+  EvictParams p = {};
+  const int elem = fp8 ? 1 : 2;
+  p.k_cache = static_cast<uint8_t*>(a->key_cache);
+  p.v_cache = static_cast<uint8_t*>(a->value_cache);
+  p.k_scales = scales ? scales->key : nullptr;
+  p.v_scales = scales ? scales->value : nullptr;
+  p.scores = a->scores;
+  p.block_tables = a->block_tables;
+  p.seq_lens = a->seq_lens;
+  p.new_lens = a->new_lens;
+  p.kept = a->kept;
+  p.status = a->status;
+  p.page_stride = (a->page_stride > 0 ? a->page_stride : (int64_t)kPageSize * a->num_kv_heads * kHeadDim) * elem;
+  p.scale_stride = scales && scales->page_stride > 0 ? scales->page_stride : a->num_kv_heads;
+  p.hkv = a->num_kv_heads;
+  p.num_pages = a->num_pages;
+  p.max_pages = a->max_pages;
+  p.hnd = a->kv_layout == SQA_KV_HND;
+  p.budget = a->budget;
+  p.recent = a->recent;
+  p.sinks = a->sinks;
+  // The largest cluster that leaves no more than two waves of the card's 2 CTAs per SM:
+  // few segments need many CTAs each to fill the card, many fill it by themselves.
+  const int segments = a->batch * a->num_kv_heads;
+  p.cluster = kEvictMaxCluster;
+  while (p.cluster > 1 && (int64_t)segments * p.cluster > 4LL * sms) p.cluster /= 2;
+  const int64_t slice = ((int64_t)a->max_pages * kPageSize + p.cluster - 1) / p.cluster;
+  p.key_cap = slice < kKeyCap ? (int)slice : kKeyCap;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return (fp8 ? launch_evict<1>(p, segments, s) : launch_evict<2>(p, segments, s)) == cudaSuccess ? SQA_OK : SQA_ERR_CUDA;
+}

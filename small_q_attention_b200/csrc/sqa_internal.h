@@ -83,6 +83,32 @@ struct MergeParams {
                                 // evenly over k CTAs (SplitKvParams::seg_split)
 };
 
+// Attention over a block-scaled e4m3 cache, and the weights of its (or a 16-bit cache's) tokens.
+struct ScaledParams {
+  const void* q;                // [B, q_len, Hq, 128] fp16 or bf16
+  const void* k_cache;          // e4m3 (16-bit too for the weights)
+  const void* v_cache;
+  const float* k_scales;        // [num_pages, hkv], scale_stride floats from page to page (nullptr: 16-bit cache)
+  const float* v_scales;
+  const int32_t* block_tables;  // [B, max_pages]
+  const int32_t* seq_lens;      // [B]
+  const int32_t* mask_lens;     // [B] or nullptr
+  const float* lse;             // weights: [B, q_len, Hq]
+  float* scores;                // weights: [num_pages, hkv, 16]
+  void* out;                    // attention: 16-bit rows, or nullptr
+  float* out_o;                 // attention: fp32 rows, or nullptr
+  float* out_lse;               // attention: or nullptr
+  unsigned int* status;
+  long long page_stride;        // elements
+  long long scale_stride;       // floats
+  int batch, q_len, hq, hkv, max_pages, num_pages;
+  int hnd, bf16;
+  float scale_log2, out_scale;
+};
+
+cudaError_t launch_scaled_attention(const ScaledParams& p, cudaStream_t stream);
+cudaError_t launch_weights(const ScaledParams& p, cudaStream_t stream);
+
 // Launchers (stream-ordered, no allocation).  Return cudaGetLastError().
 cudaError_t launch_split_kv(const SplitKvParams& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                             int grid, int smem_bytes, cudaStream_t stream);

@@ -241,6 +241,276 @@ std::tuple<at::Tensor, at::Tensor> forward_partial(
   return {o, l};
 }
 
+// ---- the block-scaled e4m3 cache and eviction by attention weight
+
+// Scales [num_pages, Hkv] fp32, K and V alike; rows may be further apart than Hkv.
+sqa_scales fill_scales(const at::Tensor& k, const at::Tensor& v, const at::Tensor& cache, int64_t hkv) {
+  for (const at::Tensor* t : {&k, &v}) {
+    TORCH_CHECK_VALUE(t->defined() && t->device() == cache.device(), "all inputs must be CUDA tensors on the same device");
+    TORCH_CHECK_VALUE(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == cache.size(0) && t->size(1) == hkv,
+                      "key_scales / value_scales must be fp32 [num_pages, Hkv]");
+    TORCH_CHECK_VALUE((hkv == 1 || t->stride(1) == 1) && (t->size(0) == 1 || t->stride(0) >= hkv) &&
+                          (t->size(0) == 1 || t->stride(0) == k.stride(0)),
+                      "key_scales / value_scales must be packed over the heads, with one page stride shared by both");
+  }
+  return sqa_scales{k.data_ptr<float>(), v.data_ptr<float>(), k.size(0) == 1 ? hkv : k.stride(0)};
+}
+
+// Memory of a call whose first word is its status word.  Eagerly one tensor per
+// (device, stream, use), grown on demand and zeroed once.  Under stream capture a
+// fresh one from the capture's own pool, its status word zeroed by the graph: two
+// captured graphs never share it, whatever streams they are replayed on.
+enum Use { kUseAttention, kUseAppend, kUseWeights, kUseEvict };
+struct UseEntry {
+  int device;
+  cudaStream_t stream;
+  Use use;
+  at::Tensor ws;
+};
+std::mutex g_use_mu;
+std::vector<UseEntry> g_use;
+
+at::Tensor memory_for(Use use, size_t need, const at::Device& dev, cudaStream_t stream) {
+  const auto bytes = at::TensorOptions().dtype(at::kByte).device(dev);
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  TORCH_CHECK(cudaStreamIsCapturing(stream, &cs) == cudaSuccess, "cudaStreamIsCapturing failed");
+  if (cs != cudaStreamCaptureStatusNone) {
+    at::Tensor ws = at::empty({(int64_t)need}, bytes);
+    check_status(sqa_workspace_init(ws.data_ptr(), std::min<size_t>(need, 256), stream), "sqa_workspace_init");
+    return ws;
+  }
+  std::lock_guard<std::mutex> lock(g_use_mu);
+  for (auto& e : g_use) {
+    if (e.device == dev.index() && e.stream == stream && e.use == use) {
+      if ((size_t)e.ws.numel() < need) e.ws = at::zeros({(int64_t)need}, bytes);
+      return e.ws;
+    }
+  }
+  g_use.push_back(UseEntry{dev.index(), stream, use, at::zeros({(int64_t)need}, bytes)});
+  return g_use.back().ws;
+}
+
+// check=True reports the bits of this call alone: earlier unchecked calls on the
+// stream may have left theirs in the word.
+void clear_status(const at::Tensor& ws, cudaStream_t stream) {
+  check_status(sqa_workspace_init(ws.data_ptr(), std::min<size_t>((size_t)ws.numel() * ws.element_size(), 256), stream),
+               "sqa_workspace_init");
+}
+
+cudaStream_t on_device(c10::cuda::OptionalCUDAGuard& guard, const at::Device& dev) {
+  if (c10::cuda::current_device() != dev.index()) guard.set_index(dev.index());
+  return at::cuda::getCurrentCUDAStream(dev.index()).stream();
+}
+
+std::tuple<at::Tensor, c10::optional<at::Tensor>> forward_scaled(
+    const at::Tensor& query, const at::Tensor& key_cache, const at::Tensor& value_cache, const at::Tensor& key_scales,
+    const at::Tensor& value_scales, const at::Tensor& block_tables, const at::Tensor& seq_lens, int64_t page_size,
+    const c10::optional<at::Tensor>& mask_lens, int64_t max_seq_len, const c10::optional<at::Tensor>& out,
+    const c10::optional<at::Tensor>& out_lse, bool return_lse, const c10::optional<at::Tensor>& workspace,
+    int64_t num_ctas, bool check, int64_t kv_layout, double sm_scale, double out_scale, int64_t min_seq_len) {
+  check_inputs(query, key_cache, value_cache, block_tables, seq_lens, page_size, mask_lens, kv_layout);
+  TORCH_CHECK_VALUE(key_cache.scalar_type() == at::kFloat8_e4m3fn, "a block-scaled cache is FP8-E4M3");
+  sqa_args a = fill_args(query, key_cache, value_cache, block_tables, seq_lens, mask_lens, max_seq_len, num_ctas, 0, 0,
+                         kv_layout, sm_scale, out_scale, min_seq_len, 0);
+  const sqa_scales scales = fill_scales(key_scales, value_scales, key_cache, a.num_kv_heads);
+  const at::Tensor o = out.has_value() ? *out : at::empty_like(query);
+  TORCH_CHECK_VALUE(o.sizes() == query.sizes() && o.is_contiguous() && o.device() == query.device() &&
+                        (o.scalar_type() == query.scalar_type() || o.scalar_type() == at::kFloat),
+                    "out must be a contiguous tensor shaped like query, of its type or fp32");
+  const bool f32 = o.scalar_type() == at::kFloat;
+  c10::optional<at::Tensor> l = out_lse;
+  if (!l.has_value() && (return_lse || f32))
+    l = at::empty(query.sizes().slice(0, 3), query.options().dtype(at::kFloat));
+  TORCH_CHECK_VALUE(!l.has_value() || (l->scalar_type() == at::kFloat && l->sizes() == query.sizes().slice(0, 3) &&
+                                       l->is_contiguous() && l->device() == query.device()),
+                    "out_lse must be a contiguous fp32 tensor [batch, q_len, Hq]");
+  if (f32) a.out_partial = o.data_ptr<float>();
+  else a.out = o.data_ptr();
+  a.out_lse = l.has_value() ? l->data_ptr<float>() : nullptr;
+  const at::Device dev = query.device();
+  c10::cuda::OptionalCUDAGuard guard;
+  const cudaStream_t stream = on_device(guard, dev);
+  int st = SQA_OK;
+  const size_t need = sqa_scaled_workspace_bytes(&a, dev.index(), &st);
+  check_status(st, "sqa_scaled_workspace_bytes");
+  TORCH_CHECK_VALUE(!workspace.has_value() || (workspace->device() == dev && workspace->is_contiguous()),
+                    "workspace must be a contiguous tensor on the query's device");
+  const at::Tensor ws = workspace.has_value() ? *workspace : memory_for(kUseAttention, need, dev, stream);
+  const size_t have = (size_t)ws.numel() * ws.element_size();
+  TORCH_CHECK_VALUE(have >= need, "workspace too small: need ", need, " bytes");
+  if (check) clear_status(ws, stream);
+  check_status(sqa_forward_scaled(&a, &scales, ws.data_ptr(), have, stream), "sqa_forward_scaled");
+  if (check) raise_device_bits(ws.data_ptr(), stream);
+  return {o, return_lse ? l : c10::nullopt};
+}
+
+void accumulate_weights(const at::Tensor& query, const at::Tensor& key_cache, const c10::optional<at::Tensor>& key_scales,
+                        const at::Tensor& block_tables, const at::Tensor& seq_lens, const at::Tensor& lse,
+                        const at::Tensor& scores, int64_t page_size, const c10::optional<at::Tensor>& mask_lens,
+                        int64_t max_seq_len, int64_t num_ctas, bool check, int64_t kv_layout, double sm_scale,
+                        int64_t min_seq_len) {
+  check_inputs(query, key_cache, key_cache, block_tables, seq_lens, page_size, mask_lens, kv_layout);
+  const sqa_args a = fill_args(query, key_cache, key_cache, block_tables, seq_lens, mask_lens, max_seq_len, num_ctas, 0,
+                               0, kv_layout, sm_scale, 1.0, min_seq_len, 0);
+  const bool fp8 = key_cache.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK_VALUE(fp8 == key_scales.has_value(), "key_scales belong to an FP8-E4M3 cache, and to no other");
+  sqa_scales scales = {};
+  if (fp8) scales = fill_scales(*key_scales, *key_scales, key_cache, a.num_kv_heads);
+  const at::Device dev = query.device();
+  TORCH_CHECK_VALUE(lse.device() == dev && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
+                        lse.sizes() == query.sizes().slice(0, 3),
+                    "lse must be a contiguous fp32 tensor [batch, q_len, Hq]");
+  TORCH_CHECK_VALUE(scores.device() == dev && scores.scalar_type() == at::kFloat && scores.is_contiguous() &&
+                        scores.sizes() == at::IntArrayRef({key_cache.size(0), (int64_t)a.num_kv_heads, kPage}),
+                    "scores must be a contiguous fp32 tensor [num_pages, Hkv, 16]");
+  c10::cuda::OptionalCUDAGuard guard;
+  const cudaStream_t stream = on_device(guard, dev);
+  const at::Tensor word = memory_for(kUseWeights, 256, dev, stream);
+  if (check) clear_status(word, stream);
+  check_status(sqa_accumulate_weights(&a, lse.data_ptr<float>(), fp8 ? &scales : nullptr, scores.data_ptr<float>(),
+                                      static_cast<uint32_t*>(word.data_ptr()), stream),
+               "sqa_accumulate_weights");
+  if (check) raise_device_bits(word.data_ptr(), stream);
+}
+
+void append_scaled(const at::Tensor& new_keys, const at::Tensor& new_values, const at::Tensor& key_cache,
+                   const at::Tensor& value_cache, const at::Tensor& key_scales, const at::Tensor& value_scales,
+                   const at::Tensor& block_tables, const at::Tensor& seq_lens, bool check, int64_t kv_layout) {
+  TORCH_CHECK_VALUE(key_cache.is_cuda(), "all inputs must be CUDA tensors");
+  const at::Device dev = key_cache.device();
+  for (const at::Tensor* t : {&new_keys, &new_values, &value_cache, &block_tables, &seq_lens})
+    TORCH_CHECK_VALUE(t->device() == dev, "all inputs must be CUDA tensors on the same device");
+  for (const at::Tensor* t : {&new_keys, &new_values, &block_tables, &seq_lens})
+    TORCH_CHECK_VALUE(t->is_contiguous(), "all inputs must be contiguous");
+  const auto nt = new_keys.scalar_type();
+  TORCH_CHECK_VALUE((nt == at::kHalf || nt == at::kBFloat16) && new_values.scalar_type() == nt,
+                    "new K/V must be FP16 or BF16, both of one type");
+  TORCH_CHECK_VALUE(key_cache.scalar_type() == at::kFloat8_e4m3fn && value_cache.scalar_type() == at::kFloat8_e4m3fn,
+                    "a block-scaled cache is FP8-E4M3");
+  TORCH_CHECK_VALUE(block_tables.scalar_type() == at::kInt && seq_lens.scalar_type() == at::kInt,
+                    "block_tables and seq_lens must be int32");
+  TORCH_CHECK_VALUE(new_keys.dim() == 4 && new_values.sizes() == new_keys.sizes(),
+                    "new_keys / new_values must be [batch, q_len, Hkv, 128]");
+  TORCH_CHECK_VALUE(key_cache.dim() == 4 && value_cache.sizes() == key_cache.sizes(),
+                    "key_cache / value_cache must be 4-D and of one shape");
+  const bool hnd = kv_layout == SQA_KV_HND;
+  const int64_t batch = new_keys.size(0), q_len = new_keys.size(1), hkv = new_keys.size(2);
+  TORCH_CHECK_VALUE(new_keys.size(3) == kHeadDim && key_cache.size(3) == kHeadDim, "the kernel supports head_dim 128");
+  TORCH_CHECK_VALUE(key_cache.size(hnd ? 2 : 1) == kPage, "page_size must be 16");
+  TORCH_CHECK_VALUE(hkv > 0 && key_cache.size(hnd ? 1 : 2) == hkv,
+                    "new K/V and the caches disagree on the number of KV heads");
+  TORCH_CHECK_VALUE(q_len >= 1, "q_len must be at least 1");
+  TORCH_CHECK_VALUE(block_tables.dim() == 2 && block_tables.size(0) == batch && seq_lens.numel() == batch,
+                    "invalid metadata: block_tables must be [batch, max_pages], seq_lens [batch]");
+  TORCH_CHECK_VALUE(key_cache.size(0) > 0 && block_tables.size(1) > 0, "empty KV cache is not supported");
+  const sqa_scales scales = fill_scales(key_scales, value_scales, key_cache, hkv);
+  const int64_t page_stride = cache_page_stride(key_cache, value_cache);
+  if (batch == 0) return;
+  c10::cuda::OptionalCUDAGuard guard;
+  const cudaStream_t stream = on_device(guard, dev);
+  const at::Tensor word = memory_for(kUseAppend, 256, dev, stream);
+  sqa_append_args a = {};
+  a.new_keys = new_keys.data_ptr();
+  a.new_values = new_values.data_ptr();
+  a.key_cache = key_cache.data_ptr();
+  a.value_cache = value_cache.data_ptr();
+  a.block_tables = block_tables.data_ptr<int32_t>();
+  a.seq_lens = seq_lens.data_ptr<int32_t>();
+  a.status = static_cast<uint32_t*>(word.data_ptr());
+  a.batch = (int32_t)batch;
+  a.q_len = (int32_t)q_len;
+  a.num_kv_heads = (int32_t)hkv;
+  a.head_dim = (int32_t)kHeadDim;
+  a.page_size = (int32_t)kPage;
+  a.num_pages = (int32_t)key_cache.size(0);
+  a.max_pages = (int32_t)block_tables.size(1);
+  a.kv_layout = (int32_t)kv_layout;
+  a.page_stride = page_stride;
+  a.kv_dtype = SQA_KV_FP8_E4M3;
+  if (check) clear_status(word, stream);
+  check_status(sqa_cache_append_scaled(&a, &scales, nt == at::kBFloat16 ? SQA_DTYPE_BF16 : SQA_DTYPE_F16, stream),
+               "sqa_cache_append_scaled");
+  if (check) raise_device_bits(word.data_ptr(), stream);
+}
+
+std::tuple<at::Tensor, at::Tensor> cache_evict(const at::Tensor& key_cache, const at::Tensor& value_cache,
+                                               const at::Tensor& scores, const at::Tensor& block_tables,
+                                               const at::Tensor& seq_lens, int64_t budget, int64_t recent, int64_t sinks,
+                                               const c10::optional<at::Tensor>& key_scales,
+                                               const c10::optional<at::Tensor>& value_scales,
+                                               const c10::optional<at::Tensor>& new_lens,
+                                               const c10::optional<at::Tensor>& kept, bool check, int64_t kv_layout) {
+  TORCH_CHECK_VALUE(key_cache.is_cuda(), "all inputs must be CUDA tensors");
+  const at::Device dev = key_cache.device();
+  for (const at::Tensor* t : {&value_cache, &scores, &block_tables, &seq_lens})
+    TORCH_CHECK_VALUE(t->device() == dev, "all inputs must be CUDA tensors on the same device");
+  for (const at::Tensor* t : {&scores, &block_tables, &seq_lens})
+    TORCH_CHECK_VALUE(t->is_contiguous(), "all inputs must be contiguous");
+  const auto kd = key_cache.scalar_type();
+  const bool fp8 = kd == at::kFloat8_e4m3fn;
+  TORCH_CHECK_VALUE((kd == at::kHalf || kd == at::kBFloat16 || fp8) && value_cache.scalar_type() == kd,
+                    "the caches must be FP16, BF16 or FP8-E4M3, both of one type");
+  TORCH_CHECK_VALUE(fp8 == key_scales.has_value() && fp8 == value_scales.has_value(),
+                    "key_scales and value_scales belong to an FP8-E4M3 cache, and to no other");
+  TORCH_CHECK_VALUE(block_tables.scalar_type() == at::kInt && seq_lens.scalar_type() == at::kInt,
+                    "block_tables and seq_lens must be int32");
+  TORCH_CHECK_VALUE(key_cache.dim() == 4 && value_cache.sizes() == key_cache.sizes(),
+                    "key_cache / value_cache must be 4-D and of one shape");
+  const bool hnd = kv_layout == SQA_KV_HND;
+  const int64_t hkv = key_cache.size(hnd ? 1 : 2);
+  TORCH_CHECK_VALUE(key_cache.size(3) == kHeadDim, "the kernel supports head_dim 128");
+  TORCH_CHECK_VALUE(key_cache.size(hnd ? 2 : 1) == kPage, "page_size must be 16");
+  TORCH_CHECK_VALUE(block_tables.dim() == 2 && seq_lens.numel() == block_tables.size(0),
+                    "invalid metadata: block_tables must be [batch, max_pages], seq_lens [batch]");
+  TORCH_CHECK_VALUE(key_cache.size(0) > 0 && hkv > 0 && block_tables.size(1) > 0, "empty KV cache is not supported");
+  TORCH_CHECK_VALUE(scores.scalar_type() == at::kFloat && scores.sizes() == at::IntArrayRef({key_cache.size(0), hkv, kPage}),
+                    "scores must be a contiguous fp32 tensor [num_pages, Hkv, 16]");
+  TORCH_CHECK_VALUE(budget >= 1 && budget <= (1 << 30), "budget must be in [1, 2^30]");
+  TORCH_CHECK_VALUE(recent >= 0 && sinks >= 0 && recent <= budget && sinks <= budget - recent,
+                    "recent and sinks must not be negative, and together at most budget");
+  sqa_scales scales = {};
+  if (fp8) scales = fill_scales(*key_scales, *value_scales, key_cache, hkv);
+  const int64_t page_stride = cache_page_stride(key_cache, value_cache);
+  const int64_t batch = block_tables.size(0);
+  const at::Tensor lens = new_lens.has_value() ? *new_lens : at::empty_like(seq_lens);
+  TORCH_CHECK_VALUE(lens.device() == dev && lens.scalar_type() == at::kInt && lens.is_contiguous() &&
+                        lens.sizes() == seq_lens.sizes() && (batch == 0 || lens.data_ptr() != seq_lens.data_ptr()),
+                    "new_lens must be a contiguous int32 tensor shaped like seq_lens, and another one");
+  const at::Tensor from = kept.has_value() ? *kept : at::empty({batch, hkv, budget}, seq_lens.options());
+  TORCH_CHECK_VALUE(from.device() == dev && from.scalar_type() == at::kInt && from.is_contiguous() &&
+                        from.sizes() == at::IntArrayRef({batch, hkv, budget}),
+                    "kept must be a contiguous int32 tensor [batch, Hkv, budget]");
+  if (batch == 0) return {lens, from};
+  c10::cuda::OptionalCUDAGuard guard;
+  const cudaStream_t stream = on_device(guard, dev);
+  const at::Tensor word = memory_for(kUseEvict, 256, dev, stream);
+  sqa_evict_args a = {};
+  a.key_cache = key_cache.data_ptr();
+  a.value_cache = value_cache.data_ptr();
+  a.scores = scores.data_ptr<float>();
+  a.block_tables = block_tables.data_ptr<int32_t>();
+  a.seq_lens = seq_lens.data_ptr<int32_t>();
+  a.new_lens = lens.data_ptr<int32_t>();
+  a.kept = from.data_ptr<int32_t>();
+  a.status = static_cast<uint32_t*>(word.data_ptr());
+  a.batch = (int32_t)batch;
+  a.num_kv_heads = (int32_t)hkv;
+  a.head_dim = (int32_t)kHeadDim;
+  a.page_size = (int32_t)kPage;
+  a.num_pages = (int32_t)key_cache.size(0);
+  a.max_pages = (int32_t)block_tables.size(1);
+  a.kv_layout = (int32_t)kv_layout;
+  a.kv_dtype = fp8 ? SQA_KV_FP8_E4M3 : SQA_KV_SAME;
+  a.budget = (int32_t)budget;
+  a.recent = (int32_t)recent;
+  a.sinks = (int32_t)sinks;
+  a.page_stride = page_stride;
+  if (check) clear_status(word, stream);
+  check_status(sqa_cache_evict(&a, fp8 ? &scales : nullptr, stream), "sqa_cache_evict");
+  if (check) raise_device_bits(word.data_ptr(), stream);
+  return {lens, from};
+}
+
 // ---- the registered operators (functional: they allocate their outputs)
 at::Tensor op_forward(const at::Tensor& query, const at::Tensor& key_cache, const at::Tensor& value_cache,
                       const at::Tensor& block_tables, const at::Tensor& seq_lens, int64_t page_size,
@@ -300,5 +570,9 @@ PYBIND11_MODULE(_sqa_torch, m) {
   m.doc() = "small-q paged MTP attention (B200): direct entry over the C ABI";
   m.def("forward", &forward, "causal paged MTP attention (see small_q_attention_b200.small_q_attention)");
   m.def("forward_partial", &forward_partial, "shard form: normalised fp32 O and natural-log LSE");
+  m.def("forward_scaled", &forward_scaled, "attention over a block-scaled e4m3 cache");
+  m.def("append_scaled", &append_scaled, "quantising append to a block-scaled e4m3 cache");
+  m.def("accumulate_weights", &accumulate_weights, "attention weight of every cached token, added to its score");
+  m.def("cache_evict", &cache_evict, "keep the tokens of the highest scores within a budget, compacted in place");
   m.def("abi_version", &sqa_abi_version);
 }

@@ -327,7 +327,7 @@ SQA_API int sqa_forward_scaled(const sqa_args* args, const sqa_scales* scales, v
  * which only `key` is read), block_tables, seq_lens, mask_lens and sm_scale as for
  * sqa_forward; value_cache and the outputs are not used.  lse: fp32 [batch, q_len,
  * num_q_heads], the natural-log log-sum-exp that the step's attention returned (a
- * row of -inf counts nothing).  The SQA_DEV_* bits are ORed into *status (may be NULL).
+ * row of -inf counts nothing).  The SQA_DEV_* bits are ORed into *status, a device word.
  * Pages must not be shared between sequences.  Asynchronous on `stream`. */
 SQA_API int sqa_accumulate_weights(const sqa_args* args, const float* lse, const sqa_scales* scales, float* scores,
                                    uint32_t* status, void* stream);

@@ -4,8 +4,9 @@
 // launch from the SM count and the shapes, encodes the two TMA tensor maps
 // over the paged caches and launches the kernels on the caller's stream.
 // Errors are status codes; no exception leaves this file.
-#include <cstdio>
+#include <algorithm>
 #include <cmath>
+#include <cstdio>
 #include <mutex>
 
 #include "../../include/small_q_attention.h"
@@ -43,6 +44,10 @@ constexpr long long kFp8LongRangeUnits = 400;
 #ifndef SQA_SEGMENT_COST_MMA
 #define SQA_SEGMENT_COST_MMA 4
 #endif
+// Block-scaled kernels: a CTA takes at least one 8-page block, and a segment start costs it
+// as much as this many pages.
+constexpr int kScaledMinPagesPerCta = 8;
+constexpr int kScaledSegmentCost = 24;
 constexpr int kSegmentCostTc = SQA_SEGMENT_COST_TC;
 constexpr int kSegmentCostMma = SQA_SEGMENT_COST_MMA;
 
@@ -545,18 +550,51 @@ int validate_scales(const sqa_args* a, const sqa_scales* s) {
 
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
-ScaledParams scaled_params(const sqa_args* a, const sqa_scales* s) {
+struct ScaledPlan {
+  int grid, seg_split, rows_pad;
+  size_t off_lse, off_o, bytes;
+};
+
+// One CTA per SM (it holds all of tensor memory), fewer for short work; with near-uniform length
+// hints and few segments, every segment is split evenly (as in make_plan).
+int make_scaled_plan(const sqa_args* a, int device, ScaledPlan* plan) {
+  const int sms = sm_count(device);
+  if (sms <= 0) return SQA_ERR_CUDA;
+  ScaledPlan pl = {};
+  const long long segments = (long long)a->batch * a->num_kv_heads;
+  long long pages = a->max_pages;
+  if (a->max_seq_len > 0) pages = std::min<long long>(pages, ((long long)a->max_seq_len + kPageSize - 1) / kPageSize);
+  long long grid = a->num_ctas > 0 ? a->num_ctas : sms;
+  if (a->num_ctas <= 0) {
+    const int min_pages = a->min_pages_per_cta > 0 ? a->min_pages_per_cta : kScaledMinPagesPerCta;
+    grid = std::max(1LL, std::min(grid, (segments * pages + min_pages - 1) / min_pages));
+    if (a->cluster != 1 && a->max_seq_len > 0 && a->min_seq_len > 0 && 100LL * a->min_seq_len >= 85LL * a->max_seq_len) {
+      const long long k = segments > 0 ? grid / segments : 0;
+      if (k >= 2 && 10 * segments * k >= 9 * grid && pages >= 16 * k) {
+        pl.seg_split = (int)k;
+        grid = segments * k;
+      }
+    }
+  }
+  pl.grid = (int)grid;
+  pl.rows_pad = warp_shape_for(a->q_len).rows_pad;
+  const size_t pieces = (size_t)(grid + segments);  // piece index = cta + segment
+  pl.off_lse = kAlign;                              // [0, 256): device status word
+  pl.off_o = align_up(pl.off_lse + pieces * pl.rows_pad * sizeof(float));
+  pl.bytes = align_up(pl.off_o + pieces * pl.rows_pad * kHeadDim * sizeof(float));
+  *plan = pl;
+  return SQA_OK;
+}
+
+ScaledParams scaled_params(const sqa_args* a, const sqa_scales* s, const ScaledPlan& pl) {
   ScaledParams p = {};
   p.q = a->query;
-  p.k_cache = a->key_cache;
-  p.v_cache = a->value_cache;
   p.k_scales = s ? s->key : nullptr;
   p.v_scales = s ? s->value : nullptr;
+  p.scale_stride = s && s->page_stride > 0 ? s->page_stride : a->num_kv_heads;
   p.block_tables = a->block_tables;
   p.seq_lens = a->seq_lens;
   p.mask_lens = a->mask_lens;
-  p.page_stride = a->page_stride > 0 ? a->page_stride : (int64_t)kPageSize * a->num_kv_heads * kHeadDim;
-  p.scale_stride = s && s->page_stride > 0 ? s->page_stride : a->num_kv_heads;
   p.batch = a->batch;
   p.q_len = a->q_len;
   p.hq = a->num_q_heads;
@@ -565,25 +603,38 @@ ScaledParams scaled_params(const sqa_args* a, const sqa_scales* s) {
   p.num_pages = a->num_pages;
   p.hnd = a->kv_layout == SQA_KV_HND;
   p.bf16 = a->dtype == SQA_DTYPE_BF16;
+  p.grid = pl.grid;
+  p.seg_cost = kScaledSegmentCost;
+  p.seg_split = pl.seg_split;
+  p.rows_pad = pl.rows_pad;
   p.scale_log2 = 1.4426950408889634f * (a->sm_scale > 0.f ? a->sm_scale : 1.f / sqrtf((float)kHeadDim));
   p.out_scale = a->out_scale != 0.f ? a->out_scale : 1.f;
   return p;
 }
+
+// The shapes and options that the block-scaled kernels take.
+int validate_scaled(const sqa_args* a) {
+  const int st = validate(a);
+  if (st != SQA_OK) return st;
+  return a->kernel != 0 || a->cluster > 1 ? SQA_ERR_UNSUPPORTED : SQA_OK;
+}
 }  // namespace
 
 size_t sqa_scaled_workspace_bytes(const sqa_args* a, int device, int* status) {
-  (void)device;
-  int st = validate(a);
+  int st = validate_scaled(a);
   if (st == SQA_OK && a->kv_dtype != SQA_KV_FP8_E4M3) st = SQA_ERR_INVALID_ARGUMENT;
-  if (st == SQA_OK && (a->kernel != 0 || a->cluster > 1)) st = SQA_ERR_UNSUPPORTED;
+  ScaledPlan pl = {};
+  if (st == SQA_OK) {
+    const int dev = current_device(device);
+    st = dev < 0 ? SQA_ERR_CUDA : make_scaled_plan(a, dev, &pl);
+  }
   if (status) *status = st;
-  return st == SQA_OK ? kAlign : 0;
+  return st == SQA_OK ? pl.bytes : 0;
 }
 
 int sqa_forward_scaled(const sqa_args* a, const sqa_scales* scales, void* workspace, size_t workspace_bytes,
                        void* stream) {
-  int st = SQA_OK;
-  const size_t need = sqa_scaled_workspace_bytes(a, -1, &st);
+  int st = validate_scaled(a);
   if (st != SQA_OK) return st;
   st = validate_scales(a, scales);
   if (st != SQA_OK) return st;
@@ -600,35 +651,60 @@ int sqa_forward_scaled(const sqa_args* a, const sqa_scales* scales, void* worksp
       !aligned4(scales->key) || !aligned4(scales->value))
     return SQA_ERR_INVALID_ARGUMENT;
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & (kAlign - 1))) return SQA_ERR_INVALID_ARGUMENT;
-  if (workspace_bytes < need) return SQA_ERR_WORKSPACE_TOO_SMALL;
-  ScaledParams p = scaled_params(a, scales);
+  const int dev = current_device(-1);
+  if (dev < 0) return SQA_ERR_CUDA;
+  ScaledPlan pl;
+  st = make_scaled_plan(a, dev, &pl);
+  if (st != SQA_OK) return st;
+  if (workspace_bytes < pl.bytes) return SQA_ERR_WORKSPACE_TOO_SMALL;
+  CUtensorMap tm_k, tm_v;
+  const bool hnd = a->kv_layout == SQA_KV_HND;
+  const uint64_t page_stride = page_stride_bytes(a->page_stride, a->num_kv_heads, 1);
+  if (!encode_cache_map(&tm_k, a->key_cache, a->num_pages, a->num_kv_heads, hnd, page_stride, true) ||
+      !encode_cache_map(&tm_v, a->value_cache, a->num_pages, a->num_kv_heads, hnd, page_stride, true))
+    return SQA_ERR_CUDA;
+  uint8_t* const ws = static_cast<uint8_t*>(workspace);
+  ScaledParams p = scaled_params(a, scales, pl);
   p.out = a->out;
   p.out_o = a->out_partial;
   p.out_lse = a->out_lse;
-  p.status = static_cast<unsigned int*>(workspace);
-  return launch_scaled_attention(p, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? SQA_OK : SQA_ERR_CUDA;
+  p.ws_lse = reinterpret_cast<float*>(ws + pl.off_lse);
+  p.ws_o = reinterpret_cast<float*>(ws + pl.off_o);
+  p.status = reinterpret_cast<unsigned int*>(ws);
+  return launch_scaled_attention(p, tm_k, tm_v, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? SQA_OK
+                                                                                                     : SQA_ERR_CUDA;
 }
 
 int sqa_accumulate_weights(const sqa_args* a, const float* lse, const sqa_scales* scales, float* scores,
                            uint32_t* status, void* stream) {
-  int st = validate(a);
+  int st = validate_scaled(a);
   if (st != SQA_OK) return st;
-  if (a->kernel != 0 || a->cluster > 1) return SQA_ERR_UNSUPPORTED;
-  if (a->kv_dtype == SQA_KV_FP8_E4M3) st = validate_scales(a, scales);  // e4m3 caches carry their scales
+  const bool fp8 = a->kv_dtype == SQA_KV_FP8_E4M3;
+  if (fp8) st = validate_scales(a, scales);  // e4m3 caches carry their scales
   else if (scales) st = SQA_ERR_INVALID_ARGUMENT;
   if (st != SQA_OK) return st;
   if (a->batch == 0) return SQA_OK;
-  if (!a->query || !a->key_cache || !a->block_tables || !a->seq_lens || !lse || !scores || (scales && !scales->key))
+  if (!a->query || !a->key_cache || !a->block_tables || !a->seq_lens || !lse || !scores || !status ||
+      (scales && !scales->key))
     return SQA_ERR_INVALID_ARGUMENT;
   if (!aligned16(a->query) || !aligned16(a->key_cache)) return SQA_ERR_INVALID_ARGUMENT;
   if (!aligned4(a->block_tables) || !aligned4(a->seq_lens) || !aligned4(a->mask_lens) || !aligned4(lse) ||
       !aligned4(scores) || !aligned4(status) || (scales && !aligned4(scales->key)))
     return SQA_ERR_INVALID_ARGUMENT;
-  ScaledParams p = scaled_params(a, scales);
+  const int dev = current_device(-1);
+  if (dev < 0) return SQA_ERR_CUDA;
+  ScaledPlan pl;
+  st = make_scaled_plan(a, dev, &pl);
+  if (st != SQA_OK) return st;
+  CUtensorMap tm_k;
+  if (!encode_cache_map(&tm_k, a->key_cache, a->num_pages, a->num_kv_heads, a->kv_layout == SQA_KV_HND,
+                        page_stride_bytes(a->page_stride, a->num_kv_heads, fp8 ? 1 : 2), fp8))
+    return SQA_ERR_CUDA;
+  ScaledParams p = scaled_params(a, scales, pl);
   p.lse = lse;
   p.scores = scores;
   p.status = status;
-  return launch_weights(p, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? SQA_OK : SQA_ERR_CUDA;
+  return launch_weights(p, tm_k, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? SQA_OK : SQA_ERR_CUDA;
 }
 
 int sqa_merge_partials(const float* parts_o, const float* parts_lse, int32_t num_parts, int64_t rows,

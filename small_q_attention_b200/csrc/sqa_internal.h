@@ -86,8 +86,6 @@ struct MergeParams {
 // Attention over a block-scaled e4m3 cache, and the weights of its (or a 16-bit cache's) tokens.
 struct ScaledParams {
   const void* q;                // [B, q_len, Hq, 128] fp16 or bf16
-  const void* k_cache;          // e4m3 (16-bit too for the weights)
-  const void* v_cache;
   const float* k_scales;        // [num_pages, hkv], scale_stride floats from page to page (nullptr: 16-bit cache)
   const float* v_scales;
   const int32_t* block_tables;  // [B, max_pages]
@@ -98,16 +96,19 @@ struct ScaledParams {
   void* out;                    // attention: 16-bit rows, or nullptr
   float* out_o;                 // attention: fp32 rows, or nullptr
   float* out_lse;               // attention: or nullptr
+  float* ws_o;                  // attention: partials of split segments [pieces, rows_pad, 128]
+  float* ws_lse;                // attention: [pieces, rows_pad]
   unsigned int* status;
-  long long page_stride;        // elements
   long long scale_stride;       // floats
   int batch, q_len, hq, hkv, max_pages, num_pages;
   int hnd, bf16;
+  int grid, seg_cost, seg_split, rows_pad;  // the schedule (sqa_schedule.cuh)
   float scale_log2, out_scale;
 };
 
-cudaError_t launch_scaled_attention(const ScaledParams& p, cudaStream_t stream);
-cudaError_t launch_weights(const ScaledParams& p, cudaStream_t stream);
+cudaError_t launch_scaled_attention(const ScaledParams& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
+                                    cudaStream_t stream);
+cudaError_t launch_weights(const ScaledParams& p, const CUtensorMap& tm_k, cudaStream_t stream);
 
 // Launchers (stream-ordered, no allocation).  Return cudaGetLastError().
 cudaError_t launch_split_kv(const SplitKvParams& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v,

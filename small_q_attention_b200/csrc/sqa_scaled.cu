@@ -1,205 +1,1109 @@
 // sqa_scaled.cu -- attention over a block-scaled e4m3 cache, and the attention weight of
-// every cached token.
+// every cached token, on the 5th-generation tensor cores.
 //
-// One CTA per (sequence, KV head) walks the sequence in tiles of 32 tokens held in
-// shared memory as fp32: scores, a running maximum and sum per row, and the output
-// accumulators in registers.
+// Orientation.  The tokens are the M side of both products: S^T = K Q^T puts token t of a
+// 128-token block (8 pages) on TMEM lane t and the query rows on columns, and O^T += V^T P^T
+// puts the head dimension on lanes and the rows on columns.  A softmax thread then owns one
+// token: its page's two scales are two scalars of the thread (a factor of every score of the
+// lane, and of every probability it writes), a token's attention weight is a sum over the
+// thread's own registers, and the M = 128 side is full whatever q_len is (with rows on M, a
+// q_len of 4 fills 16 of 128 lanes).
+//
+// Precision.  The tensor core reads the e4m3 K and V as they are (kind::f8f6f4 wants 8-bit
+// operands on both sides).  Q and P enter as PARTS e4m3 numbers each, x = x0 + x1 / 32 +
+// x2 / 1024, each the e4m3 rounding of what the parts before it left (4 significant bits a
+// part).  The parts are extra columns of the N side (free: an M = 128 product of few columns
+// is bound by reading A) with their own fp32 accumulators, joined at read-out, so that a
+// low part has its own exponent range.  Two parts hold a bf16 query exactly (8 bits) and round P
+// to 2^-9, half of bf16's own rounding; three hold an fp16 query exactly (11 bits) and
+// round P to 2^-13.  A row of Q is first scaled by a power of two that brings its largest
+// magnitude into [128, 256); P is at most 2^8 by the rule below.
+//
+// Softmax.  Per row a base b is kept; a score with its value scale, y = c ks (q . k) + lv with
+// vs = f * 2^lv, enters as E = 2^(y - b): P = f E, and the denominator sums 2^-lv E.  The value
+// scale is thus inside the running maximum, and P keeps its e4m3 range whatever the pages' value
+// scales are.  A base is raised, to the block's maximum - 4, only when some y exceeds it by more
+// than 8 (one barrier with an or-reduction a block finds that out); then l and the row's O columns
+// are rescaled.  Masked tokens and tokens behind the sequence have y = -inf by selection, so NaN in
+// their K does not matter; V rows behind the sequence are zeroed in shared memory, and a NaN in
+// the V of a draft token is zeroed and remembered, as only the rows that see the token get it.
+//
+// Weights.  w_t = sum over the rows of 2^(c ks (q . k) - lse): the same score product, summed over the
+// thread's columns and added to the token's score.  16-bit caches use kind::f16 and Q as it is.
+//
+// Warps: 0-3 softmax (one token a thread), 4 score products, 5 value products, 6 TMA
+// producer, 7 page scales.  Work is cut into CTA ranges by sqa_schedule.cuh; pieces of a split
+// segment are merged by sqa_scaled_merge_kernel.
+//
+// Pipelines (mbarriers; every wait bounded):
+//   full / empty [tiles]     producer -> issuers; K and V tiles (16 KB) alternate in one ring,
+//                            each released by the commit of the product that read it
+//   s_full / s_empty [NS]    score issuer (commit) -> softmax -> score issuer
+//   p_full / p_done [2]      softmax -> value issuer (commit) -> softmax
+//   q_ready [2]              softmax (Q of a piece, one piece ahead) -> score issuer
+//   m_full / m_empty [8]     page scales of a block -> softmax
+#include "small_q_attention.h"
 #include "sqa_internal.h"
+#include "sqa_merge_row.cuh"
 #include "sqa_ptx.cuh"
 #include "sqa_scaled.cuh"
+#include "sqa_schedule.cuh"
 
 namespace sqa {
 namespace {
 
-__device__ __forceinline__ void raise(unsigned int* status, unsigned int bits) {
-  if (status != nullptr) atomicOr(status, bits);
-}
+constexpr int kBlockPages = 8;
+constexpr int kBlock = kBlockPages * kPageSize;  // 128 tokens: the M side
+constexpr int kTileBytes = kBlock * 128;         // K or V of a block (e4m3), or one half of 16-bit K
+constexpr int kMetaSlots = 8;
+constexpr int kPBytes = kBlock * 128;
+constexpr int kScaledTcThreads = 256;
+constexpr float kNoBase = -1e30f;                // a row that has seen nothing yet
+constexpr float kRaise = 8.f, kHead = 4.f;       // raise a base that a score exceeds by 2^8, to 2^4 under it
+constexpr float kLn2f = 0.6931471805599453f;
+constexpr int kMaxLv = 60;                       // value scales enter as f * 2^lv, |lv| <= 60
 
-constexpr int kTile = 32;
-constexpr int kScaledThreads = 256;
-constexpr int kRowStride = kHeadDim + 4;
-
-struct ScaledSmem {
-  float q[kGroup * 16][kRowStride];
-  float k[kTile][kRowStride];
-  float v[kTile][kRowStride];
-  float s[kGroup * 16][kTile + 1];
-  float m[kGroup * 16], l[kGroup * 16], alpha[kGroup * 16];
+// PARTS: e4m3 parts of Q (and P): 2 or 3; 0 = 16-bit cache (weights only).
+// ROWS: query rows of a group (8, 16 or 32), G groups (2 for q_len > 8).
+template <int PARTS_, int ROWS_, int G_, bool ATTEND_>
+struct Shape {
+  static constexpr int PARTS = PARTS_, ROWS = ROWS_, G = G_;
+  static constexpr bool ATTEND = ATTEND_, F8 = PARTS_ > 0;
+  static constexpr int COLS = (F8 ? PARTS : 1) * ROWS;
+  static constexpr int N = (COLS + 15) / 16 * 16;             // score columns of a group (N of the product)
+  static constexpr int STRIDE = N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128;  // TMEM columns of a score slot
+  static constexpr int OCOLS = ATTEND ? 128 : 0;              // O columns of a group (P's row is 128 bytes)
+  static constexpr int SLOTS_FIT = (512 - G * OCOLS) / STRIDE;
+  static constexpr int NS = SLOTS_FIT < 4 ? SLOTS_FIT : 4;
+  static constexpr int Q_GROUP = F8 ? N * 128 : 2 * N * 128;  // bytes of one group's Q operand
+  static constexpr int Q_BYTES = G * Q_GROUP;
+  static constexpr int TILES = ATTEND || !F8 ? 2 : 1;         // 16 KB tiles of a block (K and V, or K's two halves)
+  static constexpr int CH = ROWS < 16 ? ROWS : 16;            // rows handled at once
+  static_assert(PARTS * ROWS <= 128 && NS >= 2, "columns");
 };
 
-// kElem: 1 = e4m3 with a scale, 2 = 16-bit.
-template <bool BF, int kElem>
-__device__ __forceinline__ float cached(const void* cache, size_t at, float scale) {
-  if constexpr (kElem == 1) {
-    return unpack_e4m3x2(static_cast<const uint8_t*>(cache)[at]).x * scale;
+struct ScaledTcParams {
+  SplitKvParams s;  // schedule, tables, outputs (s.out: 16-bit rows; s.out_o: fp32 rows; s.out_lse: optional)
+  const float* k_scales;
+  const float* v_scales;
+  long long scale_stride;
+  const float* lse;  // weights
+  float* scores;
+};
+
+struct TcSmem {
+  uint8_t* ring;
+  uint8_t* p;  // two P buffers
+  uint8_t* q;  // two Q slots
+  float4* meta;     // [kMetaSlots][8]: ks, vs, page id (bits), -
+  float* cq;        // [2][64]: log2-domain score factor of a row
+  float* base;      // [64]
+  float* alpha;     // [64]; the epilogue's 1 / l
+  float* wmax;      // [4][64]: per-warp maxima, then per-warp sums
+  uint64_t *full, *empty, *s_full, *s_empty, *p_full, *p_done, *q_ready, *m_full, *m_empty, *done;
+  uint32_t* tmem_base;
+  Schedule* sch;
+};
+
+constexpr int kFixedBytes = kMetaSlots * 8 * 16 + (2 * 64 + 64 + 64 + 4 * 64) * 4 + (2 * 4 + 2 + 2 + 2 + 2 * kMetaSlots + 1) * 8 + 64;
+
+template <class S>
+__host__ __device__ constexpr int fixed_smem() {
+  return 1024 + (S::ATTEND ? 2 * kPBytes : 0) + 2 * S::Q_BYTES + kFixedBytes;
+}
+
+template <class S>
+__device__ __forceinline__ TcSmem carve(uint8_t* smem, int tiles) {
+  TcSmem t;
+  t.ring = smem;
+  t.p = smem + (size_t)tiles * kTileBytes;
+  t.q = t.p + (S::ATTEND ? 2 * kPBytes : 0);
+  t.meta = reinterpret_cast<float4*>(t.q + 2 * S::Q_BYTES);
+  t.cq = reinterpret_cast<float*>(t.meta + kMetaSlots * 8);
+  t.base = t.cq + 2 * 64;
+  t.alpha = t.base + 64;
+  t.wmax = t.alpha + 64;
+  uint64_t* b = reinterpret_cast<uint64_t*>(t.wmax + 4 * 64);
+  t.full = b;
+  t.empty = t.full + tiles;
+  t.s_full = t.empty + tiles;
+  t.s_empty = t.s_full + 4;
+  t.p_full = t.s_empty + 4;
+  t.p_done = t.p_full + 2;
+  t.q_ready = t.p_done + 2;
+  t.m_full = t.q_ready + 2;
+  t.m_empty = t.m_full + kMetaSlots;
+  t.done = t.m_empty + kMetaSlots;
+  t.tmem_base = reinterpret_cast<uint32_t*>(t.done + 1);
+  t.sch = reinterpret_cast<Schedule*>(t.tmem_base + 2);
+  return t;
+}
+
+// The pieces of a CTA's range: f(walk, first unit, pages) for each, in order.
+template <class F>
+__device__ __forceinline__ void for_pieces(const SplitKvParams& p, const Schedule& sch, F f) {
+  SegWalk w = first_segment(p, sch);
+  int unit = sch.start;
+  while (unit < sch.end) {
+    const int seg_end = w.seg_start + w.pages;
+    const int n = min(sch.end, seg_end) - unit;
+    f(w, unit, n);
+    unit += n;
+    if (unit >= seg_end) next_segment(p, w);
+    else w.pg += n;
+  }
+}
+
+__device__ __forceinline__ int blocks_of(int pages) { return (pages + kBlockPages - 1) / kBlockPages; }
+
+// As for_pieces, by a whole warp, with the piece's page ids: f(walk, c0, n, id) for each chunk of 32
+// pages from page c0 of the piece on, lane l holding the id of page c0 + l.  The ids are read one
+// chunk ahead, across pieces too.
+template <class F>
+__device__ __forceinline__ void for_page_chunks(const SplitKvParams& p, const Schedule& sch, F f) {
+  const int lane = threadIdx.x & 31;
+  SegWalk w = first_segment(p, sch);
+  int unit = sch.start;
+  auto first_ids = [&](const SegWalk& x, int u) {
+    const int n = min(sch.end, x.seg_start + x.pages) - u;
+    return lane < n ? __ldg(p.block_tables + (size_t)x.b * p.max_pages + x.pg + lane) : 0;
+  };
+  int ids = unit < sch.end ? first_ids(w, unit) : 0;
+  while (unit < sch.end) {
+    const int n = min(sch.end, w.seg_start + w.pages) - unit;
+    const int32_t* row = p.block_tables + (size_t)w.b * p.max_pages + w.pg;
+    const int next = unit + n;
+    SegWalk wn = w;
+    if (next < sch.end) next_segment(p, wn);  // a piece ends at its segment's end or the range's
+    for (int c0 = 0; c0 < n; c0 += 32) {
+      int ahead = 0;
+      if (c0 + 32 < n) ahead = c0 + 32 + lane < n ? __ldg(row + c0 + 32 + lane) : 0;
+      else if (next < sch.end) ahead = first_ids(wn, next);
+      f(w, c0, n, ids);
+      ids = ahead;
+    }
+    unit = next;
+    w = wn;
+  }
+}
+
+// ------------------------------------------------------------------ producer (whole warp)
+template <class S>
+__device__ void produce(const ScaledTcParams& p, const Schedule& sch, const CUtensorMap* tm_k, const CUtensorMap* tm_v,
+                        const TcSmem& sm, int tiles, volatile int* abort) {
+  const uint64_t policy = l2_policy_evict_first();
+  int slot = 0, issued = 0;
+  uint32_t phase = 0;
+  unsigned int bad = 0;
+  for_page_chunks(p.s, sch, [&](const SegWalk& w, int c0, int n, int id) {
+    // NHD map: (dim, head, token, page); HND map: (dim, token, head, page)
+    const int c1 = p.s.hnd ? 0 : w.h, c2 = p.s.hnd ? w.h : 0;
+    const int cnt = min(32, n - c0);
+    for (int jb = 0; jb < cnt; jb += kBlockPages) {
+      const int np = min(kBlockPages, cnt - jb);
+      int pages[kBlockPages];
+#pragma unroll
+      for (int j = 0; j < kBlockPages; ++j) {
+        pages[j] = __shfl_sync(0xffffffffu, id, min(jb + j, 31));
+        if (j < np && (pages[j] < 0 || pages[j] >= p.s.num_pages)) {
+          bad = 1;
+          pages[j] = 0;
+        }
+      }
+#pragma unroll
+      for (int tile = 0; tile < S::TILES; ++tile) {  // K then V; or the two 64-dim halves of 16-bit K
+        bool ok = mbar_wait_bounded(smem_u32(sm.empty + slot), phase ^ 1u, abort, p.s.status, 1, issued);
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        if (ok) {
+          if (elect_one()) {
+            const uint32_t f = smem_u32(sm.full + slot);
+            mbar_arrive_expect_tx(f, np * 2048);
+            const uint32_t dst = smem_u32(sm.ring + (size_t)slot * kTileBytes);
+            const CUtensorMap* map = (S::F8 && tile == 1) ? tm_v : tm_k;
+            const int c = S::F8 ? 0 : tile * 64;
+            for (int j = 0; j < np; ++j) tma_load_4d(dst + j * 2048, map, f, c, c1, c2, pages[j], policy);
+          }
+          __syncwarp();
+          ++issued;
+        }
+        if (++slot == tiles) {
+          slot = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  });
+  const int lane = threadIdx.x & 31;
+  if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(p.s.status, 8u);  // SQA_DEV_BAD_PAGE
+  if (lane == 0 && *abort) {  // only an abort can leave loads in flight
+    for (int k = 0; k < min(issued, tiles); ++k) {
+      const int last = k + tiles * ((issued - 1 - k) / tiles);
+      if (!mbar_drain(smem_u32(sm.full + k), (uint32_t)(last / tiles) & 1u, 100000000ull))
+        atomicOr(p.s.status, 1u);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ page scales (whole warp)
+// The scales (and, for the weights, the id) of every page of a block into a meta slot.
+template <class S>
+__device__ void page_meta(const ScaledTcParams& p, const Schedule& sch, const TcSmem& sm, volatile int* abort) {
+  const int lane = threadIdx.x & 31;
+  int blk = 0;
+  for_page_chunks(p.s, sch, [&](const SegWalk& w, int c0, int n, int id) {
+    const bool in = c0 + lane < n;
+    const bool good = id >= 0 && id < p.s.num_pages;
+    float4 m = make_float4(S::F8 ? 0.f : 1.f, 0.f, __int_as_float(in && good ? id : -1), 0.f);
+    if (S::F8 && in) {
+      const size_t at = (size_t)(good ? id : 0) * p.scale_stride + w.h;
+      m.x = __ldg(p.k_scales + at);
+      if (S::ATTEND) m.y = __ldg(p.v_scales + at);
+    }
+    const int cnt = min(32, n - c0);
+    for (int jb = 0; jb < cnt; jb += kBlockPages, ++blk) {
+      const int e = blk % kMetaSlots;
+      if (blk >= kMetaSlots)
+        mbar_wait_bounded(smem_u32(sm.m_empty + e), (uint32_t)(blk / kMetaSlots - 1) & 1u, abort, p.s.status, 2, blk);
+      if (lane >= jb && lane < jb + kBlockPages) sm.meta[e * kBlockPages + lane - jb] = m;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(sm.m_full + e));
+    }
+  });
+}
+
+// ------------------------------------------------------------------ product issuers (whole warps, one elected lane)
+__device__ __forceinline__ void tc_mma_ss_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void drain_products(const ScaledTcParams& p, const TcSmem& sm) {
+  if (elect_one()) tc_commit(smem_u32(sm.done));
+  __syncwarp();
+  if (!mbar_drain(smem_u32(sm.done), 0u, 2000000000ull) && (threadIdx.x & 31) == 0)
+    atomicOr(p.s.status, 1u);
+}
+
+// S^T of (block, group) unit u into score slot u % NS.
+template <class S, bool BF>
+__device__ void issue_scores(const ScaledTcParams& p, const Schedule& sch, const TcSmem& sm, uint32_t tmem, int tiles,
+                             volatile int* abort) {
+  constexpr uint32_t kIdesc = mma_idesc_f16(128, S::N, false, false, BF && !S::F8);  // format 0: e4m3 / fp16
+  int u = 0, blk = 0, pc = 0;
+  for_pieces(p.s, sch, [&](const SegWalk&, int, int n) {
+    mbar_wait_bounded(smem_u32(sm.q_ready + (pc & 1)), (uint32_t)(pc >> 1) & 1u, abort, p.s.status, 4, pc);
+    const uint32_t q = smem_u32(sm.q + (pc & 1) * S::Q_BYTES);
+    const int nblk = blocks_of(n);
+    for (int k = 0; k < nblk; ++k, ++blk) {
+      const int t0 = blk * S::TILES;  // tile index of K (its first half)
+      mbar_wait_bounded(smem_u32(sm.full + t0 % tiles), (uint32_t)(t0 / tiles) & 1u, abort, p.s.status, 5, blk);
+      if (!S::F8) {
+        const int t1 = t0 + 1;
+        mbar_wait_bounded(smem_u32(sm.full + t1 % tiles), (uint32_t)(t1 / tiles) & 1u, abort, p.s.status, 5, blk);
+      }
+#pragma unroll
+      for (int g = 0; g < S::G; ++g, ++u) {
+        if (u >= S::NS)
+          mbar_wait_bounded(smem_u32(sm.s_empty + u % S::NS), (uint32_t)(u / S::NS - 1) & 1u, abort, p.s.status, 6, u);
+        __syncwarp();
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t d = tmem + S::G * S::OCOLS + (u % S::NS) * S::STRIDE;
+          const uint32_t qg = q + g * S::Q_GROUP;
+          if constexpr (S::F8) {
+            const uint32_t kt = smem_u32(sm.ring + (size_t)(t0 % tiles) * kTileBytes);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)  // 32 dims (32 B) a step
+              tc_mma_ss_f8(d, smem_desc_sw128(kt + kk * 32, 16, 1024), smem_desc_sw128(qg + kk * 32, 16, 1024), kIdesc,
+                           kk > 0 ? 1u : 0u);
+          } else {
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) {  // 16 dims (32 B) a step, four to a half
+              const uint32_t kt = smem_u32(sm.ring + (size_t)((t0 + (kk >> 2)) % tiles) * kTileBytes);
+              tc_mma_ss(d, smem_desc_sw128(kt + (kk & 3) * 32, 16, 1024),
+                        smem_desc_sw128(qg + (kk >> 2) * (S::N * 128) + (kk & 3) * 32, 16, 1024), kIdesc, kk > 0 ? 1u : 0u);
+            }
+          }
+          tc_commit(smem_u32(sm.s_full + u % S::NS));
+          if (g == S::G - 1) {  // the block's K may be overwritten
+            tc_commit(smem_u32(sm.empty + t0 % tiles));
+            if (!S::F8) tc_commit(smem_u32(sm.empty + (t0 + 1) % tiles));
+          }
+        }
+        __syncwarp();
+      }
+    }
+    ++pc;
+  });
+  drain_products(p, sm);
+}
+
+// O^T of group g += V^T P^T of (block, group) unit u, once P is in buffer u % 2.
+template <class S>
+__device__ void issue_values(const ScaledTcParams& p, const Schedule& sch, const TcSmem& sm, uint32_t tmem, int tiles,
+                             volatile int* abort) {
+  constexpr uint32_t kIdesc = mma_idesc_f16(128, 128, true, true, false);
+  int u = 0, blk = 0;
+  for_pieces(p.s, sch, [&](const SegWalk&, int, int n) {
+    const int nblk = blocks_of(n);
+    for (int k = 0; k < nblk; ++k, ++blk) {
+      const int t1 = blk * 2 + 1;
+      const int np = min(kBlockPages, n - k * kBlockPages);
+#pragma unroll
+      for (int g = 0; g < S::G; ++g, ++u) {
+        mbar_wait_bounded(smem_u32(sm.p_full + (u & 1)), (uint32_t)(u >> 1) & 1u, abort, p.s.status, 7, u);
+        if (g == 0)
+          mbar_wait_bounded(smem_u32(sm.full + t1 % tiles), (uint32_t)(t1 / tiles) & 1u, abort, p.s.status, 8, blk);
+        __syncwarp();
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t v = smem_u32(sm.ring + (size_t)(t1 % tiles) * kTileBytes);
+          const uint32_t pb = smem_u32(sm.p + (u & 1) * kPBytes);
+          const int steps = (np + 1) / 2;  // 32 tokens a step; the softmax zeroed an absent page's V
+          for (int kk = 0; kk < steps; ++kk)
+            tc_mma_ss_f8(tmem + g * 128, smem_desc_sw128(v + kk * 4096, kTileBytes, 1024),
+                         smem_desc_sw128(pb + kk * 4096, kTileBytes, 1024), kIdesc, (k > 0 || kk > 0) ? 1u : 0u);
+          tc_commit(smem_u32(sm.p_done + (u & 1)));
+          if (g == S::G - 1) tc_commit(smem_u32(sm.empty + t1 % tiles));
+        }
+        __syncwarp();
+      }
+    }
+  });
+  drain_products(p, sm);
+}
+
+// ------------------------------------------------------------------ softmax warps (128 threads)
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[8]) { tmem_ld8(taddr, r); }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[8]) { tmem_st8(taddr, r); }
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[16]) { tmem_st16(taddr, r); }
+
+// Barrier of the softmax threads; true when `v` is for any of them.
+__device__ __forceinline__ bool softmax_any(bool v) {
+  int r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+      "selp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((int)v)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void softmax_sync() { named_bar_sync(1, 128); }
+
+__device__ __forceinline__ int float_order(float f) {  // order-preserving int
+  const int i = __float_as_int(f);
+  return i ^ ((i >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float order_float(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
+
+// PARTS e4m3 parts of four numbers: x = part 0 + part 1 / 32 + part 2 / 1024.
+template <int PARTS>
+__device__ __forceinline__ void split4(float (&x)[4], uint32_t (&out)[3]) {
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    const uint32_t a = pack_e4m3x2(x[0], x[1]), b = pack_e4m3x2(x[2], x[3]);
+    out[i] = a | (b << 16);
+    if (i + 1 < PARTS) {
+      const float2 fa = unpack_e4m3x2(a), fb = unpack_e4m3x2(b);
+      x[0] = (x[0] - fa.x) * 32.f;
+      x[1] = (x[1] - fa.y) * 32.f;
+      x[2] = (x[2] - fb.x) * 32.f;
+      x[3] = (x[3] - fb.y) * 32.f;
+    }
+  }
+}
+
+// Q of (b, h) as the N operand of the score product, into slot `qs`: row r of part i is operand row
+// i * ROWS + r (128 B, 128-byte swizzle), and the rows' score factors.  128 threads, eight to a row.
+template <class S, bool BF>
+__device__ void write_q(const ScaledTcParams& p, const TcSmem& sm, int b, int h, int qs) {
+  const int tid = threadIdx.x;
+  const int rows = kGroup * p.s.q_len;
+  constexpr int kItems = S::G * S::ROWS * 8;
+  for (int it = tid; it < (kItems + 127) / 128 * 128; it += 128) {
+    const int r = it >> 3, c = it & 7;  // row, its 16 dims
+    const bool in = it < kItems;
+    const bool real = in && r < rows;
+    const __half* src = p.s.q + ((size_t)(b * p.s.q_len + (r >> 2)) * p.s.hq + h * kGroup + (r & 3)) * kHeadDim + c * 16;
+    uint4 x[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+    if (real) {
+      x[0] = __ldg(reinterpret_cast<const uint4*>(src));
+      x[1] = __ldg(reinterpret_cast<const uint4*>(src) + 1);
+    }
+    const int g = r / S::ROWS, rr = r % S::ROWS;
+    uint8_t* const dst = sm.q + qs * S::Q_BYTES + g * S::Q_GROUP;
+    const uint32_t w[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+    if constexpr (!S::F8) {
+      if (in) {  // 32 bytes of half c / 4: chunks 2 (c % 4) and the next
+        uint8_t* const row = dst + (c >> 2) * (S::N * 128) + (rr >> 3) * 1024 + (rr & 7) * 128;
+        const int c0 = (c & 3) * 2;
+        *reinterpret_cast<uint4*>(row + ((c0 ^ (rr & 7)) << 4)) = x[0];
+        *reinterpret_cast<uint4*>(row + (((c0 + 1) ^ (rr & 7)) << 4)) = x[1];
+        if (c == 0) sm.cq[qs * 64 + r] = p.s.scale_log2;
+      }
+    } else {
+      float f[16];
+      uint32_t top = 0;  // the row's largest magnitude, as bits (above every finite one for inf and NaN)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 a = unpack2<BF>(w[i]);
+        f[2 * i] = a.x;
+        f[2 * i + 1] = a.y;
+        top = max(top, max(__float_as_uint(a.x) & 0x7fffffffu, __float_as_uint(a.y) & 0x7fffffffu));
+      }
+#pragma unroll
+      for (int off = 1; off < 8; off <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+      // 2^e brings the largest magnitude into [128, 256); a row with an infinity or NaN is NaN
+      const bool finite = top < 0x7f800000u;
+      const int e = top > 0 ? max(-110, min(110, 134 - (int)(top >> 23))) : 0;
+      const float sc = __uint_as_float((uint32_t)(127 + e) << 23);
+      uint32_t part[3][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float y[4] = {f[4 * i] * sc, f[4 * i + 1] * sc, f[4 * i + 2] * sc, f[4 * i + 3] * sc};
+        uint32_t o[3];
+        split4<S::PARTS>(y, o);
+#pragma unroll
+        for (int k = 0; k < S::PARTS; ++k) part[k][i] = finite ? o[k] : 0x7f7f7f7fu;
+      }
+      if (in) {
+#pragma unroll
+        for (int k = 0; k < S::PARTS; ++k) {
+          const int n = k * S::ROWS + rr;
+          *reinterpret_cast<uint4*>(dst + (n >> 3) * 1024 + (n & 7) * 128 + ((c ^ (n & 7)) << 4)) =
+              make_uint4(part[k][0], part[k][1], part[k][2], part[k][3]);
+        }
+        if (c == 0) sm.cq[qs * 64 + r] = p.s.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23);
+      }
+    }
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if ((tid & 31) == 0) mbar_arrive(smem_u32(sm.q_ready + qs));
+}
+
+// Rows [c, c + CH) of a score slot, its parts joined.
+template <class S>
+__device__ __forceinline__ void read_scores(uint32_t slot, int c, float (&s)[S::CH]) {
+  if constexpr (S::F8) {
+    uint32_t raw[3][S::CH];
+#pragma unroll
+    for (int i = 0; i < S::PARTS; ++i) tmem_ld(slot + i * S::ROWS + c, raw[i]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int r = 0; r < S::CH; ++r) {
+      float x = __uint_as_float(raw[S::PARTS - 1][r]);
+#pragma unroll
+      for (int i = S::PARTS - 2; i >= 0; --i) x = fmaf(x, 1.f / 32.f, __uint_as_float(raw[i][r]));
+      s[r] = x;
+    }
   } else {
-    return unpack2<BF>(static_cast<const uint16_t*>(cache)[at]).x;
+    uint32_t raw[S::CH];
+    tmem_ld(slot + c, raw);
+    tmem_wait_ld();
+#pragma unroll
+    for (int r = 0; r < S::CH; ++r) s[r] = __uint_as_float(raw[r]);
   }
 }
 
-// Scores of tile [t0, t0 + 32) of rows `rows` into sm.s (unseen: -inf); V too for attention.
-template <bool BF, int kElem, bool kWithV>
-__device__ void load_tile(const ScaledParams& p, ScaledSmem& sm, int b, int h, int t0, int len, int mlen) {
-  const int rows = kGroup * p.q_len;
-  for (int i = threadIdx.x; i < kTile * kHeadDim; i += kScaledThreads) {
-    const int t = t0 + i / kHeadDim, d = i % kHeadDim;
-    float k = 0.f, v = 0.f;
-    if (t < len) {
-      int page = __ldg(p.block_tables + (size_t)b * p.max_pages + t / kPageSize);
-      if (page < 0 || page >= p.num_pages) {
-        raise(p.status, 8u);
-        page = 0;
+// Sum of each row over the warp's lanes: lane l gets row l / (32 / ROWS).
+template <int ROWS>
+__device__ __forceinline__ float sum_rows(float (&v)[ROWS]) {
+  const int lane = threadIdx.x & 31;
+  int n = ROWS;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    if (n > 1) {
+      n /= 2;
+      const bool upper = lane & off;
+#pragma unroll
+      for (int i = 0; i < ROWS / 2; ++i) {
+        if (i < n) {
+          const float mine = upper ? v[i + n] : v[i], other = upper ? v[i] : v[i + n];
+          v[i] = mine + __shfl_xor_sync(0xffffffffu, other, off);
+        }
       }
-      const int slot = t % kPageSize;
-      const size_t at = (size_t)page * p.page_stride +
-                        (p.hnd ? ((size_t)h * kPageSize + slot) : ((size_t)slot * p.hkv + h)) * kHeadDim + d;
-      const size_t sc = (size_t)page * p.scale_stride + h;
-      k = cached<BF, kElem>(p.k_cache, at, kElem == 1 ? p.k_scales[sc] : 1.f);
-      if (kWithV) v = cached<BF, kElem>(p.v_cache, at, p.v_scales[sc]);
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
     }
-    sm.k[i / kHeadDim][d] = k;
-    if (kWithV) sm.v[i / kHeadDim][d] = v;
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows * kTile; i += kScaledThreads) {
-    const int r = i / kTile, c = i % kTile, t = t0 + c;
-    float x = 0.f;
-    for (int d = 0; d < kHeadDim; ++d) x = fmaf(sm.q[r][d], sm.k[c][d], x);
-    sm.s[r][c] = (t < len && t < mlen - p.q_len + (r >> 2) + 1) ? x * p.scale_log2 : -INFINITY;
-  }
-  __syncthreads();
+  return v[0];
 }
 
-template <bool BF>
-__device__ void load_q(const ScaledParams& p, ScaledSmem& sm, int b, int h) {
-  for (int i = threadIdx.x; i < kGroup * p.q_len * kHeadDim; i += kScaledThreads) {
-    const int r = i / kHeadDim, d = i % kHeadDim;
-    const size_t row = (size_t)(b * p.q_len + (r >> 2)) * p.hq + h * kGroup + (r & 3);
-    sm.q[r][d] = unpack2<BF>(static_cast<const uint16_t*>(p.q)[row * kHeadDim + d]).x;
-  }
+// What the softmax threads know of a piece.
+struct Piece {
+  int len, first;  // tokens held; tokens that draft row 0 sees (its limit: mask - q_len + 1)
+};
+
+__device__ __forceinline__ Piece piece_of(const SplitKvParams& p, const SegWalk& w) {
+  const int raw = __ldg(p.seq_lens + w.b);
+  const int whole = p.mask_lens ? __ldg(p.mask_lens + w.b) : raw;
+  return Piece{min(raw, w.pages * kPageSize), whole - p.q_len + 1};
 }
 
-template <bool BF>
-__global__ void __launch_bounds__(kScaledThreads) sqa_scaled_attention_kernel(const ScaledParams p) {
-  extern __shared__ uint8_t raw[];
-  ScaledSmem& sm = *reinterpret_cast<ScaledSmem*>(raw);
-  grid_dependency_wait();
-  allow_dependent_launch();
-  const int b = blockIdx.x / p.hkv, h = blockIdx.x % p.hkv;
-  const int rows = kGroup * p.q_len, tid = threadIdx.x;
-  const int raw_len = __ldg(p.seq_lens + b);
-  const int len = min(max(raw_len, 0), p.max_pages * kPageSize);
-  const int mlen = p.mask_lens ? __ldg(p.mask_lens + b) : raw_len;
-  if (tid == 0) {
-    if (raw_len > p.max_pages * kPageSize) raise(p.status, 2u);
-    if (p.out != nullptr && raw_len < p.q_len) raise(p.status, 4u);
-  }
-  load_q<BF>(p, sm, b, h);
-  for (int r = tid; r < rows; r += kScaledThreads) {
-    sm.m[r] = -INFINITY;
-    sm.l[r] = 0.f;
-  }
-  const int d = tid % kHeadDim, r0 = tid / kHeadDim;
-  float acc[kGroup * 16 / 2];
-  for (int i = 0; i < kGroup * 16 / 2; ++i) acc[i] = 0.f;
-  __syncthreads();
-  for (int t0 = 0; t0 < len; t0 += kTile) {
-    load_tile<BF, 1, true>(p, sm, b, h, t0, len, mlen);
+template <class S, bool BF>
+__device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSmem& sm, uint32_t tmem, int tiles,
+                       volatile int* abort) {
+  constexpr int ROWS = S::ROWS, G = S::G, CH = S::CH;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;  // tid: token of a block, dimension of O
+  const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+  const int rows = kGroup * p.s.q_len;
+  int u = 0, blk = 0, pc = 0;
+  for_pieces(p.s, sch, [&](const SegWalk& w, int unit, int n) {
+    const int seg = w.b * p.s.hkv + w.h;
+    const int seg_end = w.seg_start + w.pages;
+    const bool whole = unit == w.seg_start && seg_end <= sch.end;
+    const Piece piece = piece_of(p.s, w);
+    if (pc == 0) write_q<S, BF>(p, sm, w.b, w.h, 0);
+    if (seg_end < sch.end) {  // Q of the next piece, whose slot the piece before this one is done with
+      SegWalk nw = w;
+      next_segment(p.s, nw);
+      write_q<S, BF>(p, sm, nw.b, nw.h, (pc + 1) & 1);
+    }
+    if (tid < G * ROWS) sm.base[tid] = kNoBase;
+    softmax_sync();
+    const float* const cq = sm.cq + (pc & 1) * 64;
+    float l[G][ROWS];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) l[g][r] = 0.f;
+    int nan_from = 0x7fffffff;  // first draft token whose V is NaN in dimension tid
+
+    const int nblk = blocks_of(n);
+    for (int k = 0; k < nblk; ++k, ++blk) {
+      const int np = min(kBlockPages, n - k * kBlockPages);
+      const int tok0 = (w.pg + k * kBlockPages) * kPageSize;
+      const int tok = tok0 + tid;
+      const int e = blk % kMetaSlots;
+      mbar_wait_bounded(smem_u32(sm.m_full + e), (uint32_t)(blk / kMetaSlots) & 1u, abort, p.s.status, 3, blk);
+      const float4 meta = sm.meta[e * kBlockPages + (tid >> 4)];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(sm.m_empty + e));
+      // vs = f * 2^lv
+      const int lv = max(-kMaxLv, min(kMaxLv, (int)(__float_as_uint(meta.y) >> 23) - 127));
+      const float inv_lv = __uint_as_float((uint32_t)(127 - lv) << 23);
+      const float f = meta.y * inv_lv;
+      const float flv = (float)lv;
+      const bool masked = np < kBlockPages || tok0 + kBlock > piece.first || tok0 + kBlock > piece.len;
+      // draft qi sees the token iff late < qi (every draft when negative)
+      const int late = (tid < np * kPageSize && tok < piece.len) ? tok - piece.first : 0x7fffffff;
+      const int t1 = blk * 2 + 1;  // V's tile
+
+      if (masked) {
+        // V rows behind the sequence and of absent pages: zero (they may hold NaN); draft tokens'
+        // NaN: zero, and remembered by the dimension's thread
+        mbar_wait_bounded(smem_u32(sm.full + t1 % tiles), (uint32_t)(t1 / tiles) & 1u, abort, p.s.status, 9, blk);
+        uint8_t* const v = sm.ring + (size_t)(t1 % tiles) * kTileBytes;
+        const int held = min(np * kPageSize, max(piece.len - tok0, 0));
+        const int read = (np + 1) / 2 * 32;  // rows that the product reads
+        for (int t = max(0, piece.first - tok0); t < held; ++t) {
+          uint8_t* const at = v + t * 128 + (((tid >> 4) ^ (t & 7)) << 4) + (tid & 15);
+          if ((*at & 0x7f) == 0x7f) {
+            nan_from = min(nan_from, tok0 + t);
+            *at = 0;
+          }
+        }
+        for (int c = held * 8 + tid; c < read * 8; c += 128)
+          *reinterpret_cast<uint4*>(v + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_smem();
+      }
+
+#pragma unroll
+      for (int g = 0; g < G; ++g, ++u) {
+        mbar_wait_bounded(smem_u32(sm.s_full + u % S::NS), (uint32_t)(u / S::NS) & 1u, abort, p.s.status, 10, u);
+        tc_fence_after();
+        const uint32_t slot = lanes + G * S::OCOLS + (u % S::NS) * S::STRIDE;
+        float y[ROWS];
+        float over = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < ROWS; c += CH) {
+          float s[CH];
+          read_scores<S>(slot, c, s);
+#pragma unroll
+          for (int r = 0; r < CH; r += 4) {
+            const float4 q4 = *reinterpret_cast<const float4*>(cq + g * ROWS + c + r);
+            const float4 b4 = *reinterpret_cast<const float4*>(sm.base + g * ROWS + c + r);
+            const float qq[4] = {q4.x, q4.y, q4.z, q4.w}, bb[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float x = fmaf(s[r + i], meta.x * qq[i], flv);
+              if (masked && late >= (g * ROWS + c + r + i) >> 2) x = -INFINITY;
+              y[c + r + i] = x;
+              over = fmaxf(over, x - bb[i]);
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(sm.s_empty + u % S::NS));
+        // P's buffer is free once the product before the last is done
+        if (u >= 2)
+          mbar_wait_bounded(smem_u32(sm.p_done + (u & 1)), (uint32_t)((u >> 1) - 1) & 1u, abort, p.s.status, 11, u);
+        if (softmax_any(over > kRaise)) {  // raise bases (rare after a piece's first blocks)
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r) {
+            const int m = __reduce_max_sync(0xffffffffu, float_order(y[r] == y[r] ? y[r] : -INFINITY));
+            if (lane == r) sm.wmax[warp * 64 + g * ROWS + r] = order_float(m);
+          }
+          softmax_sync();
+          if (tid < ROWS) {
+            const int r = g * ROWS + tid;
+            const float m = fmaxf(fmaxf(sm.wmax[r], sm.wmax[64 + r]), fmaxf(sm.wmax[128 + r], sm.wmax[192 + r]));
+            const float old = sm.base[r];
+            const bool up = m > old + kRaise;
+            sm.alpha[r] = up ? ex2(old - (m - kHead)) : 1.f;
+            if (up) sm.base[r] = m - kHead;
+          }
+          softmax_sync();
+          if (k > 0) {
+            // O must be stable: the group's last product is done (G = 2: waited for above)
+            if (G == 1)
+              mbar_wait_bounded(smem_u32(sm.p_done + ((u - 1) & 1)), (uint32_t)((u - 1) >> 1) & 1u, abort, p.s.status, 12, u);
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < ROWS; c += CH) {
+              float a[CH];
+#pragma unroll
+              for (int r = 0; r < CH; ++r) {
+                a[r] = sm.alpha[g * ROWS + c + r];
+                l[g][c + r] *= a[r];
+              }
+#pragma unroll
+              for (int i = 0; i < S::PARTS; ++i) {
+                uint32_t o[CH];
+                tmem_ld(lanes + g * 128 + i * ROWS + c, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int r = 0; r < CH; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * a[r]);
+                tmem_st(lanes + g * 128 + i * ROWS + c, o);
+              }
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          }
+        }
+        // P: token tid's operand row of 128 bytes, part i of row r in byte i * ROWS + r
+        uint8_t* const prow = sm.p + (u & 1) * kPBytes + (tid >> 3) * 1024 + (tid & 7) * 128;
+#pragma unroll
+        for (int c = 0; c < ROWS; c += CH) {
+          uint32_t part[3][CH / 4];
+#pragma unroll
+          for (int r = 0; r < CH; r += 4) {
+            const float4 b4 = *reinterpret_cast<const float4*>(sm.base + g * ROWS + c + r);
+            const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float ee = ex2(y[c + r + i] - bb[i]);
+              l[g][c + r + i] = fmaf(ee, inv_lv, l[g][c + r + i]);
+              x[i] = ee * f;
+            }
+            uint32_t o[3];
+            split4<S::PARTS>(x, o);
+#pragma unroll
+            for (int i = 0; i < S::PARTS; ++i) part[i][r / 4] = o[i];
+          }
+#pragma unroll
+          for (int i = 0; i < S::PARTS; ++i) {
+            const int byte = i * ROWS + c;
+            uint8_t* const at = prow + (((byte >> 4) ^ (tid & 7)) << 4) + (byte & 15);
+            if constexpr (CH == 16)
+              *reinterpret_cast<uint4*>(at) = make_uint4(part[i][0], part[i][1], part[i][2], part[i][3]);
+            else
+              *reinterpret_cast<uint2*>(at) = make_uint2(part[i][0], part[i][1]);
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(sm.p_full + (u & 1)));
+      }
+    }
+
+    // ---- epilogue: denominators, then each dimension's thread joins the parts of its rows
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float total = sum_rows<ROWS>(l[g]);
+      if (lane % (32 / ROWS) == 0) sm.wmax[warp * 64 + g * ROWS + lane / (32 / ROWS)] = total;
+    }
+    softmax_sync();
+    const int slot = (int)blockIdx.x + seg;  // workspace piece
     if (tid < rows) {
-      float m = sm.m[tid];
-      for (int c = 0; c < kTile; ++c) m = fmaxf(m, sm.s[tid][c]);
-      const float base = m == -INFINITY ? 0.f : m;
-      float l = sm.l[tid] * ex2(sm.m[tid] - base);
-      sm.alpha[tid] = ex2(sm.m[tid] - base);
-      for (int c = 0; c < kTile; ++c) {
-        const float e = ex2(sm.s[tid][c] - base);
-        sm.s[tid][c] = e;
-        l += e;
-      }
-      sm.m[tid] = m;
-      sm.l[tid] = l;
+      const float total = (sm.wmax[tid] + sm.wmax[64 + tid]) + (sm.wmax[128 + tid] + sm.wmax[192 + tid]);
+      sm.alpha[tid] = total > 0.f ? p.s.out_scale / total : total;  // 0 for a row without tokens, NaN for a NaN row
+      const float lse = total == 0.f ? -INFINITY : (sm.base[tid] + __log2f(total)) * kLn2f;
+      const size_t out_row = (size_t)(w.b * p.s.q_len + (tid >> 2)) * p.s.hq + w.h * kGroup + (tid & 3);
+      if (!whole) p.s.ws_lse[(size_t)slot * p.s.rows_pad + tid] = lse;
+      else if (p.s.out_lse) p.s.out_lse[out_row] = lse;
     }
-    __syncthreads();
+    softmax_sync();
 #pragma unroll
-    for (int i = 0; i < kGroup * 16 / 2; ++i) {
-      const int r = r0 + 2 * i;
-      if (r < rows) {
-        float a = acc[i] * sm.alpha[r];
-        for (int c = 0; c < kTile; ++c)
-          if (sm.s[r][c] != 0.f) a = fmaf(sm.s[r][c], sm.v[c][d], a);
-        acc[i] = a;
+    for (int g = 0; g < G; ++g) {  // the last products of both groups
+      const int last = u - G + g;
+      mbar_wait_bounded(smem_u32(sm.p_done + (last & 1)), (uint32_t)(last >> 1) & 1u, abort, p.s.status, 13, last);
+    }
+    tc_fence_after();
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+#pragma unroll
+      for (int c = 0; c < ROWS; c += CH) {
+        if (g * ROWS + c >= rows) break;
+        float o[CH];
+        uint32_t raw[3][CH];
+#pragma unroll
+        for (int i = 0; i < S::PARTS; ++i) tmem_ld(lanes + g * 128 + i * ROWS + c, raw[i]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int r = 0; r < CH; ++r) {
+          float x = __uint_as_float(raw[S::PARTS - 1][r]);
+#pragma unroll
+          for (int i = S::PARTS - 2; i >= 0; --i) x = fmaf(x, 1.f / 32.f, __uint_as_float(raw[i][r]));
+          const int row = g * ROWS + c + r;
+          const float inv = sm.alpha[row];
+          x = inv == 0.f ? 0.f : x * inv;
+          // draft row / 4 sees the tokens before min(len, first + row / 4)
+          if (nan_from < piece.first + (row >> 2)) x = __int_as_float(0x7fffffff);
+          o[r] = x;
+        }
+#pragma unroll
+        for (int r = 0; r < CH; ++r) {
+          const int row = g * ROWS + c + r;
+          if (row < rows) {
+            const size_t out_row = (size_t)(w.b * p.s.q_len + (row >> 2)) * p.s.hq + w.h * kGroup + (row & 3);
+            if (!whole) p.s.ws_o[((size_t)slot * p.s.rows_pad + row) * kHeadDim + tid] = o[r];
+            else if (p.s.out_o) p.s.out_o[out_row * kHeadDim + tid] = o[r];
+            else reinterpret_cast<uint16_t*>(p.s.out)[out_row * kHeadDim + tid] = (uint16_t)(pack2<BF>(o[r], 0.f) & 0xffffu);
+          }
+        }
       }
     }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < kGroup * 16 / 2; ++i) {
-    const int r = r0 + 2 * i;
-    if (r < rows) {
-      const float l = sm.l[r];
-      const float o = l > 0.f || l != l ? acc[i] * p.out_scale / l : 0.f;
-      const size_t row = (size_t)(b * p.q_len + (r >> 2)) * p.hq + h * kGroup + (r & 3);
-      if (p.out != nullptr) static_cast<uint16_t*>(p.out)[row * kHeadDim + d] = (uint16_t)(pack2<BF>(o, 0.f) & 0xffffu);
-      if (p.out_o != nullptr) p.out_o[row * kHeadDim + d] = o;
-      if (p.out_lse != nullptr && d == 0)
-        p.out_lse[row] = l > 0.f ? (sm.m[r] + log2f(l)) * 0.6931471805599453f : (l != l ? l : -INFINITY);
-    }
-  }
+    tc_fence_before();  // O is read before the next piece's first product overwrites it
+    softmax_sync();     // and so are base and alpha
+    ++pc;
+  });
 }
 
-template <bool BF, int kElem>
-__global__ void __launch_bounds__(kScaledThreads) sqa_weights_kernel(const ScaledParams p) {
-  extern __shared__ uint8_t raw[];
-  ScaledSmem& sm = *reinterpret_cast<ScaledSmem*>(raw);
+template <class S, bool BF>
+__device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const TcSmem& sm, uint32_t tmem, volatile int* abort) {
+  constexpr int ROWS = S::ROWS, G = S::G, CH = S::CH;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+  const int rows = kGroup * p.s.q_len;
+  int u = 0, blk = 0, pc = 0;
+  for_pieces(p.s, sch, [&](const SegWalk& w, int, int n) {
+    const int seg_end = w.seg_start + w.pages;
+    const Piece piece = piece_of(p.s, w);
+    const int fresh = __ldg(p.s.seq_lens + w.b) - p.s.q_len;  // tokens from here on are new
+    if (pc == 0) write_q<S, BF>(p, sm, w.b, w.h, 0);
+    if (seg_end < sch.end) {
+      SegWalk nw = w;
+      next_segment(p.s, nw);
+      write_q<S, BF>(p, sm, nw.b, nw.h, (pc + 1) & 1);
+    }
+    if (tid < G * ROWS) {  // -lse in base 2; -inf (weight 0) for padding and rows without tokens
+      float x = -INFINITY;
+      if (tid < rows) {
+        const float v = p.lse[(size_t)(w.b * p.s.q_len + (tid >> 2)) * p.s.hq + w.h * kGroup + (tid & 3)];
+        if (v != -INFINITY) x = -v * 1.4426950408889634f;
+      }
+      sm.base[tid] = x;
+    }
+    softmax_sync();
+    const float* const cq = sm.cq + (pc & 1) * 64;
+    const int nblk = blocks_of(n);
+    for (int k = 0; k < nblk; ++k, ++blk) {
+      const int np = min(kBlockPages, n - k * kBlockPages);
+      const int tok0 = (w.pg + k * kBlockPages) * kPageSize;
+      const int tok = tok0 + tid;
+      const int e = blk % kMetaSlots;
+      mbar_wait_bounded(smem_u32(sm.m_full + e), (uint32_t)(blk / kMetaSlots) & 1u, abort, p.s.status, 3, blk);
+      const float4 meta = sm.meta[e * kBlockPages + (tid >> 4)];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(sm.m_empty + e));
+      const int id = __float_as_int(meta.z);
+      const bool held = tid < np * kPageSize && tok < piece.len;
+      float* const at = p.scores + ((size_t)max(id, 0) * p.s.hkv + w.h) * kPageSize + (tid & 15);
+      const float old = (held && id >= 0 && tok < fresh) ? *at : 0.f;  // in flight during the score product
+      const bool masked = np < kBlockPages || tok0 + kBlock > piece.first || tok0 + kBlock > piece.len;
+      const int late = held ? tok - piece.first : 0x7fffffff;
+      float sum = 0.f;
+#pragma unroll
+      for (int g = 0; g < G; ++g, ++u) {
+        mbar_wait_bounded(smem_u32(sm.s_full + u % S::NS), (uint32_t)(u / S::NS) & 1u, abort, p.s.status, 10, u);
+        tc_fence_after();
+        const uint32_t slot = lanes + (u % S::NS) * S::STRIDE;
+#pragma unroll
+        for (int c = 0; c < ROWS; c += CH) {
+          float s[CH];
+          read_scores<S>(slot, c, s);
+#pragma unroll
+          for (int r = 0; r < CH; r += 4) {
+            const float4 q4 = *reinterpret_cast<const float4*>(cq + g * ROWS + c + r);
+            const float4 b4 = *reinterpret_cast<const float4*>(sm.base + g * ROWS + c + r);
+            const float qq[4] = {q4.x, q4.y, q4.z, q4.w}, bb[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float x = fmaf(s[r + i], meta.x * qq[i], bb[i]);
+              if ((masked && late >= (g * ROWS + c + r + i) >> 2) || bb[i] == -INFINITY) x = -INFINITY;
+              sum += ex2(x);
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(sm.s_empty + u % S::NS));
+      }
+      if (held && id >= 0) *at = old + sum;
+    }
+    softmax_sync();  // base has been read
+    ++pc;
+  });
+}
+
+template <class S, bool BF>
+__global__ void __launch_bounds__(kScaledTcThreads, 1)
+    sqa_scaled_tc_kernel(const ScaledTcParams p, const __grid_constant__ CUtensorMap tm_k,
+                         const __grid_constant__ CUtensorMap tm_v) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int tiles = p.s.num_stages;
+  const TcSmem sm = carve<S>(smem, tiles);
+  const int warp = threadIdx.x >> 5;
+  constexpr int kScoreWarp = 4, kValueWarp = 5, kProducerWarp = 6, kMetaWarp = 7;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < tiles; ++i) {
+      mbar_init(smem_u32(sm.full + i), 1);
+      mbar_init(smem_u32(sm.empty + i), 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(smem_u32(sm.s_full + i), 1);
+      mbar_init(smem_u32(sm.s_empty + i), 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(sm.p_full + i), 4);
+      mbar_init(smem_u32(sm.p_done + i), 1);
+      mbar_init(smem_u32(sm.q_ready + i), 4);
+    }
+    for (int i = 0; i < kMetaSlots; ++i) {
+      mbar_init(smem_u32(sm.m_full + i), 1);
+      mbar_init(smem_u32(sm.m_empty + i), 4);
+    }
+    mbar_init(smem_u32(sm.done), S::ATTEND ? 2 : 1);  // one commit from each issuer
+    fence_mbar_init();
+  }
+  if (warp == kProducerWarp && (threadIdx.x & 31) == 0) {
+    prefetch_tensormap(&tm_k);
+    if (S::ATTEND) prefetch_tensormap(&tm_v);
+  }
+  // The value issuer has nothing to do before the first P: it prefetches the CTA's first
+  // pages into L2 before the dependency wait (hints only).
+  if (warp == kValueWarp) prefetch_start<S::F8>(p.s, &tm_k, &tm_v, tiles / S::TILES * kBlockPages);
   grid_dependency_wait();
   allow_dependent_launch();
-  const int b = blockIdx.x / p.hkv, h = blockIdx.x % p.hkv;
-  const int rows = kGroup * p.q_len, tid = threadIdx.x;
-  const int raw_len = __ldg(p.seq_lens + b);
-  const int len = min(max(raw_len, 0), p.max_pages * kPageSize);
-  const int mlen = p.mask_lens ? __ldg(p.mask_lens + b) : raw_len;
-  if (tid == 0) {
-    if (raw_len > p.max_pages * kPageSize) raise(p.status, 2u);
-    if (raw_len < p.q_len) raise(p.status, 4u);
+  if (warp == kScoreWarp) {
+    tmem_alloc(smem_u32(sm.tmem_base), 512);
+    tmem_relinquish();
   }
-  load_q<BF>(p, sm, b, h);
-  for (int r = tid; r < rows; r += kScaledThreads)
-    sm.m[r] = p.lse[(size_t)(b * p.q_len + (r >> 2)) * p.hq + h * kGroup + (r & 3)] * 1.4426950408889634f;
+  if (warp == 0) build_schedule(p.s, sm.sch);
+  tc_fence_before();
   __syncthreads();
-  for (int t0 = 0; t0 < len; t0 += kTile) {
-    load_tile<BF, kElem, false>(p, sm, b, h, t0, len, mlen);
-    const int t = t0 + tid;
-    if (tid < kTile && t < len) {
-      float w = 0.f;
-      for (int r = 0; r < rows; ++r)
-        if (sm.m[r] != -INFINITY) w += ex2(sm.s[r][tid] - sm.m[r]);
-      const int page = __ldg(p.block_tables + (size_t)b * p.max_pages + t / kPageSize);
-      if (page >= 0 && page < p.num_pages) {
-        float* const at = p.scores + ((size_t)page * p.hkv + h) * kPageSize + t % kPageSize;
-        *at = t >= raw_len - p.q_len ? w : *at + w;
-      }
-    }
-    __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *sm.tmem_base;
+  const Schedule sch = *sm.sch;
+  volatile int* abort = &sm.sch->abort;
+  if (warp == kProducerWarp) {
+    produce<S>(p, sch, &tm_k, &tm_v, sm, tiles, abort);
+  } else if (warp == kMetaWarp) {
+    page_meta<S>(p, sch, sm, abort);
+  } else if (warp == kScoreWarp) {
+    issue_scores<S, BF>(p, sch, sm, tmem, tiles, abort);
+  } else if (warp == kValueWarp) {
+    if constexpr (S::ATTEND) issue_values<S>(p, sch, sm, tmem, tiles, abort);
+  } else {
+    if constexpr (S::ATTEND) attend<S, BF>(p, sch, sm, tmem, tiles, abort);
+    else weigh<S, BF>(p, sch, sm, tmem, abort);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kScoreWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
-cudaError_t launch(void (*kernel)(const ScaledParams), const ScaledParams& p, cudaStream_t stream) {
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(ScaledSmem));
+// ------------------------------------------------------------------ merge of split segments
+// As sqa_segment_merge_kernel (one warp a row, 4 rows a CTA), with a NaN part making the row NaN.
+__global__ void __launch_bounds__(128) sqa_scaled_merge_kernel(const MergeParams p) {
+  allow_dependent_launch();
+  const int s = blockIdx.x;
+  const int b = s / p.hkv, h = s - b * p.hkv;
+  const int2 info = p.seg_split
+                        ? aligned_segment_pieces(p.seq_lens, p.max_pages, p.hkv, p.seg_split, b, h)
+                        : segment_pieces(p.seq_lens, p.batch, p.max_pages, p.hkv, p.seg_cost, p.split_grid, b, h);
+  grid_dependency_wait();
+  const int row = blockIdx.y * 4 + (threadIdx.x >> 5);
+  if (row >= kGroup * p.q_len || info.y == 1) return;  // one piece: written by the split kernel
+  const int lane = threadIdx.x & 31;
+  const size_t out_row = (size_t)(b * p.q_len + (row >> 2)) * p.hq + h * kGroup + (row & 3);
+  __half* out = p.out ? p.out + out_row * kHeadDim : nullptr;
+  float* out_o = p.out_o ? p.out_o + out_row * kHeadDim : nullptr;
+  float* out_lse = p.out_lse ? p.out_lse + out_row : nullptr;
+  const size_t first = (size_t)info.x * p.piece_rows + row;
+  bool nan = false;
+  for (int i = lane; i < info.y; i += 32) {
+    const float l = __ldg(p.parts_lse + first + (size_t)i * p.piece_rows);
+    nan |= l != l;
+  }
+  if (info.y == 0) {  // no page: nothing is visible
+    if (out) reinterpret_cast<uint2*>(out)[lane] = make_uint2(0u, 0u);
+    if (out_o) reinterpret_cast<float4*>(out_o)[lane] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (out_lse && lane == 0) *out_lse = -INFINITY;
+    return;
+  }
+  merge_row<false>(p.parts_o + first * kHeadDim, (size_t)p.piece_rows * kHeadDim, p.parts_lse + first,
+                   (size_t)p.piece_rows, info.y, out, out_o, out_lse, p.bf16 != 0);
+  if (__any_sync(0xffffffffu, nan)) {
+    const float x = __int_as_float(0x7fffffff);
+    if (out) reinterpret_cast<uint2*>(out)[lane] = make_uint2(0x7fff7fffu, 0x7fff7fffu);  // NaN in fp16 and bf16
+    if (out_o) reinterpret_cast<float4*>(out_o)[lane] = make_float4(x, x, x, x);
+    if (out_lse && lane == 0) *out_lse = x;
+  }
+}
+
+// ------------------------------------------------------------------ launch
+constexpr int kMaxSmem = 227 * 1024;
+
+template <class S>
+int tiles_that_fit() {
+  const int n = (kMaxSmem - fixed_smem<S>()) / (kTileBytes + 16);
+  return n < 16 ? n / S::TILES * S::TILES : 16;
+}
+
+template <class S, bool BF>
+cudaError_t launch_shape(ScaledTcParams& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, int grid,
+                         cudaStream_t stream) {
+  auto kernel = sqa_scaled_tc_kernel<S, BF>;
+  p.s.num_stages = tiles_that_fit<S>();
+  const int smem = fixed_smem<S>() + p.s.num_stages * (kTileBytes + 16);
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (err != cudaSuccess) return err;
-  kernel<<<p.batch * p.hkv, kScaledThreads, sizeof(ScaledSmem), stream>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kScaledTcThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  err = cudaLaunchKernelEx(&cfg, kernel, p, tm_k, tm_v);
+  return err != cudaSuccess ? err : cudaGetLastError();
+}
+
+template <int PARTS, bool ATTEND, bool BF>
+cudaError_t launch_rows(ScaledTcParams& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, int grid,
+                        cudaStream_t stream) {
+  const int rows = kGroup * p.s.q_len;
+  if (rows <= 8) return launch_shape<Shape<PARTS, 8, 1, ATTEND>, BF>(p, tm_k, tm_v, grid, stream);
+  if (rows <= 16) return launch_shape<Shape<PARTS, 16, 1, ATTEND>, BF>(p, tm_k, tm_v, grid, stream);
+  if (rows <= 32) return launch_shape<Shape<PARTS, 32, 1, ATTEND>, BF>(p, tm_k, tm_v, grid, stream);
+  return launch_shape<Shape<PARTS, 32, 2, ATTEND>, BF>(p, tm_k, tm_v, grid, stream);
+}
+
+ScaledTcParams tc_params(const ScaledParams& p) {
+  ScaledTcParams t = {};
+  t.s.q = static_cast<const __half*>(p.q);
+  t.s.block_tables = p.block_tables;
+  t.s.seq_lens = p.seq_lens;
+  t.s.mask_lens = p.mask_lens;
+  t.s.out = static_cast<__half*>(p.out);
+  t.s.out_o = p.out_o;
+  t.s.out_lse = p.out_lse;
+  t.s.ws_o = p.ws_o;
+  t.s.ws_lse = p.ws_lse;
+  t.s.status = p.status;
+  t.s.batch = p.batch;
+  t.s.q_len = p.q_len;
+  t.s.hq = p.hq;
+  t.s.hkv = p.hkv;
+  t.s.max_pages = p.max_pages;
+  t.s.num_pages = p.num_pages;
+  t.s.rows_pad = p.rows_pad;
+  t.s.scale_log2 = p.scale_log2;
+  t.s.bf16 = p.bf16;
+  t.s.hnd = p.hnd;
+  t.s.out_scale = p.out_scale;
+  t.s.seg_cost = p.seg_cost;
+  t.s.seg_split = p.seg_split;
+  t.k_scales = p.k_scales;
+  t.v_scales = p.v_scales;
+  t.scale_stride = p.scale_stride;
+  t.lse = p.lse;
+  t.scores = p.scores;
+  return t;
 }
 
 }  // namespace
 
-cudaError_t launch_scaled_attention(const ScaledParams& p, cudaStream_t stream) {
-  return launch(p.bf16 ? sqa_scaled_attention_kernel<true> : sqa_scaled_attention_kernel<false>, p, stream);
+cudaError_t launch_scaled_attention(const ScaledParams& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
+                                    cudaStream_t stream) {
+  ScaledTcParams t = tc_params(p);
+  cudaError_t err = p.bf16 ? launch_rows<2, true, true>(t, tm_k, tm_v, p.grid, stream)
+                           : launch_rows<3, true, false>(t, tm_k, tm_v, p.grid, stream);
+  if (err != cudaSuccess) return err;
+  MergeParams m = {};
+  m.parts_o = p.ws_o;
+  m.parts_lse = p.ws_lse;
+  m.seq_lens = p.seq_lens;
+  m.out = static_cast<__half*>(p.out);
+  m.out_o = p.out_o;
+  m.out_lse = p.out_lse;
+  m.piece_rows = p.rows_pad;
+  m.batch = p.batch;
+  m.q_len = p.q_len;
+  m.hq = p.hq;
+  m.hkv = p.hkv;
+  m.max_pages = p.max_pages;
+  m.bf16 = p.bf16;
+  m.split_grid = p.grid;
+  m.seg_cost = p.seg_cost;
+  m.seg_split = p.seg_split;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.batch * p.hkv), (unsigned)p.q_len);  // 4 rows a CTA
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  err = cudaLaunchKernelEx(&cfg, sqa_scaled_merge_kernel, m);
+  return err != cudaSuccess ? err : cudaGetLastError();
 }
 
-cudaError_t launch_weights(const ScaledParams& p, cudaStream_t stream) {
+cudaError_t launch_weights(const ScaledParams& p, const CUtensorMap& tm_k, cudaStream_t stream) {
+  ScaledTcParams t = tc_params(p);
+  t.s.out = reinterpret_cast<__half*>(p.scores);  // only asked for being there: a length under q_len is reported
   if (p.k_scales != nullptr)
-    return launch(p.bf16 ? sqa_weights_kernel<true, 1> : sqa_weights_kernel<false, 1>, p, stream);
-  return launch(p.bf16 ? sqa_weights_kernel<true, 2> : sqa_weights_kernel<false, 2>, p, stream);
+    return p.bf16 ? launch_rows<2, false, true>(t, tm_k, tm_k, p.grid, stream)
+                  : launch_rows<3, false, false>(t, tm_k, tm_k, p.grid, stream);
+  return p.bf16 ? launch_rows<0, false, true>(t, tm_k, tm_k, p.grid, stream)
+                : launch_rows<0, false, false>(t, tm_k, tm_k, p.grid, stream);
 }
 
 }  // namespace sqa

@@ -110,17 +110,18 @@ def test_forward_scaled_refuses_scales_and_workspace(lib):
                                      (dict(kernel=1), 2), (dict(kv_dtype=0), 1), (dict(seq_lens=257), 1)])
 def test_accumulate_refuses(lib, kw, code):
     a = _args(**kw)
-    assert lib.sqa_accumulate_weights(ctypes.byref(a), 256, ctypes.byref(_scales()), 256, None, None) == code
+    assert lib.sqa_accumulate_weights(ctypes.byref(a), 256, ctypes.byref(_scales()), 256, 256, None) == code
 
 
 def test_accumulate_refuses_missing_arrays(lib):
     a = _args()
     s = ctypes.byref(_scales())
-    assert lib.sqa_accumulate_weights(ctypes.byref(a), None, s, 256, None, None) == 1
-    assert lib.sqa_accumulate_weights(ctypes.byref(a), 256, s, None, None, None) == 1
-    assert lib.sqa_accumulate_weights(ctypes.byref(a), 256, None, 256, None, None) == 1  # e4m3 without scales
+    assert lib.sqa_accumulate_weights(ctypes.byref(a), None, s, 256, 256, None) == 1
+    assert lib.sqa_accumulate_weights(ctypes.byref(a), 256, s, None, 256, None) == 1
+    assert lib.sqa_accumulate_weights(ctypes.byref(a), 256, s, 256, None, None) == 1  # no status word
+    assert lib.sqa_accumulate_weights(ctypes.byref(a), 256, None, 256, 256, None) == 1  # e4m3 without scales
     assert lib.sqa_accumulate_weights(ctypes.byref(a), 256, s, 256, 258, None) == 1
-    assert lib.sqa_accumulate_weights(None, 256, s, 256, None, None) == 1
+    assert lib.sqa_accumulate_weights(None, 256, s, 256, 256, None) == 1
 
 
 def _append_args(**kw):
@@ -183,7 +184,7 @@ def test_empty_batches_need_no_gpu(lib):
     s = ctypes.byref(_scales())
     assert lib.sqa_cache_append_scaled(ctypes.byref(_append_args(batch=0)), s, 0, None) == 0
     assert lib.sqa_cache_evict(ctypes.byref(_evict_args(batch=0)), None, None) == 0
-    assert lib.sqa_accumulate_weights(ctypes.byref(_args(batch=0)), 256, s, 256, None, None) == 0
+    assert lib.sqa_accumulate_weights(ctypes.byref(_args(batch=0)), 256, s, 256, 256, None) == 0
 
 
 def test_struct_layouts_match_the_header(tmp_path):

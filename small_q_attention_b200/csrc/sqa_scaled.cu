@@ -16,30 +16,37 @@
 // is bound by reading A) with their own fp32 accumulators, joined at read-out, so that a
 // low part has its own exponent range.  Two parts hold a bf16 query exactly (8 bits) and round P
 // to 2^-9, half of bf16's own rounding; three hold an fp16 query exactly (11 bits) and
-// round P to 2^-13.  A row of Q is first scaled by a power of two that brings its largest
-// magnitude into [128, 256); P is at most 2^8 by the rule below.
+// round P to 2^-13.  Q is first scaled by the power of two that brings the largest finite
+// magnitude of the head's rows into [128, 256); a row far below that keeps its bits down to 2^-15
+// (bf16) or 2^-20 (fp16) of the largest.  P is below 2^8 by the rule below.
 //
-// Softmax.  Per row a base b is kept; a score with its value scale, y = c ks (q . k) + lv with
-// vs = f * 2^lv, enters as E = 2^(y - b): P = f E, and the denominator sums 2^-lv E.  The value
-// scale is thus inside the running maximum, and P keeps its e4m3 range whatever the pages' value
-// scales are.  A base is raised, to the block's maximum - 4, only when some y exceeds it by more
-// than 8 (one barrier with an or-reduction a block finds that out); then l and the row's O columns
-// are rescaled.  Masked tokens and tokens behind the sequence have y = -inf by selection, so NaN in
+// Softmax.  A row keeps a base; a score with its value scale, y = c ks (q . k) + log2 vs, enters as
+// P = 2^(y - base), and the denominator sums P / vs.  The value scale is thus inside the running
+// maximum, and P keeps its e4m3 range whatever the pages' value scales are.  A base is set from the
+// first block and raised, to the block's maximum - 4, only when some y exceeds it by more than 7
+// (one barrier with an or-reduction a block finds that out); then l and the row's O columns are
+// rescaled.  Masked tokens and tokens behind the sequence have y = -inf by selection, so NaN in
 // their K does not matter; V rows behind the sequence are zeroed in shared memory, and a NaN in
 // the V of a draft token is zeroed and remembered, as only the rows that see the token get it.
 //
 // Weights.  w_t = sum over the rows of 2^(c ks (q . k) - lse): the same score product, summed over the
 // thread's columns and added to the token's score.  16-bit caches use kind::f16 and Q as it is.
 //
-// Warps: 0-3 softmax (one token a thread), 4 score products, 5 value products, 6 TMA
-// producer, 7 page scales.  Work is cut into CTA ranges by sqa_schedule.cuh; pieces of a split
+// Two softmax warpgroups, so that the scheduler always has a second warp to issue from: with
+// one, a block of 64 rows took 13.7k cycles at 0.22 instructions a cycle and scheduler.  They
+// take every other block (q_len <= 8; each with its own bases and O, joined at the end of a piece) or
+// one half of the rows each (q_len > 8).
+//
+// Warps: 0-7 softmax (one token a thread), 8 score products, 9 value products, 10 TMA
+// producer, 11 page scales.  Work is cut into CTA ranges by sqa_schedule.cuh; pieces of a split
 // segment are merged by sqa_scaled_merge_kernel.
 //
-// Pipelines (mbarriers; every wait bounded):
+// Pipelines (mbarriers; every wait bounded).  A unit u is a (block, row group); its stream u & 1
+// is the warpgroup that works on it.
 //   full / empty [tiles]     producer -> issuers; K and V tiles (16 KB) alternate in one ring,
 //                            each released by the commit of the product that read it
 //   s_full / s_empty [NS]    score issuer (commit) -> softmax -> score issuer
-//   p_full / p_done [2]      softmax -> value issuer (commit) -> softmax
+//   p_full / p_done [2]      softmax -> value issuer (commit) -> softmax, one P buffer a stream
 //   q_ready [2]              softmax (Q of a piece, one piece ahead) -> score issuer
 //   m_full / m_empty [8]     page scales of a block -> softmax
 #include "small_q_attention.h"
@@ -57,11 +64,11 @@ constexpr int kBlock = kBlockPages * kPageSize;  // 128 tokens: the M side
 constexpr int kTileBytes = kBlock * 128;         // K or V of a block (e4m3), or one half of 16-bit K
 constexpr int kMetaSlots = 8;
 constexpr int kPBytes = kBlock * 128;
-constexpr int kScaledTcThreads = 256;
-constexpr float kNoBase = -1e30f;                // a row that has seen nothing yet
-constexpr float kRaise = 8.f, kHead = 4.f;       // raise a base that a score exceeds by 2^8, to 2^4 under it
+constexpr int kSoftmaxThreads = 256;             // two warpgroups
+constexpr int kScaledTcThreads = kSoftmaxThreads + 128;
+constexpr float kRaise = 7.f, kHead = 4.f;       // raise a base that a score exceeds by 2^7, to 2^4 under it
 constexpr float kLn2f = 0.6931471805599453f;
-constexpr int kMaxLv = 60;                       // value scales enter as f * 2^lv, |lv| <= 60
+constexpr float kMinValueScale = 8.673617379884035e-19f;  // 2^-60: smaller value scales count as this
 
 // PARTS: e4m3 parts of Q (and P): 2 or 3; 0 = 16-bit cache (weights only).
 // ROWS: query rows of a group (8, 16 or 32), G groups (2 for q_len > 8).
@@ -72,8 +79,8 @@ struct Shape {
   static constexpr int COLS = (F8 ? PARTS : 1) * ROWS;
   static constexpr int N = (COLS + 15) / 16 * 16;             // score columns of a group (N of the product)
   static constexpr int STRIDE = N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128;  // TMEM columns of a score slot
-  static constexpr int OCOLS = ATTEND ? 128 : 0;              // O columns of a group (P's row is 128 bytes)
-  static constexpr int SLOTS_FIT = (512 - G * OCOLS) / STRIDE;
+  static constexpr int OCOLS = ATTEND ? 256 : 0;              // O^T of the two streams (P's row is 128 bytes)
+  static constexpr int SLOTS_FIT = (512 - OCOLS) / STRIDE;
   static constexpr int NS = SLOTS_FIT < 4 ? SLOTS_FIT : 4;
   static constexpr int Q_GROUP = F8 ? N * 128 : 2 * N * 128;  // bytes of one group's Q operand
   static constexpr int Q_BYTES = G * Q_GROUP;
@@ -95,17 +102,20 @@ struct TcSmem {
   uint8_t* ring;
   uint8_t* p;  // two P buffers
   uint8_t* q;  // two Q slots
-  float4* meta;     // [kMetaSlots][8]: ks, vs, page id (bits), -
-  float* cq;        // [2][64]: log2-domain score factor of a row
-  float* base;      // [64]
-  float* alpha;     // [64]; the epilogue's 1 / l
-  float* wmax;      // [4][64]: per-warp maxima, then per-warp sums
+  float4* meta;     // [kMetaSlots][8]: ks, log2 vs, 1 / vs, page id (bits)
+  float* base;      // [2][32]: a stream's bases (weights: -lse of the rows, [64])
+  float* delta;     // [2][32]: what a base was raised by; the epilogue's factors of O
+  float* wred;      // [8][32]: per-warp maxima, then per-warp sums
+  int* nan_from;    // [2][128]
+  float* cq;        // [2]: log2-domain score factor of a Q slot
+  unsigned int* qtop;  // [8]
   uint64_t *full, *empty, *s_full, *s_empty, *p_full, *p_done, *q_ready, *m_full, *m_empty, *done;
   uint32_t* tmem_base;
   Schedule* sch;
 };
 
-constexpr int kFixedBytes = kMetaSlots * 8 * 16 + (2 * 64 + 64 + 64 + 4 * 64) * 4 + (2 * 4 + 2 + 2 + 2 + 2 * kMetaSlots + 1) * 8 + 64;
+constexpr int kFixedBytes = kMetaSlots * 8 * 16 + (64 + 64 + 8 * 32 + 2 * 128 + 2 + 8 + 6) * 4 +
+                            (2 * 4 + 2 + 2 + 2 + 2 * kMetaSlots + 1) * 8 + 64;
 
 template <class S>
 __host__ __device__ constexpr int fixed_smem() {
@@ -119,11 +129,13 @@ __device__ __forceinline__ TcSmem carve(uint8_t* smem, int tiles) {
   t.p = smem + (size_t)tiles * kTileBytes;
   t.q = t.p + (S::ATTEND ? 2 * kPBytes : 0);
   t.meta = reinterpret_cast<float4*>(t.q + 2 * S::Q_BYTES);
-  t.cq = reinterpret_cast<float*>(t.meta + kMetaSlots * 8);
-  t.base = t.cq + 2 * 64;
-  t.alpha = t.base + 64;
-  t.wmax = t.alpha + 64;
-  uint64_t* b = reinterpret_cast<uint64_t*>(t.wmax + 4 * 64);
+  t.base = reinterpret_cast<float*>(t.meta + kMetaSlots * 8);
+  t.delta = t.base + 64;
+  t.wred = t.delta + 64;
+  t.nan_from = reinterpret_cast<int*>(t.wred + 8 * 32);
+  t.cq = reinterpret_cast<float*>(t.nan_from + 2 * 128);
+  t.qtop = reinterpret_cast<unsigned int*>(t.cq + 2);
+  uint64_t* b = reinterpret_cast<uint64_t*>(t.qtop + 8 + 6);
   t.full = b;
   t.empty = t.full + tiles;
   t.s_full = t.empty + tiles;
@@ -253,11 +265,15 @@ __device__ void page_meta(const ScaledTcParams& p, const Schedule& sch, const Tc
   for_page_chunks(p.s, sch, [&](const SegWalk& w, int c0, int n, int id) {
     const bool in = c0 + lane < n;
     const bool good = id >= 0 && id < p.s.num_pages;
-    float4 m = make_float4(S::F8 ? 0.f : 1.f, 0.f, __int_as_float(in && good ? id : -1), 0.f);
+    float4 m = make_float4(S::F8 ? 0.f : 1.f, 0.f, 1.f, __int_as_float(in && good ? id : -1));
     if (S::F8 && in) {
       const size_t at = (size_t)(good ? id : 0) * p.scale_stride + w.h;
       m.x = __ldg(p.k_scales + at);
-      if (S::ATTEND) m.y = __ldg(p.v_scales + at);
+      if (S::ATTEND) {
+        const float vs = fmaxf(__ldg(p.v_scales + at), kMinValueScale);
+        m.y = log2f(vs);
+        m.z = 1.f / vs;
+      }
     }
     const int cnt = min(32, n - c0);
     for (int jb = 0; jb < cnt; jb += kBlockPages, ++blk) {
@@ -313,7 +329,7 @@ __device__ void issue_scores(const ScaledTcParams& p, const Schedule& sch, const
         __syncwarp();
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t d = tmem + S::G * S::OCOLS + (u % S::NS) * S::STRIDE;
+          const uint32_t d = tmem + S::OCOLS + (u % S::NS) * S::STRIDE;
           const uint32_t qg = q + g * S::Q_GROUP;
           if constexpr (S::F8) {
             const uint32_t kt = smem_u32(sm.ring + (size_t)(t0 % tiles) * kTileBytes);
@@ -343,7 +359,7 @@ __device__ void issue_scores(const ScaledTcParams& p, const Schedule& sch, const
   drain_products(p, sm);
 }
 
-// O^T of group g += V^T P^T of (block, group) unit u, once P is in buffer u % 2.
+// O^T of stream u & 1 += V^T P^T of unit u, once P is in the stream's buffer.
 template <class S>
 __device__ void issue_values(const ScaledTcParams& p, const Schedule& sch, const TcSmem& sm, uint32_t tmem, int tiles,
                              volatile int* abort) {
@@ -366,8 +382,9 @@ __device__ void issue_values(const ScaledTcParams& p, const Schedule& sch, const
           const uint32_t pb = smem_u32(sm.p + (u & 1) * kPBytes);
           const int steps = (np + 1) / 2;  // 32 tokens a step; the softmax zeroed an absent page's V
           for (int kk = 0; kk < steps; ++kk)
-            tc_mma_ss_f8(tmem + g * 128, smem_desc_sw128(v + kk * 4096, kTileBytes, 1024),
-                         smem_desc_sw128(pb + kk * 4096, kTileBytes, 1024), kIdesc, (k > 0 || kk > 0) ? 1u : 0u);
+            tc_mma_ss_f8(tmem + (u & 1) * 128, smem_desc_sw128(v + kk * 4096, kTileBytes, 1024),
+                         smem_desc_sw128(pb + kk * 4096, kTileBytes, 1024), kIdesc,
+                         (k >= 3 - S::G || kk > 0) ? 1u : 0u);  // a stream's first product of a piece overwrites O
           tc_commit(smem_u32(sm.p_done + (u & 1)));
           if (g == S::G - 1) tc_commit(smem_u32(sm.empty + t1 % tiles));
         }
@@ -389,20 +406,21 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tme
 __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[8]) { tmem_st8(taddr, r); }
 __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[16]) { tmem_st16(taddr, r); }
 
-// Barrier of the softmax threads; true when `v` is for any of them.
-__device__ __forceinline__ bool softmax_any(bool v) {
+// Barrier of a softmax warpgroup; true when `v` is for any of its threads.
+__device__ __forceinline__ bool group_any(int stream, bool v) {
   int r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+      "barrier.cta.red.or.pred q, %2, 128, p;\n\t"
       "selp.b32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"((int)v)
+      : "r"((int)v), "r"(1 + stream)
       : "memory");
   return r != 0;
 }
-__device__ __forceinline__ void softmax_sync() { named_bar_sync(1, 128); }
+__device__ __forceinline__ void group_sync(int stream) { named_bar_sync(1 + stream, 128); }
+__device__ __forceinline__ void softmax_sync() { named_bar_sync(3, kSoftmaxThreads); }
 
 __device__ __forceinline__ int float_order(float f) {  // order-preserving int
   const int i = __float_as_int(f);
@@ -410,9 +428,38 @@ __device__ __forceinline__ int float_order(float f) {  // order-preserving int
 }
 __device__ __forceinline__ float order_float(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
 
-// PARTS e4m3 parts of four numbers: x = part 0 + part 1 / 32 + part 2 / 1024.
+__device__ __forceinline__ uint32_t e4m3x2_of_half2(__half2 h) {
+  return (uint32_t)__nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&h), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ __half2 half2_of_e4m3x2(uint32_t v) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v & 0xffffu), __NV_E4M3);
+  return *reinterpret_cast<const __half2*>(&h);
+}
+
+// The e4m3 parts of two probabilities below 2^8.  Differences of a number and its rounding are
+// exact.  Two parts: P rounded to fp16 first (2^-12 of it, an eighth of what the parts round
+// off); three: the first difference is taken in fp32 and rounded to fp16 (2^-16 of P).
 template <int PARTS>
-__device__ __forceinline__ void split4(float (&x)[4], uint32_t (&out)[3]) {
+__device__ __forceinline__ void split_p(float x0, float x1, uint32_t (&out)[3]) {
+  const __half2 k32 = __floats2half2_rn(32.f, 32.f);
+  __half2 rest;
+  if constexpr (PARTS == 2) {
+    const __half2 h = __floats2half2_rn(x0, x1);
+    out[0] = e4m3x2_of_half2(h);
+    rest = __hmul2(__hsub2(h, half2_of_e4m3x2(out[0])), k32);
+  } else {
+    out[0] = pack_e4m3x2(x0, x1);
+    const float2 f = unpack_e4m3x2(out[0]);
+    const __half2 h = __hmul2(__floats2half2_rn(x0 - f.x, x1 - f.y), k32);
+    out[1] = e4m3x2_of_half2(h);
+    rest = __hmul2(__hsub2(h, half2_of_e4m3x2(out[1])), k32);
+  }
+  out[PARTS - 1] = e4m3x2_of_half2(rest);
+}
+
+// PARTS e4m3 parts of four numbers, exact differences: x = part 0 + part 1 / 32 + part 2 / 1024.
+template <int PARTS>
+__device__ __forceinline__ void split_q(float (&x)[4], uint32_t (&out)[3]) {
 #pragma unroll
   for (int i = 0; i < PARTS; ++i) {
     const uint32_t a = pack_e4m3x2(x[0], x[1]), b = pack_e4m3x2(x[2], x[3]);
@@ -428,66 +475,85 @@ __device__ __forceinline__ void split4(float (&x)[4], uint32_t (&out)[3]) {
 }
 
 // Q of (b, h) as the N operand of the score product, into slot `qs`: row r of part i is operand row
-// i * ROWS + r (128 B, 128-byte swizzle), and the rows' score factors.  128 threads, eight to a row.
+// i * ROWS + r (128 B, 128-byte swizzle), and the slot's score factor.  All softmax threads, eight to
+// a row.
 template <class S, bool BF>
 __device__ void write_q(const ScaledTcParams& p, const TcSmem& sm, int b, int h, int qs) {
+  constexpr int kItems = S::G * S::ROWS * 8;
+  constexpr int kSteps = (kItems + kSoftmaxThreads - 1) / kSoftmaxThreads;
   const int tid = threadIdx.x;
   const int rows = kGroup * p.s.q_len;
-  constexpr int kItems = S::G * S::ROWS * 8;
-  for (int it = tid; it < (kItems + 127) / 128 * 128; it += 128) {
-    const int r = it >> 3, c = it & 7;  // row, its 16 dims
-    const bool in = it < kItems;
-    const bool real = in && r < rows;
-    const __half* src = p.s.q + ((size_t)(b * p.s.q_len + (r >> 2)) * p.s.hq + h * kGroup + (r & 3)) * kHeadDim + c * 16;
-    uint4 x[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-    if (real) {
-      x[0] = __ldg(reinterpret_cast<const uint4*>(src));
-      x[1] = __ldg(reinterpret_cast<const uint4*>(src) + 1);
+  uint4 x[kSteps][2];
+  uint32_t top[kSteps];  // a row's largest magnitude, as bits (above every finite one for infinity and NaN)
+  uint32_t most = 0;     // the largest of a finite row
+#pragma unroll
+  for (int st = 0; st < kSteps; ++st) {
+    const int it = st * kSoftmaxThreads + tid, r = it >> 3, c = it & 7;  // row, its 16 dims
+    x[st][0] = x[st][1] = make_uint4(0u, 0u, 0u, 0u);
+    if (r < rows) {
+      const __half* src =
+          p.s.q + ((size_t)(b * p.s.q_len + (r >> 2)) * p.s.hq + h * kGroup + (r & 3)) * kHeadDim + c * 16;
+      x[st][0] = __ldg(reinterpret_cast<const uint4*>(src));
+      x[st][1] = __ldg(reinterpret_cast<const uint4*>(src) + 1);
     }
-    const int g = r / S::ROWS, rr = r % S::ROWS;
-    uint8_t* const dst = sm.q + qs * S::Q_BYTES + g * S::Q_GROUP;
-    const uint32_t w[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
-    if constexpr (!S::F8) {
-      if (in) {  // 32 bytes of half c / 4: chunks 2 (c % 4) and the next
-        uint8_t* const row = dst + (c >> 2) * (S::N * 128) + (rr >> 3) * 1024 + (rr & 7) * 128;
-        const int c0 = (c & 3) * 2;
-        *reinterpret_cast<uint4*>(row + ((c0 ^ (rr & 7)) << 4)) = x[0];
-        *reinterpret_cast<uint4*>(row + (((c0 + 1) ^ (rr & 7)) << 4)) = x[1];
-        if (c == 0) sm.cq[qs * 64 + r] = p.s.scale_log2;
-      }
-    } else {
-      float f[16];
-      uint32_t top = 0;  // the row's largest magnitude, as bits (above every finite one for inf and NaN)
+  }
+  if constexpr (S::F8) {
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+      const uint32_t w[8] = {x[st][0].x, x[st][0].y, x[st][0].z, x[st][0].w,
+                             x[st][1].x, x[st][1].y, x[st][1].z, x[st][1].w};
+      uint32_t t = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float2 a = unpack2<BF>(w[i]);
-        f[2 * i] = a.x;
-        f[2 * i + 1] = a.y;
-        top = max(top, max(__float_as_uint(a.x) & 0x7fffffffu, __float_as_uint(a.y) & 0x7fffffffu));
+        t = max(t, max(__float_as_uint(a.x) & 0x7fffffffu, __float_as_uint(a.y) & 0x7fffffffu));
       }
 #pragma unroll
-      for (int off = 1; off < 8; off <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
-      // 2^e brings the largest magnitude into [128, 256); a row with an infinity or NaN is NaN
-      const bool finite = top < 0x7f800000u;
-      const int e = top > 0 ? max(-110, min(110, 134 - (int)(top >> 23))) : 0;
-      const float sc = __uint_as_float((uint32_t)(127 + e) << 23);
+      for (int off = 1; off < 8; off <<= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, off));
+      top[st] = t;
+      if (t < 0x7f800000u) most = max(most, t);
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    softmax_sync();  // the last call's reads of qtop are done
+    if ((tid & 31) == 0) sm.qtop[tid >> 5] = most;
+    softmax_sync();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, sm.qtop[i]);
+  }
+  // 2^e brings the largest magnitude into [128, 256)
+  const int e = most > 0 ? max(-110, min(110, 134 - (int)(most >> 23))) : 0;
+  const float sc = __uint_as_float((uint32_t)(127 + e) << 23);
+  if (tid == 0) sm.cq[qs] = p.s.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+  for (int st = 0; st < kSteps; ++st) {
+    const int it = st * kSoftmaxThreads + tid, r = it >> 3, c = it & 7;
+    if (it >= kItems) break;
+    const int rr = r % S::ROWS;
+    uint8_t* const dst = sm.q + qs * S::Q_BYTES + (r / S::ROWS) * S::Q_GROUP;
+    if constexpr (!S::F8) {  // 32 bytes of half c / 4: chunks 2 (c % 4) and the next
+      uint8_t* const row = dst + (c >> 2) * (S::N * 128) + (rr >> 3) * 1024 + (rr & 7) * 128;
+      const int c0 = (c & 3) * 2;
+      *reinterpret_cast<uint4*>(row + ((c0 ^ (rr & 7)) << 4)) = x[st][0];
+      *reinterpret_cast<uint4*>(row + (((c0 + 1) ^ (rr & 7)) << 4)) = x[st][1];
+    } else {
+      const uint32_t w[8] = {x[st][0].x, x[st][0].y, x[st][0].z, x[st][0].w,
+                             x[st][1].x, x[st][1].y, x[st][1].z, x[st][1].w};
       uint32_t part[3][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float y[4] = {f[4 * i] * sc, f[4 * i + 1] * sc, f[4 * i + 2] * sc, f[4 * i + 3] * sc};
+        const float2 a = unpack2<BF>(w[2 * i]), d = unpack2<BF>(w[2 * i + 1]);
+        float y[4] = {a.x * sc, a.y * sc, d.x * sc, d.y * sc};
         uint32_t o[3];
-        split4<S::PARTS>(y, o);
+        split_q<S::PARTS>(y, o);
 #pragma unroll
-        for (int k = 0; k < S::PARTS; ++k) part[k][i] = finite ? o[k] : 0x7f7f7f7fu;
+        for (int k = 0; k < S::PARTS; ++k)  // a row with an infinity or NaN is NaN
+          part[k][i] = top[st] < 0x7f800000u ? o[k] : 0x7f7f7f7fu;
       }
-      if (in) {
 #pragma unroll
-        for (int k = 0; k < S::PARTS; ++k) {
-          const int n = k * S::ROWS + rr;
-          *reinterpret_cast<uint4*>(dst + (n >> 3) * 1024 + (n & 7) * 128 + ((c ^ (n & 7)) << 4)) =
-              make_uint4(part[k][0], part[k][1], part[k][2], part[k][3]);
-        }
-        if (c == 0) sm.cq[qs * 64 + r] = p.s.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23);
+      for (int k = 0; k < S::PARTS; ++k) {
+        const int n = k * S::ROWS + rr;
+        *reinterpret_cast<uint4*>(dst + (n >> 3) * 1024 + (n & 7) * 128 + ((c ^ (n & 7)) << 4)) =
+            make_uint4(part[k][0], part[k][1], part[k][2], part[k][3]);
       }
     }
   }
@@ -555,14 +621,45 @@ __device__ __forceinline__ Piece piece_of(const SplitKvParams& p, const SegWalk&
   return Piece{min(raw, w.pages * kPageSize), whole - p.q_len + 1};
 }
 
+// t = y - base of a unit's rows, and their largest.  MASK: the block holds tokens that some row
+// does not see (late: see attend).
+template <class S, bool MASK>
+__device__ __forceinline__ float unit_scores(uint32_t slot, const float* base, float kc, float lv, int late, int row0,
+                                             float (&t)[S::ROWS]) {
+  float over = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < S::ROWS; c += S::CH) {
+    float s[S::CH];
+    read_scores<S>(slot, c, s);
+#pragma unroll
+    for (int r = 0; r < S::CH; r += 4) {
+      const float4 b4 = *reinterpret_cast<const float4*>(base + c + r);
+      const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = fmaf(s[r + i], kc, lv - bb[i]);
+        if (MASK && late >= (row0 + c + r + i) >> 2) x = -INFINITY;
+        t[c + r + i] = x;
+        over = fmaxf(over, x);
+      }
+    }
+  }
+  return over;
+}
+
 template <class S, bool BF>
 __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSmem& sm, uint32_t tmem, int tiles,
                        volatile int* abort) {
   constexpr int ROWS = S::ROWS, G = S::G, CH = S::CH;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;  // tid: token of a block, dimension of O
+  const int stream = threadIdx.x >> 7;
+  const int tid = threadIdx.x & 127, warp = tid >> 5, lane = tid & 31;  // tid: token of a block, dimension of O
   const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
   const int rows = kGroup * p.s.q_len;
-  int u = 0, blk = 0, pc = 0;
+  const int row0 = G == 2 ? stream * ROWS : 0;  // the stream's first row
+  float* const base = sm.base + stream * 32;
+  float* const delta = sm.delta + stream * 32;
+  float* const wred = sm.wred + stream * 4 * 32;
+  int blk = 0, pc = 0;
   for_pieces(p.s, sch, [&](const SegWalk& w, int unit, int n) {
     const int seg = w.b * p.s.hkv + w.h;
     const int seg_end = w.seg_start + w.pages;
@@ -574,236 +671,255 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
       next_segment(p.s, nw);
       write_q<S, BF>(p, sm, nw.b, nw.h, (pc + 1) & 1);
     }
-    if (tid < G * ROWS) sm.base[tid] = kNoBase;
+    if (tid < ROWS) base[tid] = 0.f;
     softmax_sync();
-    const float* const cq = sm.cq + (pc & 1) * 64;
-    float l[G][ROWS];
+    const float cq = sm.cq[pc & 1];
+    float l[ROWS];
 #pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-      for (int r = 0; r < ROWS; ++r) l[g][r] = 0.f;
+    for (int r = 0; r < ROWS; ++r) l[r] = 0.f;
     int nan_from = 0x7fffffff;  // first draft token whose V is NaN in dimension tid
 
     const int nblk = blocks_of(n);
-    for (int k = 0; k < nblk; ++k, ++blk) {
+    const int k0 = G == 2 ? 0 : (blk ^ stream) & 1;  // the stream's first block of the piece
+    for (int k = k0; k < nblk; k += 3 - G) {
+      const int bk = blk + k;
+      const int u = G == 2 ? 2 * bk + stream : bk;
+      const int v = u >> 1;  // the stream's own count
       const int np = min(kBlockPages, n - k * kBlockPages);
       const int tok0 = (w.pg + k * kBlockPages) * kPageSize;
       const int tok = tok0 + tid;
-      const int e = blk % kMetaSlots;
-      mbar_wait_bounded(smem_u32(sm.m_full + e), (uint32_t)(blk / kMetaSlots) & 1u, abort, p.s.status, 3, blk);
+      const int e = bk % kMetaSlots;
+      mbar_wait_bounded(smem_u32(sm.m_full + e), (uint32_t)(bk / kMetaSlots) & 1u, abort, p.s.status, 3, bk);
       const float4 meta = sm.meta[e * kBlockPages + (tid >> 4)];
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(sm.m_empty + e));
-      // vs = f * 2^lv
-      const int lv = max(-kMaxLv, min(kMaxLv, (int)(__float_as_uint(meta.y) >> 23) - 127));
-      const float inv_lv = __uint_as_float((uint32_t)(127 - lv) << 23);
-      const float f = meta.y * inv_lv;
-      const float flv = (float)lv;
+      const float kc = meta.x * cq;
       const bool masked = np < kBlockPages || tok0 + kBlock > piece.first || tok0 + kBlock > piece.len;
       // draft qi sees the token iff late < qi (every draft when negative)
       const int late = (tid < np * kPageSize && tok < piece.len) ? tok - piece.first : 0x7fffffff;
-      const int t1 = blk * 2 + 1;  // V's tile
 
-      if (masked) {
+      if (masked && (G == 1 || stream == 0)) {
         // V rows behind the sequence and of absent pages: zero (they may hold NaN); draft tokens'
-        // NaN: zero, and remembered by the dimension's thread
-        mbar_wait_bounded(smem_u32(sm.full + t1 % tiles), (uint32_t)(t1 / tiles) & 1u, abort, p.s.status, 9, blk);
-        uint8_t* const v = sm.ring + (size_t)(t1 % tiles) * kTileBytes;
+        // NaN: zero, and remembered by the dimension's thread.  (Two groups: the first one's product
+        // comes first.)
+        const int t1 = bk * 2 + 1;  // V's tile
+        mbar_wait_bounded(smem_u32(sm.full + t1 % tiles), (uint32_t)(t1 / tiles) & 1u, abort, p.s.status, 9, bk);
+        uint8_t* const vt = sm.ring + (size_t)(t1 % tiles) * kTileBytes;
         const int held = min(np * kPageSize, max(piece.len - tok0, 0));
         const int read = (np + 1) / 2 * 32;  // rows that the product reads
         for (int t = max(0, piece.first - tok0); t < held; ++t) {
-          uint8_t* const at = v + t * 128 + (((tid >> 4) ^ (t & 7)) << 4) + (tid & 15);
+          uint8_t* const at = vt + t * 128 + (((tid >> 4) ^ (t & 7)) << 4) + (tid & 15);
           if ((*at & 0x7f) == 0x7f) {
             nan_from = min(nan_from, tok0 + t);
             *at = 0;
           }
         }
         for (int c = held * 8 + tid; c < read * 8; c += 128)
-          *reinterpret_cast<uint4*>(v + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+          *reinterpret_cast<uint4*>(vt + c * 16) = make_uint4(0u, 0u, 0u, 0u);
         fence_proxy_async_smem();
       }
 
+      mbar_wait_bounded(smem_u32(sm.s_full + u % S::NS), (uint32_t)(u / S::NS) & 1u, abort, p.s.status, 10, u);
+      tc_fence_after();
+      const uint32_t slot = lanes + S::OCOLS + (u % S::NS) * S::STRIDE;
+      float t[ROWS];
+      const float over = masked ? unit_scores<S, true>(slot, base, kc, meta.y, late, row0, t)
+                                : unit_scores<S, false>(slot, base, kc, meta.y, late, row0, t);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(sm.s_empty + u % S::NS));
+      const bool first = k == k0;
+      const bool raise = group_any(stream, over > kRaise) || first;  // rare after a piece's first blocks
+      if (raise) {
 #pragma unroll
-      for (int g = 0; g < G; ++g, ++u) {
-        mbar_wait_bounded(smem_u32(sm.s_full + u % S::NS), (uint32_t)(u / S::NS) & 1u, abort, p.s.status, 10, u);
+        for (int r = 0; r < ROWS; ++r) {
+          const int m = __reduce_max_sync(0xffffffffu, float_order(t[r] == t[r] ? t[r] : -INFINITY));
+          if (lane == r) wred[warp * 32 + r] = order_float(m);
+        }
+        group_sync(stream);
+        if (tid < ROWS) {
+          const float m = fmaxf(fmaxf(wred[tid], wred[32 + tid]), fmaxf(wred[64 + tid], wred[96 + tid]));
+          const float d = (m > kRaise || (first && m != -INFINITY)) ? m - kHead : 0.f;
+          delta[tid] = d;
+          base[tid] += d;
+        }
+        group_sync(stream);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) t[r] -= delta[r];
+      }
+      // the stream's last product: P's buffer is free, and O stands still
+      if (v >= 1) mbar_wait_bounded(smem_u32(sm.p_done + stream), (uint32_t)(v - 1) & 1u, abort, p.s.status, 11, u);
+      if (raise && !first) {
         tc_fence_after();
-        const uint32_t slot = lanes + G * S::OCOLS + (u % S::NS) * S::STRIDE;
-        float y[ROWS];
-        float over = -INFINITY;
 #pragma unroll
         for (int c = 0; c < ROWS; c += CH) {
-          float s[CH];
-          read_scores<S>(slot, c, s);
+          float a[CH];
 #pragma unroll
-          for (int r = 0; r < CH; r += 4) {
-            const float4 q4 = *reinterpret_cast<const float4*>(cq + g * ROWS + c + r);
-            const float4 b4 = *reinterpret_cast<const float4*>(sm.base + g * ROWS + c + r);
-            const float qq[4] = {q4.x, q4.y, q4.z, q4.w}, bb[4] = {b4.x, b4.y, b4.z, b4.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float x = fmaf(s[r + i], meta.x * qq[i], flv);
-              if (masked && late >= (g * ROWS + c + r + i) >> 2) x = -INFINITY;
-              y[c + r + i] = x;
-              over = fmaxf(over, x - bb[i]);
-            }
-          }
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(sm.s_empty + u % S::NS));
-        // P's buffer is free once the product before the last is done
-        if (u >= 2)
-          mbar_wait_bounded(smem_u32(sm.p_done + (u & 1)), (uint32_t)((u >> 1) - 1) & 1u, abort, p.s.status, 11, u);
-        if (softmax_any(over > kRaise)) {  // raise bases (rare after a piece's first blocks)
-#pragma unroll
-          for (int r = 0; r < ROWS; ++r) {
-            const int m = __reduce_max_sync(0xffffffffu, float_order(y[r] == y[r] ? y[r] : -INFINITY));
-            if (lane == r) sm.wmax[warp * 64 + g * ROWS + r] = order_float(m);
-          }
-          softmax_sync();
-          if (tid < ROWS) {
-            const int r = g * ROWS + tid;
-            const float m = fmaxf(fmaxf(sm.wmax[r], sm.wmax[64 + r]), fmaxf(sm.wmax[128 + r], sm.wmax[192 + r]));
-            const float old = sm.base[r];
-            const bool up = m > old + kRaise;
-            sm.alpha[r] = up ? ex2(old - (m - kHead)) : 1.f;
-            if (up) sm.base[r] = m - kHead;
-          }
-          softmax_sync();
-          if (k > 0) {
-            // O must be stable: the group's last product is done (G = 2: waited for above)
-            if (G == 1)
-              mbar_wait_bounded(smem_u32(sm.p_done + ((u - 1) & 1)), (uint32_t)((u - 1) >> 1) & 1u, abort, p.s.status, 12, u);
-            tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < ROWS; c += CH) {
-              float a[CH];
-#pragma unroll
-              for (int r = 0; r < CH; ++r) {
-                a[r] = sm.alpha[g * ROWS + c + r];
-                l[g][c + r] *= a[r];
-              }
-#pragma unroll
-              for (int i = 0; i < S::PARTS; ++i) {
-                uint32_t o[CH];
-                tmem_ld(lanes + g * 128 + i * ROWS + c, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int r = 0; r < CH; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * a[r]);
-                tmem_st(lanes + g * 128 + i * ROWS + c, o);
-              }
-            }
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-          }
-        }
-        // P: token tid's operand row of 128 bytes, part i of row r in byte i * ROWS + r
-        uint8_t* const prow = sm.p + (u & 1) * kPBytes + (tid >> 3) * 1024 + (tid & 7) * 128;
-#pragma unroll
-        for (int c = 0; c < ROWS; c += CH) {
-          uint32_t part[3][CH / 4];
-#pragma unroll
-          for (int r = 0; r < CH; r += 4) {
-            const float4 b4 = *reinterpret_cast<const float4*>(sm.base + g * ROWS + c + r);
-            const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
-            float x[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float ee = ex2(y[c + r + i] - bb[i]);
-              l[g][c + r + i] = fmaf(ee, inv_lv, l[g][c + r + i]);
-              x[i] = ee * f;
-            }
-            uint32_t o[3];
-            split4<S::PARTS>(x, o);
-#pragma unroll
-            for (int i = 0; i < S::PARTS; ++i) part[i][r / 4] = o[i];
+          for (int r = 0; r < CH; ++r) {
+            a[r] = ex2(-delta[c + r]);
+            l[c + r] *= a[r];
           }
 #pragma unroll
           for (int i = 0; i < S::PARTS; ++i) {
-            const int byte = i * ROWS + c;
-            uint8_t* const at = prow + (((byte >> 4) ^ (tid & 7)) << 4) + (byte & 15);
-            if constexpr (CH == 16)
-              *reinterpret_cast<uint4*>(at) = make_uint4(part[i][0], part[i][1], part[i][2], part[i][3]);
-            else
-              *reinterpret_cast<uint2*>(at) = make_uint2(part[i][0], part[i][1]);
+            uint32_t o[CH];
+            tmem_ld(lanes + stream * 128 + i * ROWS + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int r = 0; r < CH; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * a[r]);
+            tmem_st(lanes + stream * 128 + i * ROWS + c, o);
           }
         }
-        fence_proxy_async_smem();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(sm.p_full + (u & 1)));
+        tmem_wait_st();
       }
-    }
-
-    // ---- epilogue: denominators, then each dimension's thread joins the parts of its rows
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const float total = sum_rows<ROWS>(l[g]);
-      if (lane % (32 / ROWS) == 0) sm.wmax[warp * 64 + g * ROWS + lane / (32 / ROWS)] = total;
-    }
-    softmax_sync();
-    const int slot = (int)blockIdx.x + seg;  // workspace piece
-    if (tid < rows) {
-      const float total = (sm.wmax[tid] + sm.wmax[64 + tid]) + (sm.wmax[128 + tid] + sm.wmax[192 + tid]);
-      sm.alpha[tid] = total > 0.f ? p.s.out_scale / total : total;  // 0 for a row without tokens, NaN for a NaN row
-      const float lse = total == 0.f ? -INFINITY : (sm.base[tid] + __log2f(total)) * kLn2f;
-      const size_t out_row = (size_t)(w.b * p.s.q_len + (tid >> 2)) * p.s.hq + w.h * kGroup + (tid & 3);
-      if (!whole) p.s.ws_lse[(size_t)slot * p.s.rows_pad + tid] = lse;
-      else if (p.s.out_lse) p.s.out_lse[out_row] = lse;
-    }
-    softmax_sync();
-#pragma unroll
-    for (int g = 0; g < G; ++g) {  // the last products of both groups
-      const int last = u - G + g;
-      mbar_wait_bounded(smem_u32(sm.p_done + (last & 1)), (uint32_t)(last >> 1) & 1u, abort, p.s.status, 13, last);
-    }
-    tc_fence_after();
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
+      // P: token tid's operand row of 128 bytes, part i of row r in byte i * ROWS + r
+      uint8_t* const prow = sm.p + stream * kPBytes + (tid >> 3) * 1024 + (tid & 7) * 128;
 #pragma unroll
       for (int c = 0; c < ROWS; c += CH) {
-        if (g * ROWS + c >= rows) break;
-        float o[CH];
-        uint32_t raw[3][CH];
+        uint32_t part[3][CH / 4];
 #pragma unroll
-        for (int i = 0; i < S::PARTS; ++i) tmem_ld(lanes + g * 128 + i * ROWS + c, raw[i]);
+        for (int r = 0; r < CH; r += 4) {
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[i] = ex2(t[c + r + i]);
+            l[c + r + i] = fmaf(x[i], meta.z, l[c + r + i]);
+          }
+          uint32_t lo[3], hi[3];
+          split_p<S::PARTS>(x[0], x[1], lo);
+          split_p<S::PARTS>(x[2], x[3], hi);
+#pragma unroll
+          for (int i = 0; i < S::PARTS; ++i) part[i][r / 4] = lo[i] | (hi[i] << 16);
+        }
+#pragma unroll
+        for (int i = 0; i < S::PARTS; ++i) {
+          const int byte = i * ROWS + c;
+          uint8_t* const at = prow + (((byte >> 4) ^ (tid & 7)) << 4) + (byte & 15);
+          if constexpr (CH == 16)
+            *reinterpret_cast<uint4*>(at) = make_uint4(part[i][0], part[i][1], part[i][2], part[i][3]);
+          else
+            *reinterpret_cast<uint2*>(at) = make_uint2(part[i][0], part[i][1]);
+        }
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(sm.p_full + stream));
+    }
+
+    // ---- epilogue: denominators and factors, then each dimension's thread joins its rows' parts
+    const float total = sum_rows<ROWS>(l);
+    if (lane % (32 / ROWS) == 0) wred[warp * 32 + lane / (32 / ROWS)] = total;
+    sm.nan_from[threadIdx.x] = nan_from;
+    softmax_sync();
+    const int slot = (int)blockIdx.x + seg;  // workspace piece
+    if (threadIdx.x < rows) {
+      const int row = threadIdx.x, r = row % ROWS;
+      auto sum_of = [&](int st) {
+        const float* x = sm.wred + st * 128 + r;
+        return (x[0] + x[32]) + (x[64] + x[96]);
+      };
+      float all, top;  // the row's denominator, in units of 2^top
+      if (G == 2) {
+        const int st = row / ROWS;
+        all = sum_of(st);
+        top = sm.base[st * 32 + r];
+        sm.delta[row] = all > 0.f ? p.s.out_scale / all : all;  // 0 for a row without tokens, NaN for a NaN row
+      } else {
+        const float l0 = sum_of(0), l1 = sum_of(1), b0 = sm.base[r], b1 = sm.base[32 + r];
+        top = l0 == 0.f ? b1 : l1 == 0.f ? b0 : fmaxf(b0, b1);
+        const float w0 = l0 == 0.f ? 0.f : ex2(b0 - top), w1 = l1 == 0.f ? 0.f : ex2(b1 - top);
+        all = l0 * w0 + l1 * w1;
+        const float f = all > 0.f ? p.s.out_scale / all : all;
+        sm.delta[r] = w0 == 0.f ? 0.f : w0 * f;
+        sm.delta[32 + r] = w1 == 0.f ? 0.f : w1 * f;
+      }
+      const float lse = all == 0.f ? -INFINITY : (top + __log2f(all)) * kLn2f;
+      const size_t out_row = (size_t)(w.b * p.s.q_len + (row >> 2)) * p.s.hq + w.h * kGroup + (row & 3);
+      if (!whole) p.s.ws_lse[(size_t)slot * p.s.rows_pad + row] = lse;
+      else if (p.s.out_lse) p.s.out_lse[out_row] = lse;
+    }
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {  // each stream's last product (a stream may have none in this piece)
+      const int last = G == 2 ? 2 * (blk + nblk - 1) + st : blk + nblk - 1 - ((blk + nblk - 1 - st) & 1);
+      if (G == 2 || last >= blk)
+        mbar_wait_bounded(smem_u32(sm.p_done + st), (uint32_t)(last >> 1) & 1u, abort, p.s.status, 13, last);
+    }
+    tc_fence_after();
+    softmax_sync();
+    nan_from = min(sm.nan_from[tid], sm.nan_from[128 + tid]);
+#pragma unroll
+    for (int c = 0; c < ROWS; c += 8) {
+      if (G == 1 && ((c >> 3) & 1) != stream) continue;  // the warpgroups share the rows
+      if (row0 + c >= rows) continue;
+      float o[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) o[r] = 0.f;
+#pragma unroll
+      for (int st = 0; st < 3 - G; ++st) {
+        const int from = G == 2 ? stream : st;
+        uint32_t raw[3][8];
+#pragma unroll
+        for (int i = 0; i < S::PARTS; ++i) tmem_ld(lanes + from * 128 + i * ROWS + c, raw[i]);
         tmem_wait_ld();
 #pragma unroll
-        for (int r = 0; r < CH; ++r) {
+        for (int r = 0; r < 8; ++r) {
           float x = __uint_as_float(raw[S::PARTS - 1][r]);
 #pragma unroll
           for (int i = S::PARTS - 2; i >= 0; --i) x = fmaf(x, 1.f / 32.f, __uint_as_float(raw[i][r]));
-          const int row = g * ROWS + c + r;
-          const float inv = sm.alpha[row];
-          x = inv == 0.f ? 0.f : x * inv;
-          // draft row / 4 sees the tokens before min(len, first + row / 4)
-          if (nan_from < piece.first + (row >> 2)) x = __int_as_float(0x7fffffff);
-          o[r] = x;
+          const float f = sm.delta[from * 32 + c + r];
+          if (f != 0.f) o[r] = fmaf(x, f, o[r]);  // a stream without tokens may hold anything
         }
+      }
 #pragma unroll
-        for (int r = 0; r < CH; ++r) {
-          const int row = g * ROWS + c + r;
-          if (row < rows) {
-            const size_t out_row = (size_t)(w.b * p.s.q_len + (row >> 2)) * p.s.hq + w.h * kGroup + (row & 3);
-            if (!whole) p.s.ws_o[((size_t)slot * p.s.rows_pad + row) * kHeadDim + tid] = o[r];
-            else if (p.s.out_o) p.s.out_o[out_row * kHeadDim + tid] = o[r];
-            else reinterpret_cast<uint16_t*>(p.s.out)[out_row * kHeadDim + tid] = (uint16_t)(pack2<BF>(o[r], 0.f) & 0xffffu);
-          }
+      for (int r = 0; r < 8; ++r) {
+        const int row = row0 + c + r;
+        // draft row / 4 sees the tokens before min(len, first + row / 4)
+        if (nan_from < piece.first + (row >> 2)) o[r] = __int_as_float(0x7fffffff);
+        if (row < rows) {
+          const size_t out_row = (size_t)(w.b * p.s.q_len + (row >> 2)) * p.s.hq + w.h * kGroup + (row & 3);
+          if (!whole) p.s.ws_o[((size_t)slot * p.s.rows_pad + row) * kHeadDim + tid] = o[r];
+          else if (p.s.out_o) p.s.out_o[out_row * kHeadDim + tid] = o[r];
+          else reinterpret_cast<uint16_t*>(p.s.out)[out_row * kHeadDim + tid] = (uint16_t)(pack2<BF>(o[r], 0.f) & 0xffffu);
         }
       }
     }
     tc_fence_before();  // O is read before the next piece's first product overwrites it
-    softmax_sync();     // and so are base and alpha
+    softmax_sync();     // and so is all that the streams share
+    blk += nblk;
     ++pc;
   });
 }
 
+template <class S, bool MASK>
+__device__ __forceinline__ float unit_weight(uint32_t slot, const float* base, float kc, int late, int row0) {
+  float sum = 0.f;
+#pragma unroll
+  for (int c = 0; c < S::ROWS; c += S::CH) {
+    float s[S::CH];
+    read_scores<S>(slot, c, s);
+#pragma unroll
+    for (int r = 0; r < S::CH; r += 4) {
+      const float4 b4 = *reinterpret_cast<const float4*>(base + c + r);
+      const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = fmaf(s[r + i], kc, bb[i]);
+        if (MASK && late >= (row0 + c + r + i) >> 2) x = -INFINITY;
+        sum += ex2(x);
+      }
+    }
+  }
+  return sum;
+}
+
 template <class S, bool BF>
 __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const TcSmem& sm, uint32_t tmem, volatile int* abort) {
-  constexpr int ROWS = S::ROWS, G = S::G, CH = S::CH;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int G = S::G;
+  const int group = threadIdx.x >> 7;  // this warpgroup's blocks: every other one
+  const int tid = threadIdx.x & 127, warp = tid >> 5, lane = tid & 31;
   const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
   const int rows = kGroup * p.s.q_len;
-  int u = 0, blk = 0, pc = 0;
+  int blk = 0, pc = 0;
   for_pieces(p.s, sch, [&](const SegWalk& w, int, int n) {
     const int seg_end = w.seg_start + w.pages;
     const Piece piece = piece_of(p.s, w);
@@ -814,27 +930,30 @@ __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const TcSmem
       next_segment(p.s, nw);
       write_q<S, BF>(p, sm, nw.b, nw.h, (pc + 1) & 1);
     }
-    if (tid < G * ROWS) {  // -lse in base 2; -inf (weight 0) for padding and rows without tokens
+    if (threadIdx.x < G * S::ROWS) {  // -lse in base 2; -inf (weight 0) for padding and rows without tokens
+      const int row = threadIdx.x;
       float x = -INFINITY;
-      if (tid < rows) {
-        const float v = p.lse[(size_t)(w.b * p.s.q_len + (tid >> 2)) * p.s.hq + w.h * kGroup + (tid & 3)];
+      if (row < rows) {
+        const float v = p.lse[(size_t)(w.b * p.s.q_len + (row >> 2)) * p.s.hq + w.h * kGroup + (row & 3)];
         if (v != -INFINITY) x = -v * 1.4426950408889634f;
       }
-      sm.base[tid] = x;
+      sm.base[row] = x;
     }
     softmax_sync();
-    const float* const cq = sm.cq + (pc & 1) * 64;
+    const float cq = sm.cq[pc & 1];
     const int nblk = blocks_of(n);
-    for (int k = 0; k < nblk; ++k, ++blk) {
+    for (int k = (blk ^ group) & 1; k < nblk; k += 2) {
+      const int bk = blk + k;
       const int np = min(kBlockPages, n - k * kBlockPages);
       const int tok0 = (w.pg + k * kBlockPages) * kPageSize;
       const int tok = tok0 + tid;
-      const int e = blk % kMetaSlots;
-      mbar_wait_bounded(smem_u32(sm.m_full + e), (uint32_t)(blk / kMetaSlots) & 1u, abort, p.s.status, 3, blk);
+      const int e = bk % kMetaSlots;
+      mbar_wait_bounded(smem_u32(sm.m_full + e), (uint32_t)(bk / kMetaSlots) & 1u, abort, p.s.status, 3, bk);
       const float4 meta = sm.meta[e * kBlockPages + (tid >> 4)];
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(sm.m_empty + e));
-      const int id = __float_as_int(meta.z);
+      const float kc = meta.x * cq;
+      const int id = __float_as_int(meta.w);
       const bool held = tid < np * kPageSize && tok < piece.len;
       float* const at = p.scores + ((size_t)max(id, 0) * p.s.hkv + w.h) * kPageSize + (tid & 15);
       const float old = (held && id >= 0 && tok < fresh) ? *at : 0.f;  // in flight during the score product
@@ -842,27 +961,13 @@ __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const TcSmem
       const int late = held ? tok - piece.first : 0x7fffffff;
       float sum = 0.f;
 #pragma unroll
-      for (int g = 0; g < G; ++g, ++u) {
+      for (int g = 0; g < G; ++g) {
+        const int u = bk * G + g;
         mbar_wait_bounded(smem_u32(sm.s_full + u % S::NS), (uint32_t)(u / S::NS) & 1u, abort, p.s.status, 10, u);
         tc_fence_after();
         const uint32_t slot = lanes + (u % S::NS) * S::STRIDE;
-#pragma unroll
-        for (int c = 0; c < ROWS; c += CH) {
-          float s[CH];
-          read_scores<S>(slot, c, s);
-#pragma unroll
-          for (int r = 0; r < CH; r += 4) {
-            const float4 q4 = *reinterpret_cast<const float4*>(cq + g * ROWS + c + r);
-            const float4 b4 = *reinterpret_cast<const float4*>(sm.base + g * ROWS + c + r);
-            const float qq[4] = {q4.x, q4.y, q4.z, q4.w}, bb[4] = {b4.x, b4.y, b4.z, b4.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float x = fmaf(s[r + i], meta.x * qq[i], bb[i]);
-              if ((masked && late >= (g * ROWS + c + r + i) >> 2) || bb[i] == -INFINITY) x = -INFINITY;
-              sum += ex2(x);
-            }
-          }
-        }
+        sum += masked ? unit_weight<S, true>(slot, sm.base + g * S::ROWS, kc, late, g * S::ROWS)
+                      : unit_weight<S, false>(slot, sm.base + g * S::ROWS, kc, late, g * S::ROWS);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(sm.s_empty + u % S::NS));
@@ -870,6 +975,7 @@ __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const TcSmem
       if (held && id >= 0) *at = old + sum;
     }
     softmax_sync();  // base has been read
+    blk += nblk;
     ++pc;
   });
 }
@@ -883,7 +989,7 @@ __global__ void __launch_bounds__(kScaledTcThreads, 1)
   const int tiles = p.s.num_stages;
   const TcSmem sm = carve<S>(smem, tiles);
   const int warp = threadIdx.x >> 5;
-  constexpr int kScoreWarp = 4, kValueWarp = 5, kProducerWarp = 6, kMetaWarp = 7;
+  constexpr int kScoreWarp = 8, kValueWarp = 9, kProducerWarp = 10, kMetaWarp = 11;
   if (threadIdx.x == 0) {
     for (int i = 0; i < tiles; ++i) {
       mbar_init(smem_u32(sm.full + i), 1);
@@ -896,11 +1002,11 @@ __global__ void __launch_bounds__(kScaledTcThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(sm.p_full + i), 4);
       mbar_init(smem_u32(sm.p_done + i), 1);
-      mbar_init(smem_u32(sm.q_ready + i), 4);
+      mbar_init(smem_u32(sm.q_ready + i), 8);
     }
     for (int i = 0; i < kMetaSlots; ++i) {
       mbar_init(smem_u32(sm.m_full + i), 1);
-      mbar_init(smem_u32(sm.m_empty + i), 4);
+      mbar_init(smem_u32(sm.m_empty + i), S::ATTEND && S::G == 2 ? 8 : 4);  // the warps that read a block's scales
     }
     mbar_init(smem_u32(sm.done), S::ATTEND ? 2 : 1);  // one commit from each issuer
     fence_mbar_init();

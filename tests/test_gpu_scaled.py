@@ -155,6 +155,30 @@ def test_attention_peaked_and_flat_rows(sqa):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("step", [0.001, 0.01, 0.05, 0.2])
+def test_attention_creeping_maximum(sqa, step, dtype):
+    """Scores that rise from token to token, so that a row's running base is passed by any amount up
+    to where it is raised, with value scales just under and just over powers of two."""
+    n = 4096
+    c = scaled_case(2, [n, n // 2 + 5], hkv=2, dtype=dtype, seed=11, spread=0.0)
+    c["query"][:] = 0.0
+    c["query"][..., 0] = 1.0
+    c["query"][:, 1, ::2, 0] = -1.0  # falls for some rows
+    k = torch.zeros_like(c["k"].float())
+    for b, row in enumerate(c["table"]):
+        for t in range(c["lens"][b]):
+            k[row[t // 16], t % 16, :, 0] = 16 + (t % 16) // 2  # within a page by e4m3's steps
+    for b, row in enumerate(c["table"]):  # from page to page by the scale
+        for j in range((c["lens"][b] + 15) // 16):
+            c["ks"][row[j]] = step * 128 ** 0.5 * (16 * j + 8) / 20
+    c["k"] = k.to(F8)
+    c["vs"][:] = 1.99
+    c["vs"][::3] = 1.01
+    out, lse = attend(sqa, to_gpu(c))
+    assert_within(out, lse, reference(c), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
 def test_attention_ignores_what_a_row_does_not_see(sqa, dtype):
     """NaN bytes and NaN or infinite scales behind the sequence and in other sequences' pages, and
     NaN in draft tokens' K and V that earlier drafts do not see."""

@@ -22,31 +22,34 @@
 //
 // Softmax.  A row keeps a base; a score with its value scale, y = c ks (q . k) + log2 vs, enters as
 // P = 2^(y - base), and the denominator sums P / vs.  The value scale is thus inside the running
-// maximum, and P keeps its e4m3 range whatever the pages' value scales are.  A base is set from the
-// first block and raised, to the block's maximum - 4, only when some y exceeds it by more than 7
-// (one barrier with an or-reduction a block finds that out); then l and the row's O columns are
-// rescaled.  Masked tokens and tokens behind the sequence have y = -inf by selection, so NaN in
-// their K does not matter; V rows behind the sequence are zeroed in shared memory, and a NaN in
-// the V of a draft token is zeroed and remembered, as only the rows that see the token get it.
+// maximum, and P keeps its e4m3 range whatever the pages' value scales are.  Bases are set from the
+// first block to its maxima - 2 and raised when some y exceeds its base by more than 8 (one
+// barrier with an or-reduction a block finds that out; then every row whose block maximum passed
+// its old one is raised, and l and O are rescaled).  Six bits of slack: with bases raised at
+// 3 bits over the maximum, two blocks in five of random data with 1% of fourfold tokens raised one,
+// at 2500 cycles each.  Masked tokens and tokens behind the sequence have y = -inf by selection, so
+// NaN in their K does not matter; V rows behind the sequence are zeroed in shared memory, and a NaN
+// in the V of a draft token is zeroed and remembered, as only the rows that see the token get it.
 //
 // Weights.  w_t = sum over the rows of 2^(c ks (q . k) - lse): the same score product, summed over the
 // thread's columns and added to the token's score.  16-bit caches use kind::f16 and Q as it is.
 //
-// Two softmax warpgroups, so that the scheduler always has a second warp to issue from: with
-// one, a block of 64 rows took 13.7k cycles at 0.22 instructions a cycle and scheduler.  They
-// take every other block (q_len <= 8; each with its own bases and O, joined at the end of a piece) or
-// one half of the rows each (q_len > 8).
+// Four softmax warpgroups, so that each scheduler has four warps to issue from and a unit of
+// 16 rows keeps its scores and sums in registers.  With one warpgroup, a block of 64 rows took
+// 13.7k cycles at 0.22 instructions a cycle and scheduler, with two of 32 rows 5k.  A unit is a
+// (block, group of 16 rows); a warpgroup takes every fourth unit, its stream: of one group always
+// (4 / G blocks apart), with its own bases and O, and the streams of a group are joined at
+// the end of a piece.
 //
-// Warps: 0-7 softmax (one token a thread), 8 score products, 9 value products, 10 TMA
-// producer, 11 page scales.  Work is cut into CTA ranges by sqa_schedule.cuh; pieces of a split
+// Warps: 0-15 softmax (one token a thread), 16 score products, 17 value products, 18 TMA
+// producer, 19 page scales.  Work is cut into CTA ranges by sqa_schedule.cuh; pieces of a split
 // segment are merged by sqa_scaled_merge_kernel.
 //
-// Pipelines (mbarriers; every wait bounded).  A unit u is a (block, row group); its stream u & 1
-// is the warpgroup that works on it.
+// Pipelines (mbarriers; every wait bounded):
 //   full / empty [tiles]     producer -> issuers; K and V tiles (16 KB) alternate in one ring,
 //                            each released by the commit of the product that read it
 //   s_full / s_empty [NS]    score issuer (commit) -> softmax -> score issuer
-//   p_full / p_done [2]      softmax -> value issuer (commit) -> softmax, one P buffer a stream
+//   p_full / p_done [4]      softmax -> value issuer (commit) -> softmax, one P buffer a stream
 //   q_ready [2]              softmax (Q of a piece, one piece ahead) -> score issuer
 //   m_full / m_empty [8]     page scales of a block -> softmax
 #include "small_q_attention.h"
@@ -63,30 +66,31 @@ constexpr int kBlockPages = 8;
 constexpr int kBlock = kBlockPages * kPageSize;  // 128 tokens: the M side
 constexpr int kTileBytes = kBlock * 128;         // K or V of a block (e4m3), or one half of 16-bit K
 constexpr int kMetaSlots = 8;
-constexpr int kPBytes = kBlock * 128;
-constexpr int kSoftmaxThreads = 256;             // two warpgroups
+constexpr int kPRow = 64;                        // bytes of a token's P: up to three parts of 16 rows
+constexpr int kPBytes = kBlock * kPRow;
+constexpr int kStreams = 4;                      // softmax warpgroups
+constexpr int kSoftmaxThreads = kStreams * 128;
 constexpr int kScaledTcThreads = kSoftmaxThreads + 128;
-constexpr float kRaise = 7.f, kHead = 4.f;       // raise a base that a score exceeds by 2^7, to 2^4 under it
+constexpr float kRaise = 8.f, kHead = 2.f;       // raise a base that a score exceeds by 2^8, to 2^2 under the maximum
 constexpr float kLn2f = 0.6931471805599453f;
 constexpr float kMinValueScale = 8.673617379884035e-19f;  // 2^-60: smaller value scales count as this
 
 // PARTS: e4m3 parts of Q (and P): 2 or 3; 0 = 16-bit cache (weights only).
-// ROWS: query rows of a group (8, 16 or 32), G groups (2 for q_len > 8).
+// ROWS: query rows of a group (8 or 16), G groups (1, 2 or 4).
 template <int PARTS_, int ROWS_, int G_, bool ATTEND_>
 struct Shape {
   static constexpr int PARTS = PARTS_, ROWS = ROWS_, G = G_;
   static constexpr bool ATTEND = ATTEND_, F8 = PARTS_ > 0;
   static constexpr int COLS = (F8 ? PARTS : 1) * ROWS;
   static constexpr int N = (COLS + 15) / 16 * 16;             // score columns of a group (N of the product)
-  static constexpr int STRIDE = N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128;  // TMEM columns of a score slot
-  static constexpr int OCOLS = ATTEND ? 256 : 0;              // O^T of the two streams (P's row is 128 bytes)
+  static constexpr int STRIDE = N <= 16 ? 16 : N <= 32 ? 32 : 64;  // TMEM columns of a score slot
+  static constexpr int OCOLS = ATTEND ? kStreams * kPRow : 0;  // O^T of the streams
   static constexpr int SLOTS_FIT = (512 - OCOLS) / STRIDE;
-  static constexpr int NS = SLOTS_FIT < 4 ? SLOTS_FIT : 4;
+  static constexpr int NS = SLOTS_FIT < 8 ? SLOTS_FIT : 8;
   static constexpr int Q_GROUP = F8 ? N * 128 : 2 * N * 128;  // bytes of one group's Q operand
   static constexpr int Q_BYTES = G * Q_GROUP;
   static constexpr int TILES = ATTEND || !F8 ? 2 : 1;         // 16 KB tiles of a block (K and V, or K's two halves)
-  static constexpr int CH = ROWS < 16 ? ROWS : 16;            // rows handled at once
-  static_assert(PARTS * ROWS <= 128 && NS >= 2, "columns");
+  static_assert(COLS <= kPRow && NS >= kStreams && kStreams % G == 0, "columns");
 };
 
 struct ScaledTcParams {
@@ -100,26 +104,26 @@ struct ScaledTcParams {
 
 struct TcSmem {
   uint8_t* ring;
-  uint8_t* p;  // two P buffers
+  uint8_t* p;  // a P buffer for each stream
   uint8_t* q;  // two Q slots
   float4* meta;     // [kMetaSlots][8]: ks, log2 vs, 1 / vs, page id (bits)
-  float* base;      // [2][32]: a stream's bases (weights: -lse of the rows, [64])
-  float* delta;     // [2][32]: what a base was raised by; the epilogue's factors of O
-  float* wred;      // [8][32]: per-warp maxima, then per-warp sums
-  int* nan_from;    // [2][128]
+  float* base;      // [4][16]: a stream's bases (weights: -lse of the rows, [64])
+  float* delta;     // [4][16]: what a base was raised by; the epilogue's factors of O
+  float* wred;      // [16][16]: per-warp maxima, then per-warp sums
+  int* nan_from;    // [4][128]
   float* cq;        // [2]: log2-domain score factor of a Q slot
-  unsigned int* qtop;  // [8]
+  unsigned int* qtop;  // [16]
   uint64_t *full, *empty, *s_full, *s_empty, *p_full, *p_done, *q_ready, *m_full, *m_empty, *done;
   uint32_t* tmem_base;
   Schedule* sch;
 };
 
-constexpr int kFixedBytes = kMetaSlots * 8 * 16 + (64 + 64 + 8 * 32 + 2 * 128 + 2 + 8 + 6) * 4 +
-                            (2 * 4 + 2 + 2 + 2 + 2 * kMetaSlots + 1) * 8 + 64;
+constexpr int kFixedBytes = kMetaSlots * 8 * 16 + (64 + 64 + 256 + kStreams * 128 + 4 + 16) * 4 +
+                            (2 * 8 + 2 * kStreams + 2 + 2 * kMetaSlots + 1) * 8 + 64;
 
 template <class S>
 __host__ __device__ constexpr int fixed_smem() {
-  return 1024 + (S::ATTEND ? 2 * kPBytes : 0) + 2 * S::Q_BYTES + kFixedBytes;
+  return 1024 + (S::ATTEND ? kStreams * kPBytes : 0) + 2 * S::Q_BYTES + kFixedBytes;
 }
 
 template <class S>
@@ -127,22 +131,22 @@ __device__ __forceinline__ TcSmem carve(uint8_t* smem, int tiles) {
   TcSmem t;
   t.ring = smem;
   t.p = smem + (size_t)tiles * kTileBytes;
-  t.q = t.p + (S::ATTEND ? 2 * kPBytes : 0);
+  t.q = t.p + (S::ATTEND ? kStreams * kPBytes : 0);
   t.meta = reinterpret_cast<float4*>(t.q + 2 * S::Q_BYTES);
   t.base = reinterpret_cast<float*>(t.meta + kMetaSlots * 8);
   t.delta = t.base + 64;
   t.wred = t.delta + 64;
-  t.nan_from = reinterpret_cast<int*>(t.wred + 8 * 32);
-  t.cq = reinterpret_cast<float*>(t.nan_from + 2 * 128);
-  t.qtop = reinterpret_cast<unsigned int*>(t.cq + 2);
-  uint64_t* b = reinterpret_cast<uint64_t*>(t.qtop + 8 + 6);
+  t.nan_from = reinterpret_cast<int*>(t.wred + 256);
+  t.cq = reinterpret_cast<float*>(t.nan_from + kStreams * 128);
+  t.qtop = reinterpret_cast<unsigned int*>(t.cq + 4);
+  uint64_t* b = reinterpret_cast<uint64_t*>(t.qtop + 16);
   t.full = b;
   t.empty = t.full + tiles;
   t.s_full = t.empty + tiles;
-  t.s_empty = t.s_full + 4;
-  t.p_full = t.s_empty + 4;
-  t.p_done = t.p_full + 2;
-  t.q_ready = t.p_done + 2;
+  t.s_empty = t.s_full + 8;
+  t.p_full = t.s_empty + 8;
+  t.p_done = t.p_full + kStreams;
+  t.q_ready = t.p_done + kStreams;
   t.m_full = t.q_ready + 2;
   t.m_empty = t.m_full + kMetaSlots;
   t.done = t.m_empty + kMetaSlots;
@@ -305,24 +309,37 @@ __device__ __forceinline__ void drain_products(const ScaledTcParams& p, const Tc
     atomicOr(p.s.status, 1u);
 }
 
+// A running position in the ring of tiles.
+struct RingPos {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int tiles) {
+    if (++slot == tiles) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
 // S^T of (block, group) unit u into score slot u % NS.
 template <class S, bool BF>
 __device__ void issue_scores(const ScaledTcParams& p, const Schedule& sch, const TcSmem& sm, uint32_t tmem, int tiles,
                              volatile int* abort) {
   constexpr uint32_t kIdesc = mma_idesc_f16(128, S::N, false, false, BF && !S::F8);  // format 0: e4m3 / fp16
-  int u = 0, blk = 0, pc = 0;
+  int u = 0, pc = 0;
+  RingPos at;
   for_pieces(p.s, sch, [&](const SegWalk&, int, int n) {
     mbar_wait_bounded(smem_u32(sm.q_ready + (pc & 1)), (uint32_t)(pc >> 1) & 1u, abort, p.s.status, 4, pc);
     const uint32_t q = smem_u32(sm.q + (pc & 1) * S::Q_BYTES);
     const int nblk = blocks_of(n);
-    for (int k = 0; k < nblk; ++k, ++blk) {
-      const int t0 = blk * S::TILES;  // tile index of K (its first half)
-      mbar_wait_bounded(smem_u32(sm.full + t0 % tiles), (uint32_t)(t0 / tiles) & 1u, abort, p.s.status, 5, blk);
-      if (!S::F8) {
-        const int t1 = t0 + 1;
-        mbar_wait_bounded(smem_u32(sm.full + t1 % tiles), (uint32_t)(t1 / tiles) & 1u, abort, p.s.status, 5, blk);
-      }
-#pragma unroll
+    for (int k = 0; k < nblk; ++k) {
+      const int k0 = at.slot;  // K's tile (its first half)
+      mbar_wait_bounded(smem_u32(sm.full + at.slot), at.phase, abort, p.s.status, 5, u);
+      at.next(tiles);
+      const int k1 = at.slot;
+      if (!S::F8) mbar_wait_bounded(smem_u32(sm.full + at.slot), at.phase, abort, p.s.status, 5, u);
+      if (S::TILES == 2) at.next(tiles);  // K's second half, or V
+#pragma unroll 1
       for (int g = 0; g < S::G; ++g, ++u) {
         if (u >= S::NS)
           mbar_wait_bounded(smem_u32(sm.s_empty + u % S::NS), (uint32_t)(u / S::NS - 1) & 1u, abort, p.s.status, 6, u);
@@ -331,24 +348,23 @@ __device__ void issue_scores(const ScaledTcParams& p, const Schedule& sch, const
         if (elect_one()) {
           const uint32_t d = tmem + S::OCOLS + (u % S::NS) * S::STRIDE;
           const uint32_t qg = q + g * S::Q_GROUP;
+          const uint32_t kt = smem_u32(sm.ring + (size_t)k0 * kTileBytes);
           if constexpr (S::F8) {
-            const uint32_t kt = smem_u32(sm.ring + (size_t)(t0 % tiles) * kTileBytes);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)  // 32 dims (32 B) a step
               tc_mma_ss_f8(d, smem_desc_sw128(kt + kk * 32, 16, 1024), smem_desc_sw128(qg + kk * 32, 16, 1024), kIdesc,
                            kk > 0 ? 1u : 0u);
           } else {
+            const uint32_t kt1 = smem_u32(sm.ring + (size_t)k1 * kTileBytes);
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk) {  // 16 dims (32 B) a step, four to a half
-              const uint32_t kt = smem_u32(sm.ring + (size_t)((t0 + (kk >> 2)) % tiles) * kTileBytes);
-              tc_mma_ss(d, smem_desc_sw128(kt + (kk & 3) * 32, 16, 1024),
+            for (int kk = 0; kk < 8; ++kk)  // 16 dims (32 B) a step, four to a half
+              tc_mma_ss(d, smem_desc_sw128((kk < 4 ? kt : kt1) + (kk & 3) * 32, 16, 1024),
                         smem_desc_sw128(qg + (kk >> 2) * (S::N * 128) + (kk & 3) * 32, 16, 1024), kIdesc, kk > 0 ? 1u : 0u);
-            }
           }
           tc_commit(smem_u32(sm.s_full + u % S::NS));
           if (g == S::G - 1) {  // the block's K may be overwritten
-            tc_commit(smem_u32(sm.empty + t0 % tiles));
-            if (!S::F8) tc_commit(smem_u32(sm.empty + (t0 + 1) % tiles));
+            tc_commit(smem_u32(sm.empty + k0));
+            if (!S::F8) tc_commit(smem_u32(sm.empty + k1));
           }
         }
         __syncwarp();
@@ -359,52 +375,69 @@ __device__ void issue_scores(const ScaledTcParams& p, const Schedule& sch, const
   drain_products(p, sm);
 }
 
-// O^T of stream u & 1 += V^T P^T of unit u, once P is in the stream's buffer.
+// Descriptor of P, MN-major with 64-byte rows (one atom of 64 rows x 8 tokens, 512 B; 64-byte swizzle).
+__device__ __forceinline__ uint64_t desc_p(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)((kPBytes >> 4) & 0x3FFFu) << 16;     // between atoms along the rows: there is one
+  d |= (uint64_t)((8 * kPRow >> 4) & 0x3FFFu) << 32;   // between groups of 8 tokens
+  d |= (uint64_t)1 << 46;                              // version
+  d |= (uint64_t)4 << 61;                              // SWIZZLE_64B
+  return d;
+}
+
+// O^T of stream u % 4 += V^T P^T of unit u, once P is in the stream's buffer.
 template <class S>
 __device__ void issue_values(const ScaledTcParams& p, const Schedule& sch, const TcSmem& sm, uint32_t tmem, int tiles,
                              volatile int* abort) {
-  constexpr uint32_t kIdesc = mma_idesc_f16(128, 128, true, true, false);
-  int u = 0, blk = 0;
+  constexpr uint32_t kIdesc = mma_idesc_f16(128, kPRow, true, true, false);
+  int u = 0;
+  RingPos at;
   for_pieces(p.s, sch, [&](const SegWalk&, int, int n) {
     const int nblk = blocks_of(n);
-    for (int k = 0; k < nblk; ++k, ++blk) {
-      const int t1 = blk * 2 + 1;
+    for (int k = 0; k < nblk; ++k) {
+      at.next(tiles);  // over K
       const int np = min(kBlockPages, n - k * kBlockPages);
-#pragma unroll
+      mbar_wait_bounded(smem_u32(sm.full + at.slot), at.phase, abort, p.s.status, 8, u);
+#pragma unroll 1
       for (int g = 0; g < S::G; ++g, ++u) {
-        mbar_wait_bounded(smem_u32(sm.p_full + (u & 1)), (uint32_t)(u >> 1) & 1u, abort, p.s.status, 7, u);
-        if (g == 0)
-          mbar_wait_bounded(smem_u32(sm.full + t1 % tiles), (uint32_t)(t1 / tiles) & 1u, abort, p.s.status, 8, blk);
+        const int st = u & (kStreams - 1);
+        mbar_wait_bounded(smem_u32(sm.p_full + st), (uint32_t)(u / kStreams) & 1u, abort, p.s.status, 7, u);
         __syncwarp();
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t v = smem_u32(sm.ring + (size_t)(t1 % tiles) * kTileBytes);
-          const uint32_t pb = smem_u32(sm.p + (u & 1) * kPBytes);
+          const uint32_t v = smem_u32(sm.ring + (size_t)at.slot * kTileBytes);
+          const uint32_t pb = smem_u32(sm.p + st * kPBytes);
           const int steps = (np + 1) / 2;  // 32 tokens a step; the softmax zeroed an absent page's V
+          // a stream's first product of a piece overwrites O
           for (int kk = 0; kk < steps; ++kk)
-            tc_mma_ss_f8(tmem + (u & 1) * 128, smem_desc_sw128(v + kk * 4096, kTileBytes, 1024),
-                         smem_desc_sw128(pb + kk * 4096, kTileBytes, 1024), kIdesc,
-                         (k >= 3 - S::G || kk > 0) ? 1u : 0u);  // a stream's first product of a piece overwrites O
-          tc_commit(smem_u32(sm.p_done + (u & 1)));
-          if (g == S::G - 1) tc_commit(smem_u32(sm.empty + t1 % tiles));
+            tc_mma_ss_f8(tmem + st * kPRow, smem_desc_sw128(v + kk * 4096, kTileBytes, 1024), desc_p(pb + kk * 32 * kPRow),
+                         kIdesc, (k >= kStreams / S::G || kk > 0) ? 1u : 0u);
+          tc_commit(smem_u32(sm.p_done + st));
+          if (g == S::G - 1) tc_commit(smem_u32(sm.empty + at.slot));
         }
         __syncwarp();
       }
+      at.next(tiles);
     }
   });
   drain_products(p, sm);
 }
 
 // ------------------------------------------------------------------ softmax warps (128 threads)
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[2]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[8]) { tmem_ld8(taddr, r); }
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
-__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[8]) { tmem_st8(taddr, r); }
-__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[16]) { tmem_st16(taddr, r); }
 
 // Barrier of a softmax warpgroup; true when `v` is for any of its threads.
 __device__ __forceinline__ bool group_any(int stream, bool v) {
@@ -420,13 +453,7 @@ __device__ __forceinline__ bool group_any(int stream, bool v) {
   return r != 0;
 }
 __device__ __forceinline__ void group_sync(int stream) { named_bar_sync(1 + stream, 128); }
-__device__ __forceinline__ void softmax_sync() { named_bar_sync(3, kSoftmaxThreads); }
-
-__device__ __forceinline__ int float_order(float f) {  // order-preserving int
-  const int i = __float_as_int(f);
-  return i ^ ((i >> 31) & 0x7fffffff);
-}
-__device__ __forceinline__ float order_float(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
+__device__ __forceinline__ void softmax_sync() { named_bar_sync(1 + kStreams, kSoftmaxThreads); }
 
 __device__ __forceinline__ uint32_t e4m3x2_of_half2(__half2 h) {
   return (uint32_t)__nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&h), __NV_SATFINITE, __NV_E4M3);
@@ -474,70 +501,63 @@ __device__ __forceinline__ void split_q(float (&x)[4], uint32_t (&out)[3]) {
   }
 }
 
-// Q of (b, h) as the N operand of the score product, into slot `qs`: row r of part i is operand row
-// i * ROWS + r (128 B, 128-byte swizzle), and the slot's score factor.  All softmax threads, eight to
-// a row.
+// Q of (b, h) as the N operand of the score product: row r of part i is operand row i * ROWS + r of its
+// group (128 B, 128-byte swizzle).  All softmax threads, eight to a row, 16 dims each.
+struct QItem {
+  uint4 x[2];
+  uint32_t top;  // the row's largest magnitude, as bits (above every finite one for infinity and NaN)
+};
+
+// The thread's part of Q into registers, and the warp's largest finite magnitude into qtop.
 template <class S, bool BF>
-__device__ void write_q(const ScaledTcParams& p, const TcSmem& sm, int b, int h, int qs) {
-  constexpr int kItems = S::G * S::ROWS * 8;
-  constexpr int kSteps = (kItems + kSoftmaxThreads - 1) / kSoftmaxThreads;
-  const int tid = threadIdx.x;
-  const int rows = kGroup * p.s.q_len;
-  uint4 x[kSteps][2];
-  uint32_t top[kSteps];  // a row's largest magnitude, as bits (above every finite one for infinity and NaN)
-  uint32_t most = 0;     // the largest of a finite row
-#pragma unroll
-  for (int st = 0; st < kSteps; ++st) {
-    const int it = st * kSoftmaxThreads + tid, r = it >> 3, c = it & 7;  // row, its 16 dims
-    x[st][0] = x[st][1] = make_uint4(0u, 0u, 0u, 0u);
-    if (r < rows) {
-      const __half* src =
-          p.s.q + ((size_t)(b * p.s.q_len + (r >> 2)) * p.s.hq + h * kGroup + (r & 3)) * kHeadDim + c * 16;
-      x[st][0] = __ldg(reinterpret_cast<const uint4*>(src));
-      x[st][1] = __ldg(reinterpret_cast<const uint4*>(src) + 1);
-    }
+__device__ __forceinline__ QItem load_q(const ScaledTcParams& p, const TcSmem& sm, int b, int h) {
+  const int r = threadIdx.x >> 3, c = threadIdx.x & 7;
+  QItem q;
+  q.x[0] = q.x[1] = make_uint4(0u, 0u, 0u, 0u);
+  q.top = 0;
+  if (r < kGroup * p.s.q_len) {
+    const __half* src = p.s.q + ((size_t)(b * p.s.q_len + (r >> 2)) * p.s.hq + h * kGroup + (r & 3)) * kHeadDim + c * 16;
+    q.x[0] = __ldg(reinterpret_cast<const uint4*>(src));
+    q.x[1] = __ldg(reinterpret_cast<const uint4*>(src) + 1);
   }
   if constexpr (S::F8) {
+    const uint32_t w[8] = {q.x[0].x, q.x[0].y, q.x[0].z, q.x[0].w, q.x[1].x, q.x[1].y, q.x[1].z, q.x[1].w};
 #pragma unroll
-    for (int st = 0; st < kSteps; ++st) {
-      const uint32_t w[8] = {x[st][0].x, x[st][0].y, x[st][0].z, x[st][0].w,
-                             x[st][1].x, x[st][1].y, x[st][1].z, x[st][1].w};
-      uint32_t t = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 a = unpack2<BF>(w[i]);
-        t = max(t, max(__float_as_uint(a.x) & 0x7fffffffu, __float_as_uint(a.y) & 0x7fffffffu));
-      }
-#pragma unroll
-      for (int off = 1; off < 8; off <<= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, off));
-      top[st] = t;
-      if (t < 0x7f800000u) most = max(most, t);
+    for (int i = 0; i < 8; ++i) {
+      const float2 a = unpack2<BF>(w[i]);
+      q.top = max(q.top, max(__float_as_uint(a.x) & 0x7fffffffu, __float_as_uint(a.y) & 0x7fffffffu));
     }
-    most = __reduce_max_sync(0xffffffffu, most);
-    softmax_sync();  // the last call's reads of qtop are done
-    if ((tid & 31) == 0) sm.qtop[tid >> 5] = most;
-    softmax_sync();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) most = max(most, sm.qtop[i]);
+    for (int off = 1; off < 8; off <<= 1) q.top = max(q.top, __shfl_xor_sync(0xffffffffu, q.top, off));
+    const uint32_t most = __reduce_max_sync(0xffffffffu, q.top < 0x7f800000u ? q.top : 0u);
+    if ((threadIdx.x & 31) == 0) sm.qtop[threadIdx.x >> 5] = most;
+  }
+  return q;
+}
+
+// After a barrier of the softmax threads: the thread's part of Q into slot `qs`.
+template <class S, bool BF>
+__device__ __forceinline__ void write_q(const ScaledTcParams& p, const TcSmem& sm, const QItem& q, int qs) {
+  const int r = threadIdx.x >> 3, c = threadIdx.x & 7;
+  uint32_t most = 0;
+  if constexpr (S::F8) {
+#pragma unroll
+    for (int i = 0; i < kSoftmaxThreads / 32; ++i) most = max(most, sm.qtop[i]);
   }
   // 2^e brings the largest magnitude into [128, 256)
   const int e = most > 0 ? max(-110, min(110, 134 - (int)(most >> 23))) : 0;
-  const float sc = __uint_as_float((uint32_t)(127 + e) << 23);
-  if (tid == 0) sm.cq[qs] = p.s.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll
-  for (int st = 0; st < kSteps; ++st) {
-    const int it = st * kSoftmaxThreads + tid, r = it >> 3, c = it & 7;
-    if (it >= kItems) break;
+  if (threadIdx.x == 0) sm.cq[qs] = p.s.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23);
+  if (r < S::G * S::ROWS) {
     const int rr = r % S::ROWS;
     uint8_t* const dst = sm.q + qs * S::Q_BYTES + (r / S::ROWS) * S::Q_GROUP;
     if constexpr (!S::F8) {  // 32 bytes of half c / 4: chunks 2 (c % 4) and the next
       uint8_t* const row = dst + (c >> 2) * (S::N * 128) + (rr >> 3) * 1024 + (rr & 7) * 128;
       const int c0 = (c & 3) * 2;
-      *reinterpret_cast<uint4*>(row + ((c0 ^ (rr & 7)) << 4)) = x[st][0];
-      *reinterpret_cast<uint4*>(row + (((c0 + 1) ^ (rr & 7)) << 4)) = x[st][1];
+      *reinterpret_cast<uint4*>(row + ((c0 ^ (rr & 7)) << 4)) = q.x[0];
+      *reinterpret_cast<uint4*>(row + (((c0 + 1) ^ (rr & 7)) << 4)) = q.x[1];
     } else {
-      const uint32_t w[8] = {x[st][0].x, x[st][0].y, x[st][0].z, x[st][0].w,
-                             x[st][1].x, x[st][1].y, x[st][1].z, x[st][1].w};
+      const float sc = __uint_as_float((uint32_t)(127 + e) << 23);
+      const uint32_t w[8] = {q.x[0].x, q.x[0].y, q.x[0].z, q.x[0].w, q.x[1].x, q.x[1].y, q.x[1].z, q.x[1].w};
       uint32_t part[3][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -547,7 +567,7 @@ __device__ void write_q(const ScaledTcParams& p, const TcSmem& sm, int b, int h,
         split_q<S::PARTS>(y, o);
 #pragma unroll
         for (int k = 0; k < S::PARTS; ++k)  // a row with an infinity or NaN is NaN
-          part[k][i] = top[st] < 0x7f800000u ? o[k] : 0x7f7f7f7fu;
+          part[k][i] = q.top < 0x7f800000u ? o[k] : 0x7f7f7f7fu;
       }
 #pragma unroll
       for (int k = 0; k < S::PARTS; ++k) {
@@ -559,37 +579,35 @@ __device__ void write_q(const ScaledTcParams& p, const TcSmem& sm, int b, int h,
   }
   fence_proxy_async_smem();
   __syncwarp();
-  if ((tid & 31) == 0) mbar_arrive(smem_u32(sm.q_ready + qs));
+  if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(sm.q_ready + qs));
 }
 
-// Rows [c, c + CH) of a score slot, its parts joined.
+// Rows [c, c + 8) of a score slot, its parts joined.
 template <class S>
-__device__ __forceinline__ void read_scores(uint32_t slot, int c, float (&s)[S::CH]) {
-  if constexpr (S::F8) {
-    uint32_t raw[3][S::CH];
+__device__ __forceinline__ void read_scores(uint32_t slot, int c, float (&s)[8]) {
+  constexpr int kParts = S::F8 ? S::PARTS : 1;
+  uint32_t raw[kParts][8];
 #pragma unroll
-    for (int i = 0; i < S::PARTS; ++i) tmem_ld(slot + i * S::ROWS + c, raw[i]);
-    tmem_wait_ld();
+  for (int i = 0; i < kParts; ++i) tmem_ld(slot + i * S::ROWS + c, raw[i]);
+  tmem_wait_ld();
 #pragma unroll
-    for (int r = 0; r < S::CH; ++r) {
-      float x = __uint_as_float(raw[S::PARTS - 1][r]);
+  for (int r = 0; r < 8; ++r) {
+    float x = __uint_as_float(raw[kParts - 1][r]);
 #pragma unroll
-      for (int i = S::PARTS - 2; i >= 0; --i) x = fmaf(x, 1.f / 32.f, __uint_as_float(raw[i][r]));
-      s[r] = x;
-    }
-  } else {
-    uint32_t raw[S::CH];
-    tmem_ld(slot + c, raw);
-    tmem_wait_ld();
-#pragma unroll
-    for (int r = 0; r < S::CH; ++r) s[r] = __uint_as_float(raw[r]);
+    for (int i = kParts - 2; i >= 0; --i) x = fmaf(x, 1.f / 32.f, __uint_as_float(raw[i][r]));
+    s[r] = x;
   }
 }
 
-// Sum of each row over the warp's lanes: lane l gets row l / (32 / ROWS).
-template <int ROWS>
-__device__ __forceinline__ float sum_rows(float (&v)[ROWS]) {
+// Each row's sum or maximum over the warp's lanes: lane l gets row l / (32 / ROWS).  Halves the rows a
+// lane holds at each step (ROWS + 1 shuffles instead of 5 ROWS).
+template <int ROWS, bool MAX>
+__device__ __forceinline__ float reduce_rows(const float (&in)[ROWS]) {
+  auto join = [](float a, float b) { return MAX ? fmaxf(a, b) : a + b; };
   const int lane = threadIdx.x & 31;
+  float v[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) v[i] = in[i];
   int n = ROWS;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
@@ -600,11 +618,11 @@ __device__ __forceinline__ float sum_rows(float (&v)[ROWS]) {
       for (int i = 0; i < ROWS / 2; ++i) {
         if (i < n) {
           const float mine = upper ? v[i + n] : v[i], other = upper ? v[i] : v[i + n];
-          v[i] = mine + __shfl_xor_sync(0xffffffffu, other, off);
+          v[i] = join(mine, __shfl_xor_sync(0xffffffffu, other, off));
         }
       }
     } else {
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
+      v[0] = join(v[0], __shfl_xor_sync(0xffffffffu, v[0], off));
     }
   }
   return v[0];
@@ -628,11 +646,11 @@ __device__ __forceinline__ float unit_scores(uint32_t slot, const float* base, f
                                              float (&t)[S::ROWS]) {
   float over = -INFINITY;
 #pragma unroll
-  for (int c = 0; c < S::ROWS; c += S::CH) {
-    float s[S::CH];
+  for (int c = 0; c < S::ROWS; c += 8) {
+    float s[8];
     read_scores<S>(slot, c, s);
 #pragma unroll
-    for (int r = 0; r < S::CH; r += 4) {
+    for (int r = 0; r < 8; r += 4) {
       const float4 b4 = *reinterpret_cast<const float4*>(base + c + r);
       const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
@@ -647,32 +665,43 @@ __device__ __forceinline__ float unit_scores(uint32_t slot, const float* base, f
   return over;
 }
 
+// The scales of block bk's page of this thread's token.
+__device__ __forceinline__ float4 read_meta(const ScaledTcParams& p, const TcSmem& sm, int bk, volatile int* abort) {
+  const int e = bk % kMetaSlots;
+  mbar_wait_bounded(smem_u32(sm.m_full + e), (uint32_t)(bk / kMetaSlots) & 1u, abort, p.s.status, 3, bk);
+  const float4 m = sm.meta[e * kBlockPages + ((threadIdx.x & 127) >> 4)];
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(sm.m_empty + e));
+  return m;
+}
+
 template <class S, bool BF>
 __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSmem& sm, uint32_t tmem, int tiles,
                        volatile int* abort) {
-  constexpr int ROWS = S::ROWS, G = S::G, CH = S::CH;
+  constexpr int ROWS = S::ROWS, G = S::G, PARTS = S::PARTS;
+  constexpr int kStep = kStreams / G;  // blocks from unit to unit of a stream
   const int stream = threadIdx.x >> 7;
   const int tid = threadIdx.x & 127, warp = tid >> 5, lane = tid & 31;  // tid: token of a block, dimension of O
   const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
   const int rows = kGroup * p.s.q_len;
-  const int row0 = G == 2 ? stream * ROWS : 0;  // the stream's first row
-  float* const base = sm.base + stream * 32;
-  float* const delta = sm.delta + stream * 32;
-  float* const wred = sm.wred + stream * 4 * 32;
+  const int group = stream % G;  // the stream's rows: row0 .. row0 + ROWS - 1
+  const int row0 = group * ROWS;
+  float* const base = sm.base + stream * 16;
+  float* const delta = sm.delta + stream * 16;
+  float* const wred = sm.wred + stream * 4 * 16;
   int blk = 0, pc = 0;
   for_pieces(p.s, sch, [&](const SegWalk& w, int unit, int n) {
     const int seg = w.b * p.s.hkv + w.h;
     const int seg_end = w.seg_start + w.pages;
     const bool whole = unit == w.seg_start && seg_end <= sch.end;
     const Piece piece = piece_of(p.s, w);
-    if (pc == 0) write_q<S, BF>(p, sm, w.b, w.h, 0);
-    if (seg_end < sch.end) {  // Q of the next piece, whose slot the piece before this one is done with
-      SegWalk nw = w;
-      next_segment(p.s, nw);
-      write_q<S, BF>(p, sm, nw.b, nw.h, (pc + 1) & 1);
+    if (pc == 0) {
+      const QItem q = load_q<S, BF>(p, sm, w.b, w.h);
+      if (tid < ROWS) base[tid] = 0.f;
+      softmax_sync();
+      write_q<S, BF>(p, sm, q, 0);
+      softmax_sync();
     }
-    if (tid < ROWS) base[tid] = 0.f;
-    softmax_sync();
     const float cq = sm.cq[pc & 1];
     float l[ROWS];
 #pragma unroll
@@ -680,28 +709,24 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
     int nan_from = 0x7fffffff;  // first draft token whose V is NaN in dimension tid
 
     const int nblk = blocks_of(n);
-    const int k0 = G == 2 ? 0 : (blk ^ stream) & 1;  // the stream's first block of the piece
-    for (int k = k0; k < nblk; k += 3 - G) {
+    const int k0 = (stream / G - blk) & (kStep - 1);  // the stream's first block of the piece
+    float4 meta = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (k0 < nblk) meta = read_meta(p, sm, blk + k0, abort);
+    for (int k = k0; k < nblk; k += kStep) {
       const int bk = blk + k;
-      const int u = G == 2 ? 2 * bk + stream : bk;
-      const int v = u >> 1;  // the stream's own count
+      const int u = bk * G + group;
+      const int v = u / kStreams;  // the stream's own count
       const int np = min(kBlockPages, n - k * kBlockPages);
       const int tok0 = (w.pg + k * kBlockPages) * kPageSize;
       const int tok = tok0 + tid;
-      const int e = bk % kMetaSlots;
-      mbar_wait_bounded(smem_u32(sm.m_full + e), (uint32_t)(bk / kMetaSlots) & 1u, abort, p.s.status, 3, bk);
-      const float4 meta = sm.meta[e * kBlockPages + (tid >> 4)];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(sm.m_empty + e));
-      const float kc = meta.x * cq;
       const bool masked = np < kBlockPages || tok0 + kBlock > piece.first || tok0 + kBlock > piece.len;
       // draft qi sees the token iff late < qi (every draft when negative)
       const int late = (tid < np * kPageSize && tok < piece.len) ? tok - piece.first : 0x7fffffff;
 
-      if (masked && (G == 1 || stream == 0)) {
+      if (masked && group == 0) {
         // V rows behind the sequence and of absent pages: zero (they may hold NaN); draft tokens'
-        // NaN: zero, and remembered by the dimension's thread.  (Two groups: the first one's product
-        // comes first.)
+        // NaN: zero, and remembered by the dimension's thread.  (The block's first group does it: its
+        // product comes first.)
         const int t1 = bk * 2 + 1;  // V's tile
         mbar_wait_bounded(smem_u32(sm.full + t1 % tiles), (uint32_t)(t1 / tiles) & 1u, abort, p.s.status, 9, bk);
         uint8_t* const vt = sm.ring + (size_t)(t1 % tiles) * kTileBytes;
@@ -723,23 +748,25 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
       tc_fence_after();
       const uint32_t slot = lanes + S::OCOLS + (u % S::NS) * S::STRIDE;
       float t[ROWS];
+      const float kc = meta.x * cq;
       const float over = masked ? unit_scores<S, true>(slot, base, kc, meta.y, late, row0, t)
                                 : unit_scores<S, false>(slot, base, kc, meta.y, late, row0, t);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(sm.s_empty + u % S::NS));
+      const float inv_vs = meta.z;
+      if (k + kStep < nblk) meta = read_meta(p, sm, bk + kStep, abort);  // off the next unit's path
       const bool first = k == k0;
       const bool raise = group_any(stream, over > kRaise) || first;  // rare after a piece's first blocks
       if (raise) {
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-          const int m = __reduce_max_sync(0xffffffffu, float_order(t[r] == t[r] ? t[r] : -INFINITY));
-          if (lane == r) wred[warp * 32 + r] = order_float(m);
-        }
+        for (int r = 0; r < ROWS; ++r) t[r] = t[r] == t[r] ? t[r] : INFINITY;  // NaN: the row will be NaN
+        const float m = reduce_rows<ROWS, true>(t);
+        if (lane % (32 / ROWS) == 0) wred[warp * 16 + lane / (32 / ROWS)] = m;
         group_sync(stream);
         if (tid < ROWS) {
-          const float m = fmaxf(fmaxf(wred[tid], wred[32 + tid]), fmaxf(wred[64 + tid], wred[96 + tid]));
-          const float d = (m > kRaise || (first && m != -INFINITY)) ? m - kHead : 0.f;
+          const float m4 = fmaxf(fmaxf(wred[tid], wred[16 + tid]), fmaxf(wred[32 + tid], wred[48 + tid]));
+          const float d = (m4 > kHead || (first && m4 != -INFINITY)) ? m4 - kHead : 0.f;
           delta[tid] = d;
           base[tid] += d;
         }
@@ -752,53 +779,51 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
       if (raise && !first) {
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < ROWS; c += CH) {
-          float a[CH];
+        for (int c = 0; c < ROWS; c += 8) {
+          float a[8];
 #pragma unroll
-          for (int r = 0; r < CH; ++r) {
+          for (int r = 0; r < 8; ++r) {
             a[r] = ex2(-delta[c + r]);
             l[c + r] *= a[r];
           }
 #pragma unroll
-          for (int i = 0; i < S::PARTS; ++i) {
-            uint32_t o[CH];
-            tmem_ld(lanes + stream * 128 + i * ROWS + c, o);
+          for (int i = 0; i < PARTS; ++i) {
+            uint32_t o[8];
+            tmem_ld(lanes + stream * kPRow + i * ROWS + c, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int r = 0; r < CH; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * a[r]);
-            tmem_st(lanes + stream * 128 + i * ROWS + c, o);
+            for (int r = 0; r < 8; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * a[r]);
+            tmem_st8(lanes + stream * kPRow + i * ROWS + c, o);
           }
         }
         tmem_wait_st();
       }
-      // P: token tid's operand row of 128 bytes, part i of row r in byte i * ROWS + r
-      uint8_t* const prow = sm.p + stream * kPBytes + (tid >> 3) * 1024 + (tid & 7) * 128;
+      // P: token tid's operand row of 64 bytes, part i of row r in byte i * ROWS + r; 16-byte chunks
+      // swizzled by token / 2
+      uint8_t* const prow = sm.p + stream * kPBytes + tid * kPRow;
+      uint32_t part[3][ROWS / 4];
 #pragma unroll
-      for (int c = 0; c < ROWS; c += CH) {
-        uint32_t part[3][CH / 4];
+      for (int r = 0; r < ROWS; r += 4) {
+        float x[4];
 #pragma unroll
-        for (int r = 0; r < CH; r += 4) {
-          float x[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x[i] = ex2(t[c + r + i]);
-            l[c + r + i] = fmaf(x[i], meta.z, l[c + r + i]);
-          }
-          uint32_t lo[3], hi[3];
-          split_p<S::PARTS>(x[0], x[1], lo);
-          split_p<S::PARTS>(x[2], x[3], hi);
-#pragma unroll
-          for (int i = 0; i < S::PARTS; ++i) part[i][r / 4] = lo[i] | (hi[i] << 16);
+        for (int i = 0; i < 4; ++i) {
+          x[i] = ex2(t[r + i]);
+          l[r + i] = fmaf(x[i], inv_vs, l[r + i]);
         }
+        uint32_t lo[3], hi[3];
+        split_p<PARTS>(x[0], x[1], lo);
+        split_p<PARTS>(x[2], x[3], hi);
 #pragma unroll
-        for (int i = 0; i < S::PARTS; ++i) {
-          const int byte = i * ROWS + c;
-          uint8_t* const at = prow + (((byte >> 4) ^ (tid & 7)) << 4) + (byte & 15);
-          if constexpr (CH == 16)
-            *reinterpret_cast<uint4*>(at) = make_uint4(part[i][0], part[i][1], part[i][2], part[i][3]);
-          else
-            *reinterpret_cast<uint2*>(at) = make_uint2(part[i][0], part[i][1]);
-        }
+        for (int i = 0; i < PARTS; ++i) part[i][r / 4] = lo[i] | (hi[i] << 16);
+      }
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) {
+        const int byte = i * ROWS;
+        uint8_t* const at = prow + (((byte >> 4) ^ ((tid >> 1) & 3)) << 4) + (byte & 15);
+        if constexpr (ROWS == 16)
+          *reinterpret_cast<uint4*>(at) = make_uint4(part[i][0], part[i][1], part[i][2], part[i][3]);
+        else
+          *reinterpret_cast<uint2*>(at) = make_uint2(part[i][0], part[i][1]);
       }
       fence_proxy_async_smem();
       tc_fence_before();
@@ -807,72 +832,82 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
     }
 
     // ---- epilogue: denominators and factors, then each dimension's thread joins its rows' parts
-    const float total = sum_rows<ROWS>(l);
-    if (lane % (32 / ROWS) == 0) wred[warp * 32 + lane / (32 / ROWS)] = total;
+    const bool more = seg_end < sch.end;  // another piece follows: its Q, for the score products
+    QItem q;
+    if (more) {
+      SegWalk nw = w;
+      next_segment(p.s, nw);
+      q = load_q<S, BF>(p, sm, nw.b, nw.h);
+    }
+    const float total = reduce_rows<ROWS, false>(l);
+    if (lane % (32 / ROWS) == 0) wred[warp * 16 + lane / (32 / ROWS)] = total;
     sm.nan_from[threadIdx.x] = nan_from;
     softmax_sync();
+    if (more) write_q<S, BF>(p, sm, q, (pc + 1) & 1);
     const int slot = (int)blockIdx.x + seg;  // workspace piece
     if (threadIdx.x < rows) {
-      const int row = threadIdx.x, r = row % ROWS;
-      auto sum_of = [&](int st) {
-        const float* x = sm.wred + st * 128 + r;
-        return (x[0] + x[32]) + (x[64] + x[96]);
-      };
-      float all, top;  // the row's denominator, in units of 2^top
-      if (G == 2) {
-        const int st = row / ROWS;
-        all = sum_of(st);
-        top = sm.base[st * 32 + r];
-        sm.delta[row] = all > 0.f ? p.s.out_scale / all : all;  // 0 for a row without tokens, NaN for a NaN row
-      } else {
-        const float l0 = sum_of(0), l1 = sum_of(1), b0 = sm.base[r], b1 = sm.base[32 + r];
-        top = l0 == 0.f ? b1 : l1 == 0.f ? b0 : fmaxf(b0, b1);
-        const float w0 = l0 == 0.f ? 0.f : ex2(b0 - top), w1 = l1 == 0.f ? 0.f : ex2(b1 - top);
-        all = l0 * w0 + l1 * w1;
-        const float f = all > 0.f ? p.s.out_scale / all : all;
-        sm.delta[r] = w0 == 0.f ? 0.f : w0 * f;
-        sm.delta[32 + r] = w1 == 0.f ? 0.f : w1 * f;
+      const int row = threadIdx.x, r = row % ROWS, g = row / ROWS;
+      float sum[kStep], top = -INFINITY, all = 0.f;  // the row's denominator `all`, in units of 2^top
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        const int st = i * G + g;
+        const float* x = sm.wred + st * 64 + r;
+        sum[i] = (x[0] + x[16]) + (x[32] + x[48]);
+        if (sum[i] != 0.f) top = fmaxf(top, sm.base[st * 16 + r]);
       }
+      float wgt[kStep];
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        wgt[i] = sum[i] == 0.f ? 0.f : ex2(sm.base[(i * G + g) * 16 + r] - top);
+        if (wgt[i] != 0.f) all += sum[i] * wgt[i];
+      }
+      const float f = all > 0.f ? p.s.out_scale / all : all;  // 0 for a row without tokens, NaN for a NaN row
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) sm.delta[(i * G + g) * 16 + r] = wgt[i] == 0.f ? 0.f : wgt[i] * f;
       const float lse = all == 0.f ? -INFINITY : (top + __log2f(all)) * kLn2f;
       const size_t out_row = (size_t)(w.b * p.s.q_len + (row >> 2)) * p.s.hq + w.h * kGroup + (row & 3);
       if (!whole) p.s.ws_lse[(size_t)slot * p.s.rows_pad + row] = lse;
       else if (p.s.out_lse) p.s.out_lse[out_row] = lse;
     }
 #pragma unroll
-    for (int st = 0; st < 2; ++st) {  // each stream's last product (a stream may have none in this piece)
-      const int last = G == 2 ? 2 * (blk + nblk - 1) + st : blk + nblk - 1 - ((blk + nblk - 1 - st) & 1);
-      if (G == 2 || last >= blk)
-        mbar_wait_bounded(smem_u32(sm.p_done + st), (uint32_t)(last >> 1) & 1u, abort, p.s.status, 13, last);
+    for (int st = 0; st < kStreams; ++st) {  // each stream's last product (it may have none in this piece)
+      const int last = ((blk + nblk) * G - 1 - st) / kStreams * kStreams + st;  // the last unit of the stream so far
+      if (last >= blk * G && last < (blk + nblk) * G)
+        mbar_wait_bounded(smem_u32(sm.p_done + st), (uint32_t)(last / kStreams) & 1u, abort, p.s.status, 13, last);
     }
     tc_fence_after();
     softmax_sync();
-    nan_from = min(sm.nan_from[tid], sm.nan_from[128 + tid]);
+    if (tid < ROWS) base[tid] = 0.f;  // for the next piece
+    nan_from = min(min(sm.nan_from[tid], sm.nan_from[128 + tid]), min(sm.nan_from[256 + tid], sm.nan_from[384 + tid]));
+    // this warpgroup's share of the rows: G * ROWS / 4 from row `stream` * that on
+    constexpr int kShare = G * ROWS / kStreams, kChunk = kShare < 4 ? kShare : 4;
+#pragma unroll 1
+    for (int c = stream * kShare; c < (stream + 1) * kShare; c += kChunk) {
+      if (c >= rows) break;
+      const int g = c / ROWS, r0 = c % ROWS;
+      float o[kChunk];
 #pragma unroll
-    for (int c = 0; c < ROWS; c += 8) {
-      if (G == 1 && ((c >> 3) & 1) != stream) continue;  // the warpgroups share the rows
-      if (row0 + c >= rows) continue;
-      float o[8];
+      for (int r = 0; r < kChunk; ++r) o[r] = 0.f;
+      uint32_t raw[kStep][3][kChunk];
 #pragma unroll
-      for (int r = 0; r < 8; ++r) o[r] = 0.f;
+      for (int i = 0; i < kStep; ++i)
 #pragma unroll
-      for (int st = 0; st < 3 - G; ++st) {
-        const int from = G == 2 ? stream : st;
-        uint32_t raw[3][8];
+        for (int j = 0; j < PARTS; ++j) tmem_ld(lanes + (i * G + g) * kPRow + j * ROWS + r0, raw[i][j]);
+      tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < S::PARTS; ++i) tmem_ld(lanes + from * 128 + i * ROWS + c, raw[i]);
-        tmem_wait_ld();
+      for (int i = 0; i < kStep; ++i) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          float x = __uint_as_float(raw[S::PARTS - 1][r]);
+        for (int r = 0; r < kChunk; ++r) {
+          float x = __uint_as_float(raw[i][PARTS - 1][r]);
 #pragma unroll
-          for (int i = S::PARTS - 2; i >= 0; --i) x = fmaf(x, 1.f / 32.f, __uint_as_float(raw[i][r]));
-          const float f = sm.delta[from * 32 + c + r];
+          for (int j = PARTS - 2; j >= 0; --j) x = fmaf(x, 1.f / 32.f, __uint_as_float(raw[i][j][r]));
+          const float f = sm.delta[(i * G + g) * 16 + r0 + r];
           if (f != 0.f) o[r] = fmaf(x, f, o[r]);  // a stream without tokens may hold anything
         }
       }
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        const int row = row0 + c + r;
+      for (int r = 0; r < kChunk; ++r) {
+        const int row = c + r;
         // draft row / 4 sees the tokens before min(len, first + row / 4)
         if (nan_from < piece.first + (row >> 2)) o[r] = __int_as_float(0x7fffffff);
         if (row < rows) {
@@ -894,11 +929,11 @@ template <class S, bool MASK>
 __device__ __forceinline__ float unit_weight(uint32_t slot, const float* base, float kc, int late, int row0) {
   float sum = 0.f;
 #pragma unroll
-  for (int c = 0; c < S::ROWS; c += S::CH) {
-    float s[S::CH];
+  for (int c = 0; c < S::ROWS; c += 8) {
+    float s[8];
     read_scores<S>(slot, c, s);
 #pragma unroll
-    for (int r = 0; r < S::CH; r += 4) {
+    for (int r = 0; r < 8; r += 4) {
       const float4 b4 = *reinterpret_cast<const float4*>(base + c + r);
       const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
@@ -912,46 +947,40 @@ __device__ __forceinline__ float unit_weight(uint32_t slot, const float* base, f
   return sum;
 }
 
+// A warpgroup takes every fourth block, all its row groups.
 template <class S, bool BF>
 __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const TcSmem& sm, uint32_t tmem, volatile int* abort) {
   constexpr int G = S::G;
-  const int group = threadIdx.x >> 7;  // this warpgroup's blocks: every other one
+  const int stream = threadIdx.x >> 7;
   const int tid = threadIdx.x & 127, warp = tid >> 5, lane = tid & 31;
   const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
   const int rows = kGroup * p.s.q_len;
+  auto row_lse = [&](int b, int h) {  // -lse in base 2; -inf (weight 0) for padding and rows without tokens
+    const int row = threadIdx.x;
+    if (row >= rows) return -INFINITY;
+    const float v = __ldg(p.lse + (size_t)(b * p.s.q_len + (row >> 2)) * p.s.hq + h * kGroup + (row & 3));
+    return v == -INFINITY ? -INFINITY : -v * 1.4426950408889634f;
+  };
   int blk = 0, pc = 0;
   for_pieces(p.s, sch, [&](const SegWalk& w, int, int n) {
     const int seg_end = w.seg_start + w.pages;
     const Piece piece = piece_of(p.s, w);
     const int fresh = __ldg(p.s.seq_lens + w.b) - p.s.q_len;  // tokens from here on are new
-    if (pc == 0) write_q<S, BF>(p, sm, w.b, w.h, 0);
-    if (seg_end < sch.end) {
-      SegWalk nw = w;
-      next_segment(p.s, nw);
-      write_q<S, BF>(p, sm, nw.b, nw.h, (pc + 1) & 1);
+    if (pc == 0) {
+      const QItem q = load_q<S, BF>(p, sm, w.b, w.h);
+      if (threadIdx.x < G * S::ROWS) sm.base[threadIdx.x] = row_lse(w.b, w.h);
+      softmax_sync();
+      write_q<S, BF>(p, sm, q, 0);
+      softmax_sync();
     }
-    if (threadIdx.x < G * S::ROWS) {  // -lse in base 2; -inf (weight 0) for padding and rows without tokens
-      const int row = threadIdx.x;
-      float x = -INFINITY;
-      if (row < rows) {
-        const float v = p.lse[(size_t)(w.b * p.s.q_len + (row >> 2)) * p.s.hq + w.h * kGroup + (row & 3)];
-        if (v != -INFINITY) x = -v * 1.4426950408889634f;
-      }
-      sm.base[row] = x;
-    }
-    softmax_sync();
     const float cq = sm.cq[pc & 1];
     const int nblk = blocks_of(n);
-    for (int k = (blk ^ group) & 1; k < nblk; k += 2) {
+    for (int k = (stream - blk) & (kStreams - 1); k < nblk; k += kStreams) {
       const int bk = blk + k;
       const int np = min(kBlockPages, n - k * kBlockPages);
       const int tok0 = (w.pg + k * kBlockPages) * kPageSize;
       const int tok = tok0 + tid;
-      const int e = bk % kMetaSlots;
-      mbar_wait_bounded(smem_u32(sm.m_full + e), (uint32_t)(bk / kMetaSlots) & 1u, abort, p.s.status, 3, bk);
-      const float4 meta = sm.meta[e * kBlockPages + (tid >> 4)];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(sm.m_empty + e));
+      const float4 meta = read_meta(p, sm, bk, abort);
       const float kc = meta.x * cq;
       const int id = __float_as_int(meta.w);
       const bool held = tid < np * kPageSize && tok < piece.len;
@@ -960,7 +989,7 @@ __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const TcSmem
       const bool masked = np < kBlockPages || tok0 + kBlock > piece.first || tok0 + kBlock > piece.len;
       const int late = held ? tok - piece.first : 0x7fffffff;
       float sum = 0.f;
-#pragma unroll
+#pragma unroll 1
       for (int g = 0; g < G; ++g) {
         const int u = bk * G + g;
         mbar_wait_bounded(smem_u32(sm.s_full + u % S::NS), (uint32_t)(u / S::NS) & 1u, abort, p.s.status, 10, u);
@@ -974,7 +1003,16 @@ __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const TcSmem
       }
       if (held && id >= 0) *at = old + sum;
     }
-    softmax_sync();  // base has been read
+    if (seg_end < sch.end) {  // the next piece's Q and rows
+      SegWalk nw = w;
+      next_segment(p.s, nw);
+      const QItem q = load_q<S, BF>(p, sm, nw.b, nw.h);
+      const float x = threadIdx.x < G * S::ROWS ? row_lse(nw.b, nw.h) : 0.f;
+      softmax_sync();
+      write_q<S, BF>(p, sm, q, (pc + 1) & 1);
+      if (threadIdx.x < G * S::ROWS) sm.base[threadIdx.x] = x;
+      softmax_sync();
+    }
     blk += nblk;
     ++pc;
   });
@@ -989,24 +1027,25 @@ __global__ void __launch_bounds__(kScaledTcThreads, 1)
   const int tiles = p.s.num_stages;
   const TcSmem sm = carve<S>(smem, tiles);
   const int warp = threadIdx.x >> 5;
-  constexpr int kScoreWarp = 8, kValueWarp = 9, kProducerWarp = 10, kMetaWarp = 11;
+  constexpr int kScoreWarp = kSoftmaxThreads / 32, kValueWarp = kScoreWarp + 1, kProducerWarp = kScoreWarp + 2,
+                kMetaWarp = kScoreWarp + 3;
   if (threadIdx.x == 0) {
     for (int i = 0; i < tiles; ++i) {
       mbar_init(smem_u32(sm.full + i), 1);
       mbar_init(smem_u32(sm.empty + i), 1);
     }
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       mbar_init(smem_u32(sm.s_full + i), 1);
       mbar_init(smem_u32(sm.s_empty + i), 4);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kStreams; ++i) {
       mbar_init(smem_u32(sm.p_full + i), 4);
       mbar_init(smem_u32(sm.p_done + i), 1);
-      mbar_init(smem_u32(sm.q_ready + i), 8);
     }
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(sm.q_ready + i), kSoftmaxThreads / 32);
     for (int i = 0; i < kMetaSlots; ++i) {
       mbar_init(smem_u32(sm.m_full + i), 1);
-      mbar_init(smem_u32(sm.m_empty + i), S::ATTEND && S::G == 2 ? 8 : 4);  // the warps that read a block's scales
+      mbar_init(smem_u32(sm.m_empty + i), S::ATTEND ? 4 * S::G : 4);  // the warps that read a block's scales
     }
     mbar_init(smem_u32(sm.done), S::ATTEND ? 2 : 1);  // one commit from each issuer
     fence_mbar_init();
@@ -1127,8 +1166,8 @@ cudaError_t launch_rows(ScaledTcParams& p, const CUtensorMap& tm_k, const CUtens
   const int rows = kGroup * p.s.q_len;
   if (rows <= 8) return launch_shape<Shape<PARTS, 8, 1, ATTEND>, BF>(p, tm_k, tm_v, grid, stream);
   if (rows <= 16) return launch_shape<Shape<PARTS, 16, 1, ATTEND>, BF>(p, tm_k, tm_v, grid, stream);
-  if (rows <= 32) return launch_shape<Shape<PARTS, 32, 1, ATTEND>, BF>(p, tm_k, tm_v, grid, stream);
-  return launch_shape<Shape<PARTS, 32, 2, ATTEND>, BF>(p, tm_k, tm_v, grid, stream);
+  if (rows <= 32) return launch_shape<Shape<PARTS, 16, 2, ATTEND>, BF>(p, tm_k, tm_v, grid, stream);
+  return launch_shape<Shape<PARTS, 16, 4, ATTEND>, BF>(p, tm_k, tm_v, grid, stream);
 }
 
 ScaledTcParams tc_params(const ScaledParams& p) {

@@ -14,22 +14,23 @@
 // x2 / 1024, each the e4m3 rounding of what the parts before it left (4 significant bits a
 // part).  The parts are extra columns of the N side (free: an M = 128 product of few columns
 // is bound by reading A) with their own fp32 accumulators, joined at read-out, so that a
-// low part has its own exponent range.  Two parts hold a bf16 query exactly (8 bits) and round P
-// to 2^-9, half of bf16's own rounding; three hold an fp16 query exactly (11 bits) and
-// round P to 2^-13.  Q is first scaled by the power of two that brings the largest finite
+// low part has its own exponent range.  Two parts hold a bf16 query exactly (8 bits), three an fp16
+// query (11 bits).  Q is first scaled by the power of two that brings the largest finite
 // magnitude of the head's rows into [128, 256); a row far below that keeps its bits down to 2^-15
-// (bf16) or 2^-20 (fp16) of the largest.  P is below 2^8 by the rule below.
+// (bf16) or 2^-20 (fp16) of the largest.  P has three parts: 2^-13 of it, and 2^-20 absolutely
+// with a row's largest P between 2^-1 and 2^8.
 //
 // Softmax.  A row keeps a base; a score with its value scale, y = c ks (q . k) + log2 vs, enters as
 // P = 2^(y - base), and the denominator sums P / vs.  The value scale is thus inside the running
 // maximum, and P keeps its e4m3 range whatever the pages' value scales are.  Bases are set from the
-// first block to its maxima - 2 and raised when some y exceeds its base by more than 8 (one
+// first block to its maxima + 1 and raised when some y exceeds its base by more than 8 (one
 // barrier with an or-reduction a block finds that out; then every row whose block maximum passed
-// its old one is raised, and l and O are rescaled).  Six bits of slack: with bases raised at
-// 3 bits over the maximum, two blocks in five of random data with 1% of fourfold tokens raised one,
-// at 2500 cycles each.  Masked tokens and tokens behind the sequence have y = -inf by selection, so
-// NaN in their K does not matter; V rows behind the sequence are zeroed in shared memory, and a NaN
-// in the V of a draft token is zeroed and remembered, as only the rows that see the token get it.
+// its old one is raised, and l and O are rescaled).  Raising costs a block as much again, and on
+// random data with 1% of fourfold tokens it came in every second to fifth block with 3 to 6 bits
+// of slack: hence 9, which the third part of P leaves room for.  Masked tokens and tokens behind
+// the sequence have y = -inf by selection, so NaN in their K does not matter; V rows behind the
+// sequence are zeroed in shared memory, and a NaN in the V of a draft token is zeroed and
+// remembered, as only the rows that see the token get it.
 //
 // Weights.  w_t = sum over the rows of 2^(c ks (q . k) - lse): the same score product, summed over the
 // thread's columns and added to the token's score.  16-bit caches use kind::f16 and Q as it is.
@@ -68,10 +69,11 @@ constexpr int kTileBytes = kBlock * 128;         // K or V of a block (e4m3), or
 constexpr int kMetaSlots = 8;
 constexpr int kPRow = 64;                        // bytes of a token's P: up to three parts of 16 rows
 constexpr int kPBytes = kBlock * kPRow;
+constexpr int kPParts = 3;                       // e4m3 parts of a probability
 constexpr int kStreams = 4;                      // softmax warpgroups
 constexpr int kSoftmaxThreads = kStreams * 128;
 constexpr int kScaledTcThreads = kSoftmaxThreads + 128;
-constexpr float kRaise = 8.f, kHead = 2.f;       // raise a base that a score exceeds by 2^8, to 2^2 under the maximum
+constexpr float kRaise = 8.f, kHead = -1.f;      // raise a base that a score exceeds by 2^8, to 2 times the maximum
 constexpr float kLn2f = 0.6931471805599453f;
 constexpr float kMinValueScale = 8.673617379884035e-19f;  // 2^-60: smaller value scales count as this
 
@@ -90,7 +92,7 @@ struct Shape {
   static constexpr int Q_GROUP = F8 ? N * 128 : 2 * N * 128;  // bytes of one group's Q operand
   static constexpr int Q_BYTES = G * Q_GROUP;
   static constexpr int TILES = ATTEND || !F8 ? 2 : 1;         // 16 KB tiles of a block (K and V, or K's two halves)
-  static_assert(COLS <= kPRow && NS >= kStreams && kStreams % G == 0, "columns");
+  static_assert(N <= 64 && kPParts * ROWS <= kPRow && NS >= kStreams && kStreams % G == 0, "columns");
 };
 
 struct ScaledTcParams {
@@ -102,57 +104,74 @@ struct ScaledTcParams {
   float* scores;
 };
 
-struct TcSmem {
-  uint8_t* ring;
-  uint8_t* p;  // a P buffer for each stream
-  uint8_t* q;  // two Q slots
-  float4* meta;     // [kMetaSlots][8]: ks, log2 vs, 1 / vs, page id (bits)
-  float* base;      // [4][16]: a stream's bases (weights: -lse of the rows, [64])
-  float* delta;     // [4][16]: what a base was raised by; the epilogue's factors of O
-  float* wred;      // [16][16]: per-warp maxima, then per-warp sums
-  int* nan_from;    // [4][128]
-  float* cq;        // [2]: log2-domain score factor of a Q slot
-  unsigned int* qtop;  // [16]
-  uint64_t *full, *empty, *s_full, *s_empty, *p_full, *p_done, *q_ready, *m_full, *m_empty, *done;
-  uint32_t* tmem_base;
-  Schedule* sch;
+// Shared memory of a CTA: everything of a fixed size first (so that its addresses are one register
+// plus constants), then the ring of tiles.
+template <class S>
+struct Smem {
+  static constexpr int kMaxTiles = 16;
+  static constexpr int P = 0;                                           // a P buffer for each stream
+  static constexpr int Q = P + (S::ATTEND ? kStreams * kPBytes : 0);    // two Q slots
+  static constexpr int META = Q + 2 * S::Q_BYTES;                       // [kMetaSlots][8]: ks, log2 vs, 1 / vs, page id (bits)
+  static constexpr int BASE = META + kMetaSlots * kBlockPages * 16;     // [4][16]: a stream's bases (weights: -lse, [64])
+  static constexpr int DELTA = BASE + 64 * 4;                           // [4][16]: raises; the epilogue's factors of O
+  static constexpr int WRED = DELTA + 64 * 4;                           // [16][16]: per-warp maxima, then sums
+  static constexpr int NAN_FROM = WRED + 256 * 4;                       // [4][128]
+  static constexpr int CQ = NAN_FROM + kStreams * 128 * 4;              // [2]: log2-domain score factor of a Q slot
+  static constexpr int QTOP = CQ + 16;                                  // [16]
+  static constexpr int SCH = QTOP + 64;
+  static constexpr int TMEM = SCH + 64;
+  static constexpr int FULL = TMEM + 16;  // barriers
+  static constexpr int EMPTY = FULL + kMaxTiles * 8;
+  static constexpr int S_FULL = EMPTY + kMaxTiles * 8;
+  static constexpr int S_EMPTY = S_FULL + 8 * 8;
+  static constexpr int P_FULL = S_EMPTY + 8 * 8;
+  static constexpr int P_DONE = P_FULL + kStreams * 8;
+  static constexpr int Q_READY = P_DONE + kStreams * 8;
+  static constexpr int M_FULL = Q_READY + 2 * 8;
+  static constexpr int M_EMPTY = M_FULL + kMetaSlots * 8;
+  static constexpr int DONE = M_EMPTY + kMetaSlots * 8;
+  static constexpr int RING = (DONE + 8 + 1023) / 1024 * 1024;
+  static_assert(sizeof(Schedule) <= 64 && META % 1024 == 0 && FULL % 8 == 0, "layout");
+
+  uint8_t* at;  // 1024-byte aligned, in shared memory
+
+  __device__ __forceinline__ uint8_t* ring(int tile) const { return at + RING + tile * kTileBytes; }
+  __device__ __forceinline__ uint8_t* p(int stream) const { return at + P + stream * kPBytes; }
+  __device__ __forceinline__ uint8_t* q(int slot) const { return at + Q + slot * S::Q_BYTES; }
+  __device__ __forceinline__ float4* meta(int slot) const { return reinterpret_cast<float4*>(at + META) + slot * kBlockPages; }
+  __device__ __forceinline__ float* base(int stream) const { return reinterpret_cast<float*>(at + BASE) + stream * 16; }
+  __device__ __forceinline__ float* delta(int stream) const { return reinterpret_cast<float*>(at + DELTA) + stream * 16; }
+  __device__ __forceinline__ float* wred(int warp) const { return reinterpret_cast<float*>(at + WRED) + warp * 16; }
+  __device__ __forceinline__ int* nan_from() const { return reinterpret_cast<int*>(at + NAN_FROM); }
+  __device__ __forceinline__ float* cq() const { return reinterpret_cast<float*>(at + CQ); }
+  __device__ __forceinline__ unsigned int* qtop() const { return reinterpret_cast<unsigned int*>(at + QTOP); }
+  __device__ __forceinline__ Schedule* sch() const { return reinterpret_cast<Schedule*>(at + SCH); }
+  __device__ __forceinline__ uint32_t* tmem() const { return reinterpret_cast<uint32_t*>(at + TMEM); }
+  __device__ __forceinline__ uint32_t bar(int group, int i = 0) const { return smem_u32(at) + group + i * 8; }
 };
 
-constexpr int kFixedBytes = kMetaSlots * 8 * 16 + (64 + 64 + 256 + kStreams * 128 + 4 + 16) * 4 +
-                            (2 * 8 + 2 * kStreams + 2 + 2 * kMetaSlots + 1) * 8 + 64;
-
-template <class S>
-__host__ __device__ constexpr int fixed_smem() {
-  return 1024 + (S::ATTEND ? kStreams * kPBytes : 0) + 2 * S::Q_BYTES + kFixedBytes;
-}
-
-template <class S>
-__device__ __forceinline__ TcSmem carve(uint8_t* smem, int tiles) {
-  TcSmem t;
-  t.ring = smem;
-  t.p = smem + (size_t)tiles * kTileBytes;
-  t.q = t.p + (S::ATTEND ? kStreams * kPBytes : 0);
-  t.meta = reinterpret_cast<float4*>(t.q + 2 * S::Q_BYTES);
-  t.base = reinterpret_cast<float*>(t.meta + kMetaSlots * 8);
-  t.delta = t.base + 64;
-  t.wred = t.delta + 64;
-  t.nan_from = reinterpret_cast<int*>(t.wred + 256);
-  t.cq = reinterpret_cast<float*>(t.nan_from + kStreams * 128);
-  t.qtop = reinterpret_cast<unsigned int*>(t.cq + 4);
-  uint64_t* b = reinterpret_cast<uint64_t*>(t.qtop + 16);
-  t.full = b;
-  t.empty = t.full + tiles;
-  t.s_full = t.empty + tiles;
-  t.s_empty = t.s_full + 8;
-  t.p_full = t.s_empty + 8;
-  t.p_done = t.p_full + kStreams;
-  t.q_ready = t.p_done + kStreams;
-  t.m_full = t.q_ready + 2;
-  t.m_empty = t.m_full + kMetaSlots;
-  t.done = t.m_empty + kMetaSlots;
-  t.tmem_base = reinterpret_cast<uint32_t*>(t.done + 1);
-  t.sch = reinterpret_cast<Schedule*>(t.tmem_base + 2);
-  return t;
+#ifndef SL
+#define SL 20
+#endif
+#ifndef SL2
+#define SL2 100
+#endif
+template <int kSleep = SL>
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort, unsigned int* status) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  for (uint32_t it = 1;; ++it) {
+    if (kSleep) __nanosleep(kSleep);
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 15u) == 0u) {
+      if (*abort) return false;
+      if (global_timer_ns() - t0 > kWaitLimitNs) {
+        *abort = 1;
+        atomicOr(status, 1u);  // SQA_DEV_TIMEOUT
+        return false;
+      }
+    }
+  }
 }
 
 // The pieces of a CTA's range: f(walk, first unit, pages) for each, in order.
@@ -206,7 +225,7 @@ __device__ __forceinline__ void for_page_chunks(const SplitKvParams& p, const Sc
 // ------------------------------------------------------------------ producer (whole warp)
 template <class S>
 __device__ void produce(const ScaledTcParams& p, const Schedule& sch, const CUtensorMap* tm_k, const CUtensorMap* tm_v,
-                        const TcSmem& sm, int tiles, volatile int* abort) {
+                        const Smem<S>& sm, int tiles, volatile int* abort) {
   const uint64_t policy = l2_policy_evict_first();
   int slot = 0, issued = 0;
   uint32_t phase = 0;
@@ -228,13 +247,13 @@ __device__ void produce(const ScaledTcParams& p, const Schedule& sch, const CUte
       }
 #pragma unroll
       for (int tile = 0; tile < S::TILES; ++tile) {  // K then V; or the two 64-dim halves of 16-bit K
-        bool ok = mbar_wait_bounded(smem_u32(sm.empty + slot), phase ^ 1u, abort, p.s.status, 1, issued);
+        bool ok = wait_for<SL2>(sm.bar(Smem<S>::EMPTY, slot), phase ^ 1u, abort, p.s.status);
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
         if (ok) {
           if (elect_one()) {
-            const uint32_t f = smem_u32(sm.full + slot);
+            const uint32_t f = sm.bar(Smem<S>::FULL, slot);
             mbar_arrive_expect_tx(f, np * 2048);
-            const uint32_t dst = smem_u32(sm.ring + (size_t)slot * kTileBytes);
+            const uint32_t dst = smem_u32(sm.ring(slot));
             const CUtensorMap* map = (S::F8 && tile == 1) ? tm_v : tm_k;
             const int c = S::F8 ? 0 : tile * 64;
             for (int j = 0; j < np; ++j) tma_load_4d(dst + j * 2048, map, f, c, c1, c2, pages[j], policy);
@@ -254,7 +273,7 @@ __device__ void produce(const ScaledTcParams& p, const Schedule& sch, const CUte
   if (lane == 0 && *abort) {  // only an abort can leave loads in flight
     for (int k = 0; k < min(issued, tiles); ++k) {
       const int last = k + tiles * ((issued - 1 - k) / tiles);
-      if (!mbar_drain(smem_u32(sm.full + k), (uint32_t)(last / tiles) & 1u, 100000000ull))
+      if (!mbar_drain(sm.bar(Smem<S>::FULL, k), (uint32_t)(last / tiles) & 1u, 100000000ull))
         atomicOr(p.s.status, 1u);
     }
   }
@@ -263,7 +282,7 @@ __device__ void produce(const ScaledTcParams& p, const Schedule& sch, const CUte
 // ------------------------------------------------------------------ page scales (whole warp)
 // The scales (and, for the weights, the id) of every page of a block into a meta slot.
 template <class S>
-__device__ void page_meta(const ScaledTcParams& p, const Schedule& sch, const TcSmem& sm, volatile int* abort) {
+__device__ void page_meta(const ScaledTcParams& p, const Schedule& sch, const Smem<S>& sm, volatile int* abort) {
   const int lane = threadIdx.x & 31;
   int blk = 0;
   for_page_chunks(p.s, sch, [&](const SegWalk& w, int c0, int n, int id) {
@@ -283,10 +302,10 @@ __device__ void page_meta(const ScaledTcParams& p, const Schedule& sch, const Tc
     for (int jb = 0; jb < cnt; jb += kBlockPages, ++blk) {
       const int e = blk % kMetaSlots;
       if (blk >= kMetaSlots)
-        mbar_wait_bounded(smem_u32(sm.m_empty + e), (uint32_t)(blk / kMetaSlots - 1) & 1u, abort, p.s.status, 2, blk);
-      if (lane >= jb && lane < jb + kBlockPages) sm.meta[e * kBlockPages + lane - jb] = m;
+        wait_for<SL2>(sm.bar(Smem<S>::M_EMPTY, e), (uint32_t)(blk / kMetaSlots - 1) & 1u, abort, p.s.status);
+      if (lane >= jb && lane < jb + kBlockPages) sm.meta(e)[lane - jb] = m;
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(sm.m_full + e));
+      if (lane == 0) mbar_arrive(sm.bar(Smem<S>::M_FULL, e));
     }
   });
 }
@@ -302,10 +321,11 @@ __device__ __forceinline__ void tc_mma_ss_f8(uint32_t d_tmem, uint64_t a_desc, u
       : "memory");
 }
 
-__device__ __forceinline__ void drain_products(const ScaledTcParams& p, const TcSmem& sm) {
-  if (elect_one()) tc_commit(smem_u32(sm.done));
+template <class S>
+__device__ __forceinline__ void drain_products(const ScaledTcParams& p, const Smem<S>& sm) {
+  if (elect_one()) tc_commit(sm.bar(Smem<S>::DONE));
   __syncwarp();
-  if (!mbar_drain(smem_u32(sm.done), 0u, 2000000000ull) && (threadIdx.x & 31) == 0)
+  if (!mbar_drain(sm.bar(Smem<S>::DONE), 0u, 2000000000ull) && (threadIdx.x & 31) == 0)
     atomicOr(p.s.status, 1u);
 }
 
@@ -323,48 +343,48 @@ struct RingPos {
 
 // S^T of (block, group) unit u into score slot u % NS.
 template <class S, bool BF>
-__device__ void issue_scores(const ScaledTcParams& p, const Schedule& sch, const TcSmem& sm, uint32_t tmem, int tiles,
+__device__ void issue_scores(const ScaledTcParams& p, const Schedule& sch, const Smem<S>& sm, uint32_t tmem, int tiles,
                              volatile int* abort) {
   constexpr uint32_t kIdesc = mma_idesc_f16(128, S::N, false, false, BF && !S::F8);  // format 0: e4m3 / fp16
   int u = 0, pc = 0;
   RingPos at;
   for_pieces(p.s, sch, [&](const SegWalk&, int, int n) {
-    mbar_wait_bounded(smem_u32(sm.q_ready + (pc & 1)), (uint32_t)(pc >> 1) & 1u, abort, p.s.status, 4, pc);
-    const uint32_t q = smem_u32(sm.q + (pc & 1) * S::Q_BYTES);
+    wait_for(sm.bar(Smem<S>::Q_READY, (pc & 1)), (uint32_t)(pc >> 1) & 1u, abort, p.s.status);
+    const uint32_t q = smem_u32(sm.q(pc & 1));
     const int nblk = blocks_of(n);
     for (int k = 0; k < nblk; ++k) {
       const int k0 = at.slot;  // K's tile (its first half)
-      mbar_wait_bounded(smem_u32(sm.full + at.slot), at.phase, abort, p.s.status, 5, u);
+      wait_for(sm.bar(Smem<S>::FULL, at.slot), at.phase, abort, p.s.status);
       at.next(tiles);
       const int k1 = at.slot;
-      if (!S::F8) mbar_wait_bounded(smem_u32(sm.full + at.slot), at.phase, abort, p.s.status, 5, u);
+      if (!S::F8) wait_for(sm.bar(Smem<S>::FULL, at.slot), at.phase, abort, p.s.status);
       if (S::TILES == 2) at.next(tiles);  // K's second half, or V
 #pragma unroll 1
       for (int g = 0; g < S::G; ++g, ++u) {
         if (u >= S::NS)
-          mbar_wait_bounded(smem_u32(sm.s_empty + u % S::NS), (uint32_t)(u / S::NS - 1) & 1u, abort, p.s.status, 6, u);
+          wait_for(sm.bar(Smem<S>::S_EMPTY, u % S::NS), (uint32_t)(u / S::NS - 1) & 1u, abort, p.s.status);
         __syncwarp();
         tc_fence_after();
         if (elect_one()) {
           const uint32_t d = tmem + S::OCOLS + (u % S::NS) * S::STRIDE;
           const uint32_t qg = q + g * S::Q_GROUP;
-          const uint32_t kt = smem_u32(sm.ring + (size_t)k0 * kTileBytes);
+          const uint32_t kt = smem_u32(sm.ring(k0));
           if constexpr (S::F8) {
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)  // 32 dims (32 B) a step
               tc_mma_ss_f8(d, smem_desc_sw128(kt + kk * 32, 16, 1024), smem_desc_sw128(qg + kk * 32, 16, 1024), kIdesc,
                            kk > 0 ? 1u : 0u);
           } else {
-            const uint32_t kt1 = smem_u32(sm.ring + (size_t)k1 * kTileBytes);
+            const uint32_t kt1 = smem_u32(sm.ring(k1));
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk)  // 16 dims (32 B) a step, four to a half
               tc_mma_ss(d, smem_desc_sw128((kk < 4 ? kt : kt1) + (kk & 3) * 32, 16, 1024),
                         smem_desc_sw128(qg + (kk >> 2) * (S::N * 128) + (kk & 3) * 32, 16, 1024), kIdesc, kk > 0 ? 1u : 0u);
           }
-          tc_commit(smem_u32(sm.s_full + u % S::NS));
+          tc_commit(sm.bar(Smem<S>::S_FULL, u % S::NS));
           if (g == S::G - 1) {  // the block's K may be overwritten
-            tc_commit(smem_u32(sm.empty + k0));
-            if (!S::F8) tc_commit(smem_u32(sm.empty + k1));
+            tc_commit(sm.bar(Smem<S>::EMPTY, k0));
+            if (!S::F8) tc_commit(sm.bar(Smem<S>::EMPTY, k1));
           }
         }
         __syncwarp();
@@ -388,7 +408,7 @@ __device__ __forceinline__ uint64_t desc_p(uint32_t saddr) {
 
 // O^T of stream u % 4 += V^T P^T of unit u, once P is in the stream's buffer.
 template <class S>
-__device__ void issue_values(const ScaledTcParams& p, const Schedule& sch, const TcSmem& sm, uint32_t tmem, int tiles,
+__device__ void issue_values(const ScaledTcParams& p, const Schedule& sch, const Smem<S>& sm, uint32_t tmem, int tiles,
                              volatile int* abort) {
   constexpr uint32_t kIdesc = mma_idesc_f16(128, kPRow, true, true, false);
   int u = 0;
@@ -398,23 +418,23 @@ __device__ void issue_values(const ScaledTcParams& p, const Schedule& sch, const
     for (int k = 0; k < nblk; ++k) {
       at.next(tiles);  // over K
       const int np = min(kBlockPages, n - k * kBlockPages);
-      mbar_wait_bounded(smem_u32(sm.full + at.slot), at.phase, abort, p.s.status, 8, u);
+      wait_for(sm.bar(Smem<S>::FULL, at.slot), at.phase, abort, p.s.status);
 #pragma unroll 1
       for (int g = 0; g < S::G; ++g, ++u) {
         const int st = u & (kStreams - 1);
-        mbar_wait_bounded(smem_u32(sm.p_full + st), (uint32_t)(u / kStreams) & 1u, abort, p.s.status, 7, u);
+        wait_for(sm.bar(Smem<S>::P_FULL, st), (uint32_t)(u / kStreams) & 1u, abort, p.s.status);
         __syncwarp();
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t v = smem_u32(sm.ring + (size_t)at.slot * kTileBytes);
-          const uint32_t pb = smem_u32(sm.p + st * kPBytes);
+          const uint32_t v = smem_u32(sm.ring(at.slot));
+          const uint32_t pb = smem_u32(sm.p(st));
           const int steps = (np + 1) / 2;  // 32 tokens a step; the softmax zeroed an absent page's V
           // a stream's first product of a piece overwrites O
           for (int kk = 0; kk < steps; ++kk)
             tc_mma_ss_f8(tmem + st * kPRow, smem_desc_sw128(v + kk * 4096, kTileBytes, 1024), desc_p(pb + kk * 32 * kPRow),
                          kIdesc, (k >= kStreams / S::G || kk > 0) ? 1u : 0u);
-          tc_commit(smem_u32(sm.p_done + st));
-          if (g == S::G - 1) tc_commit(smem_u32(sm.empty + at.slot));
+          tc_commit(sm.bar(Smem<S>::P_DONE, st));
+          if (g == S::G - 1) tc_commit(sm.bar(Smem<S>::EMPTY, at.slot));
         }
         __syncwarp();
       }
@@ -455,33 +475,32 @@ __device__ __forceinline__ bool group_any(int stream, bool v) {
 __device__ __forceinline__ void group_sync(int stream) { named_bar_sync(1 + stream, 128); }
 __device__ __forceinline__ void softmax_sync() { named_bar_sync(1 + kStreams, kSoftmaxThreads); }
 
-__device__ __forceinline__ uint32_t e4m3x2_of_half2(__half2 h) {
-  return (uint32_t)__nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&h), __NV_SATFINITE, __NV_E4M3);
+// Two fp16 (packed) -> two e4m3 (low 16 bits), nearest even; and back (exact).
+__device__ __forceinline__ uint16_t e4m3x2_of_half2(uint32_t h) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(h));
+  return r;
 }
-__device__ __forceinline__ __half2 half2_of_e4m3x2(uint32_t v) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v & 0xffffu), __NV_E4M3);
-  return *reinterpret_cast<const __half2*>(&h);
+__device__ __forceinline__ uint16_t e4m3x2_of_floats(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
 }
-
-// The e4m3 parts of two probabilities below 2^8.  Differences of a number and its rounding are
-// exact.  Two parts: P rounded to fp16 first (2^-12 of it, an eighth of what the parts round
-// off); three: the first difference is taken in fp32 and rounded to fp16 (2^-16 of P).
-template <int PARTS>
-__device__ __forceinline__ void split_p(float x0, float x1, uint32_t (&out)[3]) {
+__device__ __forceinline__ __half2 half2_of_e4m3x2(uint16_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
+  return *reinterpret_cast<const __half2*>(&r);
+}
+__device__ __forceinline__ uint32_t bits_of(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+// The three e4m3 parts of two probabilities below 2^8.  Differences of a number and its rounding
+// are exact; the first one is taken in fp32 and rounded to fp16 (2^-16 of P).
+__device__ __forceinline__ void split_p(float x0, float x1, uint16_t (&out)[3]) {
   const __half2 k32 = __floats2half2_rn(32.f, 32.f);
-  __half2 rest;
-  if constexpr (PARTS == 2) {
-    const __half2 h = __floats2half2_rn(x0, x1);
-    out[0] = e4m3x2_of_half2(h);
-    rest = __hmul2(__hsub2(h, half2_of_e4m3x2(out[0])), k32);
-  } else {
-    out[0] = pack_e4m3x2(x0, x1);
-    const float2 f = unpack_e4m3x2(out[0]);
-    const __half2 h = __hmul2(__floats2half2_rn(x0 - f.x, x1 - f.y), k32);
-    out[1] = e4m3x2_of_half2(h);
-    rest = __hmul2(__hsub2(h, half2_of_e4m3x2(out[1])), k32);
-  }
-  out[PARTS - 1] = e4m3x2_of_half2(rest);
+  out[0] = e4m3x2_of_floats(x0, x1);
+  const float2 f = __half22float2(half2_of_e4m3x2(out[0]));
+  const __half2 h = __hmul2(__floats2half2_rn(x0 - f.x, x1 - f.y), k32);
+  out[1] = e4m3x2_of_half2(bits_of(h));
+  out[2] = e4m3x2_of_half2(bits_of(__hmul2(__hsub2(h, half2_of_e4m3x2(out[1])), k32)));
 }
 
 // PARTS e4m3 parts of four numbers, exact differences: x = part 0 + part 1 / 32 + part 2 / 1024.
@@ -510,7 +529,7 @@ struct QItem {
 
 // The thread's part of Q into registers, and the warp's largest finite magnitude into qtop.
 template <class S, bool BF>
-__device__ __forceinline__ QItem load_q(const ScaledTcParams& p, const TcSmem& sm, int b, int h) {
+__device__ __forceinline__ QItem load_q(const ScaledTcParams& p, const Smem<S>& sm, int b, int h) {
   const int r = threadIdx.x >> 3, c = threadIdx.x & 7;
   QItem q;
   q.x[0] = q.x[1] = make_uint4(0u, 0u, 0u, 0u);
@@ -530,26 +549,26 @@ __device__ __forceinline__ QItem load_q(const ScaledTcParams& p, const TcSmem& s
 #pragma unroll
     for (int off = 1; off < 8; off <<= 1) q.top = max(q.top, __shfl_xor_sync(0xffffffffu, q.top, off));
     const uint32_t most = __reduce_max_sync(0xffffffffu, q.top < 0x7f800000u ? q.top : 0u);
-    if ((threadIdx.x & 31) == 0) sm.qtop[threadIdx.x >> 5] = most;
+    if ((threadIdx.x & 31) == 0) sm.qtop()[threadIdx.x >> 5] = most;
   }
   return q;
 }
 
 // After a barrier of the softmax threads: the thread's part of Q into slot `qs`.
 template <class S, bool BF>
-__device__ __forceinline__ void write_q(const ScaledTcParams& p, const TcSmem& sm, const QItem& q, int qs) {
+__device__ __forceinline__ void write_q(const ScaledTcParams& p, const Smem<S>& sm, const QItem& q, int qs) {
   const int r = threadIdx.x >> 3, c = threadIdx.x & 7;
   uint32_t most = 0;
   if constexpr (S::F8) {
 #pragma unroll
-    for (int i = 0; i < kSoftmaxThreads / 32; ++i) most = max(most, sm.qtop[i]);
+    for (int i = 0; i < kSoftmaxThreads / 32; ++i) most = max(most, sm.qtop()[i]);
   }
   // 2^e brings the largest magnitude into [128, 256)
   const int e = most > 0 ? max(-110, min(110, 134 - (int)(most >> 23))) : 0;
-  if (threadIdx.x == 0) sm.cq[qs] = p.s.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23);
+  if (threadIdx.x == 0) sm.cq()[qs] = p.s.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23);
   if (r < S::G * S::ROWS) {
     const int rr = r % S::ROWS;
-    uint8_t* const dst = sm.q + qs * S::Q_BYTES + (r / S::ROWS) * S::Q_GROUP;
+    uint8_t* const dst = sm.q(qs) + (r / S::ROWS) * S::Q_GROUP;
     if constexpr (!S::F8) {  // 32 bytes of half c / 4: chunks 2 (c % 4) and the next
       uint8_t* const row = dst + (c >> 2) * (S::N * 128) + (rr >> 3) * 1024 + (rr & 7) * 128;
       const int c0 = (c & 3) * 2;
@@ -579,7 +598,7 @@ __device__ __forceinline__ void write_q(const ScaledTcParams& p, const TcSmem& s
   }
   fence_proxy_async_smem();
   __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(sm.q_ready + qs));
+  if ((threadIdx.x & 31) == 0) mbar_arrive(sm.bar(Smem<S>::Q_READY, qs));
 }
 
 // Rows [c, c + 8) of a score slot, its parts joined.
@@ -666,19 +685,20 @@ __device__ __forceinline__ float unit_scores(uint32_t slot, const float* base, f
 }
 
 // The scales of block bk's page of this thread's token.
-__device__ __forceinline__ float4 read_meta(const ScaledTcParams& p, const TcSmem& sm, int bk, volatile int* abort) {
+template <class S>
+__device__ __forceinline__ float4 read_meta(const ScaledTcParams& p, const Smem<S>& sm, int bk, volatile int* abort) {
   const int e = bk % kMetaSlots;
-  mbar_wait_bounded(smem_u32(sm.m_full + e), (uint32_t)(bk / kMetaSlots) & 1u, abort, p.s.status, 3, bk);
-  const float4 m = sm.meta[e * kBlockPages + ((threadIdx.x & 127) >> 4)];
+  wait_for(sm.bar(Smem<S>::M_FULL, e), (uint32_t)(bk / kMetaSlots) & 1u, abort, p.s.status);
+  const float4 m = sm.meta(e)[(threadIdx.x & 127) >> 4];
   __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(sm.m_empty + e));
+  if ((threadIdx.x & 31) == 0) mbar_arrive(sm.bar(Smem<S>::M_EMPTY, e));
   return m;
 }
 
 template <class S, bool BF>
-__device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSmem& sm, uint32_t tmem, int tiles,
+__device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<S>& sm, uint32_t tmem, int tiles,
                        volatile int* abort) {
-  constexpr int ROWS = S::ROWS, G = S::G, PARTS = S::PARTS;
+  constexpr int ROWS = S::ROWS, G = S::G;
   constexpr int kStep = kStreams / G;  // blocks from unit to unit of a stream
   const int stream = threadIdx.x >> 7;
   const int tid = threadIdx.x & 127, warp = tid >> 5, lane = tid & 31;  // tid: token of a block, dimension of O
@@ -686,9 +706,9 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
   const int rows = kGroup * p.s.q_len;
   const int group = stream % G;  // the stream's rows: row0 .. row0 + ROWS - 1
   const int row0 = group * ROWS;
-  float* const base = sm.base + stream * 16;
-  float* const delta = sm.delta + stream * 16;
-  float* const wred = sm.wred + stream * 4 * 16;
+  float* const base = sm.base(stream);
+  float* const delta = sm.delta(stream);
+  float* const wred = sm.wred(stream * 4);
   int blk = 0, pc = 0;
   for_pieces(p.s, sch, [&](const SegWalk& w, int unit, int n) {
     const int seg = w.b * p.s.hkv + w.h;
@@ -702,7 +722,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
       write_q<S, BF>(p, sm, q, 0);
       softmax_sync();
     }
-    const float cq = sm.cq[pc & 1];
+    const float cq = sm.cq()[pc & 1];
     float l[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) l[r] = 0.f;
@@ -728,8 +748,8 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
         // NaN: zero, and remembered by the dimension's thread.  (The block's first group does it: its
         // product comes first.)
         const int t1 = bk * 2 + 1;  // V's tile
-        mbar_wait_bounded(smem_u32(sm.full + t1 % tiles), (uint32_t)(t1 / tiles) & 1u, abort, p.s.status, 9, bk);
-        uint8_t* const vt = sm.ring + (size_t)(t1 % tiles) * kTileBytes;
+        wait_for(sm.bar(Smem<S>::FULL, t1 % tiles), (uint32_t)(t1 / tiles) & 1u, abort, p.s.status);
+        uint8_t* const vt = sm.ring(t1 % tiles);
         const int held = min(np * kPageSize, max(piece.len - tok0, 0));
         const int read = (np + 1) / 2 * 32;  // rows that the product reads
         for (int t = max(0, piece.first - tok0); t < held; ++t) {
@@ -744,7 +764,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
         fence_proxy_async_smem();
       }
 
-      mbar_wait_bounded(smem_u32(sm.s_full + u % S::NS), (uint32_t)(u / S::NS) & 1u, abort, p.s.status, 10, u);
+      wait_for(sm.bar(Smem<S>::S_FULL, u % S::NS), (uint32_t)(u / S::NS) & 1u, abort, p.s.status);
       tc_fence_after();
       const uint32_t slot = lanes + S::OCOLS + (u % S::NS) * S::STRIDE;
       float t[ROWS];
@@ -753,14 +773,12 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
                                 : unit_scores<S, false>(slot, base, kc, meta.y, late, row0, t);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(sm.s_empty + u % S::NS));
+      if (lane == 0) mbar_arrive(sm.bar(Smem<S>::S_EMPTY, u % S::NS));
       const float inv_vs = meta.z;
       if (k + kStep < nblk) meta = read_meta(p, sm, bk + kStep, abort);  // off the next unit's path
       const bool first = k == k0;
       const bool raise = group_any(stream, over > kRaise) || first;  // rare after a piece's first blocks
       if (raise) {
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r) t[r] = t[r] == t[r] ? t[r] : INFINITY;  // NaN: the row will be NaN
         const float m = reduce_rows<ROWS, true>(t);
         if (lane % (32 / ROWS) == 0) wred[warp * 16 + lane / (32 / ROWS)] = m;
         group_sync(stream);
@@ -775,7 +793,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
         for (int r = 0; r < ROWS; ++r) t[r] -= delta[r];
       }
       // the stream's last product: P's buffer is free, and O stands still
-      if (v >= 1) mbar_wait_bounded(smem_u32(sm.p_done + stream), (uint32_t)(v - 1) & 1u, abort, p.s.status, 11, u);
+      if (v >= 1) wait_for(sm.bar(Smem<S>::P_DONE, stream), (uint32_t)(v - 1) & 1u, abort, p.s.status);
       if (raise && !first) {
         tc_fence_after();
 #pragma unroll
@@ -787,7 +805,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
             l[c + r] *= a[r];
           }
 #pragma unroll
-          for (int i = 0; i < PARTS; ++i) {
+          for (int i = 0; i < kPParts; ++i) {
             uint32_t o[8];
             tmem_ld(lanes + stream * kPRow + i * ROWS + c, o);
             tmem_wait_ld();
@@ -800,8 +818,8 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
       }
       // P: token tid's operand row of 64 bytes, part i of row r in byte i * ROWS + r; 16-byte chunks
       // swizzled by token / 2
-      uint8_t* const prow = sm.p + stream * kPBytes + tid * kPRow;
-      uint32_t part[3][ROWS / 4];
+      uint8_t* const prow = sm.p(stream) + tid * kPRow;
+      uint32_t part[kPParts][ROWS / 4];
 #pragma unroll
       for (int r = 0; r < ROWS; r += 4) {
         float x[4];
@@ -810,14 +828,14 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
           x[i] = ex2(t[r + i]);
           l[r + i] = fmaf(x[i], inv_vs, l[r + i]);
         }
-        uint32_t lo[3], hi[3];
-        split_p<PARTS>(x[0], x[1], lo);
-        split_p<PARTS>(x[2], x[3], hi);
+        uint16_t lo[kPParts], hi[kPParts];
+        split_p(x[0], x[1], lo);
+        split_p(x[2], x[3], hi);
 #pragma unroll
-        for (int i = 0; i < PARTS; ++i) part[i][r / 4] = lo[i] | (hi[i] << 16);
+        for (int i = 0; i < kPParts; ++i) part[i][r / 4] = (uint32_t)lo[i] | ((uint32_t)hi[i] << 16);
       }
 #pragma unroll
-      for (int i = 0; i < PARTS; ++i) {
+      for (int i = 0; i < kPParts; ++i) {
         const int byte = i * ROWS;
         uint8_t* const at = prow + (((byte >> 4) ^ ((tid >> 1) & 3)) << 4) + (byte & 15);
         if constexpr (ROWS == 16)
@@ -828,7 +846,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
       fence_proxy_async_smem();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(sm.p_full + stream));
+      if (lane == 0) mbar_arrive(sm.bar(Smem<S>::P_FULL, stream));
     }
 
     // ---- epilogue: denominators and factors, then each dimension's thread joins its rows' parts
@@ -841,7 +859,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
     }
     const float total = reduce_rows<ROWS, false>(l);
     if (lane % (32 / ROWS) == 0) wred[warp * 16 + lane / (32 / ROWS)] = total;
-    sm.nan_from[threadIdx.x] = nan_from;
+    sm.nan_from()[threadIdx.x] = nan_from;
     softmax_sync();
     if (more) write_q<S, BF>(p, sm, q, (pc + 1) & 1);
     const int slot = (int)blockIdx.x + seg;  // workspace piece
@@ -851,19 +869,19 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
 #pragma unroll
       for (int i = 0; i < kStep; ++i) {
         const int st = i * G + g;
-        const float* x = sm.wred + st * 64 + r;
+        const float* x = sm.wred(st * 4) + r;
         sum[i] = (x[0] + x[16]) + (x[32] + x[48]);
-        if (sum[i] != 0.f) top = fmaxf(top, sm.base[st * 16 + r]);
+        if (sum[i] != 0.f) top = fmaxf(top, sm.base(st)[r]);
       }
       float wgt[kStep];
 #pragma unroll
       for (int i = 0; i < kStep; ++i) {
-        wgt[i] = sum[i] == 0.f ? 0.f : ex2(sm.base[(i * G + g) * 16 + r] - top);
+        wgt[i] = sum[i] == 0.f ? 0.f : ex2(sm.base(i * G + g)[r] - top);
         if (wgt[i] != 0.f) all += sum[i] * wgt[i];
       }
       const float f = all > 0.f ? p.s.out_scale / all : all;  // 0 for a row without tokens, NaN for a NaN row
 #pragma unroll
-      for (int i = 0; i < kStep; ++i) sm.delta[(i * G + g) * 16 + r] = wgt[i] == 0.f ? 0.f : wgt[i] * f;
+      for (int i = 0; i < kStep; ++i) sm.delta(i * G + g)[r] = wgt[i] == 0.f ? 0.f : wgt[i] * f;
       const float lse = all == 0.f ? -INFINITY : (top + __log2f(all)) * kLn2f;
       const size_t out_row = (size_t)(w.b * p.s.q_len + (row >> 2)) * p.s.hq + w.h * kGroup + (row & 3);
       if (!whole) p.s.ws_lse[(size_t)slot * p.s.rows_pad + row] = lse;
@@ -873,12 +891,12 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
     for (int st = 0; st < kStreams; ++st) {  // each stream's last product (it may have none in this piece)
       const int last = ((blk + nblk) * G - 1 - st) / kStreams * kStreams + st;  // the last unit of the stream so far
       if (last >= blk * G && last < (blk + nblk) * G)
-        mbar_wait_bounded(smem_u32(sm.p_done + st), (uint32_t)(last / kStreams) & 1u, abort, p.s.status, 13, last);
+        wait_for(sm.bar(Smem<S>::P_DONE, st), (uint32_t)(last / kStreams) & 1u, abort, p.s.status);
     }
     tc_fence_after();
     softmax_sync();
     if (tid < ROWS) base[tid] = 0.f;  // for the next piece
-    nan_from = min(min(sm.nan_from[tid], sm.nan_from[128 + tid]), min(sm.nan_from[256 + tid], sm.nan_from[384 + tid]));
+    nan_from = min(min(sm.nan_from()[tid], sm.nan_from()[128 + tid]), min(sm.nan_from()[256 + tid], sm.nan_from()[384 + tid]));
     // this warpgroup's share of the rows: G * ROWS / 4 from row `stream` * that on
     constexpr int kShare = G * ROWS / kStreams, kChunk = kShare < 4 ? kShare : 4;
 #pragma unroll 1
@@ -888,20 +906,20 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const TcSme
       float o[kChunk];
 #pragma unroll
       for (int r = 0; r < kChunk; ++r) o[r] = 0.f;
-      uint32_t raw[kStep][3][kChunk];
+      uint32_t raw[kStep][kPParts][kChunk];
 #pragma unroll
       for (int i = 0; i < kStep; ++i)
 #pragma unroll
-        for (int j = 0; j < PARTS; ++j) tmem_ld(lanes + (i * G + g) * kPRow + j * ROWS + r0, raw[i][j]);
+        for (int j = 0; j < kPParts; ++j) tmem_ld(lanes + (i * G + g) * kPRow + j * ROWS + r0, raw[i][j]);
       tmem_wait_ld();
 #pragma unroll
       for (int i = 0; i < kStep; ++i) {
 #pragma unroll
         for (int r = 0; r < kChunk; ++r) {
-          float x = __uint_as_float(raw[i][PARTS - 1][r]);
+          float x = __uint_as_float(raw[i][kPParts - 1][r]);
 #pragma unroll
-          for (int j = PARTS - 2; j >= 0; --j) x = fmaf(x, 1.f / 32.f, __uint_as_float(raw[i][j][r]));
-          const float f = sm.delta[(i * G + g) * 16 + r0 + r];
+          for (int j = kPParts - 2; j >= 0; --j) x = fmaf(x, 1.f / 32.f, __uint_as_float(raw[i][j][r]));
+          const float f = sm.delta(i * G + g)[r0 + r];
           if (f != 0.f) o[r] = fmaf(x, f, o[r]);  // a stream without tokens may hold anything
         }
       }
@@ -949,7 +967,7 @@ __device__ __forceinline__ float unit_weight(uint32_t slot, const float* base, f
 
 // A warpgroup takes every fourth block, all its row groups.
 template <class S, bool BF>
-__device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const TcSmem& sm, uint32_t tmem, volatile int* abort) {
+__device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const Smem<S>& sm, uint32_t tmem, volatile int* abort) {
   constexpr int G = S::G;
   const int stream = threadIdx.x >> 7;
   const int tid = threadIdx.x & 127, warp = tid >> 5, lane = tid & 31;
@@ -968,12 +986,12 @@ __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const TcSmem
     const int fresh = __ldg(p.s.seq_lens + w.b) - p.s.q_len;  // tokens from here on are new
     if (pc == 0) {
       const QItem q = load_q<S, BF>(p, sm, w.b, w.h);
-      if (threadIdx.x < G * S::ROWS) sm.base[threadIdx.x] = row_lse(w.b, w.h);
+      if (threadIdx.x < G * S::ROWS) sm.base(0)[threadIdx.x] = row_lse(w.b, w.h);
       softmax_sync();
       write_q<S, BF>(p, sm, q, 0);
       softmax_sync();
     }
-    const float cq = sm.cq[pc & 1];
+    const float cq = sm.cq()[pc & 1];
     const int nblk = blocks_of(n);
     for (int k = (stream - blk) & (kStreams - 1); k < nblk; k += kStreams) {
       const int bk = blk + k;
@@ -992,14 +1010,14 @@ __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const TcSmem
 #pragma unroll 1
       for (int g = 0; g < G; ++g) {
         const int u = bk * G + g;
-        mbar_wait_bounded(smem_u32(sm.s_full + u % S::NS), (uint32_t)(u / S::NS) & 1u, abort, p.s.status, 10, u);
+        wait_for(sm.bar(Smem<S>::S_FULL, u % S::NS), (uint32_t)(u / S::NS) & 1u, abort, p.s.status);
         tc_fence_after();
         const uint32_t slot = lanes + (u % S::NS) * S::STRIDE;
-        sum += masked ? unit_weight<S, true>(slot, sm.base + g * S::ROWS, kc, late, g * S::ROWS)
-                      : unit_weight<S, false>(slot, sm.base + g * S::ROWS, kc, late, g * S::ROWS);
+        sum += masked ? unit_weight<S, true>(slot, sm.base(0) + g * S::ROWS, kc, late, g * S::ROWS)
+                      : unit_weight<S, false>(slot, sm.base(0) + g * S::ROWS, kc, late, g * S::ROWS);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(sm.s_empty + u % S::NS));
+        if (lane == 0) mbar_arrive(sm.bar(Smem<S>::S_EMPTY, u % S::NS));
       }
       if (held && id >= 0) *at = old + sum;
     }
@@ -1010,7 +1028,7 @@ __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const TcSmem
       const float x = threadIdx.x < G * S::ROWS ? row_lse(nw.b, nw.h) : 0.f;
       softmax_sync();
       write_q<S, BF>(p, sm, q, (pc + 1) & 1);
-      if (threadIdx.x < G * S::ROWS) sm.base[threadIdx.x] = x;
+      if (threadIdx.x < G * S::ROWS) sm.base(0)[threadIdx.x] = x;
       softmax_sync();
     }
     blk += nblk;
@@ -1023,31 +1041,31 @@ __global__ void __launch_bounds__(kScaledTcThreads, 1)
     sqa_scaled_tc_kernel(const ScaledTcParams p, const __grid_constant__ CUtensorMap tm_k,
                          const __grid_constant__ CUtensorMap tm_v) {
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // an offset, not a cast of an aligned address: the compiler keeps seeing shared memory
+  const Smem<S> sm{smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u)};
   const int tiles = p.s.num_stages;
-  const TcSmem sm = carve<S>(smem, tiles);
   const int warp = threadIdx.x >> 5;
   constexpr int kScoreWarp = kSoftmaxThreads / 32, kValueWarp = kScoreWarp + 1, kProducerWarp = kScoreWarp + 2,
                 kMetaWarp = kScoreWarp + 3;
   if (threadIdx.x == 0) {
     for (int i = 0; i < tiles; ++i) {
-      mbar_init(smem_u32(sm.full + i), 1);
-      mbar_init(smem_u32(sm.empty + i), 1);
+      mbar_init(sm.bar(Smem<S>::FULL, i), 1);
+      mbar_init(sm.bar(Smem<S>::EMPTY, i), 1);
     }
     for (int i = 0; i < 8; ++i) {
-      mbar_init(smem_u32(sm.s_full + i), 1);
-      mbar_init(smem_u32(sm.s_empty + i), 4);
+      mbar_init(sm.bar(Smem<S>::S_FULL, i), 1);
+      mbar_init(sm.bar(Smem<S>::S_EMPTY, i), 4);
     }
     for (int i = 0; i < kStreams; ++i) {
-      mbar_init(smem_u32(sm.p_full + i), 4);
-      mbar_init(smem_u32(sm.p_done + i), 1);
+      mbar_init(sm.bar(Smem<S>::P_FULL, i), 4);
+      mbar_init(sm.bar(Smem<S>::P_DONE, i), 1);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(sm.q_ready + i), kSoftmaxThreads / 32);
+    for (int i = 0; i < 2; ++i) mbar_init(sm.bar(Smem<S>::Q_READY, i), kSoftmaxThreads / 32);
     for (int i = 0; i < kMetaSlots; ++i) {
-      mbar_init(smem_u32(sm.m_full + i), 1);
-      mbar_init(smem_u32(sm.m_empty + i), S::ATTEND ? 4 * S::G : 4);  // the warps that read a block's scales
+      mbar_init(sm.bar(Smem<S>::M_FULL, i), 1);
+      mbar_init(sm.bar(Smem<S>::M_EMPTY, i), S::ATTEND ? 4 * S::G : 4);  // the warps that read a block's scales
     }
-    mbar_init(smem_u32(sm.done), S::ATTEND ? 2 : 1);  // one commit from each issuer
+    mbar_init(sm.bar(Smem<S>::DONE), S::ATTEND ? 2 : 1);  // one commit from each issuer
     fence_mbar_init();
   }
   if (warp == kProducerWarp && (threadIdx.x & 31) == 0) {
@@ -1060,16 +1078,16 @@ __global__ void __launch_bounds__(kScaledTcThreads, 1)
   grid_dependency_wait();
   allow_dependent_launch();
   if (warp == kScoreWarp) {
-    tmem_alloc(smem_u32(sm.tmem_base), 512);
+    tmem_alloc(smem_u32(sm.tmem()), 512);
     tmem_relinquish();
   }
-  if (warp == 0) build_schedule(p.s, sm.sch);
+  if (warp == 0) build_schedule(p.s, sm.sch());
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *sm.tmem_base;
-  const Schedule sch = *sm.sch;
-  volatile int* abort = &sm.sch->abort;
+  const uint32_t tmem = *sm.tmem();
+  const Schedule sch = *sm.sch();
+  volatile int* abort = &sm.sch()->abort;
   if (warp == kProducerWarp) {
     produce<S>(p, sch, &tm_k, &tm_v, sm, tiles, abort);
   } else if (warp == kMetaWarp) {
@@ -1133,9 +1151,9 @@ __global__ void __launch_bounds__(128) sqa_scaled_merge_kernel(const MergeParams
 constexpr int kMaxSmem = 227 * 1024;
 
 template <class S>
-int tiles_that_fit() {
-  const int n = (kMaxSmem - fixed_smem<S>()) / (kTileBytes + 16);
-  return n < 16 ? n / S::TILES * S::TILES : 16;
+constexpr int tiles_that_fit() {
+  const int n = (kMaxSmem - 1024 - Smem<S>::RING) / kTileBytes;
+  return (n < Smem<S>::kMaxTiles ? n : Smem<S>::kMaxTiles) / S::TILES * S::TILES;
 }
 
 template <class S, bool BF>
@@ -1143,7 +1161,7 @@ cudaError_t launch_shape(ScaledTcParams& p, const CUtensorMap& tm_k, const CUten
                          cudaStream_t stream) {
   auto kernel = sqa_scaled_tc_kernel<S, BF>;
   p.s.num_stages = tiles_that_fit<S>();
-  const int smem = fixed_smem<S>() + p.s.num_stages * (kTileBytes + 16);
+  const int smem = 1024 + Smem<S>::RING + p.s.num_stages * kTileBytes;
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};

@@ -90,7 +90,12 @@ __global__ void __launch_bounds__(256) sqa_cache_append_scaled_kernel(const Appe
     }
     const float need = page_scale(warp_max(amax));
     const float scale = n0 > 0 ? fmaxf(was, need) : need;
-    if (n0 > 0 && scale > was) {  // the older tokens follow the page's new scale
+    // Dividing by a power of two is multiplying by its reciprocal (exact; 64 IEEE divisions a lane
+    // made a prompt's append four times as long).  Only an old scale that another quantiser
+    // chose can be anything else.
+    const bool power = (__float_as_uint(scale) & 0x7fffffu) == 0u;
+    const float inv = 1.f / scale;
+    if (n0 > 0 && scale > was) {  // the older tokens follow the page's new scale, a power of two
       uint32_t q[kPageSize];
 #pragma unroll
       for (int s = 0; s < kPageSize; ++s) q[s] = s < n0 ? *reinterpret_cast<const uint32_t*>(dst + s * row) : 0u;
@@ -99,15 +104,23 @@ __global__ void __launch_bounds__(256) sqa_cache_append_scaled_kernel(const Appe
         if (s < n0) {
           const float2 a = unpack_e4m3x2(q[s]), c = unpack_e4m3x2(q[s] >> 16);
           *reinterpret_cast<uint32_t*>(dst + s * row) =
-              pack_e4m3x4(__fdiv_rn(a.x * was, scale), __fdiv_rn(a.y * was, scale), __fdiv_rn(c.x * was, scale),
-                          __fdiv_rn(c.y * was, scale));
+              pack_e4m3x4(a.x * was * inv, a.y * was * inv, c.x * was * inv, c.y * was * inv);
         }
       }
     }
+    if (power) {
 #pragma unroll
-    for (int s = 0; s < kPageSize; ++s) {
-      if (s >= n0 && s < n1) {
-        const float2 a = unpack2<BF>(x[s].x), c = unpack2<BF>(x[s].y);
+      for (int s = 0; s < kPageSize; ++s) {
+        if (s >= n0 && s < n1) {
+          const float2 a = unpack2<BF>(x[s].x), c = unpack2<BF>(x[s].y);
+          *reinterpret_cast<uint32_t*>(dst + s * row) = pack_e4m3x4(a.x * inv, a.y * inv, c.x * inv, c.y * inv);
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (int s = n0; s < n1; ++s) {  // not unrolled: x is read again
+        const uint2 y = __ldg(src + (size_t)(first + s - t0) * p.hkv * 32);
+        const float2 a = unpack2<BF>(y.x), c = unpack2<BF>(y.y);
         *reinterpret_cast<uint32_t*>(dst + s * row) =
             pack_e4m3x4(__fdiv_rn(a.x, scale), __fdiv_rn(a.y, scale), __fdiv_rn(c.x, scale), __fdiv_rn(c.y, scale));
       }

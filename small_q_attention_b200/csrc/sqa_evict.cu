@@ -55,18 +55,21 @@ struct EvictParams {
   int cluster, key_cap;
 };
 
+// What the CTAs of a cluster tell one another they store into each other's shared memory before
+// a cluster barrier and read from their own after it: remote stores are not waited for, while a
+// loop of remote loads cost 8 round trips (a radix pass took 4500 cycles with them).
 struct EvictShared {
-  unsigned int hist[2][256];
-  unsigned int exchange[2];  // read by the other CTAs of the cluster
-  unsigned int counts[2];    // this slice's (above, equal), read by the others
+  unsigned int hist[256];                          // this slice's
+  unsigned int hists[2][kEvictMaxCluster][256];    // every slice's, by pass parity
+  unsigned int range[kEvictMaxCluster][2];         // every slice's (lowest, highest) key
+  unsigned int counts[kEvictMaxCluster][2];        // every slice's (above, equal)
   unsigned int warp_a[kEvictWarps], warp_b[kEvictWarps];
-  unsigned int pick[2];
+  unsigned int pick[3];
 };
 
-__device__ __forceinline__ unsigned int ld_cluster_u32(const void* p, int rank) {
-  unsigned int v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_map(smem_u32(p), (uint32_t)rank)) : "memory");
-  return v;
+// `v` to the same shared-memory location of the CTA of rank `rank`.
+__device__ __forceinline__ void st_cluster_u32(void* p, int rank, unsigned int v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_map(smem_u32(p), (uint32_t)rank)), "r"(v) : "memory");
 }
 
 // Order-preserving key of a score; NaN lowest, the two zeros equal.
@@ -74,6 +77,65 @@ __device__ __forceinline__ unsigned int score_key(float f) {
   if (f != f) return 0u;
   const unsigned int u = __float_as_uint(f == 0.f ? 0.f : f);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+// The page that the warp holds (load i, row i * kRows + sub, 16 elements a lane; row r's scale in lane r) at
+// the scale of what it now holds, which is returned.  Whole warp.  Maxima are taken in fp16, which
+// holds every e4m3 number; with power-of-two scales, as the append and this kernel leave them, so
+// is the product (a factor of 2^-14..2^14; what falls below fp16's range is zero in e4m3 as
+// well), and rows that keep their scale are not touched.  Any other scale goes through fp32.
+template <int kLoads, int kRows>
+__device__ __forceinline__ float rescale_page(uint4 (&x)[kLoads], float source, int sub) {
+  float amax = 0.f, s[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    s[i] = __shfl_sync(0xffffffffu, source, i * kRows + sub);
+    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    __half2 m = __floats2half2_rn(0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      m = __hmax2(m, __hmax2(__habs2(half2_of_e4m3x2(w[c] & 0xffffu)), __habs2(half2_of_e4m3x2(w[c] >> 16))));
+    const float2 f = __half22float2(m);
+    amax = fmaxf(amax, finite_abs(fmaxf(f.x, f.y) * s[i]));
+  }
+  const float scale = page_scale(warp_max(amax));
+  const int e = (int)(__float_as_uint(scale) >> 23);
+  bool plain = true;  // every row's factor is a power of two within fp16
+  int shift[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const uint32_t u = __float_as_uint(s[i]);
+    shift[i] = (int)(u >> 23) - e;
+    plain = plain && (u & 0x7fffffu) == 0u && abs(shift[i]) <= 14;
+    if (s[i] == 0.f) {  // rows of zeros, or none
+      shift[i] = 0;
+      plain = plain && (x[i].x | x[i].y | x[i].z | x[i].w) == 0u;
+    }
+  }
+  if (__all_sync(0xffffffffu, plain)) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      if (shift[i] == 0) continue;
+      const __half2 f = __float2half2_rn(__uint_as_float((uint32_t)(shift[i] + 127) << 23));
+      uint32_t* const w = reinterpret_cast<uint32_t*>(&x[i]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        w[c] = e4m3x2_of_half2(__hmul2(half2_of_e4m3x2(w[c] & 0xffffu), f)) |
+               (e4m3x2_of_half2(__hmul2(half2_of_e4m3x2(w[c] >> 16), f)) << 16);
+    }
+  } else {
+    const float inv = 1.f / scale;  // a power of two: multiplying by it is dividing by scale
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      uint32_t* const w = reinterpret_cast<uint32_t*>(&x[i]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float2 a = unpack_e4m3x2(w[c]), d = unpack_e4m3x2(w[c] >> 16);
+        w[c] = pack_e4m3x4(a.x * s[i] * inv, a.y * s[i] * inv, d.x * s[i] * inv, d.y * s[i] * inv);
+      }
+    }
+  }
+  return scale;
 }
 
 template <int E>  // bytes per cached element: 2 (16-bit) or 1 (block-scaled e4m3)
@@ -140,20 +202,22 @@ __global__ void __launch_bounds__(kEvictThreads, 2) sqa_cache_evict_kernel(const
     sh.warp_b[warp] = hi;
   }
   __syncthreads();
-  if (tid == 0) {
+  if (tid < C) {  // this slice's range to CTA `tid`
+    lo = sh.warp_a[0];
+    hi = sh.warp_b[0];
     for (int w = 1; w < kEvictWarps; ++w) {
       lo = min(lo, sh.warp_a[w]);
       hi = max(hi, sh.warp_b[w]);
     }
-    sh.exchange[0] = lo;
-    sh.exchange[1] = hi;
+    st_cluster_u32(&sh.range[rank][0], tid, lo);
+    st_cluster_u32(&sh.range[rank][1], tid, hi);
   }
   cluster_sync_all();
   lo = 0xffffffffu;
   hi = 0u;
   for (int r = 0; r < C; ++r) {
-    lo = min(lo, ld_cluster_u32(&sh.exchange[0], r));
-    hi = max(hi, ld_cluster_u32(&sh.exchange[1], r));
+    lo = min(lo, sh.range[r][0]);
+    hi = max(hi, sh.range[r][1]);
   }
   // Kept: every key > above, and of the keys == lo the first `need` (none once `exact`).
   // Invariant: the keys above hi number want - need, those in [lo, hi] at least need.
@@ -161,19 +225,25 @@ __global__ void __launch_bounds__(kEvictThreads, 2) sqa_cache_evict_kernel(const
   bool exact = want == 0;      // nothing from [lo, hi] is needed
   unsigned int above = hi;     // keys > above are kept whatever else
   for (int pass = 0; !exact && lo < hi; ++pass) {
-    unsigned int* const hist = sh.hist[pass & 1];
     const int shift = max(0, 24 - __clz(hi - lo));  // (hi - lo) >> shift < 256
-    hist[tid] = 0u;
+    sh.hist[tid] = 0u;
     __syncthreads();
     for (int i = tid; i < count; i += kEvictThreads) {
       const unsigned int k = key_at(i);
-      if (k >= lo && k <= hi) atomicAdd(&hist[(k - lo) >> shift], 1u);
+      if (k >= lo && k <= hi) atomicAdd(&sh.hist[(k - lo) >> shift], 1u);
     }
-    cluster_sync_all();  // also: every CTA is done with the other histogram
+    __syncthreads();
+    const unsigned int mine = sh.hist[tid];
+#pragma unroll
+    for (int r = 0; r < kEvictMaxCluster; ++r)
+      if (r < C) st_cluster_u32(&sh.hists[pass & 1][rank][tid], r, mine);
+    cluster_sync_all();  // also: every CTA has read the pass before the last
     // thread t: bin 255 - t, so that an inclusive scan counts from the top
     const int bin = 255 - tid;
     unsigned int n = 0;
-    for (int r = 0; r < C; ++r) n += ld_cluster_u32(&hist[bin], r);
+#pragma unroll
+    for (int r = 0; r < kEvictMaxCluster; ++r)
+      if (r < C) n += sh.hists[pass & 1][r][bin];
     unsigned int incl = n;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -186,12 +256,10 @@ __global__ void __launch_bounds__(kEvictThreads, 2) sqa_cache_evict_kernel(const
     if (incl >= (unsigned int)need && incl - n < (unsigned int)need) {  // exactly one thread
       sh.pick[0] = (unsigned int)bin;
       sh.pick[1] = incl;
+      sh.pick[2] = n;
     }
     __syncthreads();
-    const unsigned int j = sh.pick[0], upto = sh.pick[1];  // keys of bins >= j in the range
-    const unsigned int in_bin = ld_cluster_u32(&hist[j], 0);
-    unsigned int total = in_bin;
-    for (int r = 1; r < C; ++r) total += ld_cluster_u32(&hist[j], r);
+    const unsigned int j = sh.pick[0], upto = sh.pick[1], total = sh.pick[2];  // keys of bins >= j; of bin j
     const unsigned int edge = lo + (j << shift);
     hi = edge + min(hi - edge, (1u << shift) - 1u);
     lo = edge;
@@ -221,45 +289,56 @@ __global__ void __launch_bounds__(kEvictThreads, 2) sqa_cache_evict_kernel(const
     sh.warp_b[warp] = eq;
   }
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kEvictWarps; ++w) {
+  if (tid < C) {
+    gt = eq = 0;
+    for (int w = 0; w < kEvictWarps; ++w) {
       gt += sh.warp_a[w];
       eq += sh.warp_b[w];
     }
-    sh.counts[0] = gt;
-    sh.counts[1] = eq;
+    st_cluster_u32(&sh.counts[rank][0], tid, gt);
+    st_cluster_u32(&sh.counts[rank][1], tid, eq);
   }
   cluster_sync_all();
   unsigned int gt_before = 0, eq_before = 0;
   for (int r = 0; r < rank; ++r) {
-    gt_before += ld_cluster_u32(&sh.counts[0], r);
-    eq_before += ld_cluster_u32(&sh.counts[1], r);
+    gt_before += sh.counts[r][0];
+    eq_before += sh.counts[r][1];
   }
-  for (int base = 0; base < count; base += kEvictThreads) {
-    const int i = base + tid;
-    const unsigned int k = i < count ? key_at(i) : 0u;
-    const bool is_gt = i < count && k > last, is_eq = i < count && k == last;
-    const unsigned int m_gt = __ballot_sync(0xffffffffu, is_gt), m_eq = __ballot_sync(0xffffffffu, is_eq);
+  // four consecutive tokens a thread; counts of (above, equal) packed in 16 bits each
+  for (int base = 0; base < count; base += 4 * kEvictThreads) {
+    const int i0 = base + 4 * tid;
+    unsigned int k[4], packed = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      k[i] = i0 + i < count ? key_at(i0 + i) : 0u;
+      if (i0 + i < count) packed += (k[i] > last ? 1u : 0u) + (k[i] == last ? 0x10000u : 0u);
+    }
+    unsigned int incl = packed;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const unsigned int y = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += y;
+    }
     __syncthreads();  // the last tile's counts have been read
-    if (lane == 0) {
-      sh.warp_a[warp] = __popc(m_gt);
-      sh.warp_b[warp] = __popc(m_eq);
-    }
+    if (lane == 31) sh.warp_a[warp] = incl;
     __syncthreads();
-    unsigned int g = gt_before, e = eq_before;
+    unsigned int before = incl - packed, all = 0;
     for (int w = 0; w < kEvictWarps; ++w) {
-      const unsigned int wg = sh.warp_a[w], we = sh.warp_b[w];
-      if (w < warp) {
-        g += wg;
-        e += we;
-      }
-      gt_before += wg;
-      eq_before += we;
+      const unsigned int x = sh.warp_a[w];
+      if (w < warp) before += x;
+      all += x;
     }
-    const unsigned int under = (1u << lane) - 1u;
-    g += __popc(m_gt & under);
-    e += __popc(m_eq & under);
-    if (is_gt || (is_eq && e < (unsigned int)need)) kept[p.sinks + g + min(e, (unsigned int)need)] = a0 + i;
+    unsigned int g = gt_before + (before & 0xffffu), e = eq_before + (before >> 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i0 + i >= count) break;
+      const bool is_gt = k[i] > last, is_eq = k[i] == last;
+      if (is_gt || (is_eq && e < (unsigned int)need)) kept[p.sinks + g + min(e, (unsigned int)need)] = a0 + i0 + i;
+      g += is_gt;
+      e += is_eq;
+    }
+    gt_before += all & 0xffffu;
+    eq_before += all >> 16;
   }
   for (int i = rank * kEvictThreads + tid; i < p.sinks; i += C * kEvictThreads) kept[i] = i;
   for (int i = rank * kEvictThreads + tid; i < p.recent; i += C * kEvictThreads)
@@ -275,29 +354,34 @@ __global__ void __launch_bounds__(kEvictThreads, 2) sqa_cache_evict_kernel(const
   const size_t row = p.hnd ? (size_t)kHeadDim * E : (size_t)p.hkv * kHeadDim * E;  // bytes from slot to slot
   const size_t in_row = head + (lane % kLanesPerRow) * 16;
   const int targets = (p.budget + kPageSize - 1) / kPageSize;
-  for (int base = 0; base < targets; base += C * kEvictWarps) {
+  // target page, and lane's source page and slot, of the wave from target `base` on: read a wave ahead
+  struct Source {
+    int rows, to, from, slot;
+  };
+  auto source_of = [&](int base) {
     const int target = base + rank * kEvictWarps + warp;
-    const int rows = target < targets ? min(kPageSize, p.budget - target * kPageSize) : 0;
+    Source s = {target < targets ? min(kPageSize, p.budget - target * kPageSize) : 0, 0, 0, 0};
+    if (s.rows > 0) {
+      s.to = __ldg(table + target);
+      if (lane < s.rows) {
+        const int t = __ldcg(kept + target * kPageSize + lane);
+        s.from = __ldg(table + t / kPageSize);
+        s.slot = t % kPageSize;
+      }
+    }
+    return s;
+  };
+  Source next = source_of(0);
+  for (int base = 0; base < targets; base += C * kEvictWarps) {
+    const Source src = next;
+    const int rows = src.rows, to = src.to;
     uint4 k[kLoads], v[kLoads];
     float score = 0.f, ks = 0.f, vs = 0.f;
-    int to = 0;
     if (rows > 0) {
-      to = __ldg(table + target);
-      int from = 0, slot = 0;
-      if (lane < rows) {
-        const int t = __ldcg(kept + target * kPageSize + lane);
-        from = __ldg(table + t / kPageSize);
-        slot = t % kPageSize;
-        score = __ldcg(p.scores + ((size_t)from * p.hkv + h) * kPageSize + slot);
-        if constexpr (E == 1) {
-          ks = __ldcg(p.k_scales + (size_t)from * p.scale_stride + h);
-          vs = __ldcg(p.v_scales + (size_t)from * p.scale_stride + h);
-        }
-      }
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int r = i * kRowsPerLoad + sub;
-        const int rf = __shfl_sync(0xffffffffu, from, r), rs = __shfl_sync(0xffffffffu, slot, r);
+        const int rf = __shfl_sync(0xffffffffu, src.from, r), rs = __shfl_sync(0xffffffffu, src.slot, r);
         const size_t at = (size_t)rf * p.page_stride + rs * row + in_row;
         k[i] = v[i] = make_uint4(0u, 0u, 0u, 0u);
         if (r < rows) {
@@ -305,38 +389,20 @@ __global__ void __launch_bounds__(kEvictThreads, 2) sqa_cache_evict_kernel(const
           v[i] = __ldcg(reinterpret_cast<const uint4*>(p.v_cache + at));
         }
       }
+      if (lane < rows) {
+        score = __ldcg(p.scores + ((size_t)src.from * p.hkv + h) * kPageSize + src.slot);
+        if constexpr (E == 1) {
+          ks = __ldcg(p.k_scales + (size_t)src.from * p.scale_stride + h);
+          vs = __ldcg(p.v_scales + (size_t)src.from * p.scale_stride + h);
+        }
+      }
     }
+    if (base + C * kEvictWarps < targets) next = source_of(base + C * kEvictWarps);
     cluster_sync_all();  // every source of this wave has been read
     if (rows > 0) {
       if constexpr (E == 1) {
-        // values at their source page's scale, then the target page's scale from what it now holds
-        auto rescale = [&](uint4(&x)[kLoads], float source) {
-          float amax = 0.f, s[kLoads];
-#pragma unroll
-          for (int i = 0; i < kLoads; ++i) {
-            s[i] = __shfl_sync(0xffffffffu, source, i * kRowsPerLoad + sub);
-            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const float2 a = unpack_e4m3x2(w[c]), d = unpack_e4m3x2(w[c] >> 16);
-              amax = fmaxf(amax, fmaxf(fmaxf(finite_abs(a.x * s[i]), finite_abs(a.y * s[i])),
-                                       fmaxf(finite_abs(d.x * s[i]), finite_abs(d.y * s[i]))));
-            }
-          }
-          const float scale = page_scale(warp_max(amax));
-          const float inv = 1.f / scale;  // a power of two: multiplying by it is dividing by scale
-#pragma unroll
-          for (int i = 0; i < kLoads; ++i) {
-            uint32_t* const w = reinterpret_cast<uint32_t*>(&x[i]);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const float2 a = unpack_e4m3x2(w[c]), d = unpack_e4m3x2(w[c] >> 16);
-              w[c] = pack_e4m3x4(a.x * s[i] * inv, a.y * s[i] * inv, d.x * s[i] * inv, d.y * s[i] * inv);
-            }
-          }
-          return scale;
-        };
-        const float new_ks = rescale(k, ks), new_vs = rescale(v, vs);
+        const float new_ks = rescale_page<kLoads, kRowsPerLoad>(k, ks, sub);
+        const float new_vs = rescale_page<kLoads, kRowsPerLoad>(v, vs, sub);
         if (lane == 0) {
           p.k_scales[(size_t)to * p.scale_stride + h] = new_ks;
           p.v_scales[(size_t)to * p.scale_stride + h] = new_vs;

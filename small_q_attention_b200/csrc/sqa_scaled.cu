@@ -475,32 +475,15 @@ __device__ __forceinline__ bool group_any(int stream, bool v) {
 __device__ __forceinline__ void group_sync(int stream) { named_bar_sync(1 + stream, 128); }
 __device__ __forceinline__ void softmax_sync() { named_bar_sync(1 + kStreams, kSoftmaxThreads); }
 
-// Two fp16 (packed) -> two e4m3 (low 16 bits), nearest even; and back (exact).
-__device__ __forceinline__ uint16_t e4m3x2_of_half2(uint32_t h) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(h));
-  return r;
-}
-__device__ __forceinline__ uint16_t e4m3x2_of_floats(float lo, float hi) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ __half2 half2_of_e4m3x2(uint16_t v) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
-  return *reinterpret_cast<const __half2*>(&r);
-}
-__device__ __forceinline__ uint32_t bits_of(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 // The three e4m3 parts of two probabilities below 2^8.  Differences of a number and its rounding
 // are exact; the first one is taken in fp32 and rounded to fp16 (2^-16 of P).
-__device__ __forceinline__ void split_p(float x0, float x1, uint16_t (&out)[3]) {
+__device__ __forceinline__ void split_p(float x0, float x1, uint32_t (&out)[3]) {
   const __half2 k32 = __floats2half2_rn(32.f, 32.f);
   out[0] = e4m3x2_of_floats(x0, x1);
   const float2 f = __half22float2(half2_of_e4m3x2(out[0]));
   const __half2 h = __hmul2(__floats2half2_rn(x0 - f.x, x1 - f.y), k32);
-  out[1] = e4m3x2_of_half2(bits_of(h));
-  out[2] = e4m3x2_of_half2(bits_of(__hmul2(__hsub2(h, half2_of_e4m3x2(out[1])), k32)));
+  out[1] = e4m3x2_of_half2(h);
+  out[2] = e4m3x2_of_half2(__hmul2(__hsub2(h, half2_of_e4m3x2(out[1])), k32));
 }
 
 // PARTS e4m3 parts of four numbers, exact differences: x = part 0 + part 1 / 32 + part 2 / 1024.
@@ -828,11 +811,11 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
           x[i] = ex2(t[r + i]);
           l[r + i] = fmaf(x[i], inv_vs, l[r + i]);
         }
-        uint16_t lo[kPParts], hi[kPParts];
+        uint32_t lo[kPParts], hi[kPParts];
         split_p(x[0], x[1], lo);
         split_p(x[2], x[3], hi);
 #pragma unroll
-        for (int i = 0; i < kPParts; ++i) part[i][r / 4] = (uint32_t)lo[i] | ((uint32_t)hi[i] << 16);
+        for (int i = 0; i < kPParts; ++i) part[i][r / 4] = lo[i] | (hi[i] << 16);
       }
 #pragma unroll
       for (int i = 0; i < kPParts; ++i) {

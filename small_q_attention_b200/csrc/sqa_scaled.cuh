@@ -33,6 +33,23 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+// Two packed e4m3 (low 16 bits) -> two fp16, exact; and back, to nearest even and saturating.
+__device__ __forceinline__ __half2 half2_of_e4m3x2(uint32_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)v));
+  return *reinterpret_cast<const __half2*>(&r);
+}
+__device__ __forceinline__ uint32_t e4m3x2_of_half2(__half2 h) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&h)));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2_of_floats(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 // Four floats -> four e4m3 (round to nearest even, saturating, NaN kept), first in the low byte.
 __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
   return pack_e4m3x2(a, b) | (pack_e4m3x2(c, d) << 16);

@@ -11,19 +11,27 @@
 //
 // 1. Selection.  Each CTA holds a slice of the scores as order-preserving 32-bit keys.
 //    A radix search over the range [lo, hi] that still holds the wanted rank: 256 equal
-//    bins, histograms summed over the cluster through distributed shared memory, one
-//    cluster barrier a pass, until the range is one key or a bin edge cuts off exactly
-//    the wanted count (three or four passes).  The range is taken from the scores
-//    themselves, so that the bins are used evenly (scores share their leading bits; a
-//    fixed digit would send them all to one bin and serialise its counter).
+//    bins, histograms exchanged over the cluster, one cluster barrier a pass.  The range is
+//    taken from the scores themselves, so that the bins are used evenly (scores share their
+//    leading bits; a fixed digit would send them all to one bin and serialise its counter).
+//    Once the bin of the wanted rank holds at most 256 keys, every CTA gets them all
+//    and each thread ranks one of them against the others: two exchanges for 8192 tokens
+//    where bins alone took four (2900 cycles each).  More than 256 equal keys end in a
+//    range of one key.
 // 2. Ranks.  A kept token's target is a sum of counts of earlier slices (shared through
 //    the cluster) and of a block scan; kept[] lists the kept positions.
-// 3. Moves, in place and in waves of C x 8 target pages: a warp loads the 16 source rows
+// 3. Moves, in place and in waves of C x T / 32 target pages: a warp loads the 16 source rows
 //    of its target page (K, V, scores, source scales) into registers, the cluster meets
 //    at a barrier, then every warp writes its page.  A source is never before its
 //    target, and the sources of later waves lie in pages behind this wave's targets, so
-//    nothing is overwritten before it is read.  A warp has a page's K and V (8 KB for
-//    16-bit elements) in flight at once.
+//    nothing is overwritten before it is read, and a wave's loads may be issued before the
+//    last one's stores (done for e4m3, whose pages take half the registers).
+//
+// C and T are chosen so that every cluster is resident at once where that is possible: one CTA of
+// 512 threads per SM, or two of 256.  (Clusters of 8 x 256 for 32 segments left some for a
+// second round: 36 us instead of 20 for 4 x 8192 to 2048.)
+#include <mutex>
+
 #include "small_q_attention.h"
 #include "sqa_internal.h"
 #include "sqa_ptx.cuh"
@@ -32,8 +40,8 @@
 namespace sqa {
 namespace {
 
-constexpr int kEvictThreads = 256;
-constexpr int kEvictWarps = kEvictThreads / 32;
+constexpr int kBins = 256;
+constexpr int kCandidates = 256;  // keys that are ranked directly
 constexpr int kEvictMaxCluster = 8;
 constexpr int kKeyCap = 12288;  // keys of a slice held in shared memory (48 KB); further ones are read again
 
@@ -58,13 +66,16 @@ struct EvictParams {
 // What the CTAs of a cluster tell one another they store into each other's shared memory before
 // a cluster barrier and read from their own after it: remote stores are not waited for, while a
 // loop of remote loads cost 8 round trips (a radix pass took 4500 cycles with them).
+template <int T>
 struct EvictShared {
-  unsigned int hist[256];                          // this slice's
-  unsigned int hists[2][kEvictMaxCluster][256];    // every slice's, by pass parity
+  unsigned int hist[kBins];                        // this slice's
+  unsigned int hists[2][kEvictMaxCluster][kBins];  // every slice's, by pass parity
   unsigned int range[kEvictMaxCluster][2];         // every slice's (lowest, highest) key
   unsigned int counts[kEvictMaxCluster][2];        // every slice's (above, equal)
-  unsigned int warp_a[kEvictWarps], warp_b[kEvictWarps];
-  unsigned int pick[3];
+  unsigned int cand_key[kCandidates], cand_pos[kCandidates];
+  unsigned int warp_a[T / 32], warp_b[T / 32];
+  unsigned int pick[4];
+  unsigned int fill;
 };
 
 // `v` to the same shared-memory location of the CTA of rank `rank`.
@@ -138,10 +149,12 @@ __device__ __forceinline__ float rescale_page(uint4 (&x)[kLoads], float source, 
   return scale;
 }
 
-template <int E>  // bytes per cached element: 2 (16-bit) or 1 (block-scaled e4m3)
-__global__ void __launch_bounds__(kEvictThreads, 2) sqa_cache_evict_kernel(const EvictParams p) {
+// E: bytes per cached element, 2 (16-bit) or 1 (block-scaled e4m3); T threads.
+template <int E, int T>
+__global__ void __launch_bounds__(T, 512 / T) sqa_cache_evict_kernel(const EvictParams p) {
+  constexpr int kWarps = T / 32;
   extern __shared__ unsigned int keys[];  // key_cap
-  __shared__ EvictShared sh;
+  __shared__ EvictShared<T> sh;
   grid_dependency_wait();
   allow_dependent_launch();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -151,6 +164,10 @@ __global__ void __launch_bounds__(kEvictThreads, 2) sqa_cache_evict_kernel(const
   const int b = seg / p.hkv, h = seg - b * p.hkv;
   const int len = __ldg(p.seq_lens + b);
   const int32_t* table = p.block_tables + (size_t)b * p.max_pages;
+  auto meet = [&]() {  // barrier of the cluster
+    if (C > 1) cluster_sync_all();
+    else __syncthreads();
+  };
   int32_t* const kept = p.kept + (size_t)seg * p.budget;
 
   // Sequences that stay as they are: short ones, and those whose length or pages are bad.
@@ -160,14 +177,14 @@ __global__ void __launch_bounds__(kEvictThreads, 2) sqa_cache_evict_kernel(const
   else if (pages > p.max_pages) err = 2u;  // SQA_DEV_SEQ_TOO_LONG
   else if (len > p.budget) {
     int bad = 0;
-    for (int i = tid; i < pages; i += kEvictThreads) {
+    for (int i = tid; i < pages; i += T) {
       const int id = __ldg(table + i);
       bad |= id < 0 || id >= p.num_pages;
     }
     if (__syncthreads_or(bad)) err = 8u;  // SQA_DEV_BAD_PAGE
   }
   if (err || len <= p.budget) {  // the same for every CTA of the cluster
-    for (int i = rank * kEvictThreads + tid; i < p.budget; i += C * kEvictThreads)
+    for (int i = rank * T + tid; i < p.budget; i += C * T)
       kept[i] = (!err && i < len) ? i : -1;
     if (h == 0 && rank == 0 && tid == 0) {
       p.new_lens[b] = len;
@@ -189,7 +206,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) sqa_cache_evict_kernel(const
   };
   auto key_at = [&](int i) { return i < p.key_cap ? keys[i] : read_key(i); };
   unsigned int lo = 0xffffffffu, hi = 0u;
-  for (int i = tid; i < count; i += kEvictThreads) {
+  for (int i = tid; i < count; i += T) {
     const unsigned int k = read_key(i);
     if (i < p.key_cap) keys[i] = k;
     lo = min(lo, k);
@@ -205,78 +222,112 @@ __global__ void __launch_bounds__(kEvictThreads, 2) sqa_cache_evict_kernel(const
   if (tid < C) {  // this slice's range to CTA `tid`
     lo = sh.warp_a[0];
     hi = sh.warp_b[0];
-    for (int w = 1; w < kEvictWarps; ++w) {
+    for (int w = 1; w < kWarps; ++w) {
       lo = min(lo, sh.warp_a[w]);
       hi = max(hi, sh.warp_b[w]);
     }
     st_cluster_u32(&sh.range[rank][0], tid, lo);
     st_cluster_u32(&sh.range[rank][1], tid, hi);
   }
-  cluster_sync_all();
+  meet();
   lo = 0xffffffffu;
   hi = 0u;
   for (int r = 0; r < C; ++r) {
     lo = min(lo, sh.range[r][0]);
     hi = max(hi, sh.range[r][1]);
   }
-  // Kept: every key > above, and of the keys == lo the first `need` (none once `exact`).
-  // Invariant: the keys above hi number want - need, those in [lo, hi] at least need.
+  // Kept: every key > last, and of the keys == last the first `need`.
+  // Invariant: want - need keys lie above hi, and at least `need` in [lo, hi].
   int need = want;
-  bool exact = want == 0;      // nothing from [lo, hi] is needed
-  unsigned int above = hi;     // keys > above are kept whatever else
-  for (int pass = 0; !exact && lo < hi; ++pass) {
+  bool ranked = want == 0;  // last and need are final
+  unsigned int last = hi;
+  for (int pass = 0; !ranked && lo < hi; ++pass) {
     const int shift = max(0, 24 - __clz(hi - lo));  // (hi - lo) >> shift < 256
-    sh.hist[tid] = 0u;
+    if (tid < kBins) sh.hist[tid] = 0u;
+    if (tid == 0) sh.fill = 0u;
     __syncthreads();
-    for (int i = tid; i < count; i += kEvictThreads) {
+    for (int i = tid; i < count; i += T) {
       const unsigned int k = key_at(i);
       if (k >= lo && k <= hi) atomicAdd(&sh.hist[(k - lo) >> shift], 1u);
     }
     __syncthreads();
-    const unsigned int mine = sh.hist[tid];
+    if (tid < kBins) {
+      const unsigned int mine = sh.hist[tid];
 #pragma unroll
-    for (int r = 0; r < kEvictMaxCluster; ++r)
-      if (r < C) st_cluster_u32(&sh.hists[pass & 1][rank][tid], r, mine);
-    cluster_sync_all();  // also: every CTA has read the pass before the last
-    // thread t: bin 255 - t, so that an inclusive scan counts from the top
-    const int bin = 255 - tid;
-    unsigned int n = 0;
-#pragma unroll
-    for (int r = 0; r < kEvictMaxCluster; ++r)
-      if (r < C) n += sh.hists[pass & 1][r][bin];
-    unsigned int incl = n;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const unsigned int y = __shfl_up_sync(0xffffffffu, incl, off);
-      if (lane >= off) incl += y;
+      for (int r = 0; r < kEvictMaxCluster; ++r)
+        if (r < C) st_cluster_u32(&sh.hists[pass & 1][rank][tid], r, mine);
     }
-    if (lane == 31) sh.warp_a[warp] = incl;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) incl += sh.warp_a[w];
-    if (incl >= (unsigned int)need && incl - n < (unsigned int)need) {  // exactly one thread
-      sh.pick[0] = (unsigned int)bin;
-      sh.pick[1] = incl;
-      sh.pick[2] = n;
+    meet();  // also: every CTA has read the pass before the last
+    // thread t < 256: bin 255 - t, so that an inclusive scan counts from the top
+    const int bin = kBins - 1 - tid;
+    unsigned int n = 0, incl = 0;
+    if (tid < kBins) {
+#pragma unroll
+      for (int r = 0; r < kEvictMaxCluster; ++r)
+        if (r < C) n += sh.hists[pass & 1][r][bin];
+      incl = n;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const unsigned int y = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += y;
+      }
+      if (lane == 31) sh.warp_a[warp] = incl;
     }
     __syncthreads();
-    const unsigned int j = sh.pick[0], upto = sh.pick[1], total = sh.pick[2];  // keys of bins >= j; of bin j
+    if (tid < kBins) {
+      for (int w = 0; w < warp; ++w) incl += sh.warp_a[w];
+      if (incl >= (unsigned int)need && incl - n < (unsigned int)need) {  // exactly one thread
+        sh.pick[0] = (unsigned int)bin;
+        sh.pick[1] = incl - n;  // keys above the bin, in the range
+        sh.pick[2] = n;
+      }
+    }
+    __syncthreads();
+    const unsigned int j = sh.pick[0], total = sh.pick[2];
     const unsigned int edge = lo + (j << shift);
     hi = edge + min(hi - edge, (1u << shift) - 1u);
     lo = edge;
-    above = hi;
-    if (upto == (unsigned int)need && lo > 0u) {  // the whole bin is kept: its lower edge is the limit
-      above = lo - 1u;
-      exact = true;
-    } else {
-      need -= (int)(upto - total);
+    need -= (int)sh.pick[1];
+    if (lo < hi && total <= kCandidates) {
+      // the bin's keys, with their positions, to every CTA, slice by slice
+      unsigned int at = 0;
+      for (int r = 0; r < rank; ++r) at += sh.hists[pass & 1][r][j];
+      for (int i = tid; i < count; i += T) {
+        const unsigned int k = key_at(i);
+        if (k >= lo && k <= hi) {
+          const unsigned int c = at + atomicAdd(&sh.fill, 1u);
+          for (int r = 0; r < C; ++r) {
+            st_cluster_u32(&sh.cand_key[c], r, k);
+            st_cluster_u32(&sh.cand_pos[c], r, (unsigned int)(a0 + i));
+          }
+        }
+      }
+      meet();
+      if (tid < (int)total) {  // its rank: keys above it, and equal ones before it
+        const unsigned int k = sh.cand_key[tid], t = sh.cand_pos[tid];
+        int more = 0, before = 0;
+        for (int c = 0; c < (int)total; ++c) {
+          const unsigned int kc = sh.cand_key[c];
+          more += kc > k;
+          before += kc == k && sh.cand_pos[c] < t;
+        }
+        if (more + before == need - 1) {  // the last that is kept: exactly one
+          sh.pick[0] = k;
+          sh.pick[3] = (unsigned int)(before + 1);
+        }
+      }
+      __syncthreads();
+      last = sh.pick[0];
+      need = (int)sh.pick[3];
+      ranked = true;
     }
   }
-  if (exact) need = 0;
-  const unsigned int last = exact ? above : lo;  // kept: key > last, and the first `need` with key == last
+  if (want == 0) need = 0;
+  else if (!ranked) last = lo;
 
   // ---- 2. ranks: (above, equal) counts of this slice and of the ones before it
   unsigned int gt = 0, eq = 0;
-  for (int i = tid; i < count; i += kEvictThreads) {
+  for (int i = tid; i < count; i += T) {
     const unsigned int k = key_at(i);
     gt += k > last;
     eq += k == last;
@@ -291,21 +342,21 @@ __global__ void __launch_bounds__(kEvictThreads, 2) sqa_cache_evict_kernel(const
   __syncthreads();
   if (tid < C) {
     gt = eq = 0;
-    for (int w = 0; w < kEvictWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       gt += sh.warp_a[w];
       eq += sh.warp_b[w];
     }
     st_cluster_u32(&sh.counts[rank][0], tid, gt);
     st_cluster_u32(&sh.counts[rank][1], tid, eq);
   }
-  cluster_sync_all();
+  meet();
   unsigned int gt_before = 0, eq_before = 0;
   for (int r = 0; r < rank; ++r) {
     gt_before += sh.counts[r][0];
     eq_before += sh.counts[r][1];
   }
   // four consecutive tokens a thread; counts of (above, equal) packed in 16 bits each
-  for (int base = 0; base < count; base += 4 * kEvictThreads) {
+  for (int base = 0; base < count; base += 4 * T) {
     const int i0 = base + 4 * tid;
     unsigned int k[4], packed = 0;
 #pragma unroll
@@ -323,7 +374,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) sqa_cache_evict_kernel(const
     if (lane == 31) sh.warp_a[warp] = incl;
     __syncthreads();
     unsigned int before = incl - packed, all = 0;
-    for (int w = 0; w < kEvictWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       const unsigned int x = sh.warp_a[w];
       if (w < warp) before += x;
       all += x;
@@ -340,10 +391,10 @@ __global__ void __launch_bounds__(kEvictThreads, 2) sqa_cache_evict_kernel(const
     gt_before += all & 0xffffu;
     eq_before += all >> 16;
   }
-  for (int i = rank * kEvictThreads + tid; i < p.sinks; i += C * kEvictThreads) kept[i] = i;
-  for (int i = rank * kEvictThreads + tid; i < p.recent; i += C * kEvictThreads)
+  for (int i = rank * T + tid; i < p.sinks; i += C * T) kept[i] = i;
+  for (int i = rank * T + tid; i < p.recent; i += C * T)
     kept[p.budget - p.recent + i] = len - p.recent + i;
-  cluster_sync_all();  // kept[] is complete, for every CTA of the cluster
+  meet();  // kept[] is complete, for every CTA of the cluster
 
   // ---- 3. moves, C x 8 target pages a wave
   constexpr int kLanesPerRow = kHeadDim * E / 16;     // 16 (16-bit) or 8 (e4m3) lanes hold a row
@@ -354,97 +405,160 @@ __global__ void __launch_bounds__(kEvictThreads, 2) sqa_cache_evict_kernel(const
   const size_t row = p.hnd ? (size_t)kHeadDim * E : (size_t)p.hkv * kHeadDim * E;  // bytes from slot to slot
   const size_t in_row = head + (lane % kLanesPerRow) * 16;
   const int targets = (p.budget + kPageSize - 1) / kPageSize;
-  // target page, and lane's source page and slot, of the wave from target `base` on: read a wave ahead
-  struct Source {
-    int rows, to, from, slot;
-  };
-  auto source_of = [&](int base) {
-    const int target = base + rank * kEvictWarps + warp;
-    Source s = {target < targets ? min(kPageSize, p.budget - target * kPageSize) : 0, 0, 0, 0};
-    if (s.rows > 0) {
-      s.to = __ldg(table + target);
-      if (lane < s.rows) {
-        const int t = __ldcg(kept + target * kPageSize + lane);
-        s.from = __ldg(table + t / kPageSize);
-        s.slot = t % kPageSize;
-      }
-    }
-    return s;
-  };
-  Source next = source_of(0);
-  for (int base = 0; base < targets; base += C * kEvictWarps) {
-    const Source src = next;
-    const int rows = src.rows, to = src.to;
+  struct Page {  // a wave's page: where it goes, and what the lane holds of it
+    int rows, to;
     uint4 k[kLoads], v[kLoads];
-    float score = 0.f, ks = 0.f, vs = 0.f;
-    if (rows > 0) {
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int r = i * kRowsPerLoad + sub;
-        const int rf = __shfl_sync(0xffffffffu, src.from, r), rs = __shfl_sync(0xffffffffu, src.slot, r);
-        const size_t at = (size_t)rf * p.page_stride + rs * row + in_row;
-        k[i] = v[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (r < rows) {
-          k[i] = __ldcg(reinterpret_cast<const uint4*>(p.k_cache + at));
-          v[i] = __ldcg(reinterpret_cast<const uint4*>(p.v_cache + at));
-        }
-      }
-      if (lane < rows) {
-        score = __ldcg(p.scores + ((size_t)src.from * p.hkv + h) * kPageSize + src.slot);
-        if constexpr (E == 1) {
-          ks = __ldcg(p.k_scales + (size_t)src.from * p.scale_stride + h);
-          vs = __ldcg(p.v_scales + (size_t)src.from * p.scale_stride + h);
-        }
+    float score, ks, vs;
+  };
+  auto indexes = [&](int base, Page& x, int& from, int& slot) {
+    const int target = base + rank * kWarps + warp;
+    x.rows = target < targets ? min(kPageSize, p.budget - target * kPageSize) : 0;
+    x.to = from = slot = 0;
+    if (x.rows > 0) {
+      x.to = __ldg(table + target);
+      if (lane < x.rows) {
+        const int t = __ldcg(kept + target * kPageSize + lane);
+        from = __ldg(table + t / kPageSize);
+        slot = t % kPageSize;
       }
     }
-    if (base + C * kEvictWarps < targets) next = source_of(base + C * kEvictWarps);
-    cluster_sync_all();  // every source of this wave has been read
-    if (rows > 0) {
+  };
+  auto load = [&](Page& x, int from, int slot) {
+    x.score = x.ks = x.vs = 0.f;
+    if (x.rows <= 0) return;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = i * kRowsPerLoad + sub;
+      const int rf = __shfl_sync(0xffffffffu, from, r), rs = __shfl_sync(0xffffffffu, slot, r);
+      const size_t at = (size_t)rf * p.page_stride + rs * row + in_row;
+      x.k[i] = x.v[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < x.rows) {
+        x.k[i] = __ldcg(reinterpret_cast<const uint4*>(p.k_cache + at));
+        x.v[i] = __ldcg(reinterpret_cast<const uint4*>(p.v_cache + at));
+      }
+    }
+    if (lane < x.rows) {
+      x.score = __ldcg(p.scores + ((size_t)from * p.hkv + h) * kPageSize + slot);
       if constexpr (E == 1) {
-        const float new_ks = rescale_page<kLoads, kRowsPerLoad>(k, ks, sub);
-        const float new_vs = rescale_page<kLoads, kRowsPerLoad>(v, vs, sub);
-        if (lane == 0) {
-          p.k_scales[(size_t)to * p.scale_stride + h] = new_ks;
-          p.v_scales[(size_t)to * p.scale_stride + h] = new_vs;
-        }
+        x.ks = __ldcg(p.k_scales + (size_t)from * p.scale_stride + h);
+        x.vs = __ldcg(p.v_scales + (size_t)from * p.scale_stride + h);
       }
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int r = i * kRowsPerLoad + sub;
-        if (r < rows) {
-          const size_t at = (size_t)to * p.page_stride + r * row + in_row;
-          *reinterpret_cast<uint4*>(p.k_cache + at) = k[i];
-          *reinterpret_cast<uint4*>(p.v_cache + at) = v[i];
-        }
-      }
-      if (lane < rows) p.scores[((size_t)to * p.hkv + h) * kPageSize + lane] = score;
     }
+  };
+  auto store = [&](Page& x) {
+    if (x.rows <= 0) return;
+    if constexpr (E == 1) {
+      const float new_ks = rescale_page<kLoads, kRowsPerLoad>(x.k, x.ks, sub);
+      const float new_vs = rescale_page<kLoads, kRowsPerLoad>(x.v, x.vs, sub);
+      if (lane == 0) {
+        p.k_scales[(size_t)x.to * p.scale_stride + h] = new_ks;
+        p.v_scales[(size_t)x.to * p.scale_stride + h] = new_vs;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = i * kRowsPerLoad + sub;
+      if (r < x.rows) {
+        const size_t at = (size_t)x.to * p.page_stride + r * row + in_row;
+        *reinterpret_cast<uint4*>(p.k_cache + at) = x.k[i];
+        *reinterpret_cast<uint4*>(p.v_cache + at) = x.v[i];
+      }
+    }
+    if (lane < x.rows) p.scores[((size_t)x.to * p.hkv + h) * kPageSize + lane] = x.score;
+  };
+  const int wave = C * kWarps;
+  Page x;
+  int from, slot;
+  indexes(0, x, from, slot);
+  load(x, from, slot);
+  if (wave < targets) {
+    Page ahead;  // its indexes (16-bit caches) or all of it (e4m3) while this wave's loads are under way
+    indexes(wave, ahead, from, slot);
+    for (int base = 0; base < targets; base += wave) {
+      const bool more = base + wave < targets;
+      if (E == 1 && more) load(ahead, from, slot);
+      meet();  // every source of this wave has been read
+      store(x);
+      if (more) {
+        if (E == 2) load(ahead, from, slot);
+        x = ahead;
+        if (base + 2 * wave < targets) indexes(base + 2 * wave, ahead, from, slot);
+      }
+    }
+  } else {
+    meet();
+    store(x);
   }
 }
+// Clusters of C CTAs that can be resident at once.
+template <int E, int T>
+int resident_clusters(int cluster) {
+  static std::mutex mu;
+  static int known[64][kEvictMaxCluster + 1] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  std::lock_guard<std::mutex> lock(mu);
+  if (known[dev][cluster] != 0) return known[dev][cluster];
+  auto kernel = sqa_cache_evict_kernel<E, T>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeyCap * (int)sizeof(unsigned int)) !=
+      cudaSuccess) {
+    (void)cudaGetLastError();
+    return 0;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)cluster);
+  cfg.blockDim = dim3(T);
+  cfg.dynamicSmemBytes = kKeyCap * sizeof(unsigned int);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();
+    n = 0;
+  }
+  known[dev][cluster] = n;
+  return n;
+}
 
-template <int E>
-cudaError_t launch_evict(const EvictParams& p, int segments, cudaStream_t stream) {
-  auto kernel = sqa_cache_evict_kernel<E>;
-  const int smem = p.key_cap * (int)sizeof(unsigned int);
+template <int E, int T>
+cudaError_t launch_evict(EvictParams p, int segments, int cluster, cudaStream_t stream) {
+  auto kernel = sqa_cache_evict_kernel<E, T>;
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          kKeyCap * (int)sizeof(unsigned int));
   if (err != cudaSuccess) return err;
+  p.cluster = cluster;
+  const int64_t slice = ((int64_t)p.max_pages * kPageSize + cluster - 1) / cluster;
+  p.key_cap = slice < kKeyCap ? (int)slice : kKeyCap;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(segments * p.cluster));
-  cfg.blockDim = dim3(kEvictThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3((unsigned)(segments * cluster));
+  cfg.blockDim = dim3(T);
+  cfg.dynamicSmemBytes = p.key_cap * sizeof(unsigned int);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)p.cluster;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   err = cudaLaunchKernelEx(&cfg, kernel, p);
   return err != cudaSuccess ? err : cudaGetLastError();
+}
+
+// The largest clusters of 512-thread CTAs (one a SM) that are all resident at once; where even single
+// CTAs are not, 256 threads (two a SM), in rounds if need be.
+template <int E>
+cudaError_t launch_evict_shape(const EvictParams& p, int segments, cudaStream_t stream) {
+  for (int c = kEvictMaxCluster; c >= 1; c /= 2)
+    if (resident_clusters<E, 512>(c) >= segments) return launch_evict<E, 512>(p, segments, c, stream);
+  return launch_evict<E, 256>(p, segments, 1, stream);
 }
 
 }  // namespace
@@ -481,10 +595,6 @@ extern "C" SQA_API int sqa_cache_evict(const sqa_evict_args* a, const sqa_scales
   if (scales) narrow |= reinterpret_cast<uintptr_t>(scales->key) | reinterpret_cast<uintptr_t>(scales->value);
   if ((wide & 15u) || (narrow & 3u)) return SQA_ERR_INVALID_ARGUMENT;
 
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return SQA_ERR_CUDA;
   EvictParams p = {};
   const int elem = fp8 ? 1 : 2;
   p.k_cache = static_cast<uint8_t*>(a->key_cache);
@@ -506,13 +616,8 @@ extern "C" SQA_API int sqa_cache_evict(const sqa_evict_args* a, const sqa_scales
   p.budget = a->budget;
   p.recent = a->recent;
   p.sinks = a->sinks;
-  // The largest cluster that leaves no more than two waves of the card's 2 CTAs per SM:
-  // few segments need many CTAs each to fill the card, many fill it by themselves.
   const int segments = a->batch * a->num_kv_heads;
-  p.cluster = kEvictMaxCluster;
-  while (p.cluster > 1 && (int64_t)segments * p.cluster > 4LL * sms) p.cluster /= 2;
-  const int64_t slice = ((int64_t)a->max_pages * kPageSize + p.cluster - 1) / p.cluster;
-  p.key_cap = slice < kKeyCap ? (int)slice : kKeyCap;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return (fp8 ? launch_evict<1>(p, segments, s) : launch_evict<2>(p, segments, s)) == cudaSuccess ? SQA_OK : SQA_ERR_CUDA;
+  return (fp8 ? launch_evict_shape<1>(p, segments, s) : launch_evict_shape<2>(p, segments, s)) == cudaSuccess ? SQA_OK
+                                                                                                            : SQA_ERR_CUDA;
 }

@@ -346,7 +346,7 @@ SQA_API int sqa_accumulate_weights(const sqa_args* args, const float* lse, const
 typedef struct sqa_evict_args {
   void* key_cache;             /* as in sqa_args */
   void* value_cache;
-  float* scores;               /* [num_pages, num_kv_heads, 16] */
+  float* scores;               /* [num_pages, num_kv_heads, 16], 16-byte aligned */
   const int32_t* block_tables; /* [batch, max_pages] */
   const int32_t* seq_lens;     /* [batch] */
   int32_t* new_lens;           /* [batch]; not seq_lens itself */

@@ -200,17 +200,23 @@ __global__ void __launch_bounds__(T, 512 / T) sqa_cache_evict_kernel(const Evict
   const int per = (middle + C - 1) / C;
   const int a0 = p.sinks + min(middle, rank * per);
   const int count = p.sinks + min(middle, (rank + 1) * per) - a0;
-  auto read_key = [&](int i) {
-    const int t = a0 + i;
-    return score_key(__ldcg(p.scores + ((size_t)__ldg(table + t / kPageSize) * p.hkv + h) * kPageSize + t % kPageSize));
-  };
-  auto key_at = [&](int i) { return i < p.key_cap ? keys[i] : read_key(i); };
+  const int off = a0 & 3;  // keys[] starts at a multiple of four positions: 16-byte loads of the scores
+  auto scores_of = [&](int t) { return p.scores + ((size_t)__ldg(table + t / kPageSize) * p.hkv + h) * kPageSize + t % kPageSize; };
+  auto key_at = [&](int i) { return i + off < p.key_cap ? keys[i + off] : score_key(__ldcg(scores_of(a0 + i))); };
   unsigned int lo = 0xffffffffu, hi = 0u;
-  for (int i = tid; i < count; i += T) {
-    const unsigned int k = read_key(i);
-    if (i < p.key_cap) keys[i] = k;
-    lo = min(lo, k);
-    hi = max(hi, k);
+#pragma unroll 4
+  for (int q = tid; q < (off + count + 3) / 4; q += T) {
+    const float4 f = __ldcg(reinterpret_cast<const float4*>(scores_of(a0 - off + 4 * q)));
+    const unsigned int k[4] = {score_key(f.x), score_key(f.y), score_key(f.z), score_key(f.w)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = 4 * q + i;
+      if (at < p.key_cap) keys[at] = k[i];
+      if (at >= off && at < off + count) {
+        lo = min(lo, k[i]);
+        hi = max(hi, k[i]);
+      }
+    }
   }
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
@@ -325,71 +331,58 @@ __global__ void __launch_bounds__(T, 512 / T) sqa_cache_evict_kernel(const Evict
   if (want == 0) need = 0;
   else if (!ranked) last = lo;
 
-  // ---- 2. ranks: (above, equal) counts of this slice and of the ones before it
+  // ---- 2. ranks: each thread a run of tokens (of odd length: no bank is met twice), one scan
+  const int run = ((count + T - 1) / T) | 1;
+  const int i0 = min(count, tid * run), i1 = min(count, i0 + run);
   unsigned int gt = 0, eq = 0;
-  for (int i = tid; i < count; i += T) {
+  for (int i = i0; i < i1; ++i) {
     const unsigned int k = key_at(i);
     gt += k > last;
     eq += k == last;
   }
-  gt = __reduce_add_sync(0xffffffffu, gt);
-  eq = __reduce_add_sync(0xffffffffu, eq);
+  unsigned int gt_to = gt, eq_to = eq;  // up to and with this thread's
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const unsigned int x = __shfl_up_sync(0xffffffffu, gt_to, off), y = __shfl_up_sync(0xffffffffu, eq_to, off);
+    if (lane >= off) {
+      gt_to += x;
+      eq_to += y;
+    }
+  }
   __syncthreads();  // warp_a is free
-  if (lane == 0) {
-    sh.warp_a[warp] = gt;
-    sh.warp_b[warp] = eq;
+  if (lane == 31) {
+    sh.warp_a[warp] = gt_to;
+    sh.warp_b[warp] = eq_to;
   }
   __syncthreads();
-  if (tid < C) {
-    gt = eq = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      gt += sh.warp_a[w];
-      eq += sh.warp_b[w];
+  unsigned int all_gt = 0, all_eq = 0;
+  unsigned int g = gt_to - gt, e = eq_to - eq;  // kept and equal tokens before this thread's
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) {
+      g += all_gt;
+      e += all_eq;
     }
-    st_cluster_u32(&sh.counts[rank][0], tid, gt);
-    st_cluster_u32(&sh.counts[rank][1], tid, eq);
+    all_gt += sh.warp_a[w];
+    all_eq += sh.warp_b[w];
   }
-  meet();
-  unsigned int gt_before = 0, eq_before = 0;
-  for (int r = 0; r < rank; ++r) {
-    gt_before += sh.counts[r][0];
-    eq_before += sh.counts[r][1];
+  if (C > 1) {
+    if (tid < C) {
+      st_cluster_u32(&sh.counts[rank][0], tid, all_gt);
+      st_cluster_u32(&sh.counts[rank][1], tid, all_eq);
+    }
+    meet();
+    for (int r = 0; r < rank; ++r) {
+      g += sh.counts[r][0];
+      e += sh.counts[r][1];
+    }
   }
-  // four consecutive tokens a thread; counts of (above, equal) packed in 16 bits each
-  for (int base = 0; base < count; base += 4 * T) {
-    const int i0 = base + 4 * tid;
-    unsigned int k[4], packed = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      k[i] = i0 + i < count ? key_at(i0 + i) : 0u;
-      if (i0 + i < count) packed += (k[i] > last ? 1u : 0u) + (k[i] == last ? 0x10000u : 0u);
-    }
-    unsigned int incl = packed;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const unsigned int y = __shfl_up_sync(0xffffffffu, incl, off);
-      if (lane >= off) incl += y;
-    }
-    __syncthreads();  // the last tile's counts have been read
-    if (lane == 31) sh.warp_a[warp] = incl;
-    __syncthreads();
-    unsigned int before = incl - packed, all = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      const unsigned int x = sh.warp_a[w];
-      if (w < warp) before += x;
-      all += x;
-    }
-    unsigned int g = gt_before + (before & 0xffffu), e = eq_before + (before >> 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i0 + i >= count) break;
-      const bool is_gt = k[i] > last, is_eq = k[i] == last;
-      if (is_gt || (is_eq && e < (unsigned int)need)) kept[p.sinks + g + min(e, (unsigned int)need)] = a0 + i0 + i;
-      g += is_gt;
-      e += is_eq;
-    }
-    gt_before += all & 0xffffu;
-    eq_before += all >> 16;
+  for (int i = i0; i < i1; ++i) {
+    const unsigned int k = key_at(i);
+    const bool is_gt = k > last, is_eq = k == last;
+    if (is_gt || (is_eq && e < (unsigned int)need)) kept[p.sinks + g + min(e, (unsigned int)need)] = a0 + i;
+    g += is_gt;
+    e += is_eq;
   }
   for (int i = rank * T + tid; i < p.sinks; i += C * T) kept[i] = i;
   for (int i = rank * T + tid; i < p.recent; i += C * T)
@@ -532,7 +525,7 @@ cudaError_t launch_evict(EvictParams p, int segments, int cluster, cudaStream_t 
                                          kKeyCap * (int)sizeof(unsigned int));
   if (err != cudaSuccess) return err;
   p.cluster = cluster;
-  const int64_t slice = ((int64_t)p.max_pages * kPageSize + cluster - 1) / cluster;
+  const int64_t slice = ((int64_t)p.max_pages * kPageSize + cluster - 1) / cluster + 3;  // + its start's remainder
   p.key_cap = slice < kKeyCap ? (int)slice : kKeyCap;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(segments * cluster));
@@ -588,8 +581,9 @@ extern "C" SQA_API int sqa_cache_evict(const sqa_evict_args* a, const sqa_scales
   if (!a->key_cache || !a->value_cache || !a->scores || !a->block_tables || !a->seq_lens || !a->new_lens || !a->kept ||
       a->new_lens == a->seq_lens || (scales && (!scales->key || !scales->value)))
     return SQA_ERR_INVALID_ARGUMENT;
-  const uintptr_t wide = reinterpret_cast<uintptr_t>(a->key_cache) | reinterpret_cast<uintptr_t>(a->value_cache);
-  uintptr_t narrow = reinterpret_cast<uintptr_t>(a->scores) | reinterpret_cast<uintptr_t>(a->block_tables) |
+  const uintptr_t wide = reinterpret_cast<uintptr_t>(a->key_cache) | reinterpret_cast<uintptr_t>(a->value_cache) |
+                         reinterpret_cast<uintptr_t>(a->scores);
+  uintptr_t narrow = reinterpret_cast<uintptr_t>(a->block_tables) |
                      reinterpret_cast<uintptr_t>(a->seq_lens) | reinterpret_cast<uintptr_t>(a->new_lens) |
                      reinterpret_cast<uintptr_t>(a->kept) | reinterpret_cast<uintptr_t>(a->status);
   if (scales) narrow |= reinterpret_cast<uintptr_t>(scales->key) | reinterpret_cast<uintptr_t>(scales->value);

@@ -202,19 +202,44 @@ __global__ void __launch_bounds__(T, 512 / T) sqa_cache_evict_kernel(const Evict
   const int count = p.sinks + min(middle, (rank + 1) * per) - a0;
   const int off = a0 & 3;  // keys[] starts at a multiple of four positions: 16-byte loads of the scores
   auto scores_of = [&](int t) { return p.scores + ((size_t)__ldg(table + t / kPageSize) * p.hkv + h) * kPageSize + t % kPageSize; };
-  auto key_at = [&](int i) { return i + off < p.key_cap ? keys[i + off] : score_key(__ldcg(scores_of(a0 + i))); };
-  unsigned int lo = 0xffffffffu, hi = 0u;
+  // f(i, key) for i = from, from + step, .. < to.  One loop over shared memory where it holds the whole
+  // slice: with the choice inside, no two iterations overlapped.
+  const bool held = off + count <= p.key_cap;
+  auto for_keys = [&](int from, int to, int step, auto f) {
+    if (held) {
 #pragma unroll 4
-  for (int q = tid; q < (off + count + 3) / 4; q += T) {
-    const float4 f = __ldcg(reinterpret_cast<const float4*>(scores_of(a0 - off + 4 * q)));
-    const unsigned int k[4] = {score_key(f.x), score_key(f.y), score_key(f.z), score_key(f.w)};
+      for (int i = from; i < to; i += step) f(i, keys[i + off]);
+    } else {
+#pragma unroll 1
+      for (int i = from; i < to; i += step)
+        f(i, i + off < p.key_cap ? keys[i + off] : score_key(__ldcg(scores_of(a0 + i))));
+    }
+  };
+  unsigned int lo = 0xffffffffu, hi = 0u;
+  constexpr int kAhead = 4;  // loads in flight: page ids, then scores
+  for (int q0 = tid; q0 < (off + count + 3) / 4; q0 += kAhead * T) {
+    float4 f[kAhead];
+    const float* src[kAhead];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = 4 * q + i;
-      if (at < p.key_cap) keys[at] = k[i];
-      if (at >= off && at < off + count) {
-        lo = min(lo, k[i]);
-        hi = max(hi, k[i]);
+    for (int c = 0; c < kAhead; ++c) {
+      const int q = q0 + c * T;
+      src[c] = q < (off + count + 3) / 4 ? scores_of(a0 - off + 4 * q) : nullptr;
+    }
+#pragma unroll
+    for (int c = 0; c < kAhead; ++c)
+      f[c] = src[c] ? __ldcg(reinterpret_cast<const float4*>(src[c])) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < kAhead; ++c) {
+      if (!src[c]) continue;
+      const unsigned int k[4] = {score_key(f[c].x), score_key(f[c].y), score_key(f[c].z), score_key(f[c].w)};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = 4 * (q0 + c * T) + i;
+        if (at < p.key_cap) keys[at] = k[i];
+        if (at >= off && at < off + count) {
+          lo = min(lo, k[i]);
+          hi = max(hi, k[i]);
+        }
       }
     }
   }
@@ -252,10 +277,9 @@ __global__ void __launch_bounds__(T, 512 / T) sqa_cache_evict_kernel(const Evict
     if (tid < kBins) sh.hist[tid] = 0u;
     if (tid == 0) sh.fill = 0u;
     __syncthreads();
-    for (int i = tid; i < count; i += T) {
-      const unsigned int k = key_at(i);
+    for_keys(tid, count, T, [&](int, unsigned int k) {
       if (k >= lo && k <= hi) atomicAdd(&sh.hist[(k - lo) >> shift], 1u);
-    }
+    });
     __syncthreads();
     if (tid < kBins) {
       const unsigned int mine = sh.hist[tid];
@@ -298,8 +322,7 @@ __global__ void __launch_bounds__(T, 512 / T) sqa_cache_evict_kernel(const Evict
       // the bin's keys, with their positions, to every CTA, slice by slice
       unsigned int at = 0;
       for (int r = 0; r < rank; ++r) at += sh.hists[pass & 1][r][j];
-      for (int i = tid; i < count; i += T) {
-        const unsigned int k = key_at(i);
+      for_keys(tid, count, T, [&](int i, unsigned int k) {
         if (k >= lo && k <= hi) {
           const unsigned int c = at + atomicAdd(&sh.fill, 1u);
           for (int r = 0; r < C; ++r) {
@@ -307,11 +330,12 @@ __global__ void __launch_bounds__(T, 512 / T) sqa_cache_evict_kernel(const Evict
             st_cluster_u32(&sh.cand_pos[c], r, (unsigned int)(a0 + i));
           }
         }
-      }
+      });
       meet();
       if (tid < (int)total) {  // its rank: keys above it, and equal ones before it
         const unsigned int k = sh.cand_key[tid], t = sh.cand_pos[tid];
         int more = 0, before = 0;
+#pragma unroll 4
         for (int c = 0; c < (int)total; ++c) {
           const unsigned int kc = sh.cand_key[c];
           more += kc > k;
@@ -335,11 +359,10 @@ __global__ void __launch_bounds__(T, 512 / T) sqa_cache_evict_kernel(const Evict
   const int run = ((count + T - 1) / T) | 1;
   const int i0 = min(count, tid * run), i1 = min(count, i0 + run);
   unsigned int gt = 0, eq = 0;
-  for (int i = i0; i < i1; ++i) {
-    const unsigned int k = key_at(i);
+  for_keys(i0, i1, 1, [&](int, unsigned int k) {
     gt += k > last;
     eq += k == last;
-  }
+  });
   unsigned int gt_to = gt, eq_to = eq;  // up to and with this thread's
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -377,13 +400,12 @@ __global__ void __launch_bounds__(T, 512 / T) sqa_cache_evict_kernel(const Evict
       e += sh.counts[r][1];
     }
   }
-  for (int i = i0; i < i1; ++i) {
-    const unsigned int k = key_at(i);
+  for_keys(i0, i1, 1, [&](int i, unsigned int k) {
     const bool is_gt = k > last, is_eq = k == last;
     if (is_gt || (is_eq && e < (unsigned int)need)) kept[p.sinks + g + min(e, (unsigned int)need)] = a0 + i;
     g += is_gt;
     e += is_eq;
-  }
+  });
   for (int i = rank * T + tid; i < p.sinks; i += C * T) kept[i] = i;
   for (int i = rank * T + tid; i < p.recent; i += C * T)
     kept[p.budget - p.recent + i] = len - p.recent + i;

@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(T, 512 / T) sqa_cache_evict_kernel(const Evict
     store(x);
   }
 }
-// Clusters of C CTAs that can be resident at once.
+// Clusters of C CTAs that can be resident at once (and, once per device, the kernel's shared-memory limit).
 template <int E, int T>
 int resident_clusters(int cluster) {
   static std::mutex mu;
@@ -543,9 +543,6 @@ int resident_clusters(int cluster) {
 template <int E, int T>
 cudaError_t launch_evict(EvictParams p, int segments, int cluster, cudaStream_t stream) {
   auto kernel = sqa_cache_evict_kernel<E, T>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         kKeyCap * (int)sizeof(unsigned int));
-  if (err != cudaSuccess) return err;
   p.cluster = cluster;
   const int64_t slice = ((int64_t)p.max_pages * kPageSize + cluster - 1) / cluster + 3;  // + its start's remainder
   p.key_cap = slice < kKeyCap ? (int)slice : kKeyCap;
@@ -563,7 +560,7 @@ cudaError_t launch_evict(EvictParams p, int segments, int cluster, cudaStream_t 
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  err = cudaLaunchKernelEx(&cfg, kernel, p);
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, p);
   return err != cudaSuccess ? err : cudaGetLastError();
 }
 
@@ -573,6 +570,7 @@ template <int E>
 cudaError_t launch_evict_shape(const EvictParams& p, int segments, cudaStream_t stream) {
   for (int c = kEvictMaxCluster; c >= 1; c /= 2)
     if (resident_clusters<E, 512>(c) >= segments) return launch_evict<E, 512>(p, segments, c, stream);
+  (void)resident_clusters<E, 256>(1);  // sets the shared-memory limit
   return launch_evict<E, 256>(p, segments, 1, stream);
 }
 

@@ -53,6 +53,8 @@
 //   p_full / p_done [4]      softmax -> value issuer (commit) -> softmax, one P buffer a stream
 //   q_ready [2]              softmax (Q of a piece, one piece ahead) -> score issuer
 //   m_full / m_empty [8]     page scales of a block -> softmax
+#include <atomic>
+
 #include "small_q_attention.h"
 #include "sqa_internal.h"
 #include "sqa_merge_row.cuh"
@@ -78,21 +80,22 @@ constexpr float kLn2f = 0.6931471805599453f;
 constexpr float kMinValueScale = 8.673617379884035e-19f;  // 2^-60: smaller value scales count as this
 
 // PARTS: e4m3 parts of Q (and P): 2 or 3; 0 = 16-bit cache (weights only).
-// ROWS: query rows of a group (8 or 16), G groups (1, 2 or 4).
+// ROWS: query rows of a group (8 or 16; 32 too for the weights), G groups (1, 2 or 4).
 template <int PARTS_, int ROWS_, int G_, bool ATTEND_>
 struct Shape {
   static constexpr int PARTS = PARTS_, ROWS = ROWS_, G = G_;
   static constexpr bool ATTEND = ATTEND_, F8 = PARTS_ > 0;
   static constexpr int COLS = (F8 ? PARTS : 1) * ROWS;
   static constexpr int N = (COLS + 15) / 16 * 16;             // score columns of a group (N of the product)
-  static constexpr int STRIDE = N <= 16 ? 16 : N <= 32 ? 32 : 64;  // TMEM columns of a score slot
+  static constexpr int STRIDE = N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128;  // TMEM columns of a score slot
   static constexpr int OCOLS = ATTEND ? kStreams * kPRow : 0;  // O^T of the streams
   static constexpr int SLOTS_FIT = (512 - OCOLS) / STRIDE;
   static constexpr int NS = SLOTS_FIT < 8 ? SLOTS_FIT : 8;
   static constexpr int Q_GROUP = F8 ? N * 128 : 2 * N * 128;  // bytes of one group's Q operand
   static constexpr int Q_BYTES = G * Q_GROUP;
   static constexpr int TILES = ATTEND || !F8 ? 2 : 1;         // 16 KB tiles of a block (K and V, or K's two halves)
-  static_assert(N <= 64 && kPParts * ROWS <= kPRow && NS >= kStreams && kStreams % G == 0, "columns");
+  static_assert(!ATTEND || (N <= 64 && kPParts * ROWS <= kPRow && NS >= kStreams && kStreams % G == 0), "columns");
+  static_assert(N <= 128 && NS >= 4, "columns");
 };
 
 struct ScaledTcParams {
@@ -1145,8 +1148,15 @@ cudaError_t launch_shape(ScaledTcParams& p, const CUtensorMap& tm_k, const CUten
   auto kernel = sqa_scaled_tc_kernel<S, BF>;
   p.s.num_stages = tiles_that_fit<S>();
   const int smem = 1024 + Smem<S>::RING + p.s.num_stages * kTileBytes;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<bool> configured[64];  // per device
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
+  if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (err != cudaSuccess) return err;
+    if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(kScaledTcThreads);
@@ -1167,8 +1177,13 @@ cudaError_t launch_rows(ScaledTcParams& p, const CUtensorMap& tm_k, const CUtens
   const int rows = kGroup * p.s.q_len;
   if (rows <= 8) return launch_shape<Shape<PARTS, 8, 1, ATTEND>, BF>(p, tm_k, tm_v, grid, stream);
   if (rows <= 16) return launch_shape<Shape<PARTS, 16, 1, ATTEND>, BF>(p, tm_k, tm_v, grid, stream);
-  if (rows <= 32) return launch_shape<Shape<PARTS, 16, 2, ATTEND>, BF>(p, tm_k, tm_v, grid, stream);
-  return launch_shape<Shape<PARTS, 16, 4, ATTEND>, BF>(p, tm_k, tm_v, grid, stream);
+  if constexpr (ATTEND) {
+    if (rows <= 32) return launch_shape<Shape<PARTS, 16, 2, true>, BF>(p, tm_k, tm_v, grid, stream);
+    return launch_shape<Shape<PARTS, 16, 4, true>, BF>(p, tm_k, tm_v, grid, stream);
+  } else {  // wider units: no P, no O, and K read less often
+    if (rows <= 32) return launch_shape<Shape<PARTS, 32, 1, false>, BF>(p, tm_k, tm_v, grid, stream);
+    return launch_shape<Shape<PARTS, 32, 2, false>, BF>(p, tm_k, tm_v, grid, stream);
+  }
 }
 
 ScaledTcParams tc_params(const ScaledParams& p) {

@@ -50,7 +50,7 @@
 //   full / empty [tiles]     producer -> issuers; K and V tiles (16 KB) alternate in one ring,
 //                            each released by the commit of the product that read it
 //   s_full / s_empty [NS]    score issuer (commit) -> softmax -> score issuer
-//   p_full / p_done [4]      softmax -> value issuer (commit) -> softmax, one P buffer a stream
+//   p_full / p_done [2 W]    softmax -> value issuer (commit) -> softmax, two P buffers a stream
 //   q_ready [2]              softmax (Q of a piece, one piece ahead) -> score issuer
 //   m_full / m_empty [8]     page scales of a block -> softmax
 #include <atomic>
@@ -69,33 +69,32 @@ constexpr int kBlockPages = 8;
 constexpr int kBlock = kBlockPages * kPageSize;  // 128 tokens: the M side
 constexpr int kTileBytes = kBlock * 128;         // K or V of a block (e4m3), or one half of 16-bit K
 constexpr int kMetaSlots = 8;
-constexpr int kPRow = 64;                        // bytes of a token's P: up to three parts of 16 rows
-constexpr int kPBytes = kBlock * kPRow;
 constexpr int kPParts = 3;                       // e4m3 parts of a probability
-constexpr int kStreams = 4;                      // softmax warpgroups
-constexpr int kSoftmaxThreads = kStreams * 128;
-constexpr int kScaledTcThreads = kSoftmaxThreads + 128;
 constexpr float kRaise = 8.f, kHead = -1.f;      // raise a base that a score exceeds by 2^8, to 2 times the maximum
 constexpr float kLn2f = 0.6931471805599453f;
 constexpr float kMinValueScale = 8.673617379884035e-19f;  // 2^-60: smaller value scales count as this
 
 // PARTS: e4m3 parts of Q (and P): 2 or 3; 0 = 16-bit cache (weights only).
-// ROWS: query rows of a group (8 or 16; 32 too for the weights), G groups (1, 2 or 4).
-template <int PARTS_, int ROWS_, int G_, bool ATTEND_>
+// ROWS: query rows of a group, G groups, W streams (softmax warpgroups).
+template <int PARTS_, int ROWS_, int G_, int W_, bool ATTEND_>
 struct Shape {
-  static constexpr int PARTS = PARTS_, ROWS = ROWS_, G = G_;
+  static constexpr int PARTS = PARTS_, ROWS = ROWS_, G = G_, W = W_;
   static constexpr bool ATTEND = ATTEND_, F8 = PARTS_ > 0;
+  static constexpr int SOFTMAX = W * 128, THREADS = SOFTMAX + 128;
   static constexpr int COLS = (F8 ? PARTS : 1) * ROWS;
   static constexpr int N = (COLS + 15) / 16 * 16;             // score columns of a group (N of the product)
   static constexpr int STRIDE = N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128;  // TMEM columns of a score slot
-  static constexpr int OCOLS = ATTEND ? kStreams * kPRow : 0;  // O^T of the streams
+  static constexpr int PROW = ROWS > 16 ? 128 : 64;           // bytes of a token's P: up to three parts of the rows
+  static constexpr int PBYTES = kBlock * PROW;
+  static constexpr int OCOLS = ATTEND ? W * PROW : 0;         // O^T of the streams
   static constexpr int SLOTS_FIT = (512 - OCOLS) / STRIDE;
   static constexpr int NS = SLOTS_FIT < 8 ? SLOTS_FIT : 8;
   static constexpr int Q_GROUP = F8 ? N * 128 : 2 * N * 128;  // bytes of one group's Q operand
   static constexpr int Q_BYTES = G * Q_GROUP;
   static constexpr int TILES = ATTEND || !F8 ? 2 : 1;         // 16 KB tiles of a block (K and V, or K's two halves)
-  static_assert(!ATTEND || (N <= 64 && kPParts * ROWS <= kPRow && NS >= kStreams && kStreams % G == 0), "columns");
-  static_assert(N <= 128 && NS >= 4, "columns");
+  static constexpr int Q_STEPS = (G * ROWS * 8 + SOFTMAX - 1) / SOFTMAX;
+  static_assert(!ATTEND || (kPParts * ROWS <= PROW && NS >= W && W % G == 0), "columns");
+  static_assert(N <= 128 && NS >= 2 && W <= 4 && G * ROWS <= 64, "columns");
 };
 
 struct ScaledTcParams {
@@ -112,14 +111,14 @@ struct ScaledTcParams {
 template <class S>
 struct Smem {
   static constexpr int kMaxTiles = 16;
-  static constexpr int P = 0;                                           // a P buffer for each stream
-  static constexpr int Q = P + (S::ATTEND ? kStreams * kPBytes : 0);    // two Q slots
+  static constexpr int P = 0;                                           // two P buffers for each stream
+  static constexpr int Q = P + (S::ATTEND ? S::W * 2 * S::PBYTES : 0);    // two Q slots
   static constexpr int META = Q + 2 * S::Q_BYTES;                       // [kMetaSlots][8]: ks, log2 vs, 1 / vs, page id (bits)
-  static constexpr int BASE = META + kMetaSlots * kBlockPages * 16;     // [4][16]: a stream's bases (weights: -lse, [64])
-  static constexpr int DELTA = BASE + 64 * 4;                           // [4][16]: raises; the epilogue's factors of O
-  static constexpr int WRED = DELTA + 64 * 4;                           // [16][16]: per-warp maxima, then sums
-  static constexpr int NAN_FROM = WRED + 256 * 4;                       // [4][128]
-  static constexpr int CQ = NAN_FROM + kStreams * 128 * 4;              // [2]: log2-domain score factor of a Q slot
+  static constexpr int BASE = META + kMetaSlots * kBlockPages * 16;     // [W][ROWS]: a stream's bases (weights: -lse of all rows)
+  static constexpr int DELTA = BASE + 64 * 4;                           // [W][ROWS]: raises; the epilogue's factors of O
+  static constexpr int WRED = DELTA + 64 * 4;                           // [4 W][ROWS]: per-warp maxima, then sums
+  static constexpr int NAN_FROM = WRED + 256 * 4;                       // [W][128]
+  static constexpr int CQ = NAN_FROM + S::W * 128 * 4;              // [2]: log2-domain score factor of a Q slot
   static constexpr int QTOP = CQ + 16;                                  // [16]
   static constexpr int SCH = QTOP + 64;
   static constexpr int TMEM = SCH + 64;
@@ -128,23 +127,25 @@ struct Smem {
   static constexpr int S_FULL = EMPTY + kMaxTiles * 8;
   static constexpr int S_EMPTY = S_FULL + 8 * 8;
   static constexpr int P_FULL = S_EMPTY + 8 * 8;
-  static constexpr int P_DONE = P_FULL + kStreams * 8;
-  static constexpr int Q_READY = P_DONE + kStreams * 8;
+  static constexpr int P_DONE = P_FULL + 2 * S::W * 8;
+  static constexpr int Q_READY = P_DONE + 2 * S::W * 8;
   static constexpr int M_FULL = Q_READY + 2 * 8;
   static constexpr int M_EMPTY = M_FULL + kMetaSlots * 8;
   static constexpr int DONE = M_EMPTY + kMetaSlots * 8;
   static constexpr int RING = (DONE + 8 + 1023) / 1024 * 1024;
-  static_assert(sizeof(Schedule) <= 64 && META % 1024 == 0 && FULL % 8 == 0, "layout");
+  static_assert((!S::ATTEND || S::W * S::ROWS <= 64) && sizeof(Schedule) <= 64 && META % 1024 == 0 && FULL % 8 == 0, "layout");
 
   uint8_t* at;  // 1024-byte aligned, in shared memory
 
   __device__ __forceinline__ uint8_t* ring(int tile) const { return at + RING + tile * kTileBytes; }
-  __device__ __forceinline__ uint8_t* p(int stream) const { return at + P + stream * kPBytes; }
+  // the buffer of a stream's v-th unit, and the index of its barriers
+  __device__ __forceinline__ static int pi(int stream, int v) { return 2 * stream + (v & 1); }
+  __device__ __forceinline__ uint8_t* p(int stream, int v) const { return at + P + pi(stream, v) * S::PBYTES; }
   __device__ __forceinline__ uint8_t* q(int slot) const { return at + Q + slot * S::Q_BYTES; }
   __device__ __forceinline__ float4* meta(int slot) const { return reinterpret_cast<float4*>(at + META) + slot * kBlockPages; }
-  __device__ __forceinline__ float* base(int stream) const { return reinterpret_cast<float*>(at + BASE) + stream * 16; }
-  __device__ __forceinline__ float* delta(int stream) const { return reinterpret_cast<float*>(at + DELTA) + stream * 16; }
-  __device__ __forceinline__ float* wred(int warp) const { return reinterpret_cast<float*>(at + WRED) + warp * 16; }
+  __device__ __forceinline__ float* base(int stream) const { return reinterpret_cast<float*>(at + BASE) + stream * S::ROWS; }
+  __device__ __forceinline__ float* delta(int stream) const { return reinterpret_cast<float*>(at + DELTA) + stream * S::ROWS; }
+  __device__ __forceinline__ float* wred(int warp) const { return reinterpret_cast<float*>(at + WRED) + warp * S::ROWS; }
   __device__ __forceinline__ int* nan_from() const { return reinterpret_cast<int*>(at + NAN_FROM); }
   __device__ __forceinline__ float* cq() const { return reinterpret_cast<float*>(at + CQ); }
   __device__ __forceinline__ unsigned int* qtop() const { return reinterpret_cast<unsigned int*>(at + QTOP); }
@@ -398,22 +399,23 @@ __device__ void issue_scores(const ScaledTcParams& p, const Schedule& sch, const
   drain_products(p, sm);
 }
 
-// Descriptor of P, MN-major with 64-byte rows (one atom of 64 rows x 8 tokens, 512 B; 64-byte swizzle).
+// Descriptor of P, MN-major: one atom of PROW rows (bytes) x 8 tokens, swizzled over its row.
+template <class S>
 __device__ __forceinline__ uint64_t desc_p(uint32_t saddr) {
   uint64_t d = 0;
   d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-  d |= (uint64_t)((kPBytes >> 4) & 0x3FFFu) << 16;     // between atoms along the rows: there is one
-  d |= (uint64_t)((8 * kPRow >> 4) & 0x3FFFu) << 32;   // between groups of 8 tokens
-  d |= (uint64_t)1 << 46;                              // version
-  d |= (uint64_t)4 << 61;                              // SWIZZLE_64B
+  d |= (uint64_t)((S::PBYTES >> 4) & 0x3FFFu) << 16;     // between atoms along the rows: there is one
+  d |= (uint64_t)((8 * S::PROW >> 4) & 0x3FFFu) << 32;   // between groups of 8 tokens
+  d |= (uint64_t)1 << 46;                                // version
+  d |= (uint64_t)(S::PROW == 128 ? 2 : 4) << 61;         // SWIZZLE_128B or SWIZZLE_64B
   return d;
 }
 
-// O^T of stream u % 4 += V^T P^T of unit u, once P is in the stream's buffer.
+// O^T of stream u % W += V^T P^T of unit u, once P is in the stream's buffer.
 template <class S>
 __device__ void issue_values(const ScaledTcParams& p, const Schedule& sch, const Smem<S>& sm, uint32_t tmem, int tiles,
                              volatile int* abort) {
-  constexpr uint32_t kIdesc = mma_idesc_f16(128, kPRow, true, true, false);
+  constexpr uint32_t kIdesc = mma_idesc_f16(128, S::PROW, true, true, false);
   int u = 0;
   RingPos at;
   for_pieces(p.s, sch, [&](const SegWalk&, int, int n) {
@@ -424,19 +426,19 @@ __device__ void issue_values(const ScaledTcParams& p, const Schedule& sch, const
       wait_for(sm.bar(Smem<S>::FULL, at.slot), at.phase, abort, p.s.status);
 #pragma unroll 1
       for (int g = 0; g < S::G; ++g, ++u) {
-        const int st = u & (kStreams - 1);
-        wait_for(sm.bar(Smem<S>::P_FULL, st), (uint32_t)(u / kStreams) & 1u, abort, p.s.status);
+        const int st = u % S::W, v = u / S::W;
+        wait_for(sm.bar(Smem<S>::P_FULL, sm.pi(st, v)), (uint32_t)(v >> 1) & 1u, abort, p.s.status);
         __syncwarp();
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t v = smem_u32(sm.ring(at.slot));
-          const uint32_t pb = smem_u32(sm.p(st));
+          const uint32_t vt = smem_u32(sm.ring(at.slot));
+          const uint32_t pb = smem_u32(sm.p(st, v));
           const int steps = (np + 1) / 2;  // 32 tokens a step; the softmax zeroed an absent page's V
           // a stream's first product of a piece overwrites O
           for (int kk = 0; kk < steps; ++kk)
-            tc_mma_ss_f8(tmem + st * kPRow, smem_desc_sw128(v + kk * 4096, kTileBytes, 1024), desc_p(pb + kk * 32 * kPRow),
-                         kIdesc, (k >= kStreams / S::G || kk > 0) ? 1u : 0u);
-          tc_commit(sm.bar(Smem<S>::P_DONE, st));
+            tc_mma_ss_f8(tmem + st * S::PROW, smem_desc_sw128(vt + kk * 4096, kTileBytes, 1024), desc_p<S>(pb + kk * 32 * S::PROW),
+                         kIdesc, (k >= S::W / S::G || kk > 0) ? 1u : 0u);
+          tc_commit(sm.bar(Smem<S>::P_DONE, sm.pi(st, v)));
           if (g == S::G - 1) tc_commit(sm.bar(Smem<S>::EMPTY, at.slot));
         }
         __syncwarp();
@@ -476,7 +478,10 @@ __device__ __forceinline__ bool group_any(int stream, bool v) {
   return r != 0;
 }
 __device__ __forceinline__ void group_sync(int stream) { named_bar_sync(1 + stream, 128); }
-__device__ __forceinline__ void softmax_sync() { named_bar_sync(1 + kStreams, kSoftmaxThreads); }
+template <class S>
+__device__ __forceinline__ void softmax_sync() {
+  named_bar_sync(1 + S::W, S::SOFTMAX);
+}
 
 // The three e4m3 parts of two probabilities below 2^8.  Differences of a number and its rounding
 // are exact; the first one is taken in fp32 and rounded to fp16 (2^-16 of P).
@@ -508,61 +513,74 @@ __device__ __forceinline__ void split_q(float (&x)[4], uint32_t (&out)[3]) {
 
 // Q of (b, h) as the N operand of the score product: row r of part i is operand row i * ROWS + r of its
 // group (128 B, 128-byte swizzle).  All softmax threads, eight to a row, 16 dims each.
+template <class S>
 struct QItem {
-  uint4 x[2];
-  uint32_t top;  // the row's largest magnitude, as bits (above every finite one for infinity and NaN)
+  uint4 x[S::Q_STEPS][2];
+  uint32_t top[S::Q_STEPS];  // the row's largest magnitude, as bits (above every finite one for infinity and NaN)
 };
 
 // The thread's part of Q into registers, and the warp's largest finite magnitude into qtop.
 template <class S, bool BF>
-__device__ __forceinline__ QItem load_q(const ScaledTcParams& p, const Smem<S>& sm, int b, int h) {
-  const int r = threadIdx.x >> 3, c = threadIdx.x & 7;
-  QItem q;
-  q.x[0] = q.x[1] = make_uint4(0u, 0u, 0u, 0u);
-  q.top = 0;
-  if (r < kGroup * p.s.q_len) {
-    const __half* src = p.s.q + ((size_t)(b * p.s.q_len + (r >> 2)) * p.s.hq + h * kGroup + (r & 3)) * kHeadDim + c * 16;
-    q.x[0] = __ldg(reinterpret_cast<const uint4*>(src));
-    q.x[1] = __ldg(reinterpret_cast<const uint4*>(src) + 1);
+__device__ __forceinline__ void load_q(const ScaledTcParams& p, const Smem<S>& sm, int b, int h, QItem<S>& q) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int st = 0; st < S::Q_STEPS; ++st) {
+    const int it = st * S::SOFTMAX + threadIdx.x, r = it >> 3, c = it & 7;
+    q.x[st][0] = q.x[st][1] = make_uint4(0u, 0u, 0u, 0u);
+    if (r < kGroup * p.s.q_len) {
+      const __half* src =
+          p.s.q + ((size_t)(b * p.s.q_len + (r >> 2)) * p.s.hq + h * kGroup + (r & 3)) * kHeadDim + c * 16;
+      q.x[st][0] = __ldg(reinterpret_cast<const uint4*>(src));
+      q.x[st][1] = __ldg(reinterpret_cast<const uint4*>(src) + 1);
+    }
   }
   if constexpr (S::F8) {
-    const uint32_t w[8] = {q.x[0].x, q.x[0].y, q.x[0].z, q.x[0].w, q.x[1].x, q.x[1].y, q.x[1].z, q.x[1].w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 a = unpack2<BF>(w[i]);
-      q.top = max(q.top, max(__float_as_uint(a.x) & 0x7fffffffu, __float_as_uint(a.y) & 0x7fffffffu));
+    for (int st = 0; st < S::Q_STEPS; ++st) {
+      const uint32_t w[8] = {q.x[st][0].x, q.x[st][0].y, q.x[st][0].z, q.x[st][0].w,
+                             q.x[st][1].x, q.x[st][1].y, q.x[st][1].z, q.x[st][1].w};
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 a = unpack2<BF>(w[i]);
+        top = max(top, max(__float_as_uint(a.x) & 0x7fffffffu, __float_as_uint(a.y) & 0x7fffffffu));
+      }
+#pragma unroll
+      for (int off = 1; off < 8; off <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+      q.top[st] = top;
+      if (top < 0x7f800000u) most = max(most, top);
     }
-#pragma unroll
-    for (int off = 1; off < 8; off <<= 1) q.top = max(q.top, __shfl_xor_sync(0xffffffffu, q.top, off));
-    const uint32_t most = __reduce_max_sync(0xffffffffu, q.top < 0x7f800000u ? q.top : 0u);
+    most = __reduce_max_sync(0xffffffffu, most);
     if ((threadIdx.x & 31) == 0) sm.qtop()[threadIdx.x >> 5] = most;
   }
-  return q;
 }
 
 // After a barrier of the softmax threads: the thread's part of Q into slot `qs`.
 template <class S, bool BF>
-__device__ __forceinline__ void write_q(const ScaledTcParams& p, const Smem<S>& sm, const QItem& q, int qs) {
-  const int r = threadIdx.x >> 3, c = threadIdx.x & 7;
+__device__ __forceinline__ void write_q(const ScaledTcParams& p, const Smem<S>& sm, const QItem<S>& q, int qs) {
   uint32_t most = 0;
   if constexpr (S::F8) {
 #pragma unroll
-    for (int i = 0; i < kSoftmaxThreads / 32; ++i) most = max(most, sm.qtop()[i]);
+    for (int i = 0; i < S::SOFTMAX / 32; ++i) most = max(most, sm.qtop()[i]);
   }
   // 2^e brings the largest magnitude into [128, 256)
   const int e = most > 0 ? max(-110, min(110, 134 - (int)(most >> 23))) : 0;
   if (threadIdx.x == 0) sm.cq()[qs] = p.s.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23);
-  if (r < S::G * S::ROWS) {
+#pragma unroll
+  for (int st = 0; st < S::Q_STEPS; ++st) {
+    const int it = st * S::SOFTMAX + threadIdx.x, r = it >> 3, c = it & 7;
+    if (r >= S::G * S::ROWS) break;
     const int rr = r % S::ROWS;
     uint8_t* const dst = sm.q(qs) + (r / S::ROWS) * S::Q_GROUP;
     if constexpr (!S::F8) {  // 32 bytes of half c / 4: chunks 2 (c % 4) and the next
       uint8_t* const row = dst + (c >> 2) * (S::N * 128) + (rr >> 3) * 1024 + (rr & 7) * 128;
       const int c0 = (c & 3) * 2;
-      *reinterpret_cast<uint4*>(row + ((c0 ^ (rr & 7)) << 4)) = q.x[0];
-      *reinterpret_cast<uint4*>(row + (((c0 + 1) ^ (rr & 7)) << 4)) = q.x[1];
+      *reinterpret_cast<uint4*>(row + ((c0 ^ (rr & 7)) << 4)) = q.x[st][0];
+      *reinterpret_cast<uint4*>(row + (((c0 + 1) ^ (rr & 7)) << 4)) = q.x[st][1];
     } else {
       const float sc = __uint_as_float((uint32_t)(127 + e) << 23);
-      const uint32_t w[8] = {q.x[0].x, q.x[0].y, q.x[0].z, q.x[0].w, q.x[1].x, q.x[1].y, q.x[1].z, q.x[1].w};
+      const uint32_t w[8] = {q.x[st][0].x, q.x[st][0].y, q.x[st][0].z, q.x[st][0].w,
+                             q.x[st][1].x, q.x[st][1].y, q.x[st][1].z, q.x[st][1].w};
       uint32_t part[3][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -572,7 +590,7 @@ __device__ __forceinline__ void write_q(const ScaledTcParams& p, const Smem<S>& 
         split_q<S::PARTS>(y, o);
 #pragma unroll
         for (int k = 0; k < S::PARTS; ++k)  // a row with an infinity or NaN is NaN
-          part[k][i] = q.top < 0x7f800000u ? o[k] : 0x7f7f7f7fu;
+          part[k][i] = q.top[st] < 0x7f800000u ? o[k] : 0x7f7f7f7fu;
       }
 #pragma unroll
       for (int k = 0; k < S::PARTS; ++k) {
@@ -684,8 +702,8 @@ __device__ __forceinline__ float4 read_meta(const ScaledTcParams& p, const Smem<
 template <class S, bool BF>
 __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<S>& sm, uint32_t tmem, int tiles,
                        volatile int* abort) {
-  constexpr int ROWS = S::ROWS, G = S::G;
-  constexpr int kStep = kStreams / G;  // blocks from unit to unit of a stream
+  constexpr int ROWS = S::ROWS, G = S::G, W = S::W;
+  constexpr int kStep = W / G;  // blocks from unit to unit of a stream
   const int stream = threadIdx.x >> 7;
   const int tid = threadIdx.x & 127, warp = tid >> 5, lane = tid & 31;  // tid: token of a block, dimension of O
   const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
@@ -702,11 +720,12 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
     const bool whole = unit == w.seg_start && seg_end <= sch.end;
     const Piece piece = piece_of(p.s, w);
     if (pc == 0) {
-      const QItem q = load_q<S, BF>(p, sm, w.b, w.h);
+      QItem<S> q;
+      load_q<S, BF>(p, sm, w.b, w.h, q);
       if (tid < ROWS) base[tid] = 0.f;
-      softmax_sync();
+      softmax_sync<S>();
       write_q<S, BF>(p, sm, q, 0);
-      softmax_sync();
+      softmax_sync<S>();
     }
     const float cq = sm.cq()[pc & 1];
     float l[ROWS];
@@ -721,7 +740,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
     for (int k = k0; k < nblk; k += kStep) {
       const int bk = blk + k;
       const int u = bk * G + group;
-      const int v = u / kStreams;  // the stream's own count
+      const int v = u / W;  // the stream's own count
       const int np = min(kBlockPages, n - k * kBlockPages);
       const int tok0 = (w.pg + k * kBlockPages) * kPageSize;
       const int tok = tok0 + tid;
@@ -766,10 +785,10 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
       const bool raise = group_any(stream, over > kRaise) || first;  // rare after a piece's first blocks
       if (raise) {
         const float m = reduce_rows<ROWS, true>(t);
-        if (lane % (32 / ROWS) == 0) wred[warp * 16 + lane / (32 / ROWS)] = m;
+        if (lane % (32 / ROWS) == 0) wred[warp * ROWS + lane / (32 / ROWS)] = m;
         group_sync(stream);
         if (tid < ROWS) {
-          const float m4 = fmaxf(fmaxf(wred[tid], wred[16 + tid]), fmaxf(wred[32 + tid], wred[48 + tid]));
+          const float m4 = fmaxf(fmaxf(wred[tid], wred[ROWS + tid]), fmaxf(wred[2 * ROWS + tid], wred[3 * ROWS + tid]));
           const float d = (m4 > kHead || (first && m4 != -INFINITY)) ? m4 - kHead : 0.f;
           delta[tid] = d;
           base[tid] += d;
@@ -778,9 +797,8 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) t[r] -= delta[r];
       }
-      // the stream's last product: P's buffer is free, and O stands still
-      if (v >= 1) wait_for(sm.bar(Smem<S>::P_DONE, stream), (uint32_t)(v - 1) & 1u, abort, p.s.status);
-      if (raise && !first) {
+      if (raise && !first) {  // O stands still once the stream's last product is done
+        wait_for(sm.bar(Smem<S>::P_DONE, sm.pi(stream, v - 1)), (uint32_t)((v - 1) >> 1) & 1u, abort, p.s.status);
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < ROWS; c += 8) {
@@ -793,60 +811,67 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
 #pragma unroll
           for (int i = 0; i < kPParts; ++i) {
             uint32_t o[8];
-            tmem_ld(lanes + stream * kPRow + i * ROWS + c, o);
+            tmem_ld(lanes + stream * S::PROW + i * ROWS + c, o);
             tmem_wait_ld();
 #pragma unroll
             for (int r = 0; r < 8; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * a[r]);
-            tmem_st8(lanes + stream * kPRow + i * ROWS + c, o);
+            tmem_st8(lanes + stream * S::PROW + i * ROWS + c, o);
           }
         }
         tmem_wait_st();
       }
-      // P: token tid's operand row of 64 bytes, part i of row r in byte i * ROWS + r; 16-byte chunks
-      // swizzled by token / 2
-      uint8_t* const prow = sm.p(stream) + tid * kPRow;
-      uint32_t part[kPParts][ROWS / 4];
+      // P: token tid's operand row of PROW bytes, part i of row r in byte i * ROWS + r; 16-byte chunks
+      // swizzled by the token
+      // (its buffer is free once the product before the last is done)
+      if (v >= 2) wait_for(sm.bar(Smem<S>::P_DONE, sm.pi(stream, v)), (uint32_t)((v >> 1) - 1) & 1u, abort, p.s.status);
+      uint8_t* const prow = sm.p(stream, v) + tid * S::PROW;
+      const int swizzle = S::PROW == 128 ? tid & 7 : (tid >> 1) & 3;
+      constexpr int kHalf = ROWS < 16 ? ROWS : 16;  // rows of a 16-byte chunk
 #pragma unroll
-      for (int r = 0; r < ROWS; r += 4) {
-        float x[4];
+      for (int c = 0; c < ROWS; c += kHalf) {
+        uint32_t part[kPParts][kHalf / 4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] = ex2(t[r + i]);
-          l[r + i] = fmaf(x[i], inv_vs, l[r + i]);
+        for (int r = 0; r < kHalf; r += 4) {
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[i] = ex2(t[c + r + i]);
+            l[c + r + i] = fmaf(x[i], inv_vs, l[c + r + i]);
+          }
+          uint32_t lo[kPParts], hi[kPParts];
+          split_p(x[0], x[1], lo);
+          split_p(x[2], x[3], hi);
+#pragma unroll
+          for (int i = 0; i < kPParts; ++i) part[i][r / 4] = lo[i] | (hi[i] << 16);
         }
-        uint32_t lo[kPParts], hi[kPParts];
-        split_p(x[0], x[1], lo);
-        split_p(x[2], x[3], hi);
 #pragma unroll
-        for (int i = 0; i < kPParts; ++i) part[i][r / 4] = lo[i] | (hi[i] << 16);
-      }
-#pragma unroll
-      for (int i = 0; i < kPParts; ++i) {
-        const int byte = i * ROWS;
-        uint8_t* const at = prow + (((byte >> 4) ^ ((tid >> 1) & 3)) << 4) + (byte & 15);
-        if constexpr (ROWS == 16)
-          *reinterpret_cast<uint4*>(at) = make_uint4(part[i][0], part[i][1], part[i][2], part[i][3]);
-        else
-          *reinterpret_cast<uint2*>(at) = make_uint2(part[i][0], part[i][1]);
+        for (int i = 0; i < kPParts; ++i) {
+          const int byte = i * ROWS + c;
+          uint8_t* const at = prow + (((byte >> 4) ^ swizzle) << 4) + (byte & 15);
+          if constexpr (kHalf == 16)
+            *reinterpret_cast<uint4*>(at) = make_uint4(part[i][0], part[i][1], part[i][2], part[i][3]);
+          else
+            *reinterpret_cast<uint2*>(at) = make_uint2(part[i][0], part[i][1]);
+        }
       }
       fence_proxy_async_smem();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(sm.bar(Smem<S>::P_FULL, stream));
+      if (lane == 0) mbar_arrive(sm.bar(Smem<S>::P_FULL, sm.pi(stream, v)));
     }
 
     // ---- epilogue: denominators and factors, then each dimension's thread joins its rows' parts
     const bool more = seg_end < sch.end;  // another piece follows: its Q, for the score products
-    QItem q;
+    QItem<S> q;
     if (more) {
       SegWalk nw = w;
       next_segment(p.s, nw);
-      q = load_q<S, BF>(p, sm, nw.b, nw.h);
+      load_q<S, BF>(p, sm, nw.b, nw.h, q);
     }
     const float total = reduce_rows<ROWS, false>(l);
-    if (lane % (32 / ROWS) == 0) wred[warp * 16 + lane / (32 / ROWS)] = total;
+    if (lane % (32 / ROWS) == 0) wred[warp * ROWS + lane / (32 / ROWS)] = total;
     sm.nan_from()[threadIdx.x] = nan_from;
-    softmax_sync();
+    softmax_sync<S>();
     if (more) write_q<S, BF>(p, sm, q, (pc + 1) & 1);
     const int slot = (int)blockIdx.x + seg;  // workspace piece
     if (threadIdx.x < rows) {
@@ -856,7 +881,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
       for (int i = 0; i < kStep; ++i) {
         const int st = i * G + g;
         const float* x = sm.wred(st * 4) + r;
-        sum[i] = (x[0] + x[16]) + (x[32] + x[48]);
+        sum[i] = (x[0] + x[ROWS]) + (x[2 * ROWS] + x[3 * ROWS]);
         if (sum[i] != 0.f) top = fmaxf(top, sm.base(st)[r]);
       }
       float wgt[kStep];
@@ -874,17 +899,18 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
       else if (p.s.out_lse) p.s.out_lse[out_row] = lse;
     }
 #pragma unroll
-    for (int st = 0; st < kStreams; ++st) {  // each stream's last product (it may have none in this piece)
-      const int last = ((blk + nblk) * G - 1 - st) / kStreams * kStreams + st;  // the last unit of the stream so far
+    for (int st = 0; st < W; ++st) {  // each stream's last product (it may have none in this piece)
+      const int last = ((blk + nblk) * G - 1 - st) / W * W + st;  // the last unit of the stream so far
       if (last >= blk * G && last < (blk + nblk) * G)
-        wait_for(sm.bar(Smem<S>::P_DONE, st), (uint32_t)(last / kStreams) & 1u, abort, p.s.status);
+        wait_for(sm.bar(Smem<S>::P_DONE, sm.pi(st, last / W)), (uint32_t)(last / W >> 1) & 1u, abort, p.s.status);
     }
     tc_fence_after();
-    softmax_sync();
+    softmax_sync<S>();
     if (tid < ROWS) base[tid] = 0.f;  // for the next piece
-    nan_from = min(min(sm.nan_from()[tid], sm.nan_from()[128 + tid]), min(sm.nan_from()[256 + tid], sm.nan_from()[384 + tid]));
+#pragma unroll
+    for (int st = 0; st < W; ++st) nan_from = min(nan_from, sm.nan_from()[st * 128 + tid]);
     // this warpgroup's share of the rows: G * ROWS / 4 from row `stream` * that on
-    constexpr int kShare = G * ROWS / kStreams, kChunk = kShare < 4 ? kShare : 4;
+    constexpr int kShare = G * ROWS / W, kChunk = kShare < 4 ? kShare : 4;
 #pragma unroll 1
     for (int c = stream * kShare; c < (stream + 1) * kShare; c += kChunk) {
       if (c >= rows) break;
@@ -896,7 +922,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
 #pragma unroll
       for (int i = 0; i < kStep; ++i)
 #pragma unroll
-        for (int j = 0; j < kPParts; ++j) tmem_ld(lanes + (i * G + g) * kPRow + j * ROWS + r0, raw[i][j]);
+        for (int j = 0; j < kPParts; ++j) tmem_ld(lanes + (i * G + g) * S::PROW + j * ROWS + r0, raw[i][j]);
       tmem_wait_ld();
 #pragma unroll
       for (int i = 0; i < kStep; ++i) {
@@ -923,7 +949,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
       }
     }
     tc_fence_before();  // O is read before the next piece's first product overwrites it
-    softmax_sync();     // and so is all that the streams share
+    softmax_sync<S>();     // and so is all that the streams share
     blk += nblk;
     ++pc;
   });
@@ -971,15 +997,16 @@ __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const Smem<S
     const Piece piece = piece_of(p.s, w);
     const int fresh = __ldg(p.s.seq_lens + w.b) - p.s.q_len;  // tokens from here on are new
     if (pc == 0) {
-      const QItem q = load_q<S, BF>(p, sm, w.b, w.h);
+      QItem<S> q;
+      load_q<S, BF>(p, sm, w.b, w.h, q);
       if (threadIdx.x < G * S::ROWS) sm.base(0)[threadIdx.x] = row_lse(w.b, w.h);
-      softmax_sync();
+      softmax_sync<S>();
       write_q<S, BF>(p, sm, q, 0);
-      softmax_sync();
+      softmax_sync<S>();
     }
     const float cq = sm.cq()[pc & 1];
     const int nblk = blocks_of(n);
-    for (int k = (stream - blk) & (kStreams - 1); k < nblk; k += kStreams) {
+    for (int k = (stream - blk) & (S::W - 1); k < nblk; k += S::W) {
       const int bk = blk + k;
       const int np = min(kBlockPages, n - k * kBlockPages);
       const int tok0 = (w.pg + k * kBlockPages) * kPageSize;
@@ -1010,12 +1037,13 @@ __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const Smem<S
     if (seg_end < sch.end) {  // the next piece's Q and rows
       SegWalk nw = w;
       next_segment(p.s, nw);
-      const QItem q = load_q<S, BF>(p, sm, nw.b, nw.h);
+      QItem<S> q;
+      load_q<S, BF>(p, sm, nw.b, nw.h, q);
       const float x = threadIdx.x < G * S::ROWS ? row_lse(nw.b, nw.h) : 0.f;
-      softmax_sync();
+      softmax_sync<S>();
       write_q<S, BF>(p, sm, q, (pc + 1) & 1);
       if (threadIdx.x < G * S::ROWS) sm.base(0)[threadIdx.x] = x;
-      softmax_sync();
+      softmax_sync<S>();
     }
     blk += nblk;
     ++pc;
@@ -1023,7 +1051,7 @@ __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const Smem<S
 }
 
 template <class S, bool BF>
-__global__ void __launch_bounds__(kScaledTcThreads, 1)
+__global__ void __launch_bounds__(S::THREADS, 1)
     sqa_scaled_tc_kernel(const ScaledTcParams p, const __grid_constant__ CUtensorMap tm_k,
                          const __grid_constant__ CUtensorMap tm_v) {
   extern __shared__ uint8_t smem_raw[];
@@ -1031,7 +1059,7 @@ __global__ void __launch_bounds__(kScaledTcThreads, 1)
   const Smem<S> sm{smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u)};
   const int tiles = p.s.num_stages;
   const int warp = threadIdx.x >> 5;
-  constexpr int kScoreWarp = kSoftmaxThreads / 32, kValueWarp = kScoreWarp + 1, kProducerWarp = kScoreWarp + 2,
+  constexpr int kScoreWarp = S::SOFTMAX / 32, kValueWarp = kScoreWarp + 1, kProducerWarp = kScoreWarp + 2,
                 kMetaWarp = kScoreWarp + 3;
   if (threadIdx.x == 0) {
     for (int i = 0; i < tiles; ++i) {
@@ -1042,11 +1070,13 @@ __global__ void __launch_bounds__(kScaledTcThreads, 1)
       mbar_init(sm.bar(Smem<S>::S_FULL, i), 1);
       mbar_init(sm.bar(Smem<S>::S_EMPTY, i), 4);
     }
-    for (int i = 0; i < kStreams; ++i) {
-      mbar_init(sm.bar(Smem<S>::P_FULL, i), 4);
-      mbar_init(sm.bar(Smem<S>::P_DONE, i), 1);
+    for (int i = 0; i < S::W; ++i) {
+      for (int j = 0; j < 2; ++j) {
+        mbar_init(sm.bar(Smem<S>::P_FULL, 2 * i + j), 4);
+        mbar_init(sm.bar(Smem<S>::P_DONE, 2 * i + j), 1);
+      }
     }
-    for (int i = 0; i < 2; ++i) mbar_init(sm.bar(Smem<S>::Q_READY, i), kSoftmaxThreads / 32);
+    for (int i = 0; i < 2; ++i) mbar_init(sm.bar(Smem<S>::Q_READY, i), S::SOFTMAX / 32);
     for (int i = 0; i < kMetaSlots; ++i) {
       mbar_init(sm.bar(Smem<S>::M_FULL, i), 1);
       mbar_init(sm.bar(Smem<S>::M_EMPTY, i), S::ATTEND ? 4 * S::G : 4);  // the warps that read a block's scales
@@ -1159,7 +1189,7 @@ cudaError_t launch_shape(ScaledTcParams& p, const CUtensorMap& tm_k, const CUten
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(kScaledTcThreads);
+  cfg.blockDim = dim3(S::THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -1175,14 +1205,16 @@ template <int PARTS, bool ATTEND, bool BF>
 cudaError_t launch_rows(ScaledTcParams& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, int grid,
                         cudaStream_t stream) {
   const int rows = kGroup * p.s.q_len;
-  if (rows <= 8) return launch_shape<Shape<PARTS, 8, 1, ATTEND>, BF>(p, tm_k, tm_v, grid, stream);
-  if (rows <= 16) return launch_shape<Shape<PARTS, 16, 1, ATTEND>, BF>(p, tm_k, tm_v, grid, stream);
   if constexpr (ATTEND) {
-    if (rows <= 32) return launch_shape<Shape<PARTS, 16, 2, true>, BF>(p, tm_k, tm_v, grid, stream);
-    return launch_shape<Shape<PARTS, 16, 4, true>, BF>(p, tm_k, tm_v, grid, stream);
+    if (rows <= 8) return launch_shape<Shape<PARTS, 8, 1, 2, true>, BF>(p, tm_k, tm_v, grid, stream);
+    if (rows <= 16) return launch_shape<Shape<PARTS, 16, 1, 2, true>, BF>(p, tm_k, tm_v, grid, stream);
+    if (rows <= 32) return launch_shape<Shape<PARTS, 16, 2, 2, true>, BF>(p, tm_k, tm_v, grid, stream);
+    return launch_shape<Shape<PARTS, 16, 4, 4, true>, BF>(p, tm_k, tm_v, grid, stream);
   } else {  // wider units: no P, no O, and K read less often
-    if (rows <= 32) return launch_shape<Shape<PARTS, 32, 1, false>, BF>(p, tm_k, tm_v, grid, stream);
-    return launch_shape<Shape<PARTS, 32, 2, false>, BF>(p, tm_k, tm_v, grid, stream);
+    if (rows <= 8) return launch_shape<Shape<PARTS, 8, 1, 4, false>, BF>(p, tm_k, tm_v, grid, stream);
+    if (rows <= 16) return launch_shape<Shape<PARTS, 16, 1, 4, false>, BF>(p, tm_k, tm_v, grid, stream);
+    if (rows <= 32) return launch_shape<Shape<PARTS, 32, 1, 4, false>, BF>(p, tm_k, tm_v, grid, stream);
+    return launch_shape<Shape<PARTS, 32, 2, 4, false>, BF>(p, tm_k, tm_v, grid, stream);
   }
 }
 

@@ -44,10 +44,17 @@ constexpr long long kFp8LongRangeUnits = 400;
 #ifndef SQA_SEGMENT_COST_MMA
 #define SQA_SEGMENT_COST_MMA 4
 #endif
-// Block-scaled kernels: a CTA takes at least one 8-page block, and a segment start costs it
-// as much as this many pages.
-constexpr int kScaledMinPagesPerCta = 8;
+// Block-scaled kernels.  A CTA of the attention takes at least 16 pages (two blocks), of the weights
+// 8 (q_len 4 x 4000 tokens x 1: 15.4 us with 16, 18.3 with 8, 16.5 with 32), and a
+// segment start costs it as much as 24 pages (48 ragged sequences of up to 8190: 115 us; 119 with 12,
+// 114 with 40, which costs q_len 2 as much).
+constexpr int kScaledMinPages = 16, kWeightsMinPages = 8;
 constexpr int kScaledSegmentCost = 24;
+// Attention over segments of at most 64 pages (128 for q_len <= 8 with segments for a quarter of the
+// SMs) takes one CTA a segment: nothing is left to merge.  Measured against the split at q_len 4: 600
+// tokens x 1 9.8 against 13.1 us, 1000 x 1 12.3 / 14.8, 2000 x 1 18.5 / 16.1, 600 x 8 10.3 / 16.9,
+// 2000 x 8 19.8 / 23.5, 4000 x 8 33.1 / 28.2.
+constexpr int kWholePages = 64, kWholePagesMany = 128;
 constexpr int kSegmentCostTc = SQA_SEGMENT_COST_TC;
 constexpr int kSegmentCostMma = SQA_SEGMENT_COST_MMA;
 
@@ -555,9 +562,10 @@ struct ScaledPlan {
   size_t off_lse, off_o, bytes;
 };
 
-// One CTA per SM (it holds all of tensor memory), fewer for short work; with near-uniform length
-// hints and few segments, every segment is split evenly (as in make_plan).
-int make_scaled_plan(const sqa_args* a, int device, ScaledPlan* plan) {
+// One CTA per SM (it holds all of tensor memory), fewer for short work.  Short segments of the attention
+// take one CTA each; with near-uniform length hints and few segments, every segment is split evenly
+// (as in make_plan); the weights, which have nothing to merge, split evenly whenever the CTAs suffice.
+int make_scaled_plan(const sqa_args* a, int device, bool weights, ScaledPlan* plan) {
   const int sms = sm_count(device);
   if (sms <= 0) return SQA_ERR_CUDA;
   ScaledPlan pl = {};
@@ -565,16 +573,21 @@ int make_scaled_plan(const sqa_args* a, int device, ScaledPlan* plan) {
   long long pages = a->max_pages;
   if (a->max_seq_len > 0) pages = std::min<long long>(pages, ((long long)a->max_seq_len + kPageSize - 1) / kPageSize);
   long long grid = a->num_ctas > 0 ? a->num_ctas : sms;
-  if (a->num_ctas <= 0) {
-    const int min_pages = a->min_pages_per_cta > 0 ? a->min_pages_per_cta : kScaledMinPagesPerCta;
+  if (a->num_ctas <= 0 && segments > 0) {
+    const int min_pages = a->min_pages_per_cta > 0 ? a->min_pages_per_cta : weights ? kWeightsMinPages : kScaledMinPages;
     grid = std::max(1LL, std::min(grid, (segments * pages + min_pages - 1) / min_pages));
-    if (a->cluster != 1 && a->max_seq_len > 0 && a->min_seq_len > 0 && 100LL * a->min_seq_len >= 85LL * a->max_seq_len) {
-      const long long k = segments > 0 ? grid / segments : 0;
-      if (k >= 2 && 10 * segments * k >= 9 * grid && pages >= 16 * k) {
-        pl.seg_split = (int)k;
-        grid = segments * k;
-      }
+    const bool many = a->q_len <= 8 && 4 * segments >= sms;
+    const long long even = (pages + min_pages - 1) / min_pages;  // CTAs a segment, each with its least
+    if (weights && segments * even <= sms) {
+      pl.seg_split = (int)even;
+    } else if (!weights && pages <= (many ? kWholePagesMany : kWholePages)) {
+      pl.seg_split = 1;
+    } else if (a->cluster != 1 && a->max_seq_len > 0 && a->min_seq_len > 0 &&
+               100LL * a->min_seq_len >= 85LL * a->max_seq_len) {
+      const long long k = grid / segments;
+      if (k >= 2 && 10 * segments * k >= 9 * grid && pages >= 16 * k) pl.seg_split = (int)k;
     }
+    if (pl.seg_split) grid = segments * pl.seg_split;
   }
   pl.grid = (int)grid;
   pl.rows_pad = warp_shape_for(a->q_len).rows_pad;
@@ -626,7 +639,7 @@ size_t sqa_scaled_workspace_bytes(const sqa_args* a, int device, int* status) {
   ScaledPlan pl = {};
   if (st == SQA_OK) {
     const int dev = current_device(device);
-    st = dev < 0 ? SQA_ERR_CUDA : make_scaled_plan(a, dev, &pl);
+    st = dev < 0 ? SQA_ERR_CUDA : make_scaled_plan(a, dev, false, &pl);
   }
   if (status) *status = st;
   return st == SQA_OK ? pl.bytes : 0;
@@ -654,7 +667,7 @@ int sqa_forward_scaled(const sqa_args* a, const sqa_scales* scales, void* worksp
   const int dev = current_device(-1);
   if (dev < 0) return SQA_ERR_CUDA;
   ScaledPlan pl;
-  st = make_scaled_plan(a, dev, &pl);
+  st = make_scaled_plan(a, dev, false, &pl);
   if (st != SQA_OK) return st;
   if (workspace_bytes < pl.bytes) return SQA_ERR_WORKSPACE_TOO_SMALL;
   CUtensorMap tm_k, tm_v;
@@ -694,7 +707,7 @@ int sqa_accumulate_weights(const sqa_args* a, const float* lse, const sqa_scales
   const int dev = current_device(-1);
   if (dev < 0) return SQA_ERR_CUDA;
   ScaledPlan pl;
-  st = make_scaled_plan(a, dev, &pl);
+  st = make_scaled_plan(a, dev, true, &pl);
   if (st != SQA_OK) return st;
   CUtensorMap tm_k;
   if (!encode_cache_map(&tm_k, a->key_cache, a->num_pages, a->num_kv_heads, a->kv_layout == SQA_KV_HND,

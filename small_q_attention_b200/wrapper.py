@@ -9,6 +9,10 @@ and no shape-dependent host work beyond filling one argument struct, so that
 ``run`` can be captured in a CUDA graph and replayed.  ``run`` can also append
 the step's new K/V to the cache first (``cache_append``), on the same stream.
 
+A plan with ``block_scaled=True`` takes FP8-E4M3 caches with a scale per page and KV head
+(``cache_append_scaled``, ``small_q_attention_scaled``); ``run(scores=...)`` also adds the step's
+attention weights to the cached tokens' scores, which ``evict`` cuts the cache by.
+
 The operator contract is that of ``small_q_attention`` (the upstream
 ``forward_v3``, ``src/small_q_attention/cuda.py:177-214``); this wrapper adds no
 arithmetic of its own.
@@ -24,6 +28,8 @@ from . import _native
 from .attention import (GQA_GROUP, HEAD_DIM, MAX_Q_LEN, PAGE_SIZE, _check_inputs, _fill_args, _layout_code,
                         _on_device, _raise_device_bits, _stream_handle, read_device_status)
 from .cache import cache_append
+from .eviction import accumulate_attention_weights, cache_evict
+from .scaled import cache_append_scaled, small_q_attention_scaled
 
 
 class PagedMTPAttention:
@@ -56,7 +62,7 @@ class PagedMTPAttention:
              num_ctas: int = 0, min_pages_per_cta: int = 0, kv_layout: str = "NHD",
              sm_scale: float | None = None, out_scale: float = 1.0,
              cache_dtype: torch.dtype | None = None, min_seq_len: int = 0,
-             cluster: int = 0) -> "PagedMTPAttention":
+             cluster: int = 0, block_scaled: bool = False) -> "PagedMTPAttention":
         """Fix the shapes of the following ``run`` calls and size the workspace.
 
         ``max_seq_len`` bounds ``seq_lens`` for the launch size (0: the page-table
@@ -67,7 +73,8 @@ class PagedMTPAttention:
         of few sequences run the tcgen05 kernel in thread-block clusters or with
         every segment split evenly over several CTAs (``selected_kernel`` reports
         ``2 + 100 * C`` or ``2 + 10000 * k``); a run whose lengths fall outside the
-        bounds still gives the right result.
+        bounds still gives the right result.  ``block_scaled`` plans for FP8-E4M3 caches with a
+        scale per page and KV head (``run(key_scales=..., value_scales=...)``).
         """
         if not (1 <= q_len <= MAX_Q_LEN):
             raise ValueError(f"q_len must be in [1, {MAX_Q_LEN}]")
@@ -83,21 +90,30 @@ class PagedMTPAttention:
         a.max_seq_len, a.num_ctas, a.min_pages_per_cta, a.kernel = max_seq_len, num_ctas, min_pages_per_cta, self._kernel
         a.kv_layout = _layout_code(kv_layout)
         a.min_seq_len, a.cluster = min_seq_len, cluster
-        if cache_dtype is not None and cache_dtype == getattr(torch, "float8_e4m3fn", None):
+        if block_scaled or (cache_dtype is not None and cache_dtype == getattr(torch, "float8_e4m3fn", None)):
             a.kv_dtype = _native.KV_FP8_E4M3  # fp8 caches run on the tcgen05 kernel
         lib = _native.library()
         st = ctypes.c_int(0)
-        need = int(lib.sqa_workspace_bytes(ctypes.byref(a), self.device.index, ctypes.byref(st)))
-        _native.check(st.value, "sqa_workspace_bytes")
-        picked = lib.sqa_selected_kernel(ctypes.byref(a), self.device.index)
-        if picked < 0:
-            _native.check(-picked, "sqa_selected_kernel")
+        if block_scaled:
+            if cluster not in (0, 1) or min_pages_per_cta or self._kernel == 1:
+                raise ValueError("block-scaled caches have one kernel: no kernel=1, cluster sizes or min_pages_per_cta")
+            a.kernel = 0
+            need = int(lib.sqa_scaled_workspace_bytes(ctypes.byref(a), self.device.index, ctypes.byref(st)))
+            _native.check(st.value, "sqa_scaled_workspace_bytes")
+            picked = 2
+        else:
+            need = int(lib.sqa_workspace_bytes(ctypes.byref(a), self.device.index, ctypes.byref(st)))
+            _native.check(st.value, "sqa_workspace_bytes")
+            picked = lib.sqa_selected_kernel(ctypes.byref(a), self.device.index)
+            if picked < 0:
+                _native.check(-picked, "sqa_selected_kernel")
         if self._workspace is None or self._workspace.numel() < need:
             self._workspace = torch.zeros(max(need, 1 << 16), dtype=torch.uint8, device=self.device)
         self._shape = (batch, q_len, num_kv_heads, num_pages, max_pages)
         self._max_seq_len, self._num_ctas, self._min_pages = max_seq_len, num_ctas, min_pages_per_cta
         self._kv_layout, self._sm_scale, self._out_scale = kv_layout, sm_scale, out_scale
-        self._min_seq_len, self._cluster = min_seq_len, cluster
+        self._min_seq_len, self._cluster, self._scaled = min_seq_len, cluster, block_scaled
+        self._lse = self._rows = None
         self.selected_kernel = int(picked)
         return self
 
@@ -109,10 +125,12 @@ class PagedMTPAttention:
 
     # ------------------------------------------------------------------ run
     def run(self, query, key_cache, value_cache, block_tables, seq_lens, *, out=None,
-            append_keys=None, append_values=None, check: bool = False):
+            append_keys=None, append_values=None, check: bool = False, key_scales=None, value_scales=None,
+            scores=None):
         """One step: optionally append ``append_keys/values`` ``[batch, q_len, Hkv, 128]``
         to the cache, then attend.  Returns ``out`` (allocated when not given; give
-        it when capturing a CUDA graph)."""
+        it when capturing a CUDA graph).  With ``scores`` ``[num_pages, Hkv, 16]`` the step's
+        attention weights are added to them (``accumulate_attention_weights``)."""
         if self._shape is None:
             raise RuntimeError("plan() has not been called")
         _check_inputs(query, key_cache, value_cache, block_tables, seq_lens, PAGE_SIZE, kv_layout=self._kv_layout)
@@ -130,6 +148,23 @@ class PagedMTPAttention:
             raise ValueError("out must be a contiguous tensor shaped and typed like query")
         if (append_keys is None) != (append_values is None):
             raise ValueError("append_keys and append_values go together")
+        if self._scaled != (key_scales is not None) or self._scaled != (value_scales is not None):
+            raise ValueError("key_scales and value_scales go with plan(block_scaled=True), and with no other plan")
+        if scores is not None and self._lse is None:  # kept from run to run; call once before a capture
+            self._lse = torch.empty(query.shape[:3], dtype=torch.float32, device=self.device)
+            self._rows = None if self._scaled else torch.empty(query.shape, dtype=torch.float32, device=self.device)
+        if self._scaled:
+            if append_keys is not None:
+                cache_append_scaled(append_keys, append_values, key_cache, value_cache, key_scales, value_scales,
+                                    block_tables, seq_lens, kv_layout=self._kv_layout)
+            small_q_attention_scaled(query, key_cache, value_cache, key_scales, value_scales, block_tables, seq_lens,
+                                     PAGE_SIZE, self._max_seq_len, out=out,
+                                     out_lse=self._lse if scores is not None else None, workspace=self._workspace,
+                                     num_ctas=self._num_ctas, check=check, kv_layout=self._kv_layout,
+                                     sm_scale=self._sm_scale, out_scale=self._out_scale, min_seq_len=self._min_seq_len)
+            if scores is not None:
+                self._accumulate(query, key_cache, block_tables, seq_lens, scores, key_scales)
+            return out
         if append_keys is not None:
             cache_append(append_keys, append_values, key_cache, value_cache, block_tables, seq_lens,
                          kv_layout=self._kv_layout)
@@ -137,7 +172,10 @@ class PagedMTPAttention:
                        self._num_ctas, self._min_pages, self._kernel, self._kv_layout, self._sm_scale,
                        self._out_scale)
         a.min_seq_len, a.cluster = self._min_seq_len, self._cluster
-        a.out = out.data_ptr()
+        if scores is None:
+            a.out = out.data_ptr()
+        else:  # the partial form writes the log-sum-exp too; its fp32 rows are rounded once, below
+            a.out_partial, a.out_lse = self._rows.data_ptr(), self._lse.data_ptr()
         ws = self._workspace
         with _on_device(self.device):
             code = _native.library().sqa_forward(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()),
@@ -146,4 +184,25 @@ class PagedMTPAttention:
             _native.check(code, "sqa_forward")
             if check:
                 _raise_device_bits(read_device_status(ws.data_ptr(), clear=True, device=self.device))
+        if scores is not None:
+            out.copy_(self._rows)
+            self._accumulate(query, key_cache, block_tables, seq_lens, scores, None)
         return out
+
+    def _accumulate(self, query, key_cache, block_tables, seq_lens, scores, key_scales):
+        accumulate_attention_weights(query, key_cache, block_tables, seq_lens, self._lse, scores, PAGE_SIZE,
+                                     self._max_seq_len, key_scales=key_scales, kv_layout=self._kv_layout,
+                                     sm_scale=self._sm_scale, min_seq_len=self._min_seq_len)
+
+    # ------------------------------------------------------------------ evict
+    def evict(self, key_cache, value_cache, scores, block_tables, seq_lens, budget: int, *, recent: int = 0,
+              sinks: int = 0, key_scales=None, value_scales=None, kept=None, check: bool = False):
+        """Cut every sequence longer than ``budget`` tokens by its scores (``cache_evict``, in the planned
+        layout) and ``seq_lens`` with it, in place; returns the kept positions ``[batch, Hkv, budget]``."""
+        if self._shape is None:
+            raise RuntimeError("plan() has not been called")
+        lens, kept = cache_evict(key_cache, value_cache, scores, block_tables, seq_lens, budget, recent=recent,
+                                 sinks=sinks, key_scales=key_scales, value_scales=value_scales, kept=kept, check=check,
+                                 kv_layout=self._kv_layout)
+        seq_lens.copy_(lens)
+        return kept

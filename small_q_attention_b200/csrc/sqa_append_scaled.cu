@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(256, kBlocksPerSm) sqa_cache_append_scaled_ker
 #pragma unroll
     for (int s = 0; s < kPageSize; ++s)
       x[s] = (s >= n0 && s < n1) ? __ldg(src + (size_t)(first + s - t0) * p.hkv * 32) : make_uint2(0u, 0u);
-    const float was = n0 > 0 ? *scale_at : 0.f;
+    const float was = n0 > 0 ? __ldcg(scale_at) : 0.f;
     // |x| of two 16-bit values at once, as integers (their order is that of the magnitudes); a page
     // with an infinity or NaN is looked through again for its finite values
     constexpr uint32_t kInf = BF ? 0x7f80u : 0x7c00u;
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(256, kBlocksPerSm) sqa_cache_append_scaled_ker
     if (n0 > 0 && scale > was) {  // the older tokens follow the page's new scale, a power of two
       uint32_t q[kPageSize];
 #pragma unroll
-      for (int s = 0; s < kPageSize; ++s) q[s] = s < n0 ? *reinterpret_cast<const uint32_t*>(dst + s * row) : 0u;
+      for (int s = 0; s < kPageSize; ++s) q[s] = s < n0 ? __ldcg(reinterpret_cast<const uint32_t*>(dst + s * row)) : 0u;
 #pragma unroll
       for (int s = 0; s < kPageSize; ++s) {
         if (s < n0) {

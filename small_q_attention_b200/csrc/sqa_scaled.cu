@@ -291,9 +291,9 @@ __device__ void page_meta(const ScaledTcParams& p, const Schedule& sch, const Sm
     float4 m = make_float4(S::F8 ? 0.f : 1.f, 0.f, 1.f, __int_as_float(in && good ? id : -1));
     if (S::F8 && in) {
       const size_t at = (size_t)(good ? id : 0) * p.scale_stride + w.h;
-      m.x = __ldg(p.k_scales + at);
+      m.x = __ldcg(p.k_scales + at);  // through L2: the append before may have run beside this grid's start
       if (S::ATTEND) {
-        const float vs = fmaxf(__ldg(p.v_scales + at), kMinValueScale);
+        const float vs = fmaxf(__ldcg(p.v_scales + at), kMinValueScale);
         m.y = log2f(vs);
         m.z = 1.f / vs;
       }
@@ -993,7 +993,7 @@ __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const Smem<S
   auto row_lse = [&](int b, int h) {  // -lse in base 2; -inf (weight 0) for padding and rows without tokens
     const int row = threadIdx.x;
     if (row >= rows) return -INFINITY;
-    const float v = __ldg(p.lse + (size_t)(b * p.s.q_len + (row >> 2)) * p.s.hq + h * kGroup + (row & 3));
+    const float v = __ldcg(p.lse + (size_t)(b * p.s.q_len + (row >> 2)) * p.s.hq + h * kGroup + (row & 3));
     return v == -INFINITY ? -INFINITY : -v * 1.4426950408889634f;
   };
   int blk = 0, pc = 0;
@@ -1021,7 +1021,7 @@ __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const Smem<S
       const int id = __float_as_int(meta.w);
       const bool held = tid < np * kPageSize && tok < piece.len;
       float* const at = p.scores + ((size_t)max(id, 0) * p.s.hkv + w.h) * kPageSize + (tid & 15);
-      const float old = (held && id >= 0 && tok < fresh) ? *at : 0.f;  // in flight during the score product
+      const float old = (held && id >= 0 && tok < fresh) ? __ldcg(at) : 0.f;  // in flight during the score product
       const bool masked = np < kBlockPages || tok0 + kBlock > piece.first || tok0 + kBlock > piece.len;
       const int late = held ? tok - piece.first : 0x7fffffff;
       float sum = 0.f;

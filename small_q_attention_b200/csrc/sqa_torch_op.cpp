@@ -2,7 +2,7 @@
 //
 // Two doors into the same code:
 // * TORCH_LIBRARY(sqa_b200): torch.ops.sqa_b200.small_q_attention /
-//   small_q_attention_partial, with CUDA and Meta kernels, so torch.compile and
+//   small_q_attention_partial / small_q_attention_scaled, with CUDA and Meta kernels, so torch.compile and
 //   fake-tensor tracing see a real operator instead of an opaque Python call;
 // * a pybind11 module (_sqa_torch.forward / forward_partial) that the Python
 //   entry small_q_attention() calls directly: the contract checks, argument
@@ -530,6 +530,23 @@ std::tuple<at::Tensor, at::Tensor> op_forward_partial(const at::Tensor& query, c
                          out_scale, 0, 0);
 }
 
+std::tuple<at::Tensor, at::Tensor> op_forward_scaled(const at::Tensor& query, const at::Tensor& key_cache,
+                                                     const at::Tensor& value_cache, const at::Tensor& key_scales,
+                                                     const at::Tensor& value_scales, const at::Tensor& block_tables,
+                                                     const at::Tensor& seq_lens, int64_t page_size, int64_t max_seq_len,
+                                                     int64_t kv_layout, double sm_scale, double out_scale) {
+  auto [o, l] = forward_scaled(query, key_cache, value_cache, key_scales, value_scales, block_tables, seq_lens, page_size,
+                               c10::nullopt, max_seq_len, c10::nullopt, c10::nullopt, true, c10::nullopt, 0, false,
+                               kv_layout, sm_scale, out_scale, 0);
+  return {o, *l};
+}
+
+std::tuple<at::Tensor, at::Tensor> meta_forward_scaled(const at::Tensor& query, const at::Tensor&, const at::Tensor&,
+                                                       const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                                       const at::Tensor&, int64_t, int64_t, int64_t, double, double) {
+  return {at::empty_like(query), at::empty(query.sizes().slice(0, 3), query.options().dtype(at::kFloat))};
+}
+
 at::Tensor meta_forward(const at::Tensor& query, const at::Tensor&, const at::Tensor&, const at::Tensor&,
                         const at::Tensor&, int64_t, int64_t, int64_t, int64_t, double, double) {
   return at::empty_like(query);
@@ -554,16 +571,22 @@ TORCH_LIBRARY(sqa_b200, m) {
       "small_q_attention_partial(Tensor query, Tensor key_cache, Tensor value_cache, Tensor block_tables, "
       "Tensor seq_lens, int page_size, Tensor? mask_lens=None, int max_seq_len=0, int kernel=0, int kv_layout=0, "
       "float sm_scale=0., float out_scale=1.) -> (Tensor, Tensor)");
+  m.def(
+      "small_q_attention_scaled(Tensor query, Tensor key_cache, Tensor value_cache, Tensor key_scales, "
+      "Tensor value_scales, Tensor block_tables, Tensor seq_lens, int page_size, int max_seq_len=0, int kv_layout=0, "
+      "float sm_scale=0., float out_scale=1.) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(sqa_b200, CUDA, m) {
   m.impl("small_q_attention", &op_forward);
   m.impl("small_q_attention_partial", &op_forward_partial);
+  m.impl("small_q_attention_scaled", &op_forward_scaled);
 }
 
 TORCH_LIBRARY_IMPL(sqa_b200, Meta, m) {
   m.impl("small_q_attention", &meta_forward);
   m.impl("small_q_attention_partial", &meta_forward_partial);
+  m.impl("small_q_attention_scaled", &meta_forward_scaled);
 }
 
 PYBIND11_MODULE(_sqa_torch, m) {

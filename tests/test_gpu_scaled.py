@@ -291,6 +291,36 @@ def test_attention_is_deterministic_and_graphs_do_not_share(sqa):
         assert all(torch.equal(o, e) for o, e in zip(outs, eager))
 
 
+def test_attention_compiled_and_from_two_threads(sqa):
+    """The registered operator under torch.compile's tracing, and calls from two host threads on their
+    own streams at once."""
+    import threading
+
+    cases = [scaled_case(4, [3000, 40], hkv=2, seed=s) for s in (1, 2)]
+    gs = [to_gpu(c) for c in cases]
+    want = [attend(sqa, g) for g in gs]
+    f = lambda g: torch.ops.sqa_b200.small_q_attention_scaled(  # noqa: E731
+        g["query"], g["k"], g["v"], g["ks"], g["vs"], g["table"], g["seq_lens"], 16)
+    o, lse = f(gs[0])
+    assert torch.equal(o, want[0][0]) and torch.equal(lse, want[0][1])
+    torch.cuda.synchronize()
+    bad = []
+
+    def loop(g, w):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                o, lse = attend(sqa, g)
+                torch.cuda.current_stream().synchronize()
+                bad.append(not (torch.equal(o, w[0]) and torch.equal(lse, w[1])))
+
+    threads = [threading.Thread(target=loop, args=(g, w)) for g, w in zip(gs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(bad) == 60 and not any(bad)
+
+
 def test_attention_bad_metadata(sqa):
     c = scaled_case(4, [40, 100], hkv=2, seed=4)
     g = to_gpu(c)

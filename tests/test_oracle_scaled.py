@@ -241,3 +241,15 @@ def test_no_cpu_fallback():
                  lambda: sqa.accumulate_attention_weights(*[None] * 7), lambda: sqa.cache_evict(*[None] * 6)):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+
+
+def test_the_scaled_operator_is_registered():
+    from small_q_attention_b200 import _native, build
+
+    build.build_torch_ext()
+    _native.torch_ext()
+    q = torch.empty(2, 4, 32, 128, dtype=torch.bfloat16, device="meta")
+    k = torch.empty(64, 16, 8, 128, dtype=torch.float8_e4m3fn, device="meta")
+    s, bt = torch.empty(64, 8, device="meta"), torch.empty(2, 32, dtype=torch.int32, device="meta")
+    o, lse = torch.ops.sqa_b200.small_q_attention_scaled(q, k, k, s, s, bt, torch.empty(2, dtype=torch.int32, device="meta"), 16)
+    assert o.shape == q.shape and o.dtype == torch.bfloat16 and lse.shape == (2, 4, 32) and lse.dtype == torch.float32

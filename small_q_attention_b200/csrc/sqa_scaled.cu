@@ -154,26 +154,6 @@ struct Smem {
   __device__ __forceinline__ uint32_t bar(int group, int i = 0) const { return smem_u32(at) + group + i * 8; }
 };
 
-// A bounded wait (as mbar_wait_bounded) that sleeps between polls: the softmax warps share their
-// schedulers with four warps that wait most of the time (16 x 8 x 32768: 255 us against 264 without).
-template <int kSleepNs = 20>
-__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort, unsigned int* status) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = global_timer_ns();
-  for (uint32_t it = 1;; ++it) {
-    __nanosleep(kSleepNs);
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((it & 15u) == 0u) {
-      if (*abort) return false;
-      if (global_timer_ns() - t0 > kWaitLimitNs) {
-        *abort = 1;
-        atomicOr(status, 1u);  // SQA_DEV_TIMEOUT
-        return false;
-      }
-    }
-  }
-}
-
 // The pieces of a CTA's range: f(walk, first unit, pages) for each, in order.
 template <class F>
 __device__ __forceinline__ void for_pieces(const SplitKvParams& p, const Schedule& sch, F f) {
@@ -247,7 +227,7 @@ __device__ void produce(const ScaledTcParams& p, const Schedule& sch, const CUte
       }
 #pragma unroll
       for (int tile = 0; tile < S::TILES; ++tile) {  // K then V; or the two 64-dim halves of 16-bit K
-        bool ok = wait_for<100>(sm.bar(Smem<S>::EMPTY, slot), phase ^ 1u, abort, p.s.status);
+        bool ok = mbar_wait_bounded(sm.bar(Smem<S>::EMPTY, slot), phase ^ 1u, abort, p.s.status);
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
         if (ok) {
           if (elect_one()) {
@@ -302,7 +282,7 @@ __device__ void page_meta(const ScaledTcParams& p, const Schedule& sch, const Sm
     for (int jb = 0; jb < cnt; jb += kBlockPages, ++blk) {
       const int e = blk % kMetaSlots;
       if (blk >= kMetaSlots)
-        wait_for<100>(sm.bar(Smem<S>::M_EMPTY, e), (uint32_t)(blk / kMetaSlots - 1) & 1u, abort, p.s.status);
+        mbar_wait_bounded(sm.bar(Smem<S>::M_EMPTY, e), (uint32_t)(blk / kMetaSlots - 1) & 1u, abort, p.s.status);
       if (lane >= jb && lane < jb + kBlockPages) sm.meta(e)[lane - jb] = m;
       __syncwarp();
       if (lane == 0) mbar_arrive(sm.bar(Smem<S>::M_FULL, e));
@@ -349,20 +329,20 @@ __device__ void issue_scores(const ScaledTcParams& p, const Schedule& sch, const
   int u = 0, pc = 0;
   RingPos at;
   for_pieces(p.s, sch, [&](const SegWalk&, int, int n) {
-    wait_for(sm.bar(Smem<S>::Q_READY, (pc & 1)), (uint32_t)(pc >> 1) & 1u, abort, p.s.status);
+    mbar_wait_bounded(sm.bar(Smem<S>::Q_READY, (pc & 1)), (uint32_t)(pc >> 1) & 1u, abort, p.s.status);
     const uint32_t q = smem_u32(sm.q(pc & 1));
     const int nblk = blocks_of(n);
     for (int k = 0; k < nblk; ++k) {
       const int k0 = at.slot;  // K's tile (its first half)
-      wait_for(sm.bar(Smem<S>::FULL, at.slot), at.phase, abort, p.s.status);
+      mbar_wait_bounded(sm.bar(Smem<S>::FULL, at.slot), at.phase, abort, p.s.status);
       at.next(tiles);
       const int k1 = at.slot;
-      if (!S::F8) wait_for(sm.bar(Smem<S>::FULL, at.slot), at.phase, abort, p.s.status);
+      if (!S::F8) mbar_wait_bounded(sm.bar(Smem<S>::FULL, at.slot), at.phase, abort, p.s.status);
       if (S::TILES == 2) at.next(tiles);  // K's second half, or V
 #pragma unroll 1
       for (int g = 0; g < S::G; ++g, ++u) {
         if (u >= S::NS)
-          wait_for(sm.bar(Smem<S>::S_EMPTY, u % S::NS), (uint32_t)(u / S::NS - 1) & 1u, abort, p.s.status);
+          mbar_wait_bounded(sm.bar(Smem<S>::S_EMPTY, u % S::NS), (uint32_t)(u / S::NS - 1) & 1u, abort, p.s.status);
         __syncwarp();
         tc_fence_after();
         if (elect_one()) {
@@ -419,11 +399,11 @@ __device__ void issue_values(const ScaledTcParams& p, const Schedule& sch, const
     for (int k = 0; k < nblk; ++k) {
       at.next(tiles);  // over K
       const int np = min(kBlockPages, n - k * kBlockPages);
-      wait_for(sm.bar(Smem<S>::FULL, at.slot), at.phase, abort, p.s.status);
+      mbar_wait_bounded(sm.bar(Smem<S>::FULL, at.slot), at.phase, abort, p.s.status);
 #pragma unroll 1
       for (int g = 0; g < S::G; ++g, ++u) {
         const int st = u % S::W, v = u / S::W;
-        wait_for(sm.bar(Smem<S>::P_FULL, sm.pi(st, v)), (uint32_t)(v >> 1) & 1u, abort, p.s.status);
+        mbar_wait_bounded(sm.bar(Smem<S>::P_FULL, sm.pi(st, v)), (uint32_t)(v >> 1) & 1u, abort, p.s.status);
         __syncwarp();
         tc_fence_after();
         if (elect_one()) {
@@ -688,7 +668,7 @@ __device__ __forceinline__ float unit_scores(uint32_t slot, const float* base, f
 template <class S>
 __device__ __forceinline__ float4 read_meta(const ScaledTcParams& p, const Smem<S>& sm, int bk, volatile int* abort) {
   const int e = bk % kMetaSlots;
-  wait_for(sm.bar(Smem<S>::M_FULL, e), (uint32_t)(bk / kMetaSlots) & 1u, abort, p.s.status);
+  mbar_wait_bounded(sm.bar(Smem<S>::M_FULL, e), (uint32_t)(bk / kMetaSlots) & 1u, abort, p.s.status);
   const float4 m = sm.meta(e)[(threadIdx.x & 127) >> 4];
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive(sm.bar(Smem<S>::M_EMPTY, e));
@@ -758,7 +738,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
         // NaN: zero, and remembered by the dimension's thread.  (The block's first group does it: its
         // product comes first.)
         const int t1 = bk * 2 + 1;  // V's tile
-        wait_for(sm.bar(Smem<S>::FULL, t1 % tiles), (uint32_t)(t1 / tiles) & 1u, abort, p.s.status);
+        mbar_wait_bounded(sm.bar(Smem<S>::FULL, t1 % tiles), (uint32_t)(t1 / tiles) & 1u, abort, p.s.status);
         uint8_t* const vt = sm.ring(t1 % tiles);
         const int held = min(np * kPageSize, max(piece.len - tok0, 0));
         const int read = (np + 1) / 2 * 32;  // rows that the product reads
@@ -774,7 +754,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
         fence_proxy_async_smem();
       }
 
-      wait_for(sm.bar(Smem<S>::S_FULL, u % S::NS), (uint32_t)(u / S::NS) & 1u, abort, p.s.status);
+      mbar_wait_bounded(sm.bar(Smem<S>::S_FULL, u % S::NS), (uint32_t)(u / S::NS) & 1u, abort, p.s.status);
       tc_fence_after();
       const uint32_t slot = lanes + S::OCOLS + (u % S::NS) * S::STRIDE;
       float t[ROWS];
@@ -803,7 +783,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
         for (int r = 0; r < ROWS; ++r) t[r] -= delta[r];
       }
       if (raise && !first) {  // O stands still once the stream's last product is done
-        wait_for(sm.bar(Smem<S>::P_DONE, sm.pi(stream, v - 1)), (uint32_t)((v - 1) >> 1) & 1u, abort, p.s.status);
+        mbar_wait_bounded(sm.bar(Smem<S>::P_DONE, sm.pi(stream, v - 1)), (uint32_t)((v - 1) >> 1) & 1u, abort, p.s.status);
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < ROWS; c += 8) {
@@ -828,7 +808,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
       // P: token tid's operand row of PROW bytes, part i of row r in byte i * ROWS + r; 16-byte chunks
       // swizzled by the token
       // (its buffer is free once the product before the last is done)
-      if (v >= 2) wait_for(sm.bar(Smem<S>::P_DONE, sm.pi(stream, v)), (uint32_t)((v >> 1) - 1) & 1u, abort, p.s.status);
+      if (v >= 2) mbar_wait_bounded(sm.bar(Smem<S>::P_DONE, sm.pi(stream, v)), (uint32_t)((v >> 1) - 1) & 1u, abort, p.s.status);
       uint8_t* const prow = sm.p(stream, v) + tid * S::PROW;
       const int swizzle = S::PROW == 128 ? tid & 7 : (tid >> 1) & 3;
       constexpr int kHalf = ROWS < 16 ? ROWS : 16;  // rows of a 16-byte chunk
@@ -907,7 +887,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
     for (int st = 0; st < W; ++st) {  // each stream's last product (it may have none in this piece)
       const int last = ((blk + nblk) * G - 1 - st) / W * W + st;  // the last unit of the stream so far
       if (last >= blk * G && last < (blk + nblk) * G)
-        wait_for(sm.bar(Smem<S>::P_DONE, sm.pi(st, last / W)), (uint32_t)(last / W >> 1) & 1u, abort, p.s.status);
+        mbar_wait_bounded(sm.bar(Smem<S>::P_DONE, sm.pi(st, last / W)), (uint32_t)(last / W >> 1) & 1u, abort, p.s.status);
     }
     tc_fence_after();
     softmax_sync<S>();
@@ -1028,7 +1008,7 @@ __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const Smem<S
 #pragma unroll 1
       for (int g = 0; g < G; ++g) {
         const int u = bk * G + g;
-        wait_for(sm.bar(Smem<S>::S_FULL, u % S::NS), (uint32_t)(u / S::NS) & 1u, abort, p.s.status);
+        mbar_wait_bounded(sm.bar(Smem<S>::S_FULL, u % S::NS), (uint32_t)(u / S::NS) & 1u, abort, p.s.status);
         tc_fence_after();
         const uint32_t slot = lanes + (u % S::NS) * S::STRIDE;
         sum += masked ? unit_weight<S, true>(slot, sm.base(0) + g * S::ROWS, kc, late, g * S::ROWS)

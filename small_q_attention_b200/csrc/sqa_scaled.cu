@@ -638,27 +638,33 @@ __device__ __forceinline__ Piece piece_of(const SplitKvParams& p, const SegWalk&
   return Piece{min(raw, w.pages * kPageSize), whole - p.q_len + 1};
 }
 
-// t = y - base of a unit's rows, and their largest.  MASK: the block holds tokens that some row
-// does not see (late: see attend).
-template <class S, bool MASK>
+// t = y - base of a unit's rows, and their largest; `release` is called once the scores are in registers.
+// MASK: the block holds tokens that some row does not see (late: see attend).
+template <class S, bool MASK, class F>
 __device__ __forceinline__ float unit_scores(uint32_t slot, const float* base, float kc, float lv, int late, int row0,
-                                             float (&t)[S::ROWS]) {
+                                             float (&t)[S::ROWS], F release) {
+  uint32_t raw[S::ROWS / 8][S::PARTS][8];
+#pragma unroll
+  for (int c = 0; c < S::ROWS / 8; ++c)
+#pragma unroll
+    for (int i = 0; i < S::PARTS; ++i) tmem_ld(slot + i * S::ROWS + c * 8, raw[c][i]);
+  tmem_wait_ld();
+  release();
   float over = -INFINITY;
 #pragma unroll
-  for (int c = 0; c < S::ROWS; c += 8) {
-    float s[8];
-    read_scores<S>(slot, c, s);
+  for (int r = 0; r < S::ROWS; r += 4) {
+    const float4 b4 = *reinterpret_cast<const float4*>(base + r);
+    const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
-    for (int r = 0; r < 8; r += 4) {
-      const float4 b4 = *reinterpret_cast<const float4*>(base + c + r);
-      const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
+    for (int i = 0; i < 4; ++i) {
+      const int c = (r + i) / 8, e = (r + i) % 8;
+      float s = __uint_as_float(raw[c][S::PARTS - 1][e]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x = fmaf(s[r + i], kc, lv - bb[i]);
-        if (MASK && late >= (row0 + c + r + i) >> 2) x = -INFINITY;
-        t[c + r + i] = x;
-        over = fmaxf(over, x);
-      }
+      for (int j = S::PARTS - 2; j >= 0; --j) s = fmaf(s, 1.f / 32.f, __uint_as_float(raw[c][j][e]));
+      float x = fmaf(s, kc, lv - bb[i]);
+      if (MASK && late >= (row0 + r + i) >> 2) x = -INFINITY;
+      t[r + i] = x;
+      over = fmaxf(over, x);
     }
   }
   return over;
@@ -759,11 +765,13 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
       const uint32_t slot = lanes + S::OCOLS + (u % S::NS) * S::STRIDE;
       float t[ROWS];
       const float kc = meta.x * cq;
-      const float over = masked ? unit_scores<S, true>(slot, base, kc, meta.y, late, row0, t)
-                                : unit_scores<S, false>(slot, base, kc, meta.y, late, row0, t);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(sm.bar(Smem<S>::S_EMPTY, u % S::NS));
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sm.bar(Smem<S>::S_EMPTY, u % S::NS));
+      };
+      const float over = masked ? unit_scores<S, true>(slot, base, kc, meta.y, late, row0, t, release)
+                                : unit_scores<S, false>(slot, base, kc, meta.y, late, row0, t, release);
       const float inv_vs = meta.z;
       if (k + kStep < nblk) meta = read_meta(p, sm, bk + kStep, abort);  // off the next unit's path
       const bool first = k == k0;

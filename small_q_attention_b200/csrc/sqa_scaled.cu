@@ -83,9 +83,14 @@ struct Shape {
   static constexpr int SOFTMAX = W * 128, THREADS = SOFTMAX + 128;
   static constexpr int COLS = (F8 ? PARTS : 1) * ROWS;
   static constexpr int N = (COLS + 15) / 16 * 16;             // score columns of a group (N of the product)
-  static constexpr int STRIDE = N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128;  // TMEM columns of a score slot
-  static constexpr int PROW = ROWS > 16 ? 128 : 64;           // bytes of a token's P: up to three parts of the rows
-  static constexpr int PBYTES = kBlock * PROW;
+  static constexpr int GP = ATTEND && G > 1 ? 2 : 1;          // groups that one product takes: A is read once for both
+  static constexpr int UNITS = G / GP;                        // products of a block, each for GP streams
+  static constexpr int SN = GP * N;
+  static constexpr int STRIDE = SN <= 16 ? 16 : SN <= 32 ? 32 : SN <= 64 ? 64 : 128;  // TMEM columns of a score slot
+  static constexpr int PROW = 64;                             // bytes of a token's P in a group: three parts of 16 rows
+  static constexpr int PPITCH = GP * PROW;                    // and of its operand row
+  static constexpr int PBYTES = kBlock * PPITCH;
+  static constexpr int LANES = W / GP;                        // streams of products
   static constexpr int OCOLS = ATTEND ? W * PROW : 0;         // O^T of the streams
   static constexpr int SLOTS_FIT = (512 - OCOLS) / STRIDE;
   static constexpr int NS = SLOTS_FIT < 8 ? SLOTS_FIT : 8;
@@ -93,8 +98,10 @@ struct Shape {
   static constexpr int Q_BYTES = G * Q_GROUP;
   static constexpr int TILES = ATTEND || !F8 ? 2 : 1;         // 16 KB tiles of a block (K and V, or K's two halves)
   static constexpr int Q_STEPS = (G * ROWS * 8 + SOFTMAX - 1) / SOFTMAX;
-  static_assert(!ATTEND || (kPParts * ROWS <= PROW && NS >= W && W % G == 0), "columns");
-  static_assert(N <= 128 && NS >= 2 && W <= 4 && G * ROWS <= 64, "columns");
+  static_assert(!ATTEND || (kPParts * ROWS <= PROW && W % G == 0), "columns");
+  // A slot belongs to one warpgroup (or pair): only then does a wait see no phase but the next one.
+  static_assert(NS % (ATTEND ? LANES : W * G) == 0, "slots");
+  static_assert(SN <= 128 && NS >= 2 && NS <= 8 && W <= 4 && G * ROWS <= 64, "columns");
 };
 
 struct ScaledTcParams {
@@ -111,8 +118,8 @@ struct ScaledTcParams {
 template <class S>
 struct Smem {
   static constexpr int kMaxTiles = 16;
-  static constexpr int P = 0;                                           // two P buffers for each stream
-  static constexpr int Q = P + (S::ATTEND ? S::W * 2 * S::PBYTES : 0);    // two Q slots
+  static constexpr int P = 0;                                           // two P buffers for each lane of products
+  static constexpr int Q = P + (S::ATTEND ? S::LANES * 2 * S::PBYTES : 0);    // two Q slots
   static constexpr int META = Q + 2 * S::Q_BYTES;                       // [kMetaSlots][8]: ks, log2 vs, 1 / vs, page id (bits)
   static constexpr int BASE = META + kMetaSlots * kBlockPages * 16;     // [W][ROWS]: a stream's bases (weights: -lse of all rows)
   static constexpr int DELTA = BASE + 64 * 4;                           // [W][ROWS]: raises; the epilogue's factors of O
@@ -138,9 +145,9 @@ struct Smem {
   uint8_t* at;  // 1024-byte aligned, in shared memory
 
   __device__ __forceinline__ uint8_t* ring(int tile) const { return at + RING + tile * kTileBytes; }
-  // the buffer of a stream's v-th unit, and the index of its barriers
-  __device__ __forceinline__ static int pi(int stream, int v) { return 2 * stream + (v & 1); }
-  __device__ __forceinline__ uint8_t* p(int stream, int v) const { return at + P + pi(stream, v) * S::PBYTES; }
+  // the buffer of a lane's v-th product, and the index of its barriers
+  __device__ __forceinline__ static int pi(int lane, int v) { return 2 * lane + (v & 1); }
+  __device__ __forceinline__ uint8_t* p(int lane, int v) const { return at + P + pi(lane, v) * S::PBYTES; }
   __device__ __forceinline__ uint8_t* q(int slot) const { return at + Q + slot * S::Q_BYTES; }
   __device__ __forceinline__ float4* meta(int slot) const { return reinterpret_cast<float4*>(at + META) + slot * kBlockPages; }
   __device__ __forceinline__ float* base(int stream) const { return reinterpret_cast<float*>(at + BASE) + stream * S::ROWS; }
@@ -321,11 +328,11 @@ struct RingPos {
   }
 };
 
-// S^T of (block, group) unit u into score slot u % NS.
+// S^T of product u, (block, GP groups), into score slot u % NS.
 template <class S, bool BF>
 __device__ void issue_scores(const ScaledTcParams& p, const Schedule& sch, const Smem<S>& sm, uint32_t tmem, int tiles,
                              volatile int* abort) {
-  constexpr uint32_t kIdesc = mma_idesc_f16(128, S::N, false, false, BF && !S::F8);  // format 0: e4m3 / fp16
+  constexpr uint32_t kIdesc = mma_idesc_f16(128, S::SN, false, false, BF && !S::F8);  // format 0: e4m3 / fp16
   int u = 0, pc = 0;
   RingPos at;
   for_pieces(p.s, sch, [&](const SegWalk&, int, int n) {
@@ -340,14 +347,14 @@ __device__ void issue_scores(const ScaledTcParams& p, const Schedule& sch, const
       if (!S::F8) mbar_wait_bounded(sm.bar(Smem<S>::FULL, at.slot), at.phase, abort, p.s.status);
       if (S::TILES == 2) at.next(tiles);  // K's second half, or V
 #pragma unroll 1
-      for (int g = 0; g < S::G; ++g, ++u) {
+      for (int g = 0; g < S::UNITS; ++g, ++u) {
         if (u >= S::NS)
           mbar_wait_bounded(sm.bar(Smem<S>::S_EMPTY, u % S::NS), (uint32_t)(u / S::NS - 1) & 1u, abort, p.s.status);
         __syncwarp();
         tc_fence_after();
         if (elect_one()) {
           const uint32_t d = tmem + S::OCOLS + (u % S::NS) * S::STRIDE;
-          const uint32_t qg = q + g * S::Q_GROUP;
+          const uint32_t qg = q + g * S::GP * S::Q_GROUP;
           const uint32_t kt = smem_u32(sm.ring(k0));
           if constexpr (S::F8) {
 #pragma unroll
@@ -362,7 +369,7 @@ __device__ void issue_scores(const ScaledTcParams& p, const Schedule& sch, const
                         smem_desc_sw128(qg + (kk >> 2) * (S::N * 128) + (kk & 3) * 32, 16, 1024), kIdesc, kk > 0 ? 1u : 0u);
           }
           tc_commit(sm.bar(Smem<S>::S_FULL, u % S::NS));
-          if (g == S::G - 1) {  // the block's K may be overwritten
+          if (g == S::UNITS - 1) {  // the block's K may be overwritten
             tc_commit(sm.bar(Smem<S>::EMPTY, k0));
             if (!S::F8) tc_commit(sm.bar(Smem<S>::EMPTY, k1));
           }
@@ -375,23 +382,23 @@ __device__ void issue_scores(const ScaledTcParams& p, const Schedule& sch, const
   drain_products(p, sm);
 }
 
-// Descriptor of P, MN-major: one atom of PROW rows (bytes) x 8 tokens, swizzled over its row.
+// Descriptor of P, MN-major: one atom of PPITCH rows (bytes) x 8 tokens, swizzled over its row.
 template <class S>
 __device__ __forceinline__ uint64_t desc_p(uint32_t saddr) {
   uint64_t d = 0;
   d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
   d |= (uint64_t)((S::PBYTES >> 4) & 0x3FFFu) << 16;     // between atoms along the rows: there is one
-  d |= (uint64_t)((8 * S::PROW >> 4) & 0x3FFFu) << 32;   // between groups of 8 tokens
+  d |= (uint64_t)((8 * S::PPITCH >> 4) & 0x3FFFu) << 32;  // between groups of 8 tokens
   d |= (uint64_t)1 << 46;                                // version
-  d |= (uint64_t)(S::PROW == 128 ? 2 : 4) << 61;         // SWIZZLE_128B or SWIZZLE_64B
+  d |= (uint64_t)(S::PPITCH == 128 ? 2 : 4) << 61;       // SWIZZLE_128B or SWIZZLE_64B
   return d;
 }
 
-// O^T of stream u % W += V^T P^T of unit u, once P is in the stream's buffer.
+// O^T of the streams of lane u % LANES += V^T P^T of product u, once their P is in the lane's buffer.
 template <class S>
 __device__ void issue_values(const ScaledTcParams& p, const Schedule& sch, const Smem<S>& sm, uint32_t tmem, int tiles,
                              volatile int* abort) {
-  constexpr uint32_t kIdesc = mma_idesc_f16(128, S::PROW, true, true, false);
+  constexpr uint32_t kIdesc = mma_idesc_f16(128, S::PPITCH, true, true, false);
   int u = 0;
   RingPos at;
   for_pieces(p.s, sch, [&](const SegWalk&, int, int n) {
@@ -401,8 +408,8 @@ __device__ void issue_values(const ScaledTcParams& p, const Schedule& sch, const
       const int np = min(kBlockPages, n - k * kBlockPages);
       mbar_wait_bounded(sm.bar(Smem<S>::FULL, at.slot), at.phase, abort, p.s.status);
 #pragma unroll 1
-      for (int g = 0; g < S::G; ++g, ++u) {
-        const int st = u % S::W, v = u / S::W;
+      for (int g = 0; g < S::UNITS; ++g, ++u) {
+        const int st = u % S::LANES, v = u / S::LANES;
         mbar_wait_bounded(sm.bar(Smem<S>::P_FULL, sm.pi(st, v)), (uint32_t)(v >> 1) & 1u, abort, p.s.status);
         __syncwarp();
         tc_fence_after();
@@ -412,10 +419,10 @@ __device__ void issue_values(const ScaledTcParams& p, const Schedule& sch, const
           const int steps = (np + 1) / 2;  // 32 tokens a step; the softmax zeroed an absent page's V
           // a stream's first product of a piece overwrites O
           for (int kk = 0; kk < steps; ++kk)
-            tc_mma_ss_f8(tmem + st * S::PROW, smem_desc_sw128(vt + kk * 4096, kTileBytes, 1024), desc_p<S>(pb + kk * 32 * S::PROW),
+            tc_mma_ss_f8(tmem + st * S::PPITCH, smem_desc_sw128(vt + kk * 4096, kTileBytes, 1024), desc_p<S>(pb + kk * 32 * S::PPITCH),
                          kIdesc, (k >= S::W / S::G || kk > 0) ? 1u : 0u);
           tc_commit(sm.bar(Smem<S>::P_DONE, sm.pi(st, v)));
-          if (g == S::G - 1) tc_commit(sm.bar(Smem<S>::EMPTY, at.slot));
+          if (g == S::UNITS - 1) tc_commit(sm.bar(Smem<S>::EMPTY, at.slot));
         }
         __syncwarp();
       }
@@ -692,6 +699,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
   const int rows = kGroup * p.s.q_len;
   const int group = stream % G;  // the stream's rows: row0 .. row0 + ROWS - 1
   const int row0 = group * ROWS;
+  const int plane = stream / S::GP;  // its lane of products
   float* const base = sm.base(stream);
   float* const delta = sm.delta(stream);
   float* const wred = sm.wred(stream * 4);
@@ -730,8 +738,8 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
     if (k0 < nblk) meta = read_meta(p, sm, blk + k0, abort);
     for (int k = k0; k < nblk; k += kStep) {
       const int bk = blk + k;
-      const int u = bk * G + group;
-      const int v = u / W;  // the stream's own count
+      const int u = bk * S::UNITS + group / S::GP;  // product
+      const int v = u / S::LANES;                   // the stream's own count
       const int np = min(kBlockPages, n - k * kBlockPages);
       const int tok0 = (w.pg + k * kBlockPages) * kPageSize;
       const int tok = tok0 + tid;
@@ -744,6 +752,10 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
         // NaN: zero, and remembered by the dimension's thread.  (The block's first group does it: its
         // product comes first.)
         const int t1 = bk * 2 + 1;  // V's tile
+        // The tile's last occupant is tiles / 2 > kStep blocks back: once the lane's last product is done,
+        // and with it every product before, its barrier is in no earlier phase than the one waited for.
+        if (v >= 1)
+          mbar_wait_bounded(sm.bar(Smem<S>::P_DONE, sm.pi(plane, v - 1)), (uint32_t)((v - 1) >> 1) & 1u, abort, p.s.status);
         mbar_wait_bounded(sm.bar(Smem<S>::FULL, t1 % tiles), (uint32_t)(t1 / tiles) & 1u, abort, p.s.status);
         uint8_t* const vt = sm.ring(t1 % tiles);
         const int held = min(np * kPageSize, max(piece.len - tok0, 0));
@@ -762,7 +774,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
 
       mbar_wait_bounded(sm.bar(Smem<S>::S_FULL, u % S::NS), (uint32_t)(u / S::NS) & 1u, abort, p.s.status);
       tc_fence_after();
-      const uint32_t slot = lanes + S::OCOLS + (u % S::NS) * S::STRIDE;
+      const uint32_t slot = lanes + S::OCOLS + (u % S::NS) * S::STRIDE + (group % S::GP) * S::N;
       float t[ROWS];
       const float kc = meta.x * cq;
       auto release = [&]() {
@@ -791,7 +803,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
         for (int r = 0; r < ROWS; ++r) t[r] -= delta[r];
       }
       if (raise && !first) {  // O stands still once the stream's last product is done
-        mbar_wait_bounded(sm.bar(Smem<S>::P_DONE, sm.pi(stream, v - 1)), (uint32_t)((v - 1) >> 1) & 1u, abort, p.s.status);
+        mbar_wait_bounded(sm.bar(Smem<S>::P_DONE, sm.pi(plane, v - 1)), (uint32_t)((v - 1) >> 1) & 1u, abort, p.s.status);
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < ROWS; c += 8) {
@@ -813,12 +825,12 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
         }
         tmem_wait_st();
       }
-      // P: token tid's operand row of PROW bytes, part i of row r in byte i * ROWS + r; 16-byte chunks
-      // swizzled by the token
+      // P: token tid's operand row of PPITCH bytes, in the group's 64 part i of row r in byte
+      // i * ROWS + r; 16-byte chunks swizzled by the token
       // (its buffer is free once the product before the last is done)
-      if (v >= 2) mbar_wait_bounded(sm.bar(Smem<S>::P_DONE, sm.pi(stream, v)), (uint32_t)((v >> 1) - 1) & 1u, abort, p.s.status);
-      uint8_t* const prow = sm.p(stream, v) + tid * S::PROW;
-      const int swizzle = S::PROW == 128 ? tid & 7 : (tid >> 1) & 3;
+      if (v >= 2) mbar_wait_bounded(sm.bar(Smem<S>::P_DONE, sm.pi(plane, v)), (uint32_t)((v >> 1) - 1) & 1u, abort, p.s.status);
+      uint8_t* const prow = sm.p(plane, v) + tid * S::PPITCH;
+      const int swizzle = S::PPITCH == 128 ? tid & 7 : (tid >> 1) & 3;
       constexpr int kHalf = ROWS < 16 ? ROWS : 16;  // rows of a 16-byte chunk
 #pragma unroll
       for (int c = 0; c < ROWS; c += kHalf) {
@@ -839,7 +851,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
         }
 #pragma unroll
         for (int i = 0; i < kPParts; ++i) {
-          const int byte = i * ROWS + c;
+          const int byte = (group % S::GP) * S::PROW + i * ROWS + c;
           uint8_t* const at = prow + (((byte >> 4) ^ swizzle) << 4) + (byte & 15);
           if constexpr (kHalf == 16)
             *reinterpret_cast<uint4*>(at) = make_uint4(part[i][0], part[i][1], part[i][2], part[i][3]);
@@ -850,7 +862,7 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
       fence_proxy_async_smem();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(sm.bar(Smem<S>::P_FULL, sm.pi(stream, v)));
+      if (lane == 0) mbar_arrive(sm.bar(Smem<S>::P_FULL, sm.pi(plane, v)));
     }
 
     // ---- epilogue: denominators and factors, then each dimension's thread joins its rows' parts
@@ -892,10 +904,11 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
       else if (p.s.out_lse) p.s.out_lse[out_row] = lse;
     }
 #pragma unroll
-    for (int st = 0; st < W; ++st) {  // each stream's last product (it may have none in this piece)
-      const int last = ((blk + nblk) * G - 1 - st) / W * W + st;  // the last unit of the stream so far
-      if (last >= blk * G && last < (blk + nblk) * G)
-        mbar_wait_bounded(sm.bar(Smem<S>::P_DONE, sm.pi(st, last / W)), (uint32_t)(last / W >> 1) & 1u, abort, p.s.status);
+    for (int x = 0; x < S::LANES; ++x) {  // each lane's last product (it may have none in this piece)
+      const int last = ((blk + nblk) * S::UNITS - 1 - x) / S::LANES * S::LANES + x;
+      if (last >= blk * S::UNITS && last < (blk + nblk) * S::UNITS)
+        mbar_wait_bounded(sm.bar(Smem<S>::P_DONE, sm.pi(x, last / S::LANES)), (uint32_t)(last / S::LANES >> 1) & 1u, abort,
+                          p.s.status);
     }
     tc_fence_after();
     softmax_sync<S>();
@@ -1061,13 +1074,11 @@ __global__ void __launch_bounds__(S::THREADS, 1)
     }
     for (int i = 0; i < 8; ++i) {
       mbar_init(sm.bar(Smem<S>::S_FULL, i), 1);
-      mbar_init(sm.bar(Smem<S>::S_EMPTY, i), 4);
+      mbar_init(sm.bar(Smem<S>::S_EMPTY, i), 4 * S::GP);
     }
-    for (int i = 0; i < S::W; ++i) {
-      for (int j = 0; j < 2; ++j) {
-        mbar_init(sm.bar(Smem<S>::P_FULL, 2 * i + j), 4);
-        mbar_init(sm.bar(Smem<S>::P_DONE, 2 * i + j), 1);
-      }
+    for (int i = 0; i < 2 * S::LANES; ++i) {
+      mbar_init(sm.bar(Smem<S>::P_FULL, i), 4 * S::GP);
+      mbar_init(sm.bar(Smem<S>::P_DONE, i), 1);
     }
     for (int i = 0; i < 2; ++i) mbar_init(sm.bar(Smem<S>::Q_READY, i), S::SOFTMAX / 32);
     for (int i = 0; i < kMetaSlots; ++i) {
@@ -1161,8 +1172,10 @@ constexpr int kMaxSmem = 227 * 1024;
 
 template <class S>
 constexpr int tiles_that_fit() {
-  const int n = (kMaxSmem - 1024 - Smem<S>::RING) / kTileBytes;
-  return (n < Smem<S>::kMaxTiles ? n : Smem<S>::kMaxTiles) / S::TILES * S::TILES;
+  constexpr int n = (kMaxSmem - 1024 - Smem<S>::RING) / kTileBytes;
+  constexpr int tiles = (n < Smem<S>::kMaxTiles ? n : Smem<S>::kMaxTiles) / S::TILES * S::TILES;
+  static_assert(tiles / 2 > S::W / S::G, "the ring holds more blocks than a stream skips");
+  return tiles;
 }
 
 template <class S, bool BF>
@@ -1207,7 +1220,8 @@ cudaError_t launch_rows(ScaledTcParams& p, const CUtensorMap& tm_k, const CUtens
     if (rows <= 8) return launch_shape<Shape<PARTS, 8, 1, 4, false>, BF>(p, tm_k, tm_v, grid, stream);
     if (rows <= 16) return launch_shape<Shape<PARTS, 16, 1, 4, false>, BF>(p, tm_k, tm_v, grid, stream);
     if (rows <= 32) return launch_shape<Shape<PARTS, 32, 1, 4, false>, BF>(p, tm_k, tm_v, grid, stream);
-    return launch_shape<Shape<PARTS, 32, 2, 4, false>, BF>(p, tm_k, tm_v, grid, stream);
+    // three parts of 32 rows leave four slots: two for each of two warpgroups
+    return launch_shape<Shape<PARTS, 32, 2, PARTS == 3 ? 2 : 4, false>, BF>(p, tm_k, tm_v, grid, stream);
   }
 }
 

@@ -100,6 +100,16 @@ def test_weights_masks_and_garbage(sqa, scaled):
         assert_weights(got, c, mask_lens=mask, sm_scale=0.07)
 
 
+@pytest.mark.parametrize("scaled", [False, True], ids=["16bit", "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("q_len", [1, 4, 8, 9, 16])
+def test_weights_many_blocks_a_cta(sqa, q_len, dtype, scaled):
+    """Few CTAs over long sequences: every slot and ring position is used again and again."""
+    c = weight_case(q_len, [5003, 700, 2600], 1, dtype, scaled, seed=q_len)
+    for num_ctas in (1, 2):
+        assert_weights(accumulate(sqa, gpu(c), num_ctas=num_ctas, check=True), c)
+
+
 def test_weights_sum_to_the_rows(sqa):
     """With the attention's own log-sum-exp, the new weights of a step sum to the number of rows."""
     c = weight_case(4, [1000, 33, 4], 2, torch.bfloat16, True, seed=4)

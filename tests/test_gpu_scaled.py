@@ -116,6 +116,17 @@ def test_attention_splits(sqa, num_ctas):
     assert_within(out, lse, reference(c), torch.float16)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("q_len", [1, 3, 6, 8, 9, 16])
+def test_attention_many_blocks_a_cta(sqa, q_len, dtype):
+    """Few CTAs over long sequences: every slot, buffer and ring position is used again and again."""
+    c = scaled_case(q_len, [5003, 700, 2600], hkv=1, dtype=dtype, seed=q_len)
+    g, want = to_gpu(c), reference(c)
+    for num_ctas in (1, 2):
+        out, lse = attend(sqa, g, num_ctas=num_ctas, check=True)
+        assert_within(out, lse, want, dtype)
+
+
 @pytest.mark.parametrize("q_len,batch", [(1, 1), (4, 1), (4, 3), (16, 1), (16, 2)])
 def test_attention_length_hints(sqa, q_len, batch):
     """Right whatever the bounds say: tight, loose and wrong ones."""

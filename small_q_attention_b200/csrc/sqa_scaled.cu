@@ -35,22 +35,28 @@
 // Weights.  w_t = sum over the rows of 2^(c ks (q . k) - lse): the same score product, summed over the
 // thread's columns and added to the token's score.  16-bit caches use kind::f16 and Q as it is.
 //
-// Four softmax warpgroups, so that each scheduler has four warps to issue from and a unit of
-// 16 rows keeps its scores and sums in registers.  With one warpgroup, a block of 64 rows took
-// 13.7k cycles at 0.22 instructions a cycle and scheduler, with two of 32 rows 5k.  A unit is a
-// (block, group of 16 rows); a warpgroup takes every fourth unit, its stream: of one group always
-// (4 / G blocks apart), with its own bases and O, and the streams of a group are joined at
-// the end of a piece.
+// Streams.  A unit is a (block, group of 16 rows); each of W softmax warpgroups takes every W-th unit: of
+// one group always, with its own bases and O, and the streams of a group are joined at the
+// end of a piece.  Two for up to 32 rows, four beyond (96 registers a thread): with one
+// warpgroup a block of 64 rows took 13.7k cycles, with two of 32 rows 6.9k, with four of 16
+// 3.8k; at 32 rows two beat four (237 against 248 us at 16 x 8 x 32768), and 16 rows a group beat 32
+// (237 / 241 us, fp16 243 / 290, for want of registers).  Two groups of a block share a product
+// (GP = 2, one read of K and V for both: 1 x 16 x 262144 230 -> 195 us in isolation).
 //
-// Warps: 0-15 softmax (one token a thread), 16 score products, 17 value products, 18 TMA
-// producer, 19 page scales.  Work is cut into CTA ranges by sqa_schedule.cuh; pieces of a split
+// What bounds it.  q_len 1-4 run at 5.3-5.8 TB/s (q_len 2, 16 x 32768: 187 us for 1.07 GB), near what
+// 2 KB boxes of 128-byte rows reach.  Above, the softmax warps' latency chain does: at
+// q_len 8 (235 us) leaving out P, the scores and the value products altogether still took
+// 200 us, single stages 5-11% each; the tensor pipe is 15% busy.
+//
+// Warps: 0 .. 4 W - 1 softmax (one token a thread), then one each for score products, value
+// products, TMA and page scales.  Work is cut into CTA ranges by sqa_schedule.cuh; pieces of a split
 // segment are merged by sqa_scaled_merge_kernel.
 //
 // Pipelines (mbarriers; every wait bounded):
 //   full / empty [tiles]     producer -> issuers; K and V tiles (16 KB) alternate in one ring,
 //                            each released by the commit of the product that read it
 //   s_full / s_empty [NS]    score issuer (commit) -> softmax -> score issuer
-//   p_full / p_done [2 W]    softmax -> value issuer (commit) -> softmax, two P buffers a stream
+//   p_full / p_done [2 LANES]  softmax -> value issuer (commit) -> softmax, two P buffers a lane
 //   q_ready [2]              softmax (Q of a piece, one piece ahead) -> score issuer
 //   m_full / m_empty [8]     page scales of a block -> softmax
 #include <atomic>
@@ -74,7 +80,7 @@ constexpr float kRaise = 8.f, kHead = -1.f;      // raise a base that a score ex
 constexpr float kLn2f = 0.6931471805599453f;
 constexpr float kMinValueScale = 8.673617379884035e-19f;  // 2^-60: smaller value scales count as this
 
-// PARTS: e4m3 parts of Q (and P): 2 or 3; 0 = 16-bit cache (weights only).
+// PARTS: e4m3 parts of Q, 2 or 3; 0 = 16-bit cache (weights only).
 // ROWS: query rows of a group, G groups, W streams (softmax warpgroups).
 template <int PARTS_, int ROWS_, int G_, int W_, bool ATTEND_>
 struct Shape {

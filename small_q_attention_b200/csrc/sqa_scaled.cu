@@ -439,9 +439,6 @@ __device__ void issue_values(const ScaledTcParams& p, const Schedule& sch, const
 }
 
 // ------------------------------------------------------------------ softmax warps (128 threads)
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[2]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(taddr));
-}
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[4]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])

@@ -194,6 +194,8 @@ __global__ void __launch_bounds__(T, 512 / T) sqa_cache_evict_kernel(const Evict
   }
   if (h == 0 && rank == 0 && tid == 0) p.new_lens[b] = p.budget;
 
+  __syncwarp();
+  if (C > 1) cluster_arrive_all();  // this CTA runs: the others may store into its shared memory
   // ---- 1. the key of the last score that is kept
   const int middle = len - p.sinks - p.recent;  // candidates
   const int want = p.budget - p.sinks - p.recent;
@@ -250,6 +252,7 @@ __global__ void __launch_bounds__(T, 512 / T) sqa_cache_evict_kernel(const Evict
     sh.warp_b[warp] = hi;
   }
   __syncthreads();
+  if (C > 1) cluster_wait_all();  // every CTA of the cluster runs
   if (tid < C) {  // this slice's range to CTA `tid`
     lo = sh.warp_a[0];
     hi = sh.warp_b[0];

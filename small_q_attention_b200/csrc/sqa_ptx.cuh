@@ -500,6 +500,11 @@ __host__ __device__ constexpr uint32_t mma_idesc_f16(int m, int n, bool a_mn_maj
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Its halves: work that touches no other CTA's shared memory may lie between them.
+__device__ __forceinline__ void cluster_arrive_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait_all() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // The address of the same shared-memory location in the CTA of cluster rank `rank`.
 __device__ __forceinline__ uint32_t cluster_map(uint32_t saddr, uint32_t rank) {
   uint32_t r;

@@ -243,6 +243,17 @@ def test_evict_again_and_again(sqa):
         c.update({k: g[k].cpu() for k in ("k", "v", "ks", "vs", "scores")}, seq_lens=new.cpu())
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, F8], ids=["16bit", "e4m3"])
+def test_evict_slices_of_unequal_work(sqa, dtype):
+    """CTAs of a cluster whose slices hold nothing or one score exchange their ranges at once, before the
+    others may have read theirs; the call runs back to back, so that clusters start at every moment."""
+    c = evict_case([65, 300, 66], 2, dtype, seed=11)
+    for _ in range(20):
+        g = gpu(c)
+        new, kept = evict(sqa, g, 64, recent=32, sinks=30)
+        assert_evicted(g, c, new, kept, 64, recent=32, sinks=30)
+
+
 def test_evict_bad_metadata(sqa):
     """Bad sequences are left, whole; the others are cut."""
     c = evict_case([100, 90, 80, 70, 60], 2, F8, seed=6)

@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(256) sqa_cache_append_kernel(const AppendParam
     int page = 0;
     if (len < p.q_len) {
       err = 4u;  // SQA_DEV_SEQ_TOO_SHORT: the whole sequence is skipped
-    } else if ((len + kPageSize - 1) / kPageSize > p.max_pages) {
+    } else if (page_count(len) > p.max_pages) {
       err = 2u;  // SQA_DEV_SEQ_TOO_LONG: the whole sequence is skipped
     } else {
       page = __ldg(p.block_tables + (size_t)b * p.max_pages + t / kPageSize);

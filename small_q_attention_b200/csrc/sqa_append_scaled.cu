@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(256, kBlocksPerSm) sqa_cache_append_scaled_ker
       bad |= 4u;  // SQA_DEV_SEQ_TOO_SHORT: the whole sequence is skipped
       continue;
     }
-    if ((len + kPageSize - 1) / kPageSize > p.max_pages) {
+    if (page_count(len) > p.max_pages) {
       bad |= 2u;  // SQA_DEV_SEQ_TOO_LONG: the whole sequence is skipped
       continue;
     }

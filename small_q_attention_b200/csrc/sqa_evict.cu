@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(T, 512 / T) sqa_cache_evict_kernel(const Evict
 
   // Sequences that stay as they are: short ones, and those whose length or pages are bad.
   unsigned int err = 0;
-  const int pages = (max(len, 0) + kPageSize - 1) / kPageSize;
+  const int pages = page_count(len);
   if (len < 0) err = 4u;                 // SQA_DEV_SEQ_TOO_SHORT
   else if (pages > p.max_pages) err = 2u;  // SQA_DEV_SEQ_TOO_LONG
   else if (len > p.budget) {

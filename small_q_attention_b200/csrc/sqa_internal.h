@@ -10,6 +10,11 @@ namespace sqa {
 
 constexpr int kHeadDim = 128;
 constexpr int kPageSize = 16;
+#ifdef __CUDACC__
+// Pages of `len` tokens; none for a negative length.  Lengths come from the user's device memory: rounding
+// up by an addition would wrap for the largest, and pass them as short.
+__host__ __device__ constexpr int page_count(int len) { return len > 0 ? (len - 1) / kPageSize + 1 : 0; }
+#endif
 constexpr int kGroup = 4;                 // query heads per KV head
 constexpr int kConsumerWarps = 4;
 constexpr int kThreads = (kConsumerWarps + 1) * 32;  // + one TMA producer warp

@@ -40,7 +40,7 @@ __device__ __forceinline__ int load_len(const SplitKvParams& p, int b) {
 template <bool kSpec = false>
 __device__ __forceinline__ int seq_pages(const SplitKvParams& p, int b) {
   const int len = max(load_len<kSpec>(p, b), 0);
-  return min((len + kPageSize - 1) / kPageSize, p.max_pages);
+  return min(page_count(len), p.max_pages);
 }
 
 __device__ __forceinline__ void next_segment(const SplitKvParams& p, SegWalk& w) {
@@ -81,7 +81,7 @@ __device__ __forceinline__ Schedule compute_schedule(const SplitKvParams& p) {
     int pages = 0;
     if (b < p.batch) {
       const int len = load_len<kSpec>(p, b);
-      pages = min((max(len, 0) + kPageSize - 1) / kPageSize, p.max_pages);
+      pages = min(page_count(len), p.max_pages);
       if (len > p.max_pages * kPageSize) fl |= 2u;                 // SQA_DEV_SEQ_TOO_LONG
       if (p.out != nullptr && len < p.q_len) fl |= 4u;             // SQA_DEV_SEQ_TOO_SHORT
     }
@@ -230,7 +230,7 @@ __device__ __forceinline__ Schedule even_schedule(const SplitKvParams& p) {
     int pg = 0;
     if (i < p.batch) {
       const int len = load_len<kSpec>(p, i);
-      pg = min((max(len, 0) + kPageSize - 1) / kPageSize, p.max_pages);
+      pg = min(page_count(len), p.max_pages);
       if (len > p.max_pages * kPageSize) flags |= 2u;      // SQA_DEV_SEQ_TOO_LONG
       if (p.out != nullptr && len < p.q_len) flags |= 4u;  // SQA_DEV_SEQ_TOO_SHORT
     }
@@ -289,7 +289,7 @@ __device__ __forceinline__ int2 segment_pieces(const int32_t* seq_lens, int batc
   auto pages_of = [&](int i) {
     if (i >= batch) return 0;
     const int len = max(__ldcg(seq_lens + i), 0);
-    return min((len + kPageSize - 1) / kPageSize, max_pages);
+    return min(page_count(len), max_pages);
   };
   int cached[kCachedChunks];
 #pragma unroll
@@ -336,7 +336,7 @@ __device__ __forceinline__ int2 segment_pieces(const int32_t* seq_lens, int batc
 __device__ __forceinline__ int2 aligned_segment_pieces(const int32_t* seq_lens, int max_pages, int hkv, int k,
                                                        int b, int h) {
   const int len = max(__ldcg(seq_lens + b), 0);
-  const int pages = min((len + kPageSize - 1) / kPageSize, max_pages);
+  const int pages = min(page_count(len), max_pages);
   if (pages == 0) return make_int2(0, 0);
   const int per = even_split_pages(pages, k, false);
   return make_int2((b * hkv + h) * (k + 1), (pages + per - 1) / per);

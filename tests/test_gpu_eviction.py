@@ -254,6 +254,19 @@ def test_evict_slices_of_unequal_work(sqa, dtype):
         assert_evicted(g, c, new, kept, 64, recent=32, sinks=30)
 
 
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 31 - 15, 2 ** 31 - 16])
+def test_lengths_near_the_end_of_int32(sqa, length):
+    """Rounded up to pages, they pass 32 bits: too long all the same, never short."""
+    c = evict_case([100, 90], 2, F8, seed=12)
+    c["seq_lens"] = torch.tensor([length, 90], dtype=torch.int32)
+    g = gpu(c)
+    with pytest.raises(ValueError, match="exceeds"):
+        evict(sqa, g, 32, check=True)
+    g = gpu(c)
+    new, kept = evict(sqa, g, 32)
+    assert_evicted(g, c, new, kept, 32)
+
+
 def test_evict_bad_metadata(sqa):
     """Bad sequences are left, whole; the others are cut."""
     c = evict_case([100, 90, 80, 70, 60], 2, F8, seed=6)

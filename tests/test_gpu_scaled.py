@@ -466,6 +466,26 @@ def test_append_bad_metadata(sqa):
     assert_appended(g, c)
 
 
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 31 - 15, 2 ** 31 - 16])
+def test_lengths_near_the_end_of_int32(sqa, length):
+    """Rounded up to pages, they pass 32 bits: too long all the same, never short."""
+    c = append_case(4, [20, 40, 100], 2, torch.float16, seed=8)
+    c["seq_lens"] = torch.tensor([20, length, 100], dtype=torch.int32)
+    g = to_gpu(c)
+    with pytest.raises(ValueError, match="exceeds"):
+        append(sqa, g, check=True)
+    assert_appended(g, c)
+    a = scaled_case(4, [40, 100], hkv=2, seed=8)
+    g = to_gpu(a)
+    full = 16 * g["table"].shape[1]
+    with pytest.raises(ValueError, match="exceeds"):
+        attend(sqa, dict(g, seq_lens=torch.tensor([40, length], dtype=torch.int32, device="cuda")), check=True)
+    ok = attend(sqa, g)[0]
+    clamped = attend(sqa, dict(g, seq_lens=torch.tensor([40, length], dtype=torch.int32, device="cuda")))[0]
+    torch.cuda.synchronize()
+    assert full >= 100 and torch.equal(ok[0], clamped[0])
+
+
 def test_append_strided_pool_and_refusals(sqa):
     c = append_case(6, [30, 6, 77], 4, torch.float16, seed=5)
     g = to_gpu(c)

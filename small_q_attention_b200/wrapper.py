@@ -40,7 +40,10 @@ class PagedMTPAttention:
     >>> out = attn.run(q, k_cache, v_cache, block_tables, seq_lens, out=out)   # graph-capturable
 
     ``plan`` may be called again for another shape; it reallocates only when the
-    new plan needs a larger workspace.
+    new plan needs a larger workspace, and a run with ``scores`` only when its
+    log-sum-exp (and fp32 rows) outgrow the kept ones.  A captured graph uses the memory it
+    was captured with: capture the largest plan first.  Graphs captured from one object
+    share that memory and must not be replayed at the same time.
     """
 
     def __init__(self, device: torch.device | int | None = None, *, kernel: int = 0):
@@ -53,6 +56,8 @@ class PagedMTPAttention:
             raise ValueError("kernel must be 0 (auto), 1 (warp-level) or 2 (tcgen05)")
         self._kernel = kernel
         self._workspace: torch.Tensor | None = None
+        self._lse: torch.Tensor | None = None   # flat, for runs with scores; kept and grown like the workspace
+        self._rows: torch.Tensor | None = None
         self._shape = None
         self.selected_kernel = None
 
@@ -113,7 +118,6 @@ class PagedMTPAttention:
         self._max_seq_len, self._num_ctas, self._min_pages = max_seq_len, num_ctas, min_pages_per_cta
         self._kv_layout, self._sm_scale, self._out_scale = kv_layout, sm_scale, out_scale
         self._min_seq_len, self._cluster, self._scaled = min_seq_len, cluster, block_scaled
-        self._lse = self._rows = None
         self.selected_kernel = int(picked)
         return self
 
@@ -150,20 +154,22 @@ class PagedMTPAttention:
             raise ValueError("append_keys and append_values go together")
         if self._scaled != (key_scales is not None) or self._scaled != (value_scales is not None):
             raise ValueError("key_scales and value_scales go with plan(block_scaled=True), and with no other plan")
-        if scores is not None and self._lse is None:  # kept from run to run; call once before a capture
-            self._lse = torch.empty(query.shape[:3], dtype=torch.float32, device=self.device)
-            self._rows = None if self._scaled else torch.empty(query.shape, dtype=torch.float32, device=self.device)
+        lse = rows = None
+        if scores is not None:
+            lse, self._lse = self._kept(self._lse, query.shape[:3])
+            if not self._scaled:
+                rows, self._rows = self._kept(self._rows, query.shape)
         if self._scaled:
             if append_keys is not None:
                 cache_append_scaled(append_keys, append_values, key_cache, value_cache, key_scales, value_scales,
                                     block_tables, seq_lens, kv_layout=self._kv_layout)
             small_q_attention_scaled(query, key_cache, value_cache, key_scales, value_scales, block_tables, seq_lens,
                                      PAGE_SIZE, self._max_seq_len, out=out,
-                                     out_lse=self._lse if scores is not None else None, workspace=self._workspace,
+                                     out_lse=lse, workspace=self._workspace,
                                      num_ctas=self._num_ctas, check=check, kv_layout=self._kv_layout,
                                      sm_scale=self._sm_scale, out_scale=self._out_scale, min_seq_len=self._min_seq_len)
             if scores is not None:
-                self._accumulate(query, key_cache, block_tables, seq_lens, scores, key_scales)
+                self._accumulate(query, key_cache, block_tables, seq_lens, lse, scores, key_scales)
             return out
         if append_keys is not None:
             cache_append(append_keys, append_values, key_cache, value_cache, block_tables, seq_lens,
@@ -175,7 +181,7 @@ class PagedMTPAttention:
         if scores is None:
             a.out = out.data_ptr()
         else:  # the partial form writes the log-sum-exp too; its fp32 rows are rounded once, below
-            a.out_partial, a.out_lse = self._rows.data_ptr(), self._lse.data_ptr()
+            a.out_partial, a.out_lse = rows.data_ptr(), lse.data_ptr()
         ws = self._workspace
         with _on_device(self.device):
             code = _native.library().sqa_forward(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()),
@@ -185,12 +191,19 @@ class PagedMTPAttention:
             if check:
                 _raise_device_bits(read_device_status(ws.data_ptr(), clear=True, device=self.device))
         if scores is not None:
-            out.copy_(self._rows)
-            self._accumulate(query, key_cache, block_tables, seq_lens, scores, None)
+            out.copy_(rows)
+            self._accumulate(query, key_cache, block_tables, seq_lens, lse, scores, None)
         return out
 
-    def _accumulate(self, query, key_cache, block_tables, seq_lens, scores, key_scales):
-        accumulate_attention_weights(query, key_cache, block_tables, seq_lens, self._lse, scores, PAGE_SIZE,
+    def _kept(self, buffer, shape):
+        """fp32 of ``shape`` from a kept flat buffer, and that buffer, larger if need be."""
+        n = shape.numel()
+        if buffer is None or buffer.numel() < n:
+            buffer = torch.empty(n, dtype=torch.float32, device=self.device)
+        return buffer[:n].view(shape), buffer
+
+    def _accumulate(self, query, key_cache, block_tables, seq_lens, lse, scores, key_scales):
+        accumulate_attention_weights(query, key_cache, block_tables, seq_lens, lse, scores, PAGE_SIZE,
                                      self._max_seq_len, key_scales=key_scales, kv_layout=self._kv_layout,
                                      sm_scale=self._sm_scale, min_seq_len=self._min_seq_len)
 

@@ -168,6 +168,34 @@ def test_wrapper_step_is_the_operators_and_captures(sqa, scaled):
         attn.run(query, g["k"], g["v"], g["table"], lens, **({} if scaled else dict(key_scales=1, value_scales=1)))
 
 
+@pytest.mark.parametrize("scaled", [True, False], ids=["e4m3", "16bit"])
+def test_wrapper_graph_outlives_a_smaller_plan(sqa, scaled):
+    """A graph captured with scores keeps its memory when the object is planned again and run eagerly."""
+    dtype = torch.float16
+    g, h, other = (on_gpu(fresh(scaled, dtype)) for _ in range(3))
+    lens = torch.tensor([100, 37, 150], dtype=torch.int32).cuda()
+    query = step_inputs(1, Q, dtype)[0].cuda()
+    attn = sqa.PagedMTPAttention(torch.device("cuda", 0))
+    plan = lambda n: attn.plan(n, Q, HKV, g["k"].shape[0], WIDTH, 190, block_scaled=scaled)  # noqa: E731
+    scales = lambda s: dict(key_scales=s["ks"], value_scales=s["vs"])  # noqa: E731
+    out = torch.empty_like(query)
+    plan(BATCH)
+    attn.run(query, other["k"], other["v"], other["table"], lens, scores=other["scores"], **scales(other))  # warm up
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attn.run(query, g["k"], g["v"], g["table"], lens, out=out, scores=g["scores"], **scales(g))
+    kept = attn._lse.data_ptr()
+    plan(1)
+    attn.run(query[:1], other["k"], other["v"], other["table"][:1], lens[:1], scores=other["scores"], **scales(other))
+    plan(BATCH)
+    want = attn.run(query, h["k"], h["v"], h["table"], lens, scores=h["scores"], **scales(h))
+    assert attn._lse.data_ptr() == kept
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(g["scores"], h["scores"])
+
+
 def test_wrapper_plan_refusals(sqa):
     attn = sqa.PagedMTPAttention(torch.device("cuda", 0))
     with pytest.raises(RuntimeError, match="plan"):

@@ -41,12 +41,12 @@
 // warpgroup a block of 64 rows took 13.7k cycles, with two of 32 rows 6.9k, with four of 16
 // 3.8k; at 32 rows two beat four (237 against 248 us at 16 x 8 x 32768), and 16 rows a group beat 32
 // (237 / 241 us, fp16 243 / 290, for want of registers).  Two groups of a block share a product
-// (GP = 2, one read of K and V for both: 1 x 16 x 262144 230 -> 195 us in isolation).
+// (GP = 2, one read of K and V for both: 4 x 16 x 65536 230 -> 195 us).
 //
 // What bounds it.  q_len 1-4 run at 5.3-5.8 TB/s (q_len 2, 16 x 32768: 187 us for 1.07 GB), near what
-// 2 KB boxes of 128-byte rows reach.  Above, the softmax warps' latency chain does: at
-// q_len 8 (235 us) leaving out P, the scores and the value products altogether still took
-// 200 us, single stages 5-11% each; the tensor pipe is 15% busy.
+// the loads alone reach (5.8 TB/s at q_len 4 with P, the scores and the value products left out).  Above it
+// is no one stage: at q_len 8, of 245 us, leaving out P saved 28, the scores 18, the value products
+// 38, all three 45; at q_len 16 (4 x 65536, before GP = 2), of 238 us, 29, 25, 60 and 79.
 //
 // Warps: 0 .. 4 W - 1 softmax (one token a thread), then one each for score products, value
 // products, TMA and page scales.  Work is cut into CTA ranges by sqa_schedule.cuh; pieces of a split

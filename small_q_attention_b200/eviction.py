@@ -1,7 +1,7 @@
 """Eviction from the paged cache by accumulated attention weight.
 
 Every cached token has a score per KV head, ``scores`` fp32 ``[num_pages, Hkv, 16]`` in
-the order of the cache's pages.  ``accumulate_attention_weights`` adds a step's attention
+the order of the cache's pages, 16-byte aligned for ``cache_evict``.  ``accumulate_attention_weights`` adds a step's attention
 weights to them, ``cache_evict`` keeps the tokens of the highest scores within a
 budget and compacts them in place.  Both take 16-bit caches and block-scaled FP8-E4M3
 caches.  Neither has an upstream counterpart.

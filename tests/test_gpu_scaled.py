@@ -7,7 +7,7 @@ p the probabilities and V the dequantised values:
 * a score is a sum of at most 3 x 128 products in fp32 (the query enters as at most
   three exact parts): off by at most 384 * 2^-24 * sum |q k|, and so is log2's input;
   the exponential adds 2^-22: relative error d of p, once in the numerator, once in the sum;
-* p enters the second product with 12 significant bits for fp16 queries (2^-12) and 8
+* p enters the second product with at least 12 significant bits for fp16 queries (2^-12) and 8
   for bf16 (2^-8 counts twice the rounding of 2^-9), relative, and values below 2^-18
   (bf16; 2^-22 for fp16) of a row's largest p |v| may be lost, each token at most once.
 """

@@ -10,24 +10,29 @@
 // q_len of 4 fills 16 of 128 lanes).
 //
 // Precision.  The tensor core reads the e4m3 K and V as they are (kind::f8f6f4 wants 8-bit
-// operands on both sides).  Q and P enter as PARTS e4m3 numbers each, x = x0 + x1 / 32 +
-// x2 / 1024, each the e4m3 rounding of what the parts before it left (4 significant bits a
+// operands on both sides).  Q and P enter as sums of e4m3 numbers, x = x0 + x1 / 32 +
+// x2 / 1024 .., each the e4m3 rounding of what the parts before it left (4 significant bits a
 // part).  The parts are extra columns of the N side (free: an M = 128 product of few columns
 // is bound by reading A) with their own fp32 accumulators, joined at read-out, so that a
 // low part has its own exponent range.  Two parts hold a bf16 query exactly (8 bits), three an fp16
 // query (11 bits).  Q is first scaled by the power of two that brings the largest finite
-// magnitude of the head's rows into [128, 256); a row far below that keeps its bits down to 2^-15
-// (bf16) or 2^-20 (fp16) of the largest.  P has three parts: 2^-13 of it, and 2^-20 absolutely
-// with a row's largest P between 2^-1 and 2^8.
+// magnitude of the head's rows into [128, 256); there the smallest part resolves 2^-15 (bf16) or 2^-20
+// (fp16), which is 2^-22 or 2^-27 of that magnitude, and rows far below it lose bits under that.
+// P has four parts, the last one 2^20 times too large: P is held to 2^-13 of it, below 2^-11 to
+// 2^-24, of which no more than 2^-4 of P, and lost only below 2^-30.  That matters for a row
+// that one token dominates, where the many others lie 2^-19 and further below it and still add up:
+// with three parts they left the numerator (a tail of 0.26 came out as 0.17 or 0).  Such a row's
+// base is chosen so that they lie higher (kRest).  The fourth part fits in the columns that 16 rows
+// leave unused.
 //
 // Softmax.  A row keeps a base; a score with its value scale, y = c ks (q . k) + log2 vs, enters as
 // P = 2^(y - base), and the denominator sums P / vs.  The value scale is thus inside the running
 // maximum, and P keeps its e4m3 range whatever the pages' value scales are.  Bases are set from the
-// first block to its maxima + 1 and raised when some y exceeds its base by more than 8 (one
+// first block to its maxima + 1 (less where one token dominates) and raised when some y exceeds its base by more than 8 (one
 // barrier with an or-reduction a block finds that out; then every row whose block maximum passed
 // its old one is raised, and l and O are rescaled).  Raising costs a block as much again, and on
 // random data with 1% of fourfold tokens it came in every second to fifth block with 3 to 6 bits
-// of slack: hence 9, which the third part of P leaves room for.  Masked tokens and tokens behind
+// of slack: hence 9, which the low parts of P leave room for.  Masked tokens and tokens behind
 // the sequence have y = -inf by selection, so NaN in their K does not matter; V rows behind the
 // sequence are zeroed in shared memory, and a NaN in the V of a draft token is zeroed and
 // remembered, as only the rows that see the token get it.
@@ -75,8 +80,12 @@ constexpr int kBlockPages = 8;
 constexpr int kBlock = kBlockPages * kPageSize;  // 128 tokens: the M side
 constexpr int kTileBytes = kBlock * 128;         // K or V of a block (e4m3), or one half of 16-bit K
 constexpr int kMetaSlots = 8;
-constexpr int kPParts = 3;                       // e4m3 parts of a probability
+constexpr int kPParts = 4;                       // e4m3 parts of a probability: P = p0 + p1 / 32 + p2 / 2^10 + p3 / 2^20
+constexpr float kLastPart = 1024.f;              // of p3 against p2
 constexpr float kRaise = 8.f, kHead = -1.f;      // raise a base that a score exceeds by 2^8, to 2 times the maximum
+// A row that one token dominates keeps the rest at 2^-12 or more, as far as the largest P may go for it: 2^7 in a
+// stream's first block, 2^4 later, where the next larger token would have the base raised again.
+constexpr float kRest = 12.f, kTopFirst = 7.f, kTopLater = 4.f;
 constexpr float kLn2f = 0.6931471805599453f;
 constexpr float kMinValueScale = 8.673617379884035e-19f;  // 2^-60: smaller value scales count as this
 
@@ -93,7 +102,7 @@ struct Shape {
   static constexpr int UNITS = G / GP;                        // products of a block, each for GP streams
   static constexpr int SN = GP * N;
   static constexpr int STRIDE = SN <= 16 ? 16 : SN <= 32 ? 32 : SN <= 64 ? 64 : 128;  // TMEM columns of a score slot
-  static constexpr int PROW = 64;                             // bytes of a token's P in a group: three parts of 16 rows
+  static constexpr int PROW = 64;                             // bytes of a token's P in a group: four parts of 16 rows
   static constexpr int PPITCH = GP * PROW;                    // and of its operand row
   static constexpr int PBYTES = kBlock * PPITCH;
   static constexpr int LANES = W / GP;                        // streams of products
@@ -469,15 +478,17 @@ __device__ __forceinline__ void softmax_sync() {
   named_bar_sync(1 + S::W, S::SOFTMAX);
 }
 
-// The three e4m3 parts of two probabilities below 2^8.  Differences of a number and its rounding
-// are exact; the first one is taken in fp32 and rounded to fp16 (2^-16 of P).
-__device__ __forceinline__ void split_p(float x0, float x1, uint32_t (&out)[3]) {
-  const __half2 k32 = __floats2half2_rn(32.f, 32.f);
+// The four e4m3 parts of two probabilities below 2^8.  Differences of a number and its rounding
+// are exact; 32 times the first one is taken in fp32 and rounded to fp16 (2^-16 of P, and 2^-30).  The last part
+// saturates above P = 16, where the first three hold P to 2^-13.
+__device__ __forceinline__ void split_p(float x0, float x1, uint32_t (&out)[kPParts]) {
   out[0] = e4m3x2_of_floats(x0, x1);
-  const float2 f = __half22float2(half2_of_e4m3x2(out[0]));
-  const __half2 h = __hmul2(__floats2half2_rn(x0 - f.x, x1 - f.y), k32);
+  const float2 f = __half22float2(__hmul2(half2_of_e4m3x2(out[0]), __floats2half2_rn(-32.f, -32.f)));
+  const __half2 h = __floats2half2_rn(fmaf(x0, 32.f, f.x), fmaf(x1, 32.f, f.y));
   out[1] = e4m3x2_of_half2(h);
-  out[2] = e4m3x2_of_half2(__hmul2(__hsub2(h, half2_of_e4m3x2(out[1])), k32));
+  const __half2 g = __hmul2(__hsub2(h, half2_of_e4m3x2(out[1])), __floats2half2_rn(32.f, 32.f));
+  out[2] = e4m3x2_of_half2(g);
+  out[3] = e4m3x2_of_half2(__hmul2(__hsub2(g, half2_of_e4m3x2(out[2])), __floats2half2_rn(kLastPart, kLastPart)));
 }
 
 // PARTS e4m3 parts of four numbers, exact differences: x = part 0 + part 1 / 32 + part 2 / 1024.
@@ -796,8 +807,14 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
         if (lane % (32 / ROWS) == 0) wred[warp * ROWS + lane / (32 / ROWS)] = m;
         group_sync(stream);
         if (tid < ROWS) {
-          const float m4 = fmaxf(fmaxf(wred[tid], wred[ROWS + tid]), fmaxf(wred[2 * ROWS + tid], wred[3 * ROWS + tid]));
-          const float d = (m4 > kHead || (first && m4 != -INFINITY)) ? m4 - kHead : 0.f;
+          const float w0 = wred[tid], w1 = wred[ROWS + tid], w2 = wred[2 * ROWS + tid], w3 = wred[3 * ROWS + tid];
+          const float m4 = fmaxf(fmaxf(w0, w1), fmaxf(w2, w3));
+          const float rest = fminf(fminf(w0, w1), fminf(w2, w3));  // a token that dominates is in one of the warps
+          float d = 0.f;
+          if (m4 > kHead || (first && m4 != -INFINITY)) {
+            d = fmaxf(m4 - (first ? kTopFirst : kTopLater), fminf(m4 - kHead, rest + kRest));
+            if (!first) d = fmaxf(d, 0.f);
+          }
           delta[tid] = d;
           base[tid] += d;
         }
@@ -939,7 +956,8 @@ __device__ void attend(const ScaledTcParams& p, const Schedule& sch, const Smem<
         for (int r = 0; r < kChunk; ++r) {
           float x = __uint_as_float(raw[i][kPParts - 1][r]);
 #pragma unroll
-          for (int j = kPParts - 2; j >= 0; --j) x = fmaf(x, 1.f / 32.f, __uint_as_float(raw[i][j][r]));
+          for (int j = kPParts - 2; j >= 0; --j)
+            x = fmaf(x, j == kPParts - 2 ? 1.f / kLastPart : 1.f / 32.f, __uint_as_float(raw[i][j][r]));
           const float f = sm.delta(i * G + g)[r0 + r];
           if (f != 0.f) o[r] = fmaf(x, f, o[r]);  // a stream without tokens may hold anything
         }

@@ -58,7 +58,8 @@ def small_q_attention_scaled(query, key_cache, value_cache, key_scales, value_sc
     ``[0, 2**60]`` (those below ``2**-60`` count as ``2**-60``); key scales must be finite.  Returns the rows in the query's type (or into ``out``, which may also be fp32: the
     rows before their rounding, for :func:`merge_partials`), and with ``return_lse`` also the
     fp32 natural-log log-sum-exp ``[batch, q_len, Hq]`` (-inf for a row that sees no token), which
-    :func:`accumulate_attention_weights` takes.  The other arguments are those of
+    :func:`accumulate_attention_weights` takes.  Probabilities keep 13 bits, and tokens down to ``2**-29`` of a
+    row's largest ``p * value scale`` count.  The other arguments are those of
     ``small_q_attention`` and ``small_q_attention_partial``.
 
     Without ``workspace``, eager calls share one per (device, stream) and calls under CUDA-graph

@@ -321,13 +321,14 @@ SQA_API int sqa_forward_scaled(const sqa_args* args, const sqa_scales* scales, v
 /* ---- Accumulated attention weight, and eviction by it ----
  * scores: fp32 [num_pages, num_kv_heads, 16], one value per cached token and KV head.
  * With w(b, h, t) = the sum over the rows (q_len draft tokens x 4 query heads) that see
- * token t of exp(sm_scale * q.k_t - lse[row]): the last q_len tokens of a sequence (new
- * in this step) get scores = w, the earlier ones scores += w; slots behind the sequence
- * are left.  args: query, key_cache (16-bit of args->dtype, or e4m3 with `scales`, of
+ * token t of exp(sm_scale * q.k_t - lse[row]): the last q_len tokens of the sequence (new
+ * in this step) get scores = w, the earlier ones scores += w; slots behind the tokens held
+ * are left.  A shard's mask_lens tell where the whole sequence ends: t is new from
+ * mask_lens[b] - q_len on, so a shard may hold none or some of them.  args: query, key_cache (16-bit of args->dtype, or e4m3 with `scales`, of
  * which only `key` is read), block_tables, seq_lens, mask_lens and sm_scale as for
  * sqa_forward; value_cache and the outputs are not used.  lse: fp32 [batch, q_len,
- * num_q_heads], the natural-log log-sum-exp that the step's attention returned (a
- * row of -inf counts nothing).  The SQA_DEV_* bits are ORed into *status, a device word.
+ * num_q_heads], the natural-log log-sum-exp of the step's attention over the whole sequence
+ * (of shards: the merged one, not the shard's own; a row of -inf counts nothing).  The SQA_DEV_* bits are ORed into *status, a device word.
  * Pages must not be shared between sequences.  Asynchronous on `stream`. */
 SQA_API int sqa_accumulate_weights(const sqa_args* args, const float* lse, const sqa_scales* scales, float* scores,
                                    uint32_t* status, void* stream);

@@ -131,7 +131,7 @@ def weights_reference(q, kc, ks, table, lens, lse, scores, *, mask_lens=None, sm
             for t in range(n):
                 page = int(table[b, t // PAGE])
                 old = scores[page, h, t % PAGE]
-                scores[page, h, t % PAGE] = w[t] if t >= int(lens[b]) - q_len else old + w[t]
+                scores[page, h, t % PAGE] = w[t] if t >= whole - q_len else old + w[t]
     return scores, dot
 
 

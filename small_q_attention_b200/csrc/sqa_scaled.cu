@@ -651,12 +651,13 @@ __device__ __forceinline__ float reduce_rows(const float (&in)[ROWS]) {
 // What the softmax threads know of a piece.
 struct Piece {
   int len, first;  // tokens held; tokens that draft row 0 sees (its limit: mask - q_len + 1)
+  int fresh;       // the step's own tokens, the last q_len of the whole sequence, start here
 };
 
 __device__ __forceinline__ Piece piece_of(const SplitKvParams& p, const SegWalk& w) {
   const int raw = __ldg(p.seq_lens + w.b);
   const int whole = p.mask_lens ? __ldg(p.mask_lens + w.b) : raw;
-  return Piece{min(raw, w.pages * kPageSize), whole - p.q_len + 1};
+  return Piece{min(raw, w.pages * kPageSize), whole - p.q_len + 1, whole - p.q_len};
 }
 
 // t = y - base of a unit's rows, and their largest; `release` is called once the scores are in registers.
@@ -1022,7 +1023,6 @@ __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const Smem<S
   for_pieces(p.s, sch, [&](const SegWalk& w, int, int n) {
     const int seg_end = w.seg_start + w.pages;
     const Piece piece = piece_of(p.s, w);
-    const int fresh = __ldg(p.s.seq_lens + w.b) - p.s.q_len;  // tokens from here on are new
     if (pc == 0) {
       QItem<S> q;
       load_q<S, BF>(p, sm, w.b, w.h, q);
@@ -1043,7 +1043,7 @@ __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const Smem<S
       const int id = __float_as_int(meta.w);
       const bool held = tid < np * kPageSize && tok < piece.len;
       float* const at = p.scores + ((size_t)max(id, 0) * p.s.hkv + w.h) * kPageSize + (tid & 15);
-      const float old = (held && id >= 0 && tok < fresh) ? __ldcg(at) : 0.f;  // in flight during the score product
+      const float old = (held && id >= 0 && tok < piece.fresh) ? __ldcg(at) : 0.f;  // in flight during the score product
       const bool masked = np < kBlockPages || tok0 + kBlock > piece.first || tok0 + kBlock > piece.len;
       const int late = held ? tok - piece.first : 0x7fffffff;
       float sum = 0.f;

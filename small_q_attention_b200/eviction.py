@@ -22,9 +22,12 @@ def accumulate_attention_weights(query, key_cache, block_tables, seq_lens, lse, 
     The weight of token ``t`` for KV head ``h`` is the sum over the rows (``q_len`` draft tokens x 4
     query heads) that see it of ``exp(sm_scale * q.k_t - lse[row])``, with ``lse`` ``[batch, q_len, Hq]``
     from the step's attention (``small_q_attention_partial`` or ``small_q_attention_scaled``
-    with ``return_lse``; same ``query``, cache, ``mask_lens`` and ``sm_scale``).  The last ``q_len``
+    with ``return_lse``; same ``query``, cache and ``sm_scale``).  The last ``q_len``
     tokens of a sequence are new in this step: their scores are set to their weight, whatever
-    their slots held; the earlier ones are added to.  Slots behind the sequence are left.
+    their slots held; the earlier ones are added to.  Slots behind the tokens held are left.
+    A shard of a longer sequence passes its ``mask_lens`` as it does to the attention (the whole
+    length less the shard's offset), which also tells which of its tokens, if any, are new, and
+    the merged log-sum-exp of all shards (``merge_partials`` with ``return_lse``), not its own.
     ``key_scales`` belong to an FP8-E4M3 cache.  Pages must not be shared between sequences.
     ``check=True`` synchronises and raises as ``small_q_attention`` does.
     """

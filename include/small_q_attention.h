@@ -64,7 +64,9 @@ typedef enum sqa_status {
 /* Bits of the device status word (sticky until cleared by sqa_read_device_status). */
 #define SQA_DEV_TIMEOUT 1u         /* a bounded wait gave up; output is not valid       */
 #define SQA_DEV_SEQ_TOO_LONG 2u    /* seq_lens[b] > 16 * max_pages: clamped to the table */
-#define SQA_DEV_SEQ_TOO_SHORT 4u   /* seq_lens[b] < q_len (full mode only)              */
+#define SQA_DEV_SEQ_TOO_SHORT 4u   /* seq_lens[b] < q_len (full mode only; of a shard
+                                      that a block-scaled call or sqa_accumulate_weights gets
+                                      mask_lens for it is no error)                     */
 #define SQA_DEV_BAD_PAGE 8u        /* a page id outside [0, num_pages): read as page 0  */
 #define SQA_DEV_CHECK 16u          /* a -DSQA_DEBUG_CHECKS bounds check failed; the word
                                       after the status word holds (check << 24) | index  */

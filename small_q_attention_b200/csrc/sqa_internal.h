@@ -67,6 +67,7 @@ struct SplitKvParams {
                                 // a thread-block cluster of C CTAs, partials reduced through DSMEM
   int seg_split;                // tcgen05 kernel: 0, or k >= 2 = segment blockIdx.x / k split evenly over
                                 // k CTAs (no cluster), partials merged by the merge kernel
+  int shard_lens;               // seq_lens are a shard's: below q_len they are no error
 };
 
 struct MergeParams {

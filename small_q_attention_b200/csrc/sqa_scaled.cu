@@ -1252,6 +1252,7 @@ ScaledTcParams tc_params(const ScaledParams& p) {
   t.s.block_tables = p.block_tables;
   t.s.seq_lens = p.seq_lens;
   t.s.mask_lens = p.mask_lens;
+  t.s.shard_lens = p.mask_lens != nullptr;
   t.s.out = static_cast<__half*>(p.out);
   t.s.out_o = p.out_o;
   t.s.out_lse = p.out_lse;

@@ -83,7 +83,7 @@ __device__ __forceinline__ Schedule compute_schedule(const SplitKvParams& p) {
       const int len = load_len<kSpec>(p, b);
       pages = min(page_count(len), p.max_pages);
       if (len > p.max_pages * kPageSize) fl |= 2u;                 // SQA_DEV_SEQ_TOO_LONG
-      if (p.out != nullptr && len < p.q_len) fl |= 4u;             // SQA_DEV_SEQ_TOO_SHORT
+      if (p.out != nullptr && !p.shard_lens && len < p.q_len) fl |= 4u;  // SQA_DEV_SEQ_TOO_SHORT
     }
     return pages;
   };
@@ -232,7 +232,7 @@ __device__ __forceinline__ Schedule even_schedule(const SplitKvParams& p) {
       const int len = load_len<kSpec>(p, i);
       pg = min(page_count(len), p.max_pages);
       if (len > p.max_pages * kPageSize) flags |= 2u;      // SQA_DEV_SEQ_TOO_LONG
-      if (p.out != nullptr && len < p.q_len) flags |= 4u;  // SQA_DEV_SEQ_TOO_SHORT
+      if (p.out != nullptr && !p.shard_lens && len < p.q_len) flags |= 4u;  // SQA_DEV_SEQ_TOO_SHORT
     }
     int pre = (i < b) ? pg : 0;
 #pragma unroll

@@ -37,6 +37,27 @@ def test_shards_do_what_the_whole_does(sqa, q_len, n, cuts, scaled):
     assert_weights(g["scores"], c)
 
 
+@pytest.mark.parametrize("scaled", [False, True], ids=["16bit", "e4m3"])
+def test_a_shard_may_hold_fewer_tokens_than_the_step(sqa, scaled):
+    """check=True reports a length below q_len of a whole sequence, not of a shard."""
+    c = weight_case(4, [690], 2, torch.float16, scaled, seed=6)
+    g = gpu(c)
+    two, mask = (torch.tensor([2], dtype=torch.int32).cuda() for _ in range(2))
+    last = g["table"][:, 43:44].contiguous()
+    call = lambda **kw: sqa.accumulate_attention_weights(  # noqa: E731
+        g["query"], g["k"], last, two, g["lse"], g["scores"], 16, key_scales=g["ks"], check=True, **kw)
+    call(mask_lens=mask)
+    with pytest.raises(ValueError, match="at least q_len"):
+        call()
+    if scaled:
+        attend = lambda **kw: sqa.small_q_attention_scaled(  # noqa: E731
+            g["query"], g["k"], g["v"], g["ks"], g["vs"], last, two, 16, check=True, **kw)
+        for hints in (dict(), dict(num_ctas=3)):  # both schedules
+            attend(mask_lens=mask, **hints)
+            with pytest.raises(ValueError, match="at least q_len"):
+                attend(**hints)
+
+
 def test_shards_with_their_merged_log_sum_exp(sqa):
     """The step as shards run it: fp32 rows and log-sum-exps, their merge, then the weights; they sum to the rows."""
     c = weight_case(4, [1000], 2, torch.float16, True, seed=5)

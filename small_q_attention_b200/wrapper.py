@@ -169,7 +169,7 @@ class PagedMTPAttention:
                                      num_ctas=self._num_ctas, check=check, kv_layout=self._kv_layout,
                                      sm_scale=self._sm_scale, out_scale=self._out_scale, min_seq_len=self._min_seq_len)
             if scores is not None:
-                self._accumulate(query, key_cache, block_tables, seq_lens, lse, scores, key_scales)
+                self._accumulate(query, key_cache, block_tables, seq_lens, lse, scores, key_scales, check)
             return out
         if append_keys is not None:
             cache_append(append_keys, append_values, key_cache, value_cache, block_tables, seq_lens,
@@ -189,10 +189,13 @@ class PagedMTPAttention:
                                                 ctypes.c_void_p(_stream_handle(self.device)))
             _native.check(code, "sqa_forward")
             if check:
-                _raise_device_bits(read_device_status(ws.data_ptr(), clear=True, device=self.device))
+                bits = read_device_status(ws.data_ptr(), clear=True, device=self.device)
+                if scores is not None and bool((seq_lens < query.shape[1]).any()):
+                    bits |= _native.DEV_SEQ_TOO_SHORT  # the partial form takes a shard's lengths, any of them
+                _raise_device_bits(bits)
         if scores is not None:
             out.copy_(rows)
-            self._accumulate(query, key_cache, block_tables, seq_lens, lse, scores, None)
+            self._accumulate(query, key_cache, block_tables, seq_lens, lse, scores, None, check)
         return out
 
     def _kept(self, buffer, shape):
@@ -202,9 +205,9 @@ class PagedMTPAttention:
             buffer = torch.empty(n, dtype=torch.float32, device=self.device)
         return buffer[:n].view(shape), buffer
 
-    def _accumulate(self, query, key_cache, block_tables, seq_lens, lse, scores, key_scales):
+    def _accumulate(self, query, key_cache, block_tables, seq_lens, lse, scores, key_scales, check):
         accumulate_attention_weights(query, key_cache, block_tables, seq_lens, lse, scores, PAGE_SIZE,
-                                     self._max_seq_len, key_scales=key_scales, kv_layout=self._kv_layout,
+                                     self._max_seq_len, key_scales=key_scales, check=check, kv_layout=self._kv_layout,
                                      sm_scale=self._sm_scale, min_seq_len=self._min_seq_len)
 
     # ------------------------------------------------------------------ evict

@@ -155,7 +155,12 @@ class PagedMTPAttention:
         if self._scaled != (key_scales is not None) or self._scaled != (value_scales is not None):
             raise ValueError("key_scales and value_scales go with plan(block_scaled=True), and with no other plan")
         lse = rows = None
-        if scores is not None:
+        if scores is not None:  # refused before the append and the attention have run
+            if not self._scaled and key_cache.dtype == getattr(torch, "float8_e4m3fn", None):
+                raise ValueError("scores need 16-bit caches or plan(block_scaled=True): an FP8 cache with one scale has no weights")
+            if (not isinstance(scores, torch.Tensor) or scores.device != self.device or scores.dtype != torch.float32
+                    or scores.shape != (shape[3], shape[2], PAGE_SIZE) or not scores.is_contiguous()):
+                raise ValueError("scores must be a contiguous fp32 tensor [num_pages, Hkv, 16] on the planned device")
             lse, self._lse = self._kept(self._lse, query.shape[:3])
             if not self._scaled:
                 rows, self._rows = self._kept(self._rows, query.shape)

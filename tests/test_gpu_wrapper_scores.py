@@ -51,3 +51,36 @@ def test_checked_run_with_scores_reports_bad_metadata(sqa, scaled):
             assert torch.equal(g["scores"], before)
     attn.run(query, g["k"], g["v"], g["table"], lengths(100, Q, 150), scores=g["scores"], check=True, **scales(g))
     assert not torch.equal(g["scores"], before)
+
+
+def bytes_of(g):
+    return [g[k].view(torch.uint8).clone() for k in ("k", "v", "scores")]
+
+
+def test_scores_of_a_single_scale_fp8_plan_are_refused_before_the_step(sqa):
+    g = on_gpu(fresh(True, torch.float16))
+    query, *new = [x.cuda() for x in step_inputs(1, Q, torch.float16)]
+    attn = planned(sqa, g, False, cache_dtype=F8)
+    before, out = bytes_of(g), torch.full_like(query, 7.0)
+    lens = lengths(100, 37, 150)
+    new8 = [x.clamp(-448, 448).to(F8) for x in new]
+    with pytest.raises(ValueError, match="block_scaled"):
+        attn.run(query, g["k"], g["v"], g["table"], lens, out=out, append_keys=new8[0], append_values=new8[1], scores=g["scores"])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(before, bytes_of(g))) and (out == 7.0).all()
+    attn.run(query, g["k"], g["v"], g["table"], lens, out=out, append_keys=new8[0], append_values=new8[1], check=True)
+    assert not (out == 7.0).any()
+
+
+@SCALED
+def test_scores_of_the_wrong_kind_are_refused_before_the_step(sqa, scaled):
+    g = on_gpu(fresh(scaled, torch.float16))
+    query, *new = [x.cuda() for x in step_inputs(1, Q, torch.float16)]
+    attn = planned(sqa, g, scaled)
+    before, out = bytes_of(g), torch.full_like(query, 7.0)
+    for s in (g["scores"][:-1], g["scores"].double(), g["scores"].cpu(), g["scores"].transpose(0, 1), g["scores"][..., :8], 3):
+        with pytest.raises(ValueError, match="scores"):
+            attn.run(query, g["k"], g["v"], g["table"], lengths(100, 37, 150), out=out, append_keys=new[0], append_values=new[1],
+                     scores=s, **scales(g))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(before, bytes_of(g))) and (out == 7.0).all()

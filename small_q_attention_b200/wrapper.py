@@ -41,9 +41,9 @@ class PagedMTPAttention:
 
     ``plan`` may be called again for another shape; it reallocates only when the
     new plan needs a larger workspace, and a run with ``scores`` only when its
-    log-sum-exp (and fp32 rows) outgrow the kept ones.  A captured graph uses the memory it
-    was captured with: capture the largest plan first.  Graphs captured from one object
-    share that memory and must not be replayed at the same time.
+    log-sum-exp (and fp32 rows) outgrow the kept ones.  Outgrown memory is kept (each new buffer is
+    at least twice as large as the last), so a graph captured before can still be replayed.
+    Graphs captured from one object share its memory and must not be replayed at the same time.
     """
 
     def __init__(self, device: torch.device | int | None = None, *, kernel: int = 0):
@@ -58,6 +58,7 @@ class PagedMTPAttention:
         self._workspace: torch.Tensor | None = None
         self._lse: torch.Tensor | None = None   # flat, for runs with scores; kept and grown like the workspace
         self._rows: torch.Tensor | None = None
+        self._outgrown: list[torch.Tensor] = []  # captured graphs and calls in flight may still use them
         self._shape = None
         self.selected_kernel = None
 
@@ -113,7 +114,7 @@ class PagedMTPAttention:
             if picked < 0:
                 _native.check(-picked, "sqa_selected_kernel")
         if self._workspace is None or self._workspace.numel() < need:
-            self._workspace = torch.zeros(max(need, 1 << 16), dtype=torch.uint8, device=self.device)
+            self._workspace = self._grown(self._workspace, max(need, 1 << 16), torch.uint8)
         self._shape = (batch, q_len, num_kv_heads, num_pages, max_pages)
         self._max_seq_len, self._num_ctas, self._min_pages = max_seq_len, num_ctas, min_pages_per_cta
         self._kv_layout, self._sm_scale, self._out_scale = kv_layout, sm_scale, out_scale
@@ -207,8 +208,15 @@ class PagedMTPAttention:
         """fp32 of ``shape`` from a kept flat buffer, and that buffer, larger if need be."""
         n = shape.numel()
         if buffer is None or buffer.numel() < n:
-            buffer = torch.empty(n, dtype=torch.float32, device=self.device)
+            buffer = self._grown(buffer, n, torch.float32)
         return buffer[:n].view(shape), buffer
+
+    def _grown(self, buffer, n, dtype):
+        """A zeroed buffer of at least ``n`` elements in place of ``buffer``, which is kept."""
+        if buffer is not None:
+            self._outgrown.append(buffer)
+            n = max(n, 2 * buffer.numel())
+        return torch.zeros(n, dtype=dtype, device=self.device)
 
     def _accumulate(self, query, key_cache, block_tables, seq_lens, lse, scores, key_scales, check):
         accumulate_attention_weights(query, key_cache, block_tables, seq_lens, lse, scores, PAGE_SIZE,

@@ -84,3 +84,31 @@ def test_scores_of_the_wrong_kind_are_refused_before_the_step(sqa, scaled):
                      scores=s, **scales(g))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(before, bytes_of(g))) and (out == 7.0).all()
+
+
+@SCALED
+def test_graph_outlives_a_larger_plan(sqa, scaled):
+    """A graph captured on a small plan replays after larger plans have outgrown its memory and the allocator
+    has given out everything that was freed."""
+    g, h, other = (on_gpu(fresh(scaled, torch.float16)) for _ in range(3))
+    lens = lengths(100, 37, 150)
+    query = step_inputs(1, Q, torch.float16)[0].cuda()
+    attn = planned(sqa, g, scaled, batch=1)
+    attn.run(query[:1], other["k"], other["v"], other["table"][:1], lens[:1], scores=other["scores"], **scales(other))  # warm up
+    torch.cuda.synchronize()
+    graph, out = torch.cuda.CUDAGraph(), torch.empty_like(query[:1])
+    with torch.cuda.graph(graph):
+        attn.run(query[:1], g["k"], g["v"], g["table"][:1], lens[:1], out=out, scores=g["scores"], **scales(g))
+    used = [x.data_ptr() for x in (attn.workspace, attn._lse, attn._rows) if x is not None]
+    attn.plan(BATCH, Q, HKV, g["k"].shape[0], WIDTH, 190, block_scaled=scaled, num_ctas=2000)  # a larger workspace
+    attn.run(query, other["k"], other["v"], other["table"], lens, scores=other["scores"], **scales(other))
+    assert attn.workspace.data_ptr() != used[0] and attn._lse.data_ptr() != used[1]
+    torch.cuda.synchronize()
+    taken = [torch.full((n,), 0xA5, dtype=torch.uint8, device="cuda") for n in (512, 4096, 1 << 16, 1 << 18, 1 << 20) for _ in range(64)]
+    assert not {x.data_ptr() for x in taken} & set(used)
+    attn.plan(1, Q, HKV, g["k"].shape[0], WIDTH, 190, block_scaled=scaled)
+    want = attn.run(query[:1], h["k"], h["v"], h["table"][:1], lens[:1], scores=h["scores"], **scales(h))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(g["scores"], h["scores"])
+    assert all((x == 0xA5).all() for x in taken)

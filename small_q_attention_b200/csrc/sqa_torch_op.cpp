@@ -307,11 +307,13 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> forward_scaled(
     const at::Tensor& value_scales, const at::Tensor& block_tables, const at::Tensor& seq_lens, int64_t page_size,
     const c10::optional<at::Tensor>& mask_lens, int64_t max_seq_len, const c10::optional<at::Tensor>& out,
     const c10::optional<at::Tensor>& out_lse, bool return_lse, const c10::optional<at::Tensor>& workspace,
-    int64_t num_ctas, bool check, int64_t kv_layout, double sm_scale, double out_scale, int64_t min_seq_len) {
+    int64_t num_ctas, bool check, int64_t kv_layout, double sm_scale, double out_scale, int64_t min_seq_len,
+    int64_t cluster) {
   check_inputs(query, key_cache, value_cache, block_tables, seq_lens, page_size, mask_lens, kv_layout);
   TORCH_CHECK_VALUE(key_cache.scalar_type() == at::kFloat8_e4m3fn, "a block-scaled cache is FP8-E4M3");
   sqa_args a = fill_args(query, key_cache, value_cache, block_tables, seq_lens, mask_lens, max_seq_len, num_ctas, 0, 0,
-                         kv_layout, sm_scale, out_scale, min_seq_len, 0);
+                         kv_layout, sm_scale, out_scale, min_seq_len, cluster);
+  TORCH_CHECK_VALUE(cluster == 0 || cluster == 1, "cluster must be 0 or 1 for a block-scaled cache");
   const sqa_scales scales = fill_scales(key_scales, value_scales, key_cache, a.num_kv_heads);
   const at::Tensor o = out.has_value() ? *out : at::empty_like(query);
   TORCH_CHECK_VALUE(o.sizes() == query.sizes() && o.is_contiguous() && o.device() == query.device() &&
@@ -537,7 +539,7 @@ std::tuple<at::Tensor, at::Tensor> op_forward_scaled(const at::Tensor& query, co
                                                      int64_t kv_layout, double sm_scale, double out_scale) {
   auto [o, l] = forward_scaled(query, key_cache, value_cache, key_scales, value_scales, block_tables, seq_lens, page_size,
                                c10::nullopt, max_seq_len, c10::nullopt, c10::nullopt, true, c10::nullopt, 0, false,
-                               kv_layout, sm_scale, out_scale, 0);
+                               kv_layout, sm_scale, out_scale, 0, 0);
   return {o, *l};
 }
 
@@ -593,7 +595,12 @@ PYBIND11_MODULE(_sqa_torch, m) {
   m.doc() = "small-q paged MTP attention (B200): direct entry over the C ABI";
   m.def("forward", &forward, "causal paged MTP attention (see small_q_attention_b200.small_q_attention)");
   m.def("forward_partial", &forward_partial, "shard form: normalised fp32 O and natural-log LSE");
-  m.def("forward_scaled", &forward_scaled, "attention over a block-scaled e4m3 cache");
+  m.def("forward_scaled", &forward_scaled, "attention over a block-scaled e4m3 cache", py::arg("query"),
+        py::arg("key_cache"), py::arg("value_cache"), py::arg("key_scales"), py::arg("value_scales"),
+        py::arg("block_tables"), py::arg("seq_lens"), py::arg("page_size"), py::arg("mask_lens"),
+        py::arg("max_seq_len"), py::arg("out"), py::arg("out_lse"), py::arg("return_lse"), py::arg("workspace"),
+        py::arg("num_ctas"), py::arg("check"), py::arg("kv_layout"), py::arg("sm_scale"), py::arg("out_scale"),
+        py::arg("min_seq_len"), py::arg("cluster") = 0);
   m.def("append_scaled", &append_scaled, "quantising append to a block-scaled e4m3 cache");
   m.def("accumulate_weights", &accumulate_weights, "attention weight of every cached token, added to its score");
   m.def("cache_evict", &cache_evict, "keep the tokens of the highest scores within a budget, compacted in place");

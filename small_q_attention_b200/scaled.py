@@ -50,7 +50,7 @@ def small_q_attention_scaled(query, key_cache, value_cache, key_scales, value_sc
                              page_size: int, max_seq_len: int = 0, *, out=None, out_lse=None, return_lse: bool = False,
                              mask_lens=None, workspace=None, num_ctas: int = 0, check: bool = False,
                              kv_layout: str = "NHD", sm_scale: float | None = None, out_scale: float = 1.0,
-                             min_seq_len: int = 0):
+                             min_seq_len: int = 0, cluster: int = 0):
     """``small_q_attention`` over a block-scaled FP8-E4M3 cache.
 
     ``query`` is FP16 or BF16; K is ``key_scales * key_cache`` and V ``value_scales *
@@ -60,7 +60,8 @@ def small_q_attention_scaled(query, key_cache, value_cache, key_scales, value_sc
     fp32 natural-log log-sum-exp ``[batch, q_len, Hq]`` (-inf for a row that sees no token), which
     :func:`accumulate_attention_weights` takes.  Probabilities keep 13 bits, and tokens down to ``2**-29`` of a
     row's largest ``p * value scale`` count.  The other arguments are those of
-    ``small_q_attention`` and ``small_q_attention_partial``.
+    ``small_q_attention`` and ``small_q_attention_partial``; ``cluster`` is 0 or 1 (1: near-uniform
+    bounds do not make every segment split evenly).
 
     Without ``workspace``, eager calls share one per (device, stream) and calls under CUDA-graph
     capture take one from the graph's own memory pool.
@@ -71,7 +72,7 @@ def small_q_attention_scaled(query, key_cache, value_cache, key_scales, value_sc
         o, lse = _native.torch_ext().forward_scaled(
             query, key_cache, value_cache, key_scales, value_scales, block_tables, seq_lens, page_size, mask_lens,
             max_seq_len, out, out_lse, return_lse, workspace, num_ctas, check, _layout_code(kv_layout),
-            0.0 if sm_scale is None else sm_scale, out_scale, min_seq_len)
+            0.0 if sm_scale is None else sm_scale, out_scale, min_seq_len, cluster)
     except TypeError as e:
         raise ValueError(f"all inputs must be CUDA tensors ({e})") from None
     return (o, lse) if return_lse else o

@@ -173,7 +173,8 @@ class PagedMTPAttention:
                                      PAGE_SIZE, self._max_seq_len, out=out,
                                      out_lse=lse, workspace=self._workspace,
                                      num_ctas=self._num_ctas, check=check, kv_layout=self._kv_layout,
-                                     sm_scale=self._sm_scale, out_scale=self._out_scale, min_seq_len=self._min_seq_len)
+                                     sm_scale=self._sm_scale, out_scale=self._out_scale, min_seq_len=self._min_seq_len,
+                                     cluster=self._cluster)
             if scores is not None:
                 self._accumulate(query, key_cache, block_tables, seq_lens, lse, scores, key_scales, check)
             return out

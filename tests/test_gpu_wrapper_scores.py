@@ -112,3 +112,20 @@ def test_graph_outlives_a_larger_plan(sqa, scaled):
     torch.cuda.synchronize()
     assert torch.equal(out, want) and torch.equal(g["scores"], h["scores"])
     assert all((x == 0xA5).all() for x in taken)
+
+
+def test_block_scaled_plan_hands_on_its_cluster_option(sqa, monkeypatch):
+    """cluster=1 turns the even split off in the plan and in the run alike: with a workspace for one, not the other."""
+    import small_q_attention_b200.wrapper as w
+
+    g = on_gpu(fresh(True, torch.float16))
+    query = step_inputs(1, Q, torch.float16)[0].cuda()
+    seen = []
+    call = w.small_q_attention_scaled
+    monkeypatch.setattr(w, "small_q_attention_scaled", lambda *a, **kw: (seen.append(kw.get("cluster")), call(*a, **kw))[1])
+    outs = [planned(sqa, g, True, min_seq_len=180, cluster=c).run(query, g["k"], g["v"], g["table"], lengths(190, 185, 180),
+                                                                  check=True, **scales(g)) for c in (0, 1)]
+    assert seen == [0, 1]
+    assert torch.allclose(outs[0].float(), outs[1].float(), rtol=2e-3, atol=1e-3)
+    with pytest.raises(ValueError, match="cluster"):
+        call(query, g["k"], g["v"], g["ks"], g["vs"], g["table"], lengths(190, 185, 180), 16, cluster=2)

@@ -60,7 +60,8 @@ def cache_evict(key_cache, value_cache, scores, block_tables, seq_lens, budget: 
     ``kept`` (int32 ``[batch, Hkv, budget]``) holds the position each target came from, -1 behind
     the last.  Pages must not be shared between sequences or listed twice.  With ``check=True``
     the call synchronises and raises ``ValueError`` for a negative length or one beyond the page
-    table and ``IndexError`` for a page id outside the cache; those sequences are left.
+    table and ``IndexError`` for a page id outside the cache; those sequences are left, the others
+    are cut, and a ``new_lens`` that was passed in holds every sequence's length.
     """
     if not _cuda_available():
         raise RuntimeError("CUDA is required for the cache-eviction kernel")

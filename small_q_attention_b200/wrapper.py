@@ -228,11 +228,16 @@ class PagedMTPAttention:
     def evict(self, key_cache, value_cache, scores, block_tables, seq_lens, budget: int, *, recent: int = 0,
               sinks: int = 0, key_scales=None, value_scales=None, kept=None, check: bool = False):
         """Cut every sequence longer than ``budget`` tokens by its scores (``cache_evict``, in the planned
-        layout) and ``seq_lens`` with it, in place; returns the kept positions ``[batch, Hkv, budget]``."""
+        layout) and ``seq_lens`` with it, in place; returns the kept positions ``[batch, Hkv, budget]``.
+        Where ``check=True`` raises for some sequences, the others are cut all the same, lengths too."""
         if self._shape is None:
             raise RuntimeError("plan() has not been called")
-        lens, kept = cache_evict(key_cache, value_cache, scores, block_tables, seq_lens, budget, recent=recent,
-                                 sinks=sinks, key_scales=key_scales, value_scales=value_scales, kept=kept, check=check,
-                                 kv_layout=self._kv_layout)
-        seq_lens.copy_(lens)
-        return kept
+        if not isinstance(seq_lens, torch.Tensor):
+            raise ValueError("all inputs must be CUDA tensors")
+        lens = seq_lens.clone()
+        try:
+            return cache_evict(key_cache, value_cache, scores, block_tables, seq_lens, budget, recent=recent, sinks=sinks,
+                               key_scales=key_scales, value_scales=value_scales, new_lens=lens, kept=kept, check=check,
+                               kv_layout=self._kv_layout)[1]
+        finally:  # raised after the launch: the caches are cut; refused before it: lens is what it was
+            seq_lens.copy_(lens)

@@ -129,3 +129,24 @@ def test_block_scaled_plan_hands_on_its_cluster_option(sqa, monkeypatch):
     assert torch.allclose(outs[0].float(), outs[1].float(), rtol=2e-3, atol=1e-3)
     with pytest.raises(ValueError, match="cluster"):
         call(query, g["k"], g["v"], g["ks"], g["vs"], g["table"], lengths(190, 185, 180), 16, cluster=2)
+
+
+@SCALED
+def test_checked_eviction_that_raises_leaves_lengths_and_caches_in_step(sqa, scaled):
+    """One bad page: that sequence is left, the others are cut, and the lengths say so although the call raised."""
+    g, h = on_gpu(fresh(scaled, torch.float16)), on_gpu(fresh(scaled, torch.float16))
+    attn = planned(sqa, g, scaled)
+    bad = g["table"].clone()
+    bad[1, 2] = 10 ** 6
+    lens = lengths(150, 120, 40)
+    with pytest.raises(IndexError):
+        attn.evict(g["k"], g["v"], g["scores"], bad, lens, 64, recent=8, sinks=2, check=True, **scales(g))
+    assert lens.tolist() == [64, 120, 40]
+    new, _ = sqa.cache_evict(h["k"], h["v"], h["scores"], bad, lengths(150, 120, 40), 64, recent=8, sinks=2, **scales(h))
+    assert new.tolist() == [64, 120, 40] and all(torch.equal(a, b) for a, b in zip(bytes_of(g), bytes_of(h)))
+    for kw in (dict(recent=65), dict(sinks=-1), dict(key_scales=3)):  # refused before the launch
+        with pytest.raises(ValueError):
+            attn.evict(g["k"], g["v"], g["scores"], g["table"], lens, 64, **{**scales(g), **kw})
+    assert lens.tolist() == [64, 120, 40] and all(torch.equal(a, b) for a, b in zip(bytes_of(g), bytes_of(h)))
+    with pytest.raises(ValueError):
+        attn.evict(g["k"], g["v"], g["scores"], g["table"], None, 64, **scales(g))

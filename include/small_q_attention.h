@@ -352,8 +352,9 @@ typedef struct sqa_evict_args {
   float* scores;               /* [num_pages, num_kv_heads, 16], 16-byte aligned */
   const int32_t* block_tables; /* [batch, max_pages] */
   const int32_t* seq_lens;     /* [batch] */
-  int32_t* new_lens;           /* [batch]; not seq_lens itself */
-  int32_t* kept;               /* [batch, num_kv_heads, budget] */
+  int32_t* new_lens;           /* [batch] */
+  int32_t* kept;               /* [batch, num_kv_heads, budget]; new_lens and kept overlap neither each other nor
+                                  seq_lens or block_tables */
   uint32_t* status;            /* device status word or NULL */
   int32_t batch;
   int32_t num_kv_heads;

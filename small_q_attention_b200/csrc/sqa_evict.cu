@@ -578,6 +578,11 @@ cudaError_t launch_evict_shape(const EvictParams& p, int segments, cudaStream_t 
   return launch_evict<E, 256>(p, segments, 1, stream);
 }
 
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
+}
+
 }  // namespace
 }  // namespace sqa
 
@@ -603,7 +608,13 @@ extern "C" SQA_API int sqa_cache_evict(const sqa_evict_args* a, const sqa_scales
     return SQA_ERR_UNSUPPORTED;
   if (a->batch == 0) return SQA_OK;
   if (!a->key_cache || !a->value_cache || !a->scores || !a->block_tables || !a->seq_lens || !a->new_lens || !a->kept ||
-      a->new_lens == a->seq_lens || (scales && (!scales->key || !scales->value)))
+      (scales && (!scales->key || !scales->value)))
+    return SQA_ERR_INVALID_ARGUMENT;
+  // CTAs read lengths and tables while others write their results
+  const int64_t lens = 4 * (int64_t)a->batch, tables = lens * a->max_pages, kept = lens * a->num_kv_heads * a->budget;
+  if (overlap(a->new_lens, lens, a->seq_lens, lens) || overlap(a->new_lens, lens, a->block_tables, tables) ||
+      overlap(a->kept, kept, a->seq_lens, lens) || overlap(a->kept, kept, a->block_tables, tables) ||
+      overlap(a->kept, kept, a->new_lens, lens))
     return SQA_ERR_INVALID_ARGUMENT;
   const uintptr_t wide = reinterpret_cast<uintptr_t>(a->key_cache) | reinterpret_cast<uintptr_t>(a->value_cache) |
                          reinterpret_cast<uintptr_t>(a->scores);

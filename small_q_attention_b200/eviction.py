@@ -56,7 +56,7 @@ def cache_evict(key_cache, value_cache, scores, block_tables, seq_lens, budget: 
     block-scaled cache that is written gets the smallest power-of-two scale for the values it
     now holds.  Sequences of at most ``budget`` tokens are left as they are.
 
-    ``new_lens`` (int32, shaped like ``seq_lens``, another tensor) is ``min(seq_lens, budget)``;
+    ``new_lens`` (int32, shaped like ``seq_lens``, memory of its own) is ``min(seq_lens, budget)``;
     ``kept`` (int32 ``[batch, Hkv, budget]``) holds the position each target came from, -1 behind
     the last.  Pages must not be shared between sequences or listed twice.  With ``check=True``
     the call synchronises and raises ``ValueError`` for a negative length or one beyond the page

@@ -314,8 +314,9 @@ SQA_API int sqa_cache_append_scaled(const sqa_append_args* args, const sqa_scale
  * args as for sqa_forward with kv_dtype = SQA_KV_FP8_E4M3, except: with `out`, out_lse
  * may be given too (fp32 [batch, q_len, num_q_heads], as in partial mode); kernel must
  * be 0 and cluster 0 or 1.  Scales are finite; key scales have any sign, value scales lie
- * in [0, 2^60], and those below 2^-60 count as 2^-60.  Needs sqa_scaled_workspace_bytes() bytes of workspace, zeroed
- * once with sqa_workspace_init; the status word is read with sqa_read_device_status. */
+ * in [0, 2^30], and those below 2^-60 count as 2^-60: over these 90 bits every token whose
+ * probability is 2^-34 or more of the largest counts in the denominator.  Needs
+ * sqa_scaled_workspace_bytes() bytes of workspace, zeroed once with sqa_workspace_init; the status word is read with sqa_read_device_status. */
 SQA_API size_t sqa_scaled_workspace_bytes(const sqa_args* args, int device, int* status);
 SQA_API int sqa_forward_scaled(const sqa_args* args, const sqa_scales* scales, void* workspace,
                                size_t workspace_bytes, void* stream);

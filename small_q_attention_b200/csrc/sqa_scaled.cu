@@ -87,7 +87,9 @@ constexpr float kRaise = 8.f, kHead = -1.f;      // raise a base that a score ex
 // stream's first block, 2^4 later, where the next larger token would have the base raised again.
 constexpr float kRest = 12.f, kTopFirst = 7.f, kTopLater = 4.f;
 constexpr float kLn2f = 0.6931471805599453f;
-constexpr float kMinValueScale = 8.673617379884035e-19f;  // 2^-60: smaller value scales count as this
+// 2^-60: smaller value scales count as this.  With none over 2^30, the documented limit, y - base underflows (under
+// -126) only for tokens of 2^-35 and less of the largest probability; over 2^60 it would from 2^-5 on.
+constexpr float kMinValueScale = 8.673617379884035e-19f;
 
 // PARTS: e4m3 parts of Q, 2 or 3; 0 = 16-bit cache (weights only).
 // ROWS: query rows of a group, G groups, W streams (softmax warpgroups).

@@ -54,9 +54,10 @@ def small_q_attention_scaled(query, key_cache, value_cache, key_scales, value_sc
     """``small_q_attention`` over a block-scaled FP8-E4M3 cache.
 
     ``query`` is FP16 or BF16; K is ``key_scales * key_cache`` and V ``value_scales *
-    value_cache`` per page and head.  Value scales must lie in
-    ``[0, 2**60]`` (those below ``2**-60`` count as ``2**-60``); key scales must be finite.  Returns the rows in the query's type (or into ``out``, which may also be fp32: the
-    rows before their rounding, for :func:`merge_partials`), and with ``return_lse`` also the
+    value_cache`` per page and head.  Value scales must lie in ``[0, 2**30]`` (those below ``2**-60``,
+    an all-zero page's among them, count as ``2**-60``); key scales must be finite.  Returns the rows in
+    the query's type (or into ``out``, which may also be fp32: the rows before their rounding, for
+    :func:`merge_partials`), and with ``return_lse`` also the
     fp32 natural-log log-sum-exp ``[batch, q_len, Hq]`` (-inf for a row that sees no token), which
     :func:`accumulate_attention_weights` takes.  Probabilities keep 13 bits, and tokens down to ``2**-29`` of a
     row's largest ``p * value scale`` count.  The other arguments are those of

@@ -156,3 +156,42 @@ def test_the_same_call_gives_the_same_bits(sqa, q_len):
         want = attend(sqa, c).clone()
         for _ in range(10):
             assert torch.equal(attend(sqa, c), want)
+
+
+@DTYPES
+@pytest.mark.parametrize("q_len", [1, 4, 8, 16])
+@pytest.mark.parametrize("largest", [2.0 ** 30, 1.0, 2.0 ** -20])
+def test_pages_of_zeros_beside_the_largest_value_scale(sqa, q_len, largest, dtype):
+    """Tokens whose values are zero (their pages' scale is the append's 2^-100, or 0) count in the denominator in full, 0 to
+    20 bits below the one page that holds values at the largest scale allowed, and so do those of a small scale.
+
+    Bounds.  A score less its base is fma(s, c, log2 scale - base), |values| below 128 over these 90 bits of scales
+    and 20 of scores: two roundings of 2^-18 at most, the same for all tokens of one page.  The log-sum-exp adds
+    one of 2^-19 (top + log2 sum, below 64), log2's own 2^-22, the exponential's 2^-22 and the product's half step of
+    2^-20: ln 2 (2^-17 + 2^-19 + 2^-22) + 2^-22 + 2^-20 < 2^-16.4.  An output takes the first two in its
+    numerator and in its sum, the exponential's, and the parts' 2^-13: (2^-13 + 2^-15) of it."""
+    n = 4096
+    g = torch.Generator().manual_seed(q_len)
+    table = torch.randperm(n // 16, generator=g).to(torch.int32).view(1, -1)
+    at = table[0].long()
+    query = torch.zeros(1, q_len, 4, 128)
+    query[..., 0] = torch.linspace(0, 20, 4 * q_len).view(1, q_len, 4) * math.log(2) * 128 ** 0.5 / 7
+    k, v = torch.zeros(n // 16, 16, 1, 128), torch.zeros(n // 16, 16, 1, 128)
+    k[at[37], :, 0, 0] = 448
+    v[at[37]] = 200 + 100 * torch.rand(16, 1, 128, generator=g)
+    v[at[90:95]] = 100
+    vs = torch.full((n // 16, 1), 2.0 ** -100)
+    vs[at[::3]] = 0.0
+    vs[at[90:95]] = 2.0 ** -60
+    vs[at[37]] = largest
+    c = dict(q_len=q_len, table=table, seq_lens=torch.tensor([n], dtype=torch.int32), query=query.to(dtype), k=k.to(F8), v=v.to(F8),
+             ks=torch.full((n // 16, 1), 1 / 64.0), vs=vs)
+    for num_ctas in (0, 1):
+        out = torch.empty(query.shape, device="cuda")
+        out, lse = attend(sqa, c, num_ctas=num_ctas, out=out, return_lse=True)
+        x = 7.0 * c["query"][..., 0].double() * 128 ** -0.5  # of the page's 16 tokens; the others' is 0
+        seen = n - q_len + 1 + torch.arange(q_len)[:, None].double()
+        total = 16 * torch.exp(x) + seen - 16
+        want = (torch.exp(x) / total)[..., None] * largest * v[at[37], :, 0].to(F8).double().sum(dim=0)
+        assert ((lse.cpu().double() - total.log()).abs() <= 2.0 ** -16.4).all()
+        assert ((out.cpu().double() - want).abs() <= (2.0 ** -13 + 2.0 ** -15) * want).all()

@@ -51,10 +51,26 @@ constexpr long long kFp8LongRangeUnits = 400;
 constexpr int kScaledMinPages = 16, kWeightsMinPages = 8;
 constexpr int kScaledSegmentCost = 24;
 // Attention over segments of at most 64 pages (128 for q_len <= 8 with segments for a quarter of the
-// SMs) takes one CTA a segment: nothing is left to merge.  Measured against the split at q_len 4: 600
-// tokens x 1 9.8 against 13.1 us, 1000 x 1 12.3 / 14.8, 2000 x 1 18.5 / 16.1, 600 x 8 10.3 / 16.9,
-// 2000 x 8 19.8 / 23.5, 4000 x 8 33.1 / 28.2.
-constexpr int kWholePages = 64, kWholePagesMany = 128;
+// SMs) takes one CTA a segment: nothing is left to merge.  More segments than SMs run in waves of CTAs, each
+// with its start, where the split has one start a CTA and few pieces to merge: that pays for q_len 5
+// and up, for 3-4 in up to two waves and for 1-2 in two waves of up to 40 pages.
+// Measured, one CTA a segment against the split (us; B sequences of 8 heads, equal lengths):
+//   q_len 4   B 1:  600 tokens 9.5 / 17.4, 1000 11.9 / 17.6     B 16: 600 12.5 / 21.9, 2000 21.7 / 30.9
+//             B 32: 600 24.4 / 29.5, 2000 43.3 / 48.2           B 64: 600 49.3 / 48.3, 2000 87.2 / 84.1
+//   q_len 1   B 16: 2000 19.8 / 24.7    B 32: 600 22.0 / 23.6, 2000 39.5 / 36.9    B 64: 600 44.3 / 35.8
+//   q_len 8   B 64: 600 56.6 / 60.9, 2000 100.9 / 102.3    q_len 16  B 64: 600 73.9 / 99.7, 1000 92.9 / 120.4
+// The table's limits hold for ragged batches too, whose lengths the host does not see.  With 20 or 37 sequences of
+// equal lengths, just over one and under two waves, the split would be faster (q_len 3, 20 x 2000: 39.9 / 31.3;
+// q_len 1, 37 x 600: 23.5 / 19.8); with lengths from a quarter of that up it is slower (23.0 / 27.0, 21.8 / 26.6).
+constexpr int kWholePages = 64, kWholePagesMany = 128, kWholePagesWaves = 40;
+
+int whole_pages(int q_len, long long segments, int sms) {
+  if (segments > sms && q_len <= 4) {
+    if (segments > 2LL * sms) return 0;
+    if (q_len <= 2) return kWholePagesWaves;
+  }
+  return q_len <= 8 && 4 * segments >= sms ? kWholePagesMany : kWholePages;
+}
 constexpr int kSegmentCostTc = SQA_SEGMENT_COST_TC;
 constexpr int kSegmentCostMma = SQA_SEGMENT_COST_MMA;
 
@@ -576,11 +592,10 @@ int make_scaled_plan(const sqa_args* a, int device, bool weights, ScaledPlan* pl
   if (a->num_ctas <= 0 && segments > 0) {
     const int min_pages = a->min_pages_per_cta > 0 ? a->min_pages_per_cta : weights ? kWeightsMinPages : kScaledMinPages;
     grid = std::max(1LL, std::min(grid, (segments * pages + min_pages - 1) / min_pages));
-    const bool many = a->q_len <= 8 && 4 * segments >= sms;
     const long long even = (pages + min_pages - 1) / min_pages;  // CTAs a segment, each with its least
     if (weights && segments * even <= sms) {
       pl.seg_split = (int)even;
-    } else if (!weights && pages <= (many ? kWholePagesMany : kWholePages)) {
+    } else if (!weights && pages <= whole_pages(a->q_len, segments, sms)) {
       pl.seg_split = 1;
     } else if (a->cluster != 1 && a->max_seq_len > 0 && a->min_seq_len > 0 &&
                100LL * a->min_seq_len >= 85LL * a->max_seq_len) {

@@ -127,13 +127,22 @@ bool encode_cache_map_uncached(CUtensorMap* map, const void* base, int num_pages
   const cuuint64_t strides[3] = {row, hnd ? row * kPageSize : row * hkv, (cuuint64_t)page_stride};
   const cuuint32_t box[4] = {fp8 ? 128u : 64u, hnd ? (cuuint32_t)kPageSize : 1u, hnd ? 1u : (cuuint32_t)kPageSize, 1u};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
-  return fn(map, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base),
-            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B,
-            // L2 fills of one head's row: 256 B for 16-bit elements, 128 B for fp8 (a
-            // 256-byte fill there would also fetch the neighbouring head's row)
-            fp8 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  auto encode = [&] {
+    return fn(map, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base),
+              dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B,
+              // L2 fills of one head's row: 256 B for 16-bit elements, 128 B for fp8 (a
+              // 256-byte fill there would also fetch the neighbouring head's row)
+              fp8 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    // A host thread's first CUDA call: unlike the runtime's calls, a driver call binds no context to the thread.
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+  }
+  return r == CUDA_SUCCESS;
 }
 
 // A serving loop passes the same caches on every call: keep the last few

@@ -21,6 +21,7 @@
 #include <torch/extension.h>
 #include <torch/library.h>
 
+#include <memory>
 #include <mutex>
 #include <string>
 #include <tuple>
@@ -133,23 +134,32 @@ void check_status(int code, const char* what) {
   TORCH_CHECK(false, msg);
 }
 
+// The memory of one call.  A registered operator runs without Python's lock, so calls from two host threads on
+// one stream meet here: the launches of a call that use a shared workspace hold `turn`, or the
+// other call's kernels would come between its split and its merge.
+struct CallMemory {
+  at::Tensor ws;
+  std::shared_ptr<std::mutex> turn;  // null: the call's own memory, or the caller's
+  std::unique_lock<std::mutex> hold() const { return turn ? std::unique_lock<std::mutex>(*turn) : std::unique_lock<std::mutex>(); }
+};
+
 // One workspace per (device, stream), grown on demand; the status word of a
 // new one starts zeroed.  (A caller's explicit workspace is used as given.)
 struct WsEntry {
   int device;
   cudaStream_t stream;
-  at::Tensor ws;
+  CallMemory mem;
 };
 std::mutex g_ws_mu;
 std::vector<WsEntry> g_ws;
 
-std::pair<void*, size_t> workspace_for(const sqa_args& a, const at::Device& dev, cudaStream_t stream,
-                                       const c10::optional<at::Tensor>& workspace) {
+CallMemory workspace_for(const sqa_args& a, const at::Device& dev, cudaStream_t stream,
+                         const c10::optional<at::Tensor>& workspace) {
   if (workspace.has_value()) {
     const at::Tensor& w = *workspace;
     TORCH_CHECK_VALUE(w.device() == dev && w.is_contiguous(),
                       "workspace must be a contiguous tensor on the query's device");
-    return {w.data_ptr(), (size_t)w.numel() * w.element_size()};
+    return {w, nullptr};
   }
   int st = SQA_OK;
   const size_t need = sqa_workspace_bytes(&a, dev.index(), &st);
@@ -157,14 +167,15 @@ std::pair<void*, size_t> workspace_for(const sqa_args& a, const at::Device& dev,
   std::lock_guard<std::mutex> lock(g_ws_mu);
   for (auto& e : g_ws) {
     if (e.device == dev.index() && e.stream == stream) {
-      if ((size_t)e.ws.numel() < need) e.ws = at::zeros({(int64_t)std::max<size_t>(need, 1 << 20)},
-                                                        at::TensorOptions().dtype(at::kByte).device(dev));
-      return {e.ws.data_ptr(), (size_t)e.ws.numel()};
+      if ((size_t)e.mem.ws.numel() < need) e.mem.ws = at::zeros({(int64_t)std::max<size_t>(need, 1 << 20)},
+                                                                at::TensorOptions().dtype(at::kByte).device(dev));
+      return e.mem;
     }
   }
   g_ws.push_back(WsEntry{dev.index(), stream,
-                         at::zeros({(int64_t)std::max<size_t>(need, 1 << 20)}, at::TensorOptions().dtype(at::kByte).device(dev))});
-  return {g_ws.back().ws.data_ptr(), (size_t)g_ws.back().ws.numel()};
+                         {at::zeros({(int64_t)std::max<size_t>(need, 1 << 20)}, at::TensorOptions().dtype(at::kByte).device(dev)),
+                          std::make_shared<std::mutex>()}});
+  return g_ws.back().mem;
 }
 
 // check=True: synchronise and raise what the upstream CPU reference raises
@@ -184,8 +195,10 @@ void launch(sqa_args& a, const at::Tensor& q, const c10::optional<at::Tensor>& w
   c10::cuda::OptionalCUDAGuard guard;
   if (c10::cuda::current_device() != dev.index()) guard.set_index(dev.index());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
-  auto [ws, ws_bytes] = workspace_for(a, dev, stream, workspace);
-  const int code = sqa_forward(&a, ws, ws_bytes, stream);
+  const CallMemory mem = workspace_for(a, dev, stream, workspace);
+  const auto turn = mem.hold();
+  void* const ws = mem.ws.data_ptr();
+  const int code = sqa_forward(&a, ws, (size_t)mem.ws.numel() * mem.ws.element_size(), stream);
   if (code == SQA_ERR_WORKSPACE_TOO_SMALL && workspace.has_value()) {
     int st = SQA_OK;
     TORCH_CHECK_VALUE(false, "workspace too small: need ", sqa_workspace_bytes(&a, dev.index(), &st), " bytes");
@@ -265,29 +278,29 @@ struct UseEntry {
   int device;
   cudaStream_t stream;
   Use use;
-  at::Tensor ws;
+  CallMemory mem;
 };
 std::mutex g_use_mu;
 std::vector<UseEntry> g_use;
 
-at::Tensor memory_for(Use use, size_t need, const at::Device& dev, cudaStream_t stream) {
+CallMemory memory_for(Use use, size_t need, const at::Device& dev, cudaStream_t stream) {
   const auto bytes = at::TensorOptions().dtype(at::kByte).device(dev);
   cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
   TORCH_CHECK(cudaStreamIsCapturing(stream, &cs) == cudaSuccess, "cudaStreamIsCapturing failed");
   if (cs != cudaStreamCaptureStatusNone) {
     at::Tensor ws = at::empty({(int64_t)need}, bytes);
     check_status(sqa_workspace_init(ws.data_ptr(), std::min<size_t>(need, 256), stream), "sqa_workspace_init");
-    return ws;
+    return {ws, nullptr};
   }
   std::lock_guard<std::mutex> lock(g_use_mu);
   for (auto& e : g_use) {
     if (e.device == dev.index() && e.stream == stream && e.use == use) {
-      if ((size_t)e.ws.numel() < need) e.ws = at::zeros({(int64_t)need}, bytes);
-      return e.ws;
+      if ((size_t)e.mem.ws.numel() < need) e.mem.ws = at::zeros({(int64_t)need}, bytes);
+      return e.mem;
     }
   }
-  g_use.push_back(UseEntry{dev.index(), stream, use, at::zeros({(int64_t)need}, bytes)});
-  return g_use.back().ws;
+  g_use.push_back(UseEntry{dev.index(), stream, use, {at::zeros({(int64_t)need}, bytes), std::make_shared<std::mutex>()}});
+  return g_use.back().mem;
 }
 
 // check=True reports the bits of this call alone: earlier unchecked calls on the
@@ -337,9 +350,11 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> forward_scaled(
   check_status(st, "sqa_scaled_workspace_bytes");
   TORCH_CHECK_VALUE(!workspace.has_value() || (workspace->device() == dev && workspace->is_contiguous()),
                     "workspace must be a contiguous tensor on the query's device");
-  const at::Tensor ws = workspace.has_value() ? *workspace : memory_for(kUseAttention, need, dev, stream);
+  const CallMemory mem = workspace.has_value() ? CallMemory{*workspace, nullptr} : memory_for(kUseAttention, need, dev, stream);
+  const at::Tensor& ws = mem.ws;
   const size_t have = (size_t)ws.numel() * ws.element_size();
   TORCH_CHECK_VALUE(have >= need, "workspace too small: need ", need, " bytes");
+  const auto turn = mem.hold();
   if (check) clear_status(ws, stream);
   check_status(sqa_forward_scaled(&a, &scales, ws.data_ptr(), have, stream), "sqa_forward_scaled");
   if (check) raise_device_bits(ws.data_ptr(), stream);
@@ -367,7 +382,9 @@ void accumulate_weights(const at::Tensor& query, const at::Tensor& key_cache, co
                     "scores must be a contiguous fp32 tensor [num_pages, Hkv, 16]");
   c10::cuda::OptionalCUDAGuard guard;
   const cudaStream_t stream = on_device(guard, dev);
-  const at::Tensor word = memory_for(kUseWeights, 256, dev, stream);
+  const CallMemory mem = memory_for(kUseWeights, 256, dev, stream);
+  const auto turn = mem.hold();
+  const at::Tensor& word = mem.ws;
   if (check) clear_status(word, stream);
   check_status(sqa_accumulate_weights(&a, lse.data_ptr<float>(), fp8 ? &scales : nullptr, scores.data_ptr<float>(),
                                       static_cast<uint32_t*>(word.data_ptr()), stream),
@@ -410,7 +427,9 @@ void append_scaled(const at::Tensor& new_keys, const at::Tensor& new_values, con
   if (batch == 0) return;
   c10::cuda::OptionalCUDAGuard guard;
   const cudaStream_t stream = on_device(guard, dev);
-  const at::Tensor word = memory_for(kUseAppend, 256, dev, stream);
+  const CallMemory mem = memory_for(kUseAppend, 256, dev, stream);
+  const auto turn = mem.hold();
+  const at::Tensor& word = mem.ws;
   sqa_append_args a = {};
   a.new_keys = new_keys.data_ptr();
   a.new_values = new_values.data_ptr();
@@ -485,7 +504,9 @@ std::tuple<at::Tensor, at::Tensor> cache_evict(const at::Tensor& key_cache, cons
   if (batch == 0) return {lens, from};
   c10::cuda::OptionalCUDAGuard guard;
   const cudaStream_t stream = on_device(guard, dev);
-  const at::Tensor word = memory_for(kUseEvict, 256, dev, stream);
+  const CallMemory mem = memory_for(kUseEvict, 256, dev, stream);
+  const auto turn = mem.hold();
+  const at::Tensor& word = mem.ws;
   sqa_evict_args a = {};
   a.key_cache = key_cache.data_ptr();
   a.value_cache = value_cache.data_ptr();

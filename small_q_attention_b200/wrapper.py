@@ -43,7 +43,8 @@ class PagedMTPAttention:
     new plan needs a larger workspace, and a run with ``scores`` only when its
     log-sum-exp (and fp32 rows) outgrow the kept ones.  Outgrown memory is kept (each new buffer is
     at least twice as large as the last), so a graph captured before can still be replayed.
-    Graphs captured from one object share its memory and must not be replayed at the same time.
+    Graphs captured from one object share its memory and must not be replayed at the same time;
+    neither must two host threads or streams run one object at once.
     """
 
     def __init__(self, device: torch.device | int | None = None, *, kernel: int = 0):

@@ -1047,7 +1047,9 @@ __device__ void weigh(const ScaledTcParams& p, const Schedule& sch, const Smem<S
       float* const at = p.scores + ((size_t)max(id, 0) * p.s.hkv + w.h) * kPageSize + (tid & 15);
       const float old = (held && id >= 0 && tok < piece.fresh) ? __ldcg(at) : 0.f;  // in flight during the score product
       const bool masked = np < kBlockPages || tok0 + kBlock > piece.first || tok0 + kBlock > piece.len;
-      const int late = held ? tok - piece.first : 0x7fffffff;
+      // draft qi sees the token iff late < qi.  Of a token that no draft sees the padding rows must not see it
+      // either: their scores are 0 times its K, NaN for a K or a scale that is not finite.
+      const int late = held && tok - piece.first < p.s.q_len - 1 ? tok - piece.first : 0x7fffffff;
       float sum = 0.f;
 #pragma unroll 1
       for (int g = 0; g < G; ++g) {

@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(T, 512 / T) sqa_cache_evict_kernel(const Evict
     kept[p.budget - p.recent + i] = len - p.recent + i;
   meet();  // kept[] is complete, for every CTA of the cluster
 
-  // ---- 3. moves, C x 8 target pages a wave
+  // ---- 3. moves, C x T / 32 target pages a wave
   constexpr int kLanesPerRow = kHeadDim * E / 16;     // 16 (16-bit) or 8 (e4m3) lanes hold a row
   constexpr int kRowsPerLoad = 32 / kLanesPerRow;     // rows a warp loads at once
   constexpr int kLoads = kPageSize / kRowsPerLoad;

@@ -1119,7 +1119,7 @@ __global__ void __launch_bounds__(S::THREADS, 1)
   }
   // The value issuer has nothing to do before the first P: it prefetches the CTA's first
   // pages into L2 before the dependency wait (hints only).
-  if (warp == kValueWarp) prefetch_start<S::F8>(p.s, &tm_k, &tm_v, tiles / S::TILES * kBlockPages);
+  if (warp == kValueWarp) prefetch_start<S::F8, S::ATTEND>(p.s, &tm_k, &tm_v, tiles / S::TILES * kBlockPages);
   grid_dependency_wait();
   allow_dependent_launch();
   if (warp == kScoreWarp) {

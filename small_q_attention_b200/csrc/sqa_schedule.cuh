@@ -349,7 +349,7 @@ __device__ __forceinline__ int2 aligned_segment_pieces(const int32_t* seq_lens, 
 // be stale: they only steer prefetches (nothing is consumed or written, and a
 // page id outside the pool is skipped), and every value is read again after
 // the wait.  The loads after the wait then find their lines in L2.
-template <bool F8>
+template <bool F8, bool kValues = true>  // kValues: V is read too
 __device__ __forceinline__ void prefetch_start(const SplitKvParams& p, const CUtensorMap* tm_k,
                                                const CUtensorMap* tm_v, int budget) {
   const int lane = threadIdx.x & 31;
@@ -375,12 +375,14 @@ __device__ __forceinline__ void prefetch_start(const SplitKvParams& p, const CUt
         const int k1 = p.hnd ? 0 : h, k2 = p.hnd ? h : 0;  // NHD (dim, head, token, page); HND (dim, token, head, page)
         if constexpr (F8) {  // fp8 maps: one 128-dim box per page
           tma_prefetch_4d(tm_k, 0, k1, k2, id);
-          tma_prefetch_4d(tm_v, 0, k1, k2, id);
+          if (kValues) tma_prefetch_4d(tm_v, 0, k1, k2, id);
         } else {  // 16-bit maps: two 64-dim boxes per page
           tma_prefetch_4d(tm_k, 0, k1, k2, id);
           tma_prefetch_4d(tm_k, 64, k1, k2, id);
-          tma_prefetch_4d(tm_v, 0, k1, k2, id);
-          tma_prefetch_4d(tm_v, 64, k1, k2, id);
+          if (kValues) {
+            tma_prefetch_4d(tm_v, 0, k1, k2, id);
+            tma_prefetch_4d(tm_v, 64, k1, k2, id);
+          }
         }
       }
     }

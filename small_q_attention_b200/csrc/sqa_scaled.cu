@@ -48,10 +48,12 @@
 // (237 / 241 us, fp16 243 / 290, for want of registers).  Two groups of a block share a product
 // (GP = 2, one read of K and V for both: 4 x 16 x 65536 230 -> 195 us).
 //
-// What bounds it.  q_len 1-4 run at 5.3-5.8 TB/s (q_len 2, 16 x 32768: 187 us for 1.07 GB), near what
+// What bounds it.  q_len 1-4 run at 5.2-5.7 TB/s (q_len 2, 16 x 32768: 190 us for 1.07 GB), near what
 // the loads alone reach (5.8 TB/s at q_len 4 with P, the scores and the value products left out).  Above it
-// is no one stage: at q_len 8, of 245 us, leaving out P saved 28, the scores 18, the value products
-// 38, all three 45; at q_len 16 (4 x 65536, before GP = 2), of 238 us, 29, 25, 60 and 79.
+// is the softmax threads' work, more than any one stage: with three parts of P, at q_len 8, of 245 us,
+// leaving out P saved 28, the scores 18, the value products 38, all three 45; at q_len 16 (4 x 65536, before
+// GP = 2), of 238 us, 29, 25, 60 and 79.  The fourth part took q_len 8 from 241 to 261 us and q_len 16 (1 x 262144)
+// from 194 to 219, where the SM now issues 2.6 instructions a cycle.
 //
 // Warps: 0 .. 4 W - 1 softmax (one token a thread), then one each for score products, value
 // products, TMA and page scales.  Work is cut into CTA ranges by sqa_schedule.cuh; pieces of a split

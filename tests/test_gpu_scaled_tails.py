@@ -122,7 +122,7 @@ def test_tail_under_a_dominant_token_that_comes_later(sqa, q_len, dtype):
 
 @DTYPES
 @pytest.mark.parametrize("q_len", [2, 8])
-def test_tail_under_two_dominant_tokens_of_one_block(sqa, q_len, dtype):
+def test_tail_under_dominant_tokens_in_every_run_of_a_block(sqa, q_len, dtype):
     """All four runs of 32 tokens of the first block hold one: its largest P is 2^-1, and the floor is the parts' own."""
     c = dominated(q_len, 32768, [0, 40, 70, 127], dtype, seed=q_len, low=10.0, high=14.0)
     assert_tail(attend(sqa, c, num_ctas=1), c, lambda y, limit: -1.0)
